@@ -49,6 +49,7 @@ typedef enum qfg_status {
 typedef enum qfg_dtype {
   QFG_FLOAT = 1,
   QFG_UINT8 = 2,        /* block-16 NVFP4, [K, N * 9 / 16] */
+  QFG_INT8 = 3,         /* rows and weights with a scale for each row and column (RmsNormQuant, RowQuant, QuantGemm) */
   QFG_INT64 = 7,
   QFG_FLOAT16 = 10,
   QFG_BFLOAT16 = 16,
@@ -303,6 +304,43 @@ QFG_API int qfg_peer_free(void* ptr);
 
 /* Fold `ranks` gathered key rows (keys[rank * m + row]) into idx[row] / val[row]. */
 QFG_API int qfg_lmhead_combine(const uint64_t* keys, int ranks, int64_t m, int64_t* idx, float* val, void* stream);
+
+/* ---------------------------------------------------------------- eight-bit rows
+ * An eight-bit block, no counterpart in the reference: rows of activations in INT8 or E4M3 with a scale each, and their product
+ * with a weight of the same type that has a scale for each column.  Matrices may have rows further apart than they are long (`ld*`,
+ * in elements); their last dimension is contiguous.  Rows and weights may begin anywhere that their element type may; the
+ * kernels are fastest where bases and row distances are multiples of 16 bytes.
+ *
+ * RmsNormQuant: h = x + residual, rounded to its type, is kept (residual == NULL: h is x, and `h` is not written); y_i = h_i *
+ * rsqrt(mean(h^2) + eps) * (weight_offset + weight_i); then as RowQuant.  `dtype` (BFLOAT16, FLOAT16, FLOAT) is that of x, residual and h,
+ * `weight_dtype` the same or FLOAT, `q_dtype` INT8 or FLOAT8E4M3FN.  q is [rows, n], scale FP32 [rows], h [rows, n], all contiguous; h may be
+ * the residual or x itself where that is contiguous.
+ *
+ * RowQuant: y = x, or swish(x) * u in FP32 where u is given; scale = max(max_i |y_i|, 2^-100) / top with top = 127 (INT8) or 448 (E4M3); q_i = y_i /
+ * scale, rounded to nearest, ties to even.  A row whose largest value, or whose sum of squares in a norm, is not a finite FP32
+ * number has scale NaN and q 0.
+ *
+ * rows == 0 is a no-op; 1 <= n <= INT_MAX / 2. */
+QFG_API int qfg_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype,
+                              float weight_offset, float eps, int64_t rows, int64_t n, int q_dtype, void* q, float* scale, void* h,
+                              void* stream);
+QFG_API int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q,
+                          float* scale, void* stream);
+
+/* QuantGemm: out[m, n] = (sum_k x[m, k] w[k, n]) * x_scale[m] * w_scale[n].  INT8 products are summed in 32-bit integers, which is
+ * exact (k <= 131071 of them cannot overflow), E4M3 products in FP32; the sum is scaled in FP32 and rounded once to `out_dtype`
+ * (BFLOAT16, FLOAT16 or FLOAT).  `w_scale` (host floats, one per column, uploaded once here; NULL: ones).
+ * `dtype` is that of x and of w, INT8 or FLOAT8E4M3FN; x_scale FP32 [m] on the device.  The weight is [k][n] with rows ldw apart (QFG_ORDER_N: its
+ * columns lie beside one another) or [n][k] (QFG_ORDER_K).  m == 0 is a no-op.  Nothing is allocated and the call may be captured. */
+typedef enum qfg_order { QFG_ORDER_N = 0, QFG_ORDER_K = 1 } qfg_order;
+typedef struct qfg_quant_gemm qfg_quant_gemm;
+QFG_API int qfg_quant_gemm_create(const float* w_scale, size_t n_w_scale, int out_dtype, qfg_quant_gemm** out);
+QFG_API int qfg_quant_gemm_compute(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx, const float* x_scale, int64_t m, int64_t k,
+                                   const void* w, int64_t ldw, int order, int64_t n, void* out, int64_t ldo, void* stream);
+/* "plan" = "rows per tile,CTAs that split K,pair,CTAs per SM" pins the launch shape ("" gives the choice back); one that does not exist is an error
+ * of the call.  "give_up" = 1, for tests: no operand comes, and what waits for it gives up and writes NaN. */
+QFG_API int qfg_quant_gemm_set_option(qfg_quant_gemm* op, const char* key, const char* value);
+QFG_API void qfg_quant_gemm_destroy(qfg_quant_gemm* op);
 
 /* Measurement aid, no counterpart in the reference: sweeps `bytes` of device memory at `buf` (16-byte aligned) with
  * 128-bit read-only loads and writes nothing (`sink`, 4 bytes of device memory or null, is never stored to on

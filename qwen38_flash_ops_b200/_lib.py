@@ -15,7 +15,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("QFG_LIBRARY") or os.path.join(_HERE, "libqfg_b200.so")
 
 QFG_OK, QFG_FAIL, QFG_INVALID_ARGUMENT = 0, 1, 2
-QFG_FLOAT, QFG_UINT8, QFG_INT64, QFG_FLOAT16, QFG_BFLOAT16, QFG_FLOAT8E4M3FN = 1, 2, 7, 10, 16, 17
+QFG_FLOAT, QFG_UINT8, QFG_INT8, QFG_INT64, QFG_FLOAT16, QFG_BFLOAT16, QFG_FLOAT8E4M3FN = 1, 2, 3, 7, 10, 16, 17
+QFG_ORDER_N, QFG_ORDER_K = 0, 1
 
 # every symbol include/qfg.h declares
 EXPORTS = (
@@ -27,6 +28,8 @@ EXPORTS = (
     "qfg_untile_hc_create", "qfg_untile_hc_compute", "qfg_untile_hc_destroy",
     "qfg_shared_expert_down_create", "qfg_shared_expert_down_compute", "qfg_shared_expert_down_set_option",
     "qfg_shared_expert_down_destroy",
+    "qfg_rmsnorm_quant", "qfg_row_quant",
+    "qfg_quant_gemm_create", "qfg_quant_gemm_compute", "qfg_quant_gemm_set_option", "qfg_quant_gemm_destroy",
     "qfg_lmhead_workspace_bytes", "qfg_lmhead_create", "qfg_lmhead_compute", "qfg_lmhead_static_max_rows",
     "qfg_lmhead_compute_static", "qfg_lmhead_set_option",
     "qfg_lmhead_destroy", "qfg_lmhead_combine",
@@ -99,6 +102,15 @@ def load() -> ctypes.CDLL:
     lib.qfg_untile_hc_compute.argtypes = [c_void_p, POINTER(Tensor2D), c_void_p, c_void_p]
     lib.qfg_untile_hc_destroy.argtypes = [c_void_p]
     lib.qfg_untile_hc_destroy.restype = None
+    lib.qfg_rmsnorm_quant.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, c_float, c_int64, c_int64, c_int,
+                                      c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.qfg_row_quant.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]
+    lib.qfg_quant_gemm_create.argtypes = [POINTER(c_float), c_size_t, c_int, POINTER(c_void_p)]
+    lib.qfg_quant_gemm_compute.argtypes = [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_int64,
+                                           c_void_p, c_int64, c_void_p]
+    lib.qfg_quant_gemm_set_option.argtypes = [c_void_p, c_char_p, c_char_p]
+    lib.qfg_quant_gemm_destroy.argtypes = [c_void_p]
+    lib.qfg_quant_gemm_destroy.restype = None
     lib.qfg_lmhead_exchange_bytes.restype = c_size_t
     lib.qfg_lmhead_compute_sharded.argtypes = [c_void_p, c_void_p, c_int64, c_int64, POINTER(Tensor2D), c_int64, c_int64,
                                                c_void_p, POINTER(LmExchange), c_void_p, c_void_p, c_void_p, c_void_p]

@@ -22,17 +22,24 @@ struct Entries {
   decltype(&qfg_dequant_compute) dequant;
   decltype(&qfg_lmhead_compute) lmhead;
   decltype(&qfg_shared_expert_down_compute) shared_expert_down;
+  decltype(&qfg_rmsnorm_quant) rmsnorm_quant;
+  decltype(&qfg_row_quant) row_quant;
+  decltype(&qfg_quant_gemm_compute) quant_gemm;
 } g_lib;
 
-// A plain dense CUDA tensor, or null: no subclass, no wrapper of a transform, nothing without memory of its own.
-const at::Tensor* Dense(PyObject* o) {
+// A plain CUDA tensor, or null: no subclass, no wrapper of a transform, nothing without memory of its own.
+const at::Tensor* Plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   const c10::DispatchKeySet keys = t.key_set();
   if (!t.defined() || !keys.has(c10::DispatchKey::CUDA) || keys.has(c10::DispatchKey::Python) || keys.has(c10::DispatchKey::FuncTorchBatched) ||
-      keys.has(c10::DispatchKey::FuncTorchGradWrapper) || keys.has(c10::DispatchKey::Functionalize) || !t.has_storage() || !t.is_contiguous())
+      keys.has(c10::DispatchKey::FuncTorchGradWrapper) || keys.has(c10::DispatchKey::Functionalize) || !t.has_storage())
     return nullptr;
   return &t;
+}
+const at::Tensor* Dense(PyObject* o) {  // a contiguous one
+  const at::Tensor* t = Plain(o);
+  return t != nullptr && t->is_contiguous() ? t : nullptr;
 }
 const at::Tensor* Bf16(PyObject* o) {
   const at::Tensor* t = Dense(o);
@@ -243,6 +250,134 @@ PyObject* SharedExpertDown(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// ---- eight-bit rows
+int Code(at::ScalarType t) {  // 0: none of the types here
+  switch (t) {
+    case at::kBFloat16: return QFG_BFLOAT16;
+    case at::kHalf: return QFG_FLOAT16;
+    case at::kFloat: return QFG_FLOAT;
+    case at::kChar: return QFG_INT8;
+    case at::kFloat8_e4m3fn: return QFG_FLOAT8E4M3FN;
+    default: return 0;
+  }
+}
+bool Float(const at::Tensor& t) { return Code(t.scalar_type()) != 0 && t.element_size() > 1; }
+bool EightBits(const at::Tensor& t) { return Code(t.scalar_type()) != 0 && t.element_size() == 1; }
+bool OnCurrent(const at::Tensor& t) { return t.get_device() == c10::cuda::current_device(); }
+// Rows that are evenly spaced, on the current device: contiguous, or a matrix whose rows are further apart.
+struct Rows {
+  const at::Tensor* t = nullptr;
+  int64_t rows = 0, n = 0, ld = 0;
+};
+bool ToRows(PyObject* o, Rows* r) {
+  r->t = Plain(o);
+  if (r->t == nullptr || r->t->dim() < 1 || r->t->size(-1) < 1 || !OnCurrent(*r->t)) return false;
+  r->n = r->t->size(-1);
+  r->rows = r->t->numel() / r->n;
+  r->ld = r->n;
+  if (r->t->is_contiguous()) return true;
+  r->ld = r->t->dim() == 2 ? r->t->stride(0) : 0;
+  return r->ld >= r->n && (r->t->stride(1) == 1 || r->n == 1);
+}
+
+// rmsnorm_quant(eps, weight_offset, fp8, x, weight, residual or None) -> (q, scale) or (q, scale, h)
+PyObject* RmsNormQuant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    Rows x, r;
+    if (n_args != 6 || !PyFloat_CheckExact(a[0]) || !PyFloat_CheckExact(a[1]) || (a[2] != Py_True && a[2] != Py_False) || !ToRows(a[3], &x)) return None();
+    const at::Tensor* w = Dense(a[4]);
+    const bool added = a[5] != Py_None;
+    if (w == nullptr || !Float(*x.t) || (w->scalar_type() != x.t->scalar_type() && w->scalar_type() != at::kFloat) || w->numel() != x.n || !OnCurrent(*w))
+      return None();
+    if (added && (!ToRows(a[5], &r) || r.t->scalar_type() != x.t->scalar_type() || r.t->sizes() != x.t->sizes())) return None();
+    const bool fp8 = a[2] == Py_True;
+    const at::Tensor q = at::empty(x.t->sizes(), x.t->options().dtype(fp8 ? at::kFloat8_e4m3fn : at::kChar)),
+                     scale = at::empty(x.t->sizes().slice(0, x.t->dim() - 1), x.t->options().dtype(at::kFloat));
+    at::Tensor h;
+    if (added) h = at::empty(x.t->sizes(), x.t->options());
+    const int dtype = Code(x.t->scalar_type()), w_dtype = Code(w->scalar_type());
+    const float offset = static_cast<float>(PyFloat_AS_DOUBLE(a[1])), eps = static_cast<float>(PyFloat_AS_DOUBLE(a[0]));
+    const void *xp = x.t->data_ptr(), *rp = added ? r.t->data_ptr() : nullptr, *wp = w->data_ptr();
+    void *const qp = q.data_ptr(), *const hp = added ? h.data_ptr() : nullptr, *const stream = Stream();
+    float* const sp = scale.data_ptr<float>();
+    const int code = Call([&] {
+      return g_lib.rmsnorm_quant(dtype, xp, x.ld, rp, r.ld, wp, w_dtype, offset, eps, x.rows, x.n, fp8 ? QFG_FLOAT8E4M3FN : QFG_INT8, qp, sp, hp, stream);
+    });
+    return code != 0 ? PyLong_FromLong(code) : added ? TupleOf({q, scale, h}) : TupleOf({q, scale});
+  });
+}
+
+// row_quant(fp8, x, u or None) -> (q, scale)
+PyObject* RowQuant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    Rows x, u;
+    if (n_args != 3 || (a[0] != Py_True && a[0] != Py_False) || !ToRows(a[1], &x) || !Float(*x.t)) return None();
+    const bool gated = a[2] != Py_None, fp8 = a[0] == Py_True;
+    if (gated && (!ToRows(a[2], &u) || u.t->scalar_type() != x.t->scalar_type() || u.t->sizes() != x.t->sizes())) return None();
+    const at::Tensor q = at::empty(x.t->sizes(), x.t->options().dtype(fp8 ? at::kFloat8_e4m3fn : at::kChar)),
+                     scale = at::empty(x.t->sizes().slice(0, x.t->dim() - 1), x.t->options().dtype(at::kFloat));
+    const int dtype = Code(x.t->scalar_type());
+    const void *xp = x.t->data_ptr(), *up = gated ? u.t->data_ptr() : nullptr;
+    void *const qp = q.data_ptr(), *const stream = Stream();
+    float* const sp = scale.data_ptr<float>();
+    const int code = Call([&] { return g_lib.row_quant(dtype, xp, x.ld, up, u.ld, x.rows, x.n, fp8 ? QFG_FLOAT8E4M3FN : QFG_INT8, qp, sp, stream); });
+    return code != 0 ? PyLong_FromLong(code) : TupleOf({q, scale});
+  });
+}
+
+// quant_gemm(handle, output type, x, x_scale, w) -> out
+PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    Rows x;
+    if (n_args != 5 || !ToRows(a[2], &x) || !EightBits(*x.t)) return None();
+    const void* op = PyLong_AsVoidPtr(a[0]);
+    const long out_dtype = PyLong_AsLong(a[1]);
+    const at::Tensor *xs = Dense(a[3]), *w = Plain(a[4]);
+    if (PyErr_Occurred() || op == nullptr || xs == nullptr || w == nullptr || xs->scalar_type() != at::kFloat || xs->numel() != x.rows || !OnCurrent(*xs) ||
+        w->dim() != 2 || w->scalar_type() != x.t->scalar_type() || w->size(0) != x.n || w->size(1) < 1 || !OnCurrent(*w))
+      return None();
+    const int64_t n = w->size(1), k = x.n;
+    int order;
+    int64_t ldw;
+    if (w->stride(1) == 1 && w->stride(0) >= n) {
+      order = QFG_ORDER_N, ldw = w->stride(0);
+    } else if (w->stride(0) == 1 && w->stride(1) >= k) {
+      order = QFG_ORDER_K, ldw = w->stride(1);
+    } else {
+      return None();
+    }
+    c10::SmallVector<int64_t, 6> shape(x.t->sizes().begin(), x.t->sizes().end());
+    shape.back() = n;
+    const at::Tensor out = at::empty(shape, x.t->options().dtype(out_dtype == QFG_BFLOAT16 ? at::kBFloat16 : out_dtype == QFG_FLOAT16 ? at::kHalf : at::kFloat));
+    const int dtype = Code(x.t->scalar_type());
+    const void *xp = x.t->data_ptr(), *wp = w->data_ptr();
+    const float* const sp = xs->data_ptr<float>();
+    void *const yp = out.data_ptr(), *const stream = Stream();
+    const int code =
+        Call([&] { return g_lib.quant_gemm(static_cast<const qfg_quant_gemm*>(op), dtype, xp, x.ld, sp, x.rows, k, wp, ldw, order, n, yp, n, stream); });
+    return code != 0 ? PyLong_FromLong(code) : THPVariable_Wrap(out);
+  });
+}
+
+template <typename T>
+bool Address(PyObject* o, T* fn) {
+  void* p = PyLong_AsVoidPtr(o);
+  if (p == nullptr && !PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
+  *fn = reinterpret_cast<T>(p);
+  return p != nullptr;
+}
+// bind_rows(address, ...): the entry points of eight-bit rows, in the order of Entries
+PyObject* BindRows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  if (n_args != 3) {
+    PyErr_SetString(PyExc_TypeError, "bind_rows takes three addresses");
+    return nullptr;
+  }
+  Entries e = g_lib;
+  if (!Address(a[0], &e.rmsnorm_quant) || !Address(a[1], &e.row_quant) || !Address(a[2], &e.quant_gemm)) return nullptr;
+  g_lib = e;
+  Py_RETURN_NONE;
+}
+
 // bind(address, ...) in the order of Entries
 PyObject* Bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   void* p[5];
@@ -272,6 +407,10 @@ PyMethodDef g_methods[] = {QFG_METHOD("bind", Bind),
                            QFG_METHOD("dequant", Dequant),
                            QFG_METHOD("lmhead", LmHead),
                            QFG_METHOD("shared_expert_down", SharedExpertDown),
+                           QFG_METHOD("bind_rows", BindRows),
+                           QFG_METHOD("rmsnorm_quant", RmsNormQuant),
+                           QFG_METHOD("row_quant", RowQuant),
+                           QFG_METHOD("quant_gemm", QuantGemm),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

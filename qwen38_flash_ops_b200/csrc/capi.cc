@@ -113,6 +113,15 @@ struct qfg_shared_expert_down {
   qfg_skinny_gemm gemm;
 };
 
+struct qfg_quant_gemm {
+  int out_dtype = QFG_BFLOAT16;
+  int device = 0;
+  float* d_w_scale = nullptr;
+  size_t w_scale_len = 0;
+  qfg::QuantPlan plan;  // bm > 0: set_option("plan", ...)
+  int give_up = 0;
+};
+
 struct qfg_untile_hc {
   int kind = 0;
   float* d_w_scale = nullptr;
@@ -664,6 +673,157 @@ int qfg_shared_expert_down_set_option(qfg_shared_expert_down* op, const char* ke
 void qfg_shared_expert_down_destroy(qfg_shared_expert_down* op) {
   if (op == nullptr) return;
   cudaFree(op->gemm.d_w_scale);
+  delete op;
+}
+
+// ------------------------------------------------------------------------------ eight-bit rows
+namespace {
+
+size_t ElementBytes(int dtype) { return dtype == QFG_FLOAT ? 4 : dtype == QFG_BFLOAT16 || dtype == QFG_FLOAT16 ? 2 : 0; }  // 0: no type of rows
+bool Aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+bool EightBits(int dtype) { return dtype == QFG_INT8 || dtype == QFG_FLOAT8E4M3FN; }
+
+int RunRowQuant(const char* name, qfg::RowQuantCall& c, int q_dtype, void* stream) {
+  const size_t elem = ElementBytes(c.dtype);
+  if (elem == 0) return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": rows must be BF16/FP16/FP32");
+  if (!EightBits(q_dtype)) return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": q must be INT8 or FP8 E4M3FN");
+  const bool added = c.norm && c.residual != nullptr;
+  if (c.rows < 0 || c.n < 1 || c.n > INT_MAX / 2 || c.ldx < c.n || (added && c.ldr < c.n) || (c.u != nullptr && c.ldu < c.n))
+    return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": bad shape");
+  if (c.rows == 0) return QFG_OK;
+  if (c.x == nullptr || c.q == nullptr || c.scale == nullptr || (c.norm && c.weight == nullptr) || (added && c.h == nullptr))
+    return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": null argument");
+  if (!Aligned(c.x, elem) || !Aligned(c.u, elem) || !Aligned(c.residual, elem) || !Aligned(c.h, elem) || !Aligned(c.scale, 4) ||
+      (c.norm && !Aligned(c.weight, ElementBytes(c.weight_dtype))))
+    return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": misaligned argument");
+  c.fp8 = q_dtype == QFG_FLOAT8E4M3FN;
+  const cudaError_t err = qfg::LaunchRowQuant(c, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? QFG_OK : Fail(QFG_FAIL, std::string(name) + ": " + cudaGetErrorString(err));
+}
+
+}  // namespace
+
+int qfg_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype,
+                      float weight_offset, float eps, int64_t rows, int64_t n, int q_dtype, void* q, float* scale, void* h, void* stream) {
+  if (weight_dtype != dtype && weight_dtype != QFG_FLOAT)
+    return Fail(QFG_INVALID_ARGUMENT, "RmsNormQuant: the weight must have the type of x, or FP32");
+  if (!(eps >= 0.f)) return Fail(QFG_INVALID_ARGUMENT, "RmsNormQuant: eps must not be negative");
+  qfg::RowQuantCall c;
+  c.norm = true;
+  c.dtype = dtype;
+  c.x = x;
+  c.ldx = ldx;
+  c.residual = residual;
+  c.ldr = ldr;
+  c.weight = weight;
+  c.weight_dtype = weight_dtype;
+  c.weight_offset = weight_offset;
+  c.eps = eps;
+  c.rows = rows;
+  c.n = n;
+  c.q = static_cast<uint8_t*>(q);
+  c.scale = scale;
+  c.h = residual != nullptr ? h : nullptr;
+  return RunRowQuant("RmsNormQuant", c, q_dtype, stream);
+}
+
+int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q, float* scale,
+                  void* stream) {
+  qfg::RowQuantCall c;
+  c.dtype = dtype;
+  c.x = x;
+  c.ldx = ldx;
+  c.u = u;
+  c.ldu = ldu;
+  c.rows = rows;
+  c.n = n;
+  c.q = static_cast<uint8_t*>(q);
+  c.scale = scale;
+  return RunRowQuant("RowQuant", c, q_dtype, stream);
+}
+
+int qfg_quant_gemm_create(const float* w_scale, size_t n_w_scale, int out_dtype, qfg_quant_gemm** out) {
+  if (out == nullptr) return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: null handle pointer");
+  *out = nullptr;
+  if (ElementBytes(out_dtype) == 0) return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: the output must be BF16/FP16/FP32");
+  if ((w_scale == nullptr) != (n_w_scale == 0)) return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: bad w_scale");
+  qfg_quant_gemm* op = nullptr;
+  try {
+    op = new qfg_quant_gemm();
+    op->out_dtype = out_dtype;
+    cudaError_t err = qfg::ConfigureQuantKernels();
+    if (err == cudaSuccess) err = cudaGetDevice(&op->device);
+    if (err != cudaSuccess) throw std::runtime_error(std::string("QuantGemm: ") + cudaGetErrorString(err));
+    op->d_w_scale = UploadScales(w_scale, n_w_scale, "QuantGemm");
+    op->w_scale_len = n_w_scale;
+  } catch (const std::exception& e) {
+    delete op;
+    return Fail(QFG_FAIL, e.what());
+  }
+  *out = op;
+  return QFG_OK;
+}
+
+int qfg_quant_gemm_compute(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx, const float* x_scale, int64_t m, int64_t k, const void* w,
+                           int64_t ldw, int order, int64_t n, void* out, int64_t ldo, void* stream) {
+  if (op == nullptr) return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: null node");
+  try {
+    if (!EightBits(dtype)) throw InvalidArgument("QuantGemm: x and the weight must be INT8 or FP8 E4M3FN");
+    if (order != QFG_ORDER_N && order != QFG_ORDER_K) throw InvalidArgument("QuantGemm: bad order of the weight");
+    if (m < 0 || m > INT_MAX / 2 || k < 1 || k > INT_MAX / 2 || n < 1 || n > INT_MAX / 2 || ldx < k || ldw < (order == QFG_ORDER_K ? k : n) || ldo < n)
+      throw InvalidArgument("QuantGemm: bad shape");
+    if (dtype == QFG_INT8 && k > 131071) throw InvalidArgument("QuantGemm: K over 131071 can overflow a sum of INT8 products");
+    if (op->w_scale_len != 0 && op->w_scale_len != static_cast<size_t>(n)) throw InvalidArgument("QuantGemm: w_scale must have one value per column");
+    if (m == 0) return QFG_OK;
+    if (x == nullptr || x_scale == nullptr || w == nullptr || out == nullptr) throw InvalidArgument("QuantGemm: null argument");
+    if (!Aligned(x_scale, 4) || !Aligned(out, ElementBytes(op->out_dtype))) throw InvalidArgument("QuantGemm: misaligned argument");
+    int device = -1;
+    if (cudaGetDevice(&device) != cudaSuccess || device != op->device)  // the scales are on the node's own
+      throw std::runtime_error(std::string("QuantGemm: ") + cudaGetErrorString(cudaErrorInvalidDevice));
+    qfg::QuantCall c;
+    c.x = static_cast<const uint8_t*>(x);
+    c.ldx = m == 1 ? (k + 15) / 16 * 16 : ldx;  // one row is at any distance from the next
+    c.m = m;
+    c.k = k;
+    c.x_scale = x_scale;
+    c.w = static_cast<const uint8_t*>(w);
+    c.ldw = ldw;
+    c.n = n;
+    c.order_k = order == QFG_ORDER_K;
+    c.fp8 = dtype == QFG_FLOAT8E4M3FN;
+    c.w_scale = op->d_w_scale;
+    c.out = out;
+    c.ldo = ldo;
+    c.out_type = op->out_dtype;
+    c.give_up = op->give_up;
+    const qfg::QuantPlan plan = op->plan.bm > 0 ? op->plan : qfg::ChooseQuantPlan(c);
+    if (!qfg::LaunchQuantGemm(c, plan, static_cast<cudaStream_t>(stream))) throw std::runtime_error("QuantGemm: a tensor map could not be made");
+    return QFG_OK;
+  } catch (const InvalidArgument& e) {
+    return Fail(QFG_INVALID_ARGUMENT, e.what());
+  } catch (const std::exception& e) {
+    return Fail(QFG_FAIL, e.what());
+  }
+}
+
+int qfg_quant_gemm_set_option(qfg_quant_gemm* op, const char* key, const char* value) {
+  if (op == nullptr || key == nullptr || value == nullptr) return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: null argument");
+  if (std::strcmp(key, "give_up") == 0) {
+    op->give_up = std::atoi(value) != 0;
+  } else if (std::strcmp(key, "plan") == 0) {
+    qfg::QuantPlan plan;
+    if (*value != 0 && (std::sscanf(value, "%d,%d,%d,%d", &plan.bm, &plan.split, &plan.pair, &plan.per_sm) < 1 || plan.bm < 1))
+      return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: plan is \"rows per tile,split,pair,per SM\"");
+    op->plan = plan;
+  } else {
+    return Fail(QFG_INVALID_ARGUMENT, std::string("QuantGemm: unknown option ") + key);
+  }
+  return QFG_OK;
+}
+
+void qfg_quant_gemm_destroy(qfg_quant_gemm* op) {
+  if (op == nullptr) return;
+  cudaFree(op->d_w_scale);
   delete op;
 }
 

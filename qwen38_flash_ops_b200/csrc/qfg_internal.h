@@ -299,4 +299,53 @@ bool LaunchDenseShared(int mode, const GemmParams& p, int64_t m, const DenseTcPl
 // untile_hc.cu
 cudaError_t LaunchUntileHc(bool fp8, const void* w, void* out, const float* scale, int kind, cudaStream_t stream);
 
+// quant_gemm.cu
+struct QuantCall {
+  const uint8_t* x = nullptr;  // [m][k], rows ldx bytes apart
+  int64_t ldx = 0, m = 0, k = 0;
+  const float* x_scale = nullptr;
+  const uint8_t* w = nullptr;  // [k][n], or [n][k] where order_k; rows ldw bytes apart
+  int64_t ldw = 0, n = 0;
+  int order_k = 0;
+  bool fp8 = false;
+  const float* w_scale = nullptr;  // or null
+  void* out = nullptr;             // [m][n], rows ldo elements apart
+  int64_t ldo = 0;
+  int out_type = QFG_BFLOAT16;
+  int give_up = 0;  // testing
+};
+struct QuantPlan {
+  int bm = 0;      // rows of x per tile: a multiple of 16, at most 256
+  int split = 1;   // CTAs (a cluster) that share the K range of a tile
+  int pair = 0;    // two CTAs per tile of 256 columns
+  int per_sm = 1;  // CTAs whose shared memory fits an SM together, 1 or 2
+};
+cudaError_t ConfigureQuantKernels();  // on the current device
+QuantPlan ChooseQuantPlan(const QuantCall& call);  // throws std::runtime_error
+// false, nothing launched: a tensor map that could not be made.  Throws std::runtime_error (a launch shape that does not exist, a
+// launch that failed).
+bool LaunchQuantGemm(const QuantCall& call, const QuantPlan& plan, cudaStream_t stream);
+
+// row_quant.cu
+struct RowQuantCall {
+  int dtype = 0;  // of x, u or residual, and h
+  const void* x = nullptr;
+  int64_t ldx = 0;  // elements from row to row
+  const void* u = nullptr;  // act: swish(x) * u where given
+  int64_t ldu = 0;
+  // norm: RMS norm of x (+ residual, the sum kept in h) times (weight_offset + weight)
+  bool norm = false;
+  const void* residual = nullptr;
+  int64_t ldr = 0;
+  const void* weight = nullptr;
+  int weight_dtype = 0;
+  float weight_offset = 0.f, eps = 0.f;
+  int64_t rows = 0, n = 0;
+  bool fp8 = false;
+  uint8_t* q = nullptr;
+  float* scale = nullptr;
+  void* h = nullptr;
+};
+cudaError_t LaunchRowQuant(const RowQuantCall& call, cudaStream_t stream);
+
 }  // namespace qfg

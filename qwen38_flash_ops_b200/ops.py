@@ -28,6 +28,8 @@ _DTYPES = {
     torch.uint8: _lib.QFG_UINT8,
     torch.float8_e4m3fn: _lib.QFG_FLOAT8E4M3FN,
 }
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_EIGHT_BITS = {torch.int8: _lib.QFG_INT8, torch.float8_e4m3fn: _lib.QFG_FLOAT8E4M3FN}
 
 
 # The host's part of a call is longer than the smallest kernels, so a call of the ordinary form goes through csrc/calls.cc,
@@ -46,7 +48,8 @@ except ImportError as e:
                   f"`make -C {os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')}` builds it", RuntimeWarning)
     _handed_back = lambda *args: None
     _calls = SimpleNamespace(bind=_handed_back, skinny_gemm=_handed_back, argmax_rows=_handed_back, dequant=_handed_back,
-                             lmhead=_handed_back, shared_expert_down=_handed_back)
+                             lmhead=_handed_back, shared_expert_down=_handed_back, bind_rows=_handed_back, rmsnorm_quant=_handed_back,
+                             row_quant=_handed_back, quant_gemm=_handed_back)
 _bound = False
 
 
@@ -58,6 +61,8 @@ def _load():
         _calls.bind(*[ctypes.cast(getattr(lib, name), c_void_p).value
                       for name in ("qfg_skinny_gemm_compute", "qfg_argmax_rows", "qfg_dequant_compute", "qfg_lmhead_compute",
                                    "qfg_shared_expert_down_compute")])
+        _calls.bind_rows(*[ctypes.cast(getattr(lib, name), c_void_p).value
+                           for name in ("qfg_rmsnorm_quant", "qfg_row_quant", "qfg_quant_gemm_compute")])
         _bound = True
     return lib
 
@@ -319,6 +324,186 @@ class UntileHcBf16:
         if h:
             self._lib.qfg_untile_hc_destroy(h)
             self._h = None
+
+
+def _refuse(message: str):
+    raise QfgError(_lib.QFG_INVALID_ARGUMENT, message)
+
+
+def _rows(op: str, name: str, t: torch.Tensor, dtypes):
+    """(rows, length, elements from row to row) of a tensor whose last dimension is contiguous and whose rows are evenly spaced."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        _refuse(f"{op}: {name} must be a tensor on the current CUDA device")
+    if t.dtype not in dtypes:
+        _refuse(f"{op}: {name} must be {' / '.join(str(d).removeprefix('torch.') for d in dtypes)}, not {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        _refuse(f"{op}: {name} has no elements in a row")
+    n = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // n, n, n
+    try:
+        flat = t.view(-1, n)
+    except RuntimeError:
+        _refuse(f"{op}: the rows of {name} must be evenly spaced")
+    if (n > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < n):
+        _refuse(f"{op}: the rows of {name} must be contiguous and must not overlap")
+    return flat.shape[0], n, max(n, flat.stride(0))
+
+
+def _given(op: str, name: str, t, shape, dtype, contiguous=True):
+    """Checks an output that the caller gave."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != torch.cuda.current_device() or t.dtype != dtype or t.shape != shape:
+        _refuse(f"{op}: {name} must be a {str(dtype).removeprefix('torch.')} tensor of shape {list(shape)} on the current CUDA device")
+    if contiguous and not t.is_contiguous():
+        _refuse(f"{op}: {name} must be contiguous")
+    return t
+
+
+class RmsNormQuant:
+    """Root-mean-square norm with the residual's addition, in eight bits with a scale for each row.
+
+    h = x + residual, rounded to its type (without a residual h is x); y = h * rsqrt(mean(h^2) + eps) * (weight_offset + weight)
+    in FP32; scale = max(max|y|, 2^-100) / 127 (torch.int8) or / 448 (torch.float8_e4m3fn); q = y / scale rounded to nearest.
+    x, residual: [..., n] in BF16, FP16 or FP32; weight: [n], of the same type or FP32.  Returns (q, scale), with a residual (q, scale, h).
+    A row with a value that is not finite, or whose sum of squares is not, has scale NaN and q 0."""
+
+    def __init__(self, eps: float = 1e-6, weight_offset: float = 0.0, dtype: torch.dtype = torch.int8):
+        self._lib = _load()
+        if dtype not in _EIGHT_BITS:
+            _refuse("RmsNormQuant: dtype must be torch.int8 or torch.float8_e4m3fn")
+        if not float(eps) >= 0.0:
+            _refuse("RmsNormQuant: eps must not be negative")
+        self.eps, self.weight_offset, self.dtype = float(eps), float(weight_offset), dtype
+        self._fp8 = dtype == torch.float8_e4m3fn
+
+    def __call__(self, x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, out=None):
+        """`out`: optional (q, scale) or (q, scale, h) to write into; h may be the residual, or x."""
+        if out is None:
+            r = _calls.rmsnorm_quant(self.eps, self.weight_offset, self._fp8, x, weight, residual)
+            if r is not None:
+                return r if r.__class__ is tuple else check(r)
+        op = "RmsNormQuant"
+        rows, n, ldx = _rows(op, "x", x, _FLOATS)
+        _, wn, _ = _rows(op, "weight", weight, (x.dtype, torch.float32))
+        if weight.numel() != n or wn != n or not weight.is_contiguous():
+            _refuse(f"{op}: weight must be a contiguous tensor of {n} elements")
+        ldr = 0
+        if residual is not None:
+            _, _, ldr = _rows(op, "residual", residual, (x.dtype,))
+            if residual.shape != x.shape:
+                _refuse(f"{op}: the residual must have the shape of x")
+        if out is None:
+            q, scale = torch.empty(x.shape, dtype=self.dtype, device=x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+            h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+        else:
+            if len(out) != (2 if residual is None else 3):
+                _refuse(f"{op}: out must be (q, scale), with a residual (q, scale, h)")
+            q, scale = _given(op, "q", out[0], x.shape, self.dtype), _given(op, "scale", out[1], x.shape[:-1], torch.float32)
+            h = _given(op, "h", out[2], x.shape, x.dtype) if residual is not None else None
+        check(self._lib.qfg_rmsnorm_quant(_DTYPES[x.dtype], x.data_ptr(), ldx, residual.data_ptr() if residual is not None else None, ldr,
+                                          weight.data_ptr(), _DTYPES[weight.dtype], self.weight_offset, self.eps, rows, n, _EIGHT_BITS[self.dtype],
+                                          q.data_ptr(), scale.data_ptr(), h.data_ptr() if h is not None else None, _stream_ptr()))
+        return (q, scale) if h is None else (q, scale, h)
+
+
+class RowQuant:
+    """Rows in eight bits with a scale each: of x, or with u of swish(x) * u, x / (1 + exp(-x)) * u in FP32.
+
+    x, u: [..., n] in BF16, FP16 or FP32, whose rows may be further apart than they are long (the halves of a gate and up
+    projection).  Returns (q, scale) as RmsNormQuant does."""
+
+    def __init__(self, dtype: torch.dtype = torch.int8):
+        self._lib = _load()
+        if dtype not in _EIGHT_BITS:
+            _refuse("RowQuant: dtype must be torch.int8 or torch.float8_e4m3fn")
+        self.dtype = dtype
+        self._fp8 = dtype == torch.float8_e4m3fn
+
+    def __call__(self, x: torch.Tensor, u: torch.Tensor | None = None, out=None):
+        if out is None:
+            r = _calls.row_quant(self._fp8, x, u)
+            if r is not None:
+                return r if r.__class__ is tuple else check(r)
+        op = "RowQuant"
+        rows, n, ldx = _rows(op, "x", x, _FLOATS)
+        ldu = 0
+        if u is not None:
+            _, _, ldu = _rows(op, "u", u, (x.dtype,))
+            if u.shape != x.shape:
+                _refuse(f"{op}: u must have the shape of x")
+        if out is None:
+            q, scale = torch.empty(x.shape, dtype=self.dtype, device=x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        else:
+            if len(out) != 2:
+                _refuse(f"{op}: out must be (q, scale)")
+            q, scale = _given(op, "q", out[0], x.shape, self.dtype), _given(op, "scale", out[1], x.shape[:-1], torch.float32)
+        check(self._lib.qfg_row_quant(_DTYPES[x.dtype], x.data_ptr(), ldx, u.data_ptr() if u is not None else None, ldu, rows, n,
+                                      _EIGHT_BITS[self.dtype], q.data_ptr(), scale.data_ptr(), _stream_ptr()))
+        return q, scale
+
+
+class QuantGemm:
+    """out = (x @ w) * x_scale[:, None] * w_scale: eight-bit rows by an eight-bit weight, torch.int8 summed exactly in 32-bit
+    integers (K up to 131071), torch.float8_e4m3fn in FP32; the sum is scaled in FP32 and rounded once to `out_dtype`.
+
+    Attributes: optional `w_scale` (a value per column), `out_dtype` (BF16, FP16 or FP32).  Inputs: x [..., K] and its row scales
+    x_scale [...] (FP32), as RmsNormQuant and RowQuant return them; w [K, N] of the type of x, with either dimension
+    contiguous (a checkpoint's [N, K] weight goes in as its .t())."""
+
+    def __init__(self, w_scale=None, out_dtype: torch.dtype = torch.bfloat16):
+        lib = _load()
+        self._lib = lib
+        self._h = c_void_p()
+        if out_dtype not in _FLOATS:
+            _refuse("QuantGemm: out_dtype must be torch.bfloat16, torch.float16 or torch.float32")
+        if w_scale is not None and len(w_scale) > 0:
+            keep, ptr = _lib.f32_array(w_scale)
+            n = keep.size
+        else:
+            keep, ptr, n = None, None, 0
+        self.out_dtype, self._code = out_dtype, _DTYPES[out_dtype]
+        check(lib.qfg_quant_gemm_create(ptr, n, self._code, ctypes.byref(self._h)))
+        self._p = self._h.value
+
+    def set_option(self, key: str, value) -> None:
+        check(self._lib.qfg_quant_gemm_set_option(self._h, key.encode(), str(value).encode()))
+
+    def __call__(self, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None):
+        """`out`: optional [..., N] of out_dtype to write into; its rows may be further apart than they are long."""
+        if out is None:
+            r = _calls.quant_gemm(self._p, self._code, x, x_scale, w)
+            if r is not None:
+                return r if r.__class__ is not int else check(r)
+        op = "QuantGemm"
+        m, k, ldx = _rows(op, "x", x, tuple(_EIGHT_BITS))
+        _rows(op, "x_scale", x_scale.unsqueeze(-1) if isinstance(x_scale, torch.Tensor) else x_scale, (torch.float32,))
+        if x_scale.numel() != m or not x_scale.is_contiguous():
+            _refuse(f"{op}: x_scale must be a contiguous tensor with one value per row of x")
+        if not isinstance(w, torch.Tensor) or not w.is_cuda or w.get_device() != torch.cuda.current_device() or w.dtype != x.dtype or w.dim() != 2:
+            _refuse(f"{op}: the weight must be a matrix of the type of x on the current CUDA device")
+        if w.shape[0] != k or w.shape[1] < 1:
+            _refuse(f"{op}: the weight must have {k} rows")
+        n = w.shape[1]
+        if w.stride(1) == 1 and w.stride(0) >= n:
+            order, ldw = _lib.QFG_ORDER_N, w.stride(0)
+        elif w.stride(0) == 1 and w.stride(1) >= k:
+            order, ldw = _lib.QFG_ORDER_K, w.stride(1)
+        else:
+            _refuse(f"{op}: one dimension of the weight must be contiguous, and the other's rows must not overlap")
+        shape = x.shape[:-1] + (n,)
+        if out is None:
+            out = torch.empty(shape, dtype=self.out_dtype, device=x.device)
+        _given(op, "out", out, shape, self.out_dtype, contiguous=False)
+        _, _, ldo = _rows(op, "out", out, (self.out_dtype,))
+        check(self._lib.qfg_quant_gemm_compute(self._h, _EIGHT_BITS[x.dtype], x.data_ptr(), ldx, x_scale.data_ptr(), m, k, w.data_ptr(), ldw, order, n,
+                                               out.data_ptr(), ldo, _stream_ptr()))
+        return out
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            self._lib.qfg_quant_gemm_destroy(h)
+            self._h = self._p = None
 
 
 class LmHeadArgmax:

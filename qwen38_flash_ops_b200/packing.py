@@ -71,6 +71,15 @@ def quantize_fp8_per_column(w: np.ndarray):
     return q, s
 
 
+def quantize_int8_per_column(w: np.ndarray):
+    """Per-column INT8: s_col = amax_col / 127 (float32), q = round(w / s_col), ties to even.
+    Returns (q int8 [K, N], s_col float32 [N])."""
+    w = np.asarray(w, dtype=np.float32)
+    amax = np.maximum(np.abs(w).max(axis=0), np.float32(1e-8))
+    s = (amax / np.float32(127.0)).astype(np.float32)
+    return np.clip(np.rint(w / s[None, :]), -127.0, 127.0).astype(np.int8), s
+
+
 def e2m1_encode(x: np.ndarray) -> np.ndarray:
     """Nearest E2M1 code (sign | 3-bit magnitude index), ties to the even code, saturating at 6."""
     x = np.asarray(x, dtype=np.float64)

@@ -41,3 +41,10 @@ def quantize_fp8_per_column_torch(w: torch.Tensor):
     s = (amax / 448.0).float()
     q = (w.float() / s[None, :]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
     return q, s
+
+
+def quantize_int8_per_column_torch(w: torch.Tensor):
+    amax = w.float().abs().amax(dim=0).clamp(min=1e-8)
+    s = (amax / 127.0).float()
+    q = (w.float() / s[None, :]).round().clamp(-127.0, 127.0).to(torch.int8)
+    return q, s
