@@ -43,11 +43,12 @@ constexpr int kTileN = 128;               // columns of w per CTA
 constexpr int kTileK = 128;               // k per stage: one swizzled row of a K-major operand
 constexpr int kWBytes = kTileN * kTileK;  // of a stage
 constexpr int kRing = 12;                 // stages at most
-constexpr int kLoaderWarps = 8;
-constexpr int kBatch = 4;                 // 16-byte pieces a loading thread has in hand
+constexpr int kCopyWarps = 8, kShiftWarps = 8;  // LOADERS
+constexpr int kRawPitch = 144;            // bytes of a row as it is copied: 128 of them lie in nine aligned pieces of sixteen
+constexpr int kRawMost = 4;               // stages of that at most
 constexpr int kPitch = 80;                // bytes of a row of 32 columns in an epilogue warp's buffer: rows 16 bytes apart in the banks
-constexpr int kOutBuffers = 4 * 32 * kPitch;
-constexpr int kScaleBuffers = 4 * 256 * 4;  // each epilogue warp's copy of its rows' scales
+constexpr int kWarpBuffer = 32 * kPitch + 256 * 4;  // that, and the warp's copy of its rows' scales
+constexpr int kEarlyRows = 32;              // SPLIT: tiles of up to so many rows have room beside the stages for the other CTAs' sums
 constexpr int kMostColumns = 512;           // of tensor memory
 constexpr int kMaxSplit = 8;                // CTAs that share K
 
@@ -58,16 +59,17 @@ struct QuantParams {
   const float *x_scale, *w_scale;
   void* out;
   long long ldo;
-  int M, N, K, ksteps, bm, m_tiles, tiles, stages, sets;
+  int M, N, K, ksteps, bm, m_tiles, n_tiles, group, tiles, stages, sets, raw_stages;
   int order_k;           // the weight is stored [n][k]
   int x_loads, w_loads;  // LOADERS: which operands do not come by tensor copies
+  int raw_at;            // where the rows of those are copied to, behind everything else
   int out_type;          // a qfg_dtype
   int out_vec;           // rows of the output lie on 16 bytes
   int give_up;           // testing: no stage comes
 };
 
 struct QuantCtl {
-  unsigned long long full[kRing], empty[kRing], acc_full[2], acc_empty[2];
+  unsigned long long full[kRing], empty[kRing], raw_full[kRawMost], raw_empty[kRawMost], acc_full[2], acc_empty[2], sums;
   uint32_t tmem;
   volatile uint32_t fault;
 };
@@ -95,8 +97,9 @@ template <bool FP8>
 __device__ __forceinline__ float Sum(uint32_t v) {
   return FP8 ? __uint_as_float(v) : __int2float_rn(static_cast<int>(v));
 }
-__device__ __forceinline__ uint32_t Pack(int type, float lo, float hi) {
-  if (type == QFG_BFLOAT16) {
+template <bool BF16>
+__device__ __forceinline__ uint32_t Pack(float lo, float hi) {
+  if constexpr (BF16) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
@@ -104,122 +107,161 @@ __device__ __forceinline__ uint32_t Pack(int type, float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A word into the shared memory of a CTA of the cluster, which counts itself in on a barrier there.
+__device__ __forceinline__ void StoreAsync(uint32_t addr, uint32_t v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void ClusterArrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void ClusterWait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 struct At {
   int n0, m0;
 };
-// the tiles of one block of columns follow one another, so the SMs share its weights in L2
+// Tiles go down `group` row blocks, then on to the next column block, and through all of these before the next group: the tiles of a wave then share
+// about as many rows of x as columns of w in L2.
 template <bool PAIR>
 __device__ __forceinline__ At Locate(const QuantParams& p, int tile, int rank) {
-  const int nt = tile / p.m_tiles;
-  return {nt * (PAIR ? 2 * kTileN : kTileN) + (PAIR ? rank * kTileN : 0), (tile - nt * p.m_tiles) * p.bm};
+  const int g = tile / (p.group * p.n_tiles), rest = tile - g * p.group * p.n_tiles, rows = min(p.group, p.m_tiles - g * p.group), nt = rest / rows;
+  return {nt * (PAIR ? 2 * kTileN : kTileN) + (PAIR ? rank * kTileN : 0), (g * p.group + rest - nt * rows) * p.bm};
 }
 
-// ------------------------------------------------------------------------------ loading warps
-// The words that hold `valid` bytes from `pos` on, of a tensor of `span` bytes that begins anywhere.  A word that the tensor only
-// begins or ends in is put together of the tensor's own bytes.
-__device__ __forceinline__ void LoadWords(const uint8_t* base, long long pos, int valid, long long span, uint32_t (&w)[5]) {
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(base) + static_cast<uintptr_t>(pos)) & 3);
-  const long long first = pos - shift;
-#pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const long long at = first + 4 * i;
-    w[i] = 0;
-    if (valid > 0 && 4 * i < shift + valid) {
-      if (at >= 0 && at + 4 <= span) {
-        w[i] = *reinterpret_cast<const uint32_t*>(base + at);
-      } else {
-        for (int b = 0; b < 4; ++b) {
-          if (at + b >= 0 && at + b < span) w[i] |= static_cast<uint32_t>(base[at + b]) << (8 * b);
+// ------------------------------------------------------------------------------ operands off 16 bytes
+// Rows that tensor copies cannot address come in two steps.  Copying warps fetch the aligned pieces of sixteen bytes that hold a row's 128 into a ring of
+// their own, asynchronously, and shifting warps move the rows from there to where the MMA reads them, a word a lane.  Those have no copies of
+// their own in flight: the proxy fence behind their stores would wait for them.  (One set of warps that loaded words and stored them took 2.8 us a
+// stage of 208 rows.)  No byte outside the tensor is read: the last piece is copied in part, and one that begins before the tensor byte by byte.
+struct Unaligned {  // which rows a stage takes: the weight's, then those of x
+  const uint8_t *x, *w;
+  int w_rows, rows;
+  __device__ __forceinline__ explicit Unaligned(const QuantParams& p)
+      : x(BehindWait(p.x)), w(BehindWait(p.w)), w_rows(p.w_loads ? kTileK : 0), rows(w_rows + (p.x_loads ? p.bm : 0)) {}
+};
+struct StageRows {  // of an operand in one stage
+  const uint8_t *row, *begin, *end;  // the first row's first byte; the tensor
+  long long ld;
+  int rows, valid;  // rows that the tensor has from there on, and bytes of each
+};
+__device__ __forceinline__ StageRows RowsOf(const QuantParams& p, const Unaligned& u, bool of_w, const At& t, int k0) {
+  if (!of_w) return {u.x + t.m0 * p.ldx + k0, u.x, u.x + p.x_span, p.ldx, p.M - t.m0, min(kTileK, p.K - k0)};
+  const int row = p.order_k ? t.n0 : k0, col = p.order_k ? k0 : t.n0;
+  return {u.w + row * p.ldw + col, u.w, u.w + p.w_span, p.ldw, (p.order_k ? p.N : p.K) - row, min(kTileK, (p.order_k ? p.K : p.N) - col)};
+}
+
+__device__ __forceinline__ void CopyRole(const QuantParams& p, QuantCtl& ctl, int warp, int lane, int kbeg, int kcount, int first_tile, int tile_step, uint32_t raw) {
+  const uint32_t full0 = Smem(&ctl.raw_full[0]), empty0 = Smem(&ctl.raw_empty[0]);
+  const Unaligned u(p);
+  const uint32_t slot_bytes = static_cast<uint32_t>(u.rows * kRawPitch);
+  // a warp takes three rows at a time, nine lanes each
+  constexpr int kPieces = kRawPitch / 16, kPass = 3 * kCopyWarps;
+  const int sub = lane / kPieces, piece = lane - sub * kPieces, first = sub < 3 ? warp * 3 + sub : INT_MAX / 2;
+  int slot = 0, round = 0;
+  if (p.give_up) return;
+  auto copy = [&](const StageRows& s, int stored, uint32_t to) {  // `stored`: rows that the stage has
+    const int rows = min(s.rows, stored);
+    const uint8_t* at = s.row + first * s.ld;
+    const long long step = kPass * s.ld;
+    uint32_t dst = to + static_cast<uint32_t>(first * kRawPitch + piece * 16);
+#pragma unroll 4
+    for (int r = first; r < rows; r += kPass, at += step, dst += kPass * kRawPitch) {
+      const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+      const uint8_t* const src = at + (16 * piece - off);
+      if (16 * piece < off + s.valid) {
+        if (src >= s.begin) {
+          const long long left = s.end - src;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(static_cast<int>(left < 16 ? left : 16)) : "memory");
+        } else {
+          for (int e = 0; e < 16; ++e) {
+            if (src + e >= s.begin && src + e < s.end) asm volatile("st.shared.u8 [%0], %1;" ::"r"(dst + e), "r"(static_cast<uint32_t>(src[e])) : "memory");
+          }
+          __threadfence_block();  // the arrival below is that of the copies
         }
+      }
+    }
+  };
+  for (int tile = first_tile; tile < p.tiles; tile += tile_step) {
+    const At t = Locate<false>(p, tile, 0);
+    for (int k = 0; k < kcount; ++k) {
+      if (round > 0 && !BarWait(empty0 + slot * 8, static_cast<uint32_t>((round - 1) & 1), ctl)) return;
+      const uint32_t to = raw + static_cast<uint32_t>(slot) * slot_bytes;
+      if (p.w_loads) copy(RowsOf(p, u, true, t, (kbeg + k) * kTileK), kTileK, to);
+      if (p.x_loads) copy(RowsOf(p, u, false, t, (kbeg + k) * kTileK), p.bm, to + static_cast<uint32_t>(u.w_rows * kRawPitch));
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full0 + slot * 8) : "memory");
+      if (++slot == p.raw_stages) {
+        slot = 0;
+        ++round;
       }
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // nothing lands behind the end of the block
 }
 
-// Fills every stage's share of the operands that tensor copies cannot address.  A piece is 16 bytes of a row of either operand;
-// a thread's next pieces are asked for before those in hand are stored.
-__device__ __forceinline__ void LoaderRole(const QuantParams& p, QuantCtl& ctl, int thread, int kbeg, int kcount, int first_tile, int tile_step, uint32_t smem,
-                                           uint32_t stage_bytes) {
-  const uint32_t full0 = Smem(&ctl.full[0]), empty0 = Smem(&ctl.empty[0]);
-  const uint8_t *const x = BehindWait(p.x), *const w = BehindWait(p.w);
-  const int w_rows = p.w_loads ? kTileK : 0, pieces = (w_rows + (p.x_loads ? p.bm : 0)) * 8;
-  const int batches = (pieces + kLoaderWarps * 32 * kBatch - 1) / (kLoaderWarps * 32 * kBatch);
-  const int mine = ((p.tiles - first_tile + tile_step - 1) / tile_step) * kcount;  // stages in all
-  if (p.give_up) return;
-  uint32_t next[kBatch][5], words[kBatch][5];
-  int next_valid[kBatch], valid[kBatch], next_shift[kBatch], shift[kBatch];
-  auto load = [&](int stage_index, int batch) {
-    const int turn = stage_index / kcount, k0 = (kbeg + stage_index - turn * kcount) * kTileK;
-    const At t = Locate<false>(p, first_tile + turn * tile_step, 0);
+__device__ __forceinline__ void ShiftRole(const QuantParams& p, QuantCtl& ctl, int warp, int lane, int kbeg, int kcount, int first_tile, int tile_step, uint32_t smem,
+                                          uint32_t stage_bytes, uint32_t raw) {
+  const uint32_t rfull0 = Smem(&ctl.raw_full[0]), rempty0 = Smem(&ctl.raw_empty[0]), full0 = Smem(&ctl.full[0]), empty0 = Smem(&ctl.empty[0]);
+  const Unaligned u(p);
+  const uint32_t slot_bytes = static_cast<uint32_t>(u.rows * kRawPitch);
+  int slot = 0, stage = 0, round = 0;
+  uint32_t raw_parity = 0;
+  // warp w takes rows w, w + 8, ..., all of the same place in the swizzle, eight loads ahead of the stores
+  const uint32_t swizzled = static_cast<uint32_t>(warp * 128 + (((lane >> 2) ^ (warp & 7)) * 16) + (lane & 3) * 4);
+  auto shift = [&](const StageRows& s, int stored, uint32_t from, uint32_t to) {
+    constexpr int kAtOnce = 8;
+    const uint32_t low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(s.row)), ld = static_cast<uint32_t>(s.ld);  // only the place in sixteen bytes counts
+    const int left = s.valid - 4 * lane;
+    const uint32_t mask = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * left);
+    for (int r0 = warp; r0 < stored; r0 += kAtOnce * kShiftWarps) {
+      uint32_t lo[kAtOnce], hi[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int piece = (batch * kBatch + j) * (kLoaderWarps * 32) + thread, r = piece >> 3, c = (piece & 7) * 16;
-      const bool of_w = r < w_rows;
-      // rows and bytes of a row, of the operand as it is stored
-      const int row = of_w ? (p.order_k ? t.n0 : k0) + r : t.m0 + r - w_rows, rows = of_w ? (p.order_k ? p.N : p.K) : p.M;
-      const int col = (of_w && !p.order_k ? t.n0 : k0) + c, cols = of_w && !p.order_k ? p.N : p.K;
-      const uint8_t* const base = of_w ? w : x;
-      const long long pos = static_cast<long long>(row) * (of_w ? p.ldw : p.ldx) + col;
-      next_valid[j] = piece < pieces && row < rows ? min(16, cols - col) : 0;
-      next_shift[j] = static_cast<int>((reinterpret_cast<uintptr_t>(base) + static_cast<uintptr_t>(pos)) & 3) * 8;
-      LoadWords(base, pos, next_valid[j], of_w ? p.w_span : p.x_span, next[j]);
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int r = r0 + j * kShiftWarps;
+        const uint32_t off = (low + static_cast<uint32_t>(r) * ld) & 15, at = from + static_cast<uint32_t>(r * kRawPitch + 4 * lane) + (off & ~3u);
+        lo[j] = hi[j] = 0;
+        if (r < stored) {
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(lo[j]) : "r"(at));
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(hi[j]) : "r"(at + 4));  // within the row's pieces, unless off is 0 and it is not needed
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int r = r0 + j * kShiftWarps;
+        const uint32_t off = (low + static_cast<uint32_t>(r) * ld) & 15, v = r < s.rows ? __funnelshift_r(lo[j], hi[j], (off & 3) * 8) & mask : 0u;
+        if (r < stored) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + static_cast<uint32_t>((r - warp) * 128)), "r"(v) : "memory");
+      }
     }
   };
-  load(0, 0);
-  int stage = 0;
-  uint32_t parity = 1;
-#pragma unroll 1
-  for (int s = 0; s < mine; ++s) {
-#pragma unroll 1
-    for (int b = 0; b < batches; ++b) {
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        valid[j] = next_valid[j];
-        shift[j] = next_shift[j];
-#pragma unroll
-        for (int i = 0; i < 5; ++i) words[j][i] = next[j][i];
+  for (int tile = first_tile; tile < p.tiles; tile += tile_step) {
+    const At t = Locate<false>(p, tile, 0);
+    for (int k = 0; k < kcount; ++k) {
+      if (round > 0 && !BarWait(empty0 + stage * 8, static_cast<uint32_t>((round - 1) & 1), ctl)) return;
+      if (!BarWait(rfull0 + slot * 8, raw_parity, ctl)) return;
+      const uint32_t from = raw + static_cast<uint32_t>(slot) * slot_bytes, to = smem + static_cast<uint32_t>(stage) * stage_bytes + swizzled;
+      if (p.w_loads) shift(RowsOf(p, u, true, t, (kbeg + k) * kTileK), kTileK, from, to);
+      if (p.x_loads) shift(RowsOf(p, u, false, t, (kbeg + k) * kTileK), p.bm, from + static_cast<uint32_t>(u.w_rows * kRawPitch), to + kWBytes);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        BarArrive(full0 + stage * 8);
+        BarArrive(rempty0 + slot * 8);
       }
-      if (b + 1 < batches) {
-        load(s, b + 1);
-      } else if (s + 1 < mine) {
-        load(s + 1, 0);
+      if (++stage == p.stages) {
+        stage = 0;
+        ++round;
       }
-      if (b == 0 && s >= p.stages && !BarWait(empty0 + stage * 8, parity, ctl)) return;
-      const uint32_t dst = smem + static_cast<uint32_t>(stage) * stage_bytes;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int piece = (b * kBatch + j) * (kLoaderWarps * 32) + thread, r = piece >> 3, c = piece & 7;
-        if (piece >= pieces) continue;
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = __funnelshift_r(words[j][i], words[j][i + 1], shift[j]);
-          const int left = valid[j] - 4 * i;
-          if (left < 4) v[i] = left <= 0 ? 0u : v[i] & (0xFFFFFFFFu >> (32 - 8 * left));
-        }
-        const int row = r < w_rows ? r : r - w_rows;
-        Sts128(dst + (r < w_rows ? 0u : static_cast<uint32_t>(kWBytes)) + static_cast<uint32_t>(row * 128 + ((c ^ (row & 7)) * 16)), v);
+      if (++slot == p.raw_stages) {
+        slot = 0;
+        raw_parity ^= 1u;
       }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if ((thread & 31) == 0) BarArrive(full0 + stage * 8);
-    if (++stage == p.stages) {
-      stage = 0;
-      parity ^= 1u;
     }
   }
 }
 
 // ------------------------------------------------------------------------------ the kernel
-template <bool LOADERS>
-constexpr int QuantThreads() {
-  return 32 * (6 + (LOADERS ? kLoaderWarps : 0));
-}
+template <bool PAIR, bool LOADERS>
+constexpr int kThreads = 32 * (6 + (PAIR ? 4 : 0) + (LOADERS ? kCopyWarps + kShiftWarps : 0));
 
 // SPLIT: one tile per cluster.  PAIR and the others never together.
 template <bool FP8, bool PAIR, bool SPLIT, bool LOADERS>
-__global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(const __grid_constant__ QuantParams p) {
+__global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(const __grid_constant__ QuantParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ QuantCtl ctl;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -233,27 +275,65 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
   const int xrows = PAIR ? p.bm / 2 : p.bm;
   const uint32_t stage_bytes = static_cast<uint32_t>(kWBytes + xrows * kTileK);
   const uint32_t full0 = Smem(&ctl.full[0]), empty0 = Smem(&ctl.empty[0]), accf0 = Smem(&ctl.acc_full[0]), acce0 = Smem(&ctl.acc_empty[0]);
-  const bool copies = !LOADERS || !p.x_loads || !p.w_loads;
+  const bool load_w = !LOADERS || !p.w_loads, load_x = !LOADERS || !p.x_loads;
+  constexpr int kEpilogueWarps = PAIR ? 8 : 4;
   int acc_cols = 32;
   while (acc_cols < p.sets * p.bm) acc_cols *= 2;
+  // SPLIT: the rows of the tile that this rank finishes, and where their sums come together, [rank][row][column]
+  const int tile_rows = SPLIT ? min(p.bm, p.M - Locate<false>(p, first_tile, 0).m0) : 0, share = (p.bm + csize - 1) / csize;
+  const int my_rows = max(0, min(share, tile_rows - rank * share));
+  const bool early = p.bm <= kEarlyRows;  // beside the stages: peers may send theirs while this CTA still multiplies
+  const uint32_t recv = smem + (early ? static_cast<uint32_t>(p.stages) * stage_bytes : 0u);
 
-  if (tid == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      BarInit(full0 + i * 8, (copies ? 1 : 0) + (LOADERS ? kLoaderWarps : 0));
-      BarInit(empty0 + i * 8, 1);
+  // The copying warp makes the barriers itself, so that its first copies are on their way while the other warps set up.
+  int c_tile = first_tile, c_k = 0, c_stage = 0, c_round = 0;
+  At c_at = Locate<PAIR>(p, first_tile, rank);
+  const uint32_t mine = static_cast<uint32_t>((load_w ? kWBytes : 0) + (load_x ? xrows * kTileK : 0));
+  auto copy_stage = [&]() {
+    const At t = c_at;
+    const uint32_t bar = PAIR ? MapRank(full0 + c_stage * 8, 0) : full0 + c_stage * 8;
+    const uint32_t dst = smem + static_cast<uint32_t>(c_stage) * stage_bytes;
+    const int k0 = (kbeg + c_k) * kTileK;
+    if (ElectOne()) {
+      if (rank == 0 || !PAIR) BarExpect(full0 + c_stage * 8, PAIR ? 2 * mine : mine);
+      if (load_w) TmaLoad<PAIR>(dst, &p.wmap, p.order_k ? k0 : t.n0, p.order_k ? t.n0 : k0, bar);
+      if (load_x) TmaLoad<PAIR>(dst + kWBytes, &p.xmap, k0, t.m0 + (PAIR ? rank * xrows : 0), bar);
     }
-    for (int i = 0; i < 2; ++i) {
-      BarInit(accf0 + i * 8, 1);
-      BarInit(acce0 + i * 8, 4 * (PAIR ? 2 : 1));
+    __syncwarp();
+    if (++c_stage == p.stages) {
+      c_stage = 0;
+      ++c_round;
     }
-    ctl.fault = static_cast<uint32_t>(p.give_up);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 4 && lane == 0) {
-    if (!LOADERS || !p.x_loads) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.xmap) : "memory");
-    if (!LOADERS || !p.w_loads) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.wmap) : "memory");
-  }
-  if (warp == 5) {
+    if (++c_k == kcount) {
+      c_k = 0;
+      c_tile += tile_step;
+      c_at = Locate<PAIR>(p, c_tile, rank);
+    }
+  };
+  const bool copies = p.give_up == 0 && (load_w || load_x);
+  if (warp == 4) {
+    if (lane == 0) {
+      if (load_x) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.xmap) : "memory");
+      if (load_w) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.wmap) : "memory");
+      for (int i = 0; i < p.stages; ++i) {
+        BarInit(full0 + i * 8, (load_w || load_x ? 1 : 0) + (LOADERS ? kShiftWarps : 0));
+        BarInit(empty0 + i * 8, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        BarInit(accf0 + i * 8, 1);
+        BarInit(acce0 + i * 8, kEpilogueWarps * (PAIR ? 2 : 1));
+      }
+      for (int i = 0; LOADERS && i < p.raw_stages; ++i) {
+        BarInit(Smem(&ctl.raw_full[i]), kCopyWarps * 32);
+        BarInit(Smem(&ctl.raw_empty[i]), kShiftWarps);
+      }
+      BarInit(Smem(&ctl.sums), 1);
+      ctl.fault = static_cast<uint32_t>(p.give_up);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      if (SPLIT && early && my_rows > 0) BarExpect(Smem(&ctl.sums), static_cast<uint32_t>(csize * my_rows * kTileN * 4));
+    }
+    __syncwarp();
+  } else if (warp == 5) {
     if constexpr (PAIR) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Smem(&ctl.tmem)), "r"(acc_cols) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -263,38 +343,56 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
     }
   }
   FenceBefore();
-  GridDependencyWait();
-  __syncthreads();
+  if (PAIR || warp != 4) {
+    GridDependencyWait();
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory");
+  } else {  // this warp waits for nothing that the others set up, only they for its barriers
+    asm volatile("bar.arrive 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory");
+    GridDependencyWait();
+  }
   if constexpr (PAIR) cg::this_cluster().sync();  // the leader's barriers exist before the peer arrives on them
+  if constexpr (SPLIT) ClusterArrive();           // as do those that the peers' sums will count themselves in on
   FenceAfter();
-  const uint32_t tmem = ctl.tmem;
+  const uint32_t tmem = PAIR || warp != 4 ? ctl.tmem : 0;
 
-  if (warp < 4) {
-    // ---- epilogue
+  if (warp < 4 || (PAIR && warp >= 6)) {
+    // ---- epilogue; a warp reaches the 32 columns of w that its number says.  Of a pair's eight, two share them and take the rows by 32 in turn.
     const float* const x_scale = BehindWait(p.x_scale);
-    uint8_t* const bufs = smem_ptr + static_cast<size_t>(p.stages) * stage_bytes;
-    const uint32_t buf = Smem(bufs) + static_cast<uint32_t>(warp * 32 * kPitch);
-    float* const xs = reinterpret_cast<float*>(bufs + kOutBuffers) + warp * 256;
+    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;
+    uint8_t* const bufs = smem_ptr + static_cast<size_t>(p.stages) * stage_bytes + (quarter + 4 * half) * kWarpBuffer;
+    const uint32_t buf = Smem(bufs);
+    float* const xs = reinterpret_cast<float*>(bufs + 32 * kPitch);
     int it = 0;
     bool good = true;  // false from the first wait that ran out: the tiles that are left become NaN
     for (int tile = first_tile; tile < p.tiles; tile += tile_step, ++it) {
       const int b = p.sets == 2 ? it & 1 : 0, turn = p.sets == 2 ? it >> 1 : it;
       const At t = Locate<PAIR>(p, tile, rank);
-      const int n = t.n0 + 32 * warp;  // the warp's first column
+      const int n = t.n0 + 32 * quarter;  // the warp's first column
       if constexpr (!SPLIT) {
         for (int i = lane; i < p.bm; i += 32) xs[i] = t.m0 + i < p.M ? x_scale[t.m0 + i] : 0.f;
         __syncwarp();
       }
+      // asked for ahead of the wait: a trip to memory
+      float ws[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+      if (!SPLIT && p.w_scale != nullptr) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int col = p.out_type == QFG_FLOAT ? n + lane : n + 8 * h + (lane >> 2);
+          if (col < p.N) ws[h >> 1][h & 1] = p.w_scale[col];
+        }
+      }
       good = good && BarWait(accf0 + b * 8, static_cast<uint32_t>(turn & 1), ctl);
       __syncwarp();
       FenceAfter();
-      const uint32_t src = tmem + (static_cast<uint32_t>(32 * warp) << 16) + static_cast<uint32_t>(b * p.bm);
+      const uint32_t src = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(b * p.bm);
       if (SPLIT || p.out_type == QFG_FLOAT) {
         // a lane is a column, a register a row
-        const float ws = !SPLIT && p.w_scale != nullptr && n + lane < p.N ? p.w_scale[n + lane] : 1.f;
-        // where the stages were: after a wait that ran out, copies may still be landing there
-        for (int i = 0; SPLIT && i < 16 && !good; ++i) __nanosleep(1000000);
-        for (int c = 0; c < p.bm; c += 16) {
+        if constexpr (SPLIT) {
+          ClusterWait();
+          // where the stages were: after a wait that ran out, copies may still be landing there
+          for (int i = 0; i < 16 && !good && !early; ++i) __nanosleep(1000000);
+        }
+        for (int c = 16 * half; c < (SPLIT ? tile_rows : p.bm); c += PAIR ? 32 : 16) {
           uint32_t v[16];
           asm volatile(
               "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -303,31 +401,42 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
               : "r"(src + static_cast<uint32_t>(c)));
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           if constexpr (SPLIT) {
-            uint32_t* const part = reinterpret_cast<uint32_t*>(smem_ptr) + c * kTileN + 32 * warp + lane;
+            if (early) {
+              int owner = c / share, row = c - owner * share;
+              const uint32_t slot = recv + static_cast<uint32_t>((rank * share * kTileN + 32 * quarter + lane) * 4);
+              uint32_t to = MapRank(slot, owner), bar = MapRank(Smem(&ctl.sums), owner);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) part[i * kTileN] = v[i];
+              for (int i = 0; i < 16; ++i) {
+                if (good && c + i < tile_rows) StoreAsync(to + static_cast<uint32_t>(row * (kTileN * 4)), v[i], bar);
+                if (++row == share && c + i + 1 < tile_rows) {
+                  row = 0;
+                  ++owner;
+                  to = MapRank(slot, owner);
+                  bar = MapRank(Smem(&ctl.sums), owner);
+                }
+              }
+            } else {
+              uint32_t* const part = reinterpret_cast<uint32_t*>(smem_ptr) + c * kTileN + 32 * quarter + lane;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) part[i * kTileN] = v[i];
+            }
           } else if (n + lane < p.N) {
             float* const out = static_cast<float*>(p.out) + static_cast<long long>(t.m0 + c) * p.ldo + n + lane;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              if (t.m0 + c + i < p.M) out[i * p.ldo] = good ? Sum<FP8>(v[i]) * xs[c + i] * ws : __uint_as_float(0x7FFFFFFFu);
+              if (t.m0 + c + i < p.M) out[i * p.ldo] = good ? Sum<FP8>(v[i]) * xs[c + i] * ws[0][0] : __uint_as_float(0x7FFFFFFFu);
             }
           }
         }
       } else {
         // 8 x 8 fragments, columns of w down and rows of x across, transposed through shared memory for stores of 16 bytes
-        const int g = lane >> 2, t2 = (lane & 3) * 2, row = lane >> 2, chunk = lane & 3;
-        float ws[2][2];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int col = n + 8 * h + g;
-          ws[h >> 1][h & 1] = p.w_scale != nullptr && col < p.N ? p.w_scale[col] : 1.f;
-        }
+        const int t2 = (lane & 3) * 2, row = lane >> 2, chunk = lane & 3;
         const int rows = min(p.bm, p.M - t.m0), cols = p.N - n;
         uint16_t* const out = static_cast<uint16_t*>(p.out) + static_cast<long long>(t.m0) * p.ldo + n;
         const uint32_t st = buf + static_cast<uint32_t>((((lane >> 4) & 1) * 8 + (lane & 7)) * kPitch + ((lane >> 3) & 1) * 16);
         const uint32_t ld = buf + static_cast<uint32_t>(row * kPitch + chunk * 16);
-        for (int c = 0; c < p.bm; c += 32) {
+        auto finish = [&](auto type) {
+        for (int c = 32 * half; c < p.bm; c += PAIR ? 64 : 32) {
           uint32_t v[2][2][8];  // [lower, upper 16 columns][16 rows][fragments]
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -354,7 +463,7 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
                 for (int i = 0; i < 4; ++i) {
                   const float2 s = i < 2 ? s0 : s1;
                   const float lo = Sum<FP8>(v[h][k][2 * i]) * s.x * ws[h][i & 1], hi = Sum<FP8>(v[h][k][2 * i + 1]) * s.y * ws[h][i & 1];
-                  w[i] = good ? Pack(p.out_type, lo, hi) : 0x7FFF7FFFu;
+                  w[i] = good ? Pack<decltype(type)::value>(lo, hi) : 0x7FFF7FFFu;
                 }
                 asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(st + k * (16 * kPitch) + h * 32), "r"(w[0]),
                              "r"(w[1]), "r"(w[2]), "r"(w[3])
@@ -374,12 +483,18 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
               }
             }
           } else {
-            const uint16_t* const from = reinterpret_cast<const uint16_t*>(bufs + warp * 32 * kPitch) + lane;
+            const uint16_t* const from = reinterpret_cast<const uint16_t*>(bufs) + lane;
             const int last = min(32, rows - c);
             for (int r = 0; r < last; ++r) {
               if (lane < cols) out[static_cast<long long>(c + r) * p.ldo + lane] = from[r * (kPitch / 2)];
             }
           }
+        }
+        };
+        if (p.out_type == QFG_BFLOAT16) {
+          finish(std::true_type());
+        } else {
+          finish(std::false_type());
         }
       }
       FenceBefore();
@@ -388,32 +503,7 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
     }
   } else if (warp == 4) {
     // ---- tensor copies
-    int stage = 0, round = 0;
-    bool good = p.give_up == 0 && copies;
-    const bool load_w = !LOADERS || !p.w_loads, load_x = !LOADERS || !p.x_loads;
-    const uint32_t mine = static_cast<uint32_t>((load_w ? kWBytes : 0) + (load_x ? xrows * kTileK : 0));
-    for (int tile = first_tile; tile < p.tiles && good; tile += tile_step) {
-      const At t = Locate<PAIR>(p, tile, rank);
-      for (int k = 0; k < kcount; ++k) {
-        if (round > 0 && !BarWait(empty0 + stage * 8, static_cast<uint32_t>((round - 1) & 1), ctl)) {
-          good = false;
-          break;
-        }
-        const uint32_t bar = PAIR ? MapRank(full0 + stage * 8, 0) : full0 + stage * 8;
-        const uint32_t dst = smem + static_cast<uint32_t>(stage) * stage_bytes;
-        const int k0 = (kbeg + k) * kTileK;
-        if (ElectOne()) {
-          if (rank == 0 || !PAIR) BarExpect(full0 + stage * 8, PAIR ? 2 * mine : mine);
-          if (load_w) TmaLoad<PAIR>(dst, &p.wmap, p.order_k ? k0 : t.n0, p.order_k ? t.n0 : k0, bar);
-          if (load_x) TmaLoad<PAIR>(dst + kWBytes, &p.xmap, k0, t.m0 + (PAIR ? rank * xrows : 0), bar);
-        }
-        __syncwarp();
-        if (++stage == p.stages) {
-          stage = 0;
-          ++round;
-        }
-      }
-    }
+    while (copies && c_tile < p.tiles && (c_round == 0 || BarWait(empty0 + c_stage * 8, static_cast<uint32_t>((c_round - 1) & 1), ctl))) copy_stage();
   } else if (warp == 5) {
     // ---- MMAs (the leader's, for both CTAs of a pair)
     if (!PAIR || rank == 0) {
@@ -453,47 +543,61 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
       }
     }
   } else if constexpr (LOADERS) {
-    LoaderRole(p, ctl, tid - 6 * 32, kbeg, kcount, first_tile, tile_step, smem, stage_bytes);
+    const uint32_t raw = smem + static_cast<uint32_t>(p.raw_at);
+    if (warp < 6 + kCopyWarps) {
+      CopyRole(p, ctl, warp - 6, lane, kbeg, kcount, first_tile, tile_step, raw);
+    } else {
+      ShiftRole(p, ctl, warp - 6 - kCopyWarps, lane, kbeg, kcount, first_tile, tile_step, smem, stage_bytes, raw);
+    }
   }
 
   if constexpr (SPLIT) {
-    // the ranks' sums meet: rank r finishes rows [r bm / C, (r + 1) bm / C) of the tile, adding in rank order
+    // rank r finishes rows [r share, (r + 1) share) of the tile, adding in rank order.  Early tiles: every rank has sent the sums of those rows here,
+    // which saves one of the two times that the ranks would have to meet; larger ones are read from where they are.
     cg::cluster_group cluster = cg::this_cluster();
-    FenceBefore();
-    cluster.sync();
     const At t = Locate<false>(p, first_tile, 0);
-    const uint32_t* const part = reinterpret_cast<const uint32_t*>(smem_ptr);
     const float* const x_scale = BehindWait(p.x_scale);
-    const int r0 = rank * p.bm / csize, r1 = (rank + 1) * p.bm / csize;
-    const int c = lane * 4, n = t.n0 + c, cols = p.N - n;
-    const int rows = min(r1, p.M - t.m0), warps = static_cast<int>(blockDim.x) / 32;
-    float ws[4];
+    const int c = lane * 4, n = t.n0 + c, cols = p.N - n, m_first = t.m0 + rank * share;
+    const int warps = static_cast<int>(blockDim.x) / 32;
+    // asked for ahead of the waits: trips to memory
+    float ws[4], x_first = warp < my_rows ? x_scale[m_first + warp] : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) ws[e] = p.w_scale != nullptr && e < cols ? p.w_scale[n + e] : 1.f;
-    uint32_t bad = 0;  // a rank gave up
+    if (warp >= 4) ClusterWait();
+    ClusterArrive();
+    if (!early) ClusterWait();
+    bool bad = false;
+    if (early) {
+      bad = my_rows > 0 && !BarWaitCluster(Smem(&ctl.sums), 0, ctl);
+    } else {
 #pragma unroll
-    for (int r = 0; r < kMaxSplit; ++r) {
-      if (r < csize) bad |= *cluster.map_shared_rank(const_cast<const uint32_t*>(&ctl.fault), r);
+      for (int r = 0; r < kMaxSplit; ++r) {
+        if (r < csize) bad |= *cluster.map_shared_rank(const_cast<const uint32_t*>(&ctl.fault), r) != 0;
+      }
     }
+    const uint8_t* const here = smem_ptr + (recv - smem) + c * 4;
     // ROWS rows a warp at a time, so that the loads of all of them and of all ranks are on their way together
     auto add_up = [&](auto rows_tag, auto ranks_tag) {
       constexpr int ROWS = decltype(rows_tag)::value, RANKS = decltype(ranks_tag)::value;
-      for (int m0 = r0 + warp; m0 < rows; m0 += warps * ROWS) {
+      for (int m0 = warp; m0 < my_rows; m0 += warps * ROWS) {
         uint4 v[ROWS][RANKS];
         float xs[ROWS];
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
           const int m = m0 + i * warps;
-          xs[i] = m < rows ? x_scale[t.m0 + m] : 0.f;
+          xs[i] = m == warp ? x_first : m < my_rows ? x_scale[m_first + m] : 0.f;
 #pragma unroll
           for (int r = 0; r < RANKS; ++r) {
-            if (r < csize && m < rows) v[i][r] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(part, r) + m * kTileN + c);
+            if (r < csize && m < my_rows) {
+              v[i][r] = early ? *reinterpret_cast<const uint4*>(here + (r * share + m) * (kTileN * 4))
+                              : *reinterpret_cast<const uint4*>(cluster.map_shared_rank(reinterpret_cast<const uint32_t*>(smem_ptr), r) + (rank * share + m) * kTileN + c);
+            }
           }
         }
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
           const int m = m0 + i * warps;
-          if (m >= rows) break;
+          if (m >= my_rows) break;
           uint32_t s[4] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w};
 #pragma unroll
           for (int r = 1; r < RANKS; ++r) {
@@ -506,7 +610,7 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
           float y[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[e] = bad ? __uint_as_float(0x7FFFFFFFu) : Sum<FP8>(s[e]) * xs[i] * ws[e];
-          const long long at = static_cast<long long>(t.m0 + m) * p.ldo + n;
+          const long long at = static_cast<long long>(m_first + m) * p.ldo + n;
           if (p.out_type == QFG_FLOAT) {
             float* const dst = static_cast<float*>(p.out) + at;
             if (p.out_vec && cols >= 4) {
@@ -519,7 +623,8 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
             }
           } else {
             uint16_t* const dst = static_cast<uint16_t*>(p.out) + at;
-            const uint2 o = make_uint2(Pack(p.out_type, y[0], y[1]), Pack(p.out_type, y[2], y[3]));
+            const uint2 o = p.out_type == QFG_BFLOAT16 ? make_uint2(Pack<true>(y[0], y[1]), Pack<true>(y[2], y[3]))
+                                                       : make_uint2(Pack<false>(y[0], y[1]), Pack<false>(y[2], y[3]));
             if (p.out_vec && cols >= 4) {
               *reinterpret_cast<uint2*>(dst) = o;
             } else {
@@ -535,15 +640,17 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
     if (csize <= 2) {
       add_up(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
     } else if (csize <= 4) {
-      add_up(std::integral_constant<int, 3>(), std::integral_constant<int, 4>());
+      add_up(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
     } else {
-      add_up(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
+      add_up(std::integral_constant<int, 2>(), std::integral_constant<int, kMaxSplit>());
     }
   }
+  if (SPLIT && !early) ClusterArrive();  // nothing more is read from the others
   if (ctl.fault) __nanosleep(100000);  // copies of a CTA that gave up may still be landing
   FenceBefore();
   __syncthreads();
-  if constexpr (PAIR || SPLIT) cg::this_cluster().sync();  // no CTA leaves while a peer still reads its shared memory
+  if constexpr (PAIR) cg::this_cluster().sync();  // no CTA leaves while its peer's MMAs still read its shared memory
+  if constexpr (SPLIT) ClusterWait();
   if (warp == 5) {
     if constexpr (PAIR) {
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(acc_cols) : "memory");
@@ -553,10 +660,16 @@ __global__ void __launch_bounds__(QuantThreads<LOADERS>(), 1) QuantGemmKernel(co
   }
 }
 
+#ifndef QGROUP
+#define QGROUP 8
+#endif
 // ------------------------------------------------------------------------------ host
 constexpr int kSmemPerSm = 233472;                                      // of an SM; a CTA takes 1 KB of it beside its own
 constexpr int kStatic = (static_cast<int>(sizeof(QuantCtl)) + 127) / 128 * 128;
-constexpr int kFixed = 1024 + kOutBuffers + kScaleBuffers;              // beside the stages
+// bytes beside the stages
+int Fixed(const QuantPlan& plan) {
+  return 1024 + (plan.pair ? 8 : 4) * kWarpBuffer + (plan.split > 1 && plan.bm <= kEarlyRows ? std::max(0, (kEarlyRows + kMaxSplit) * kTileN * 4 - 4 * kWarpBuffer) : 0);
+}
 
 int SmemLimit(int per_sm) { return kSmemPerSm / per_sm - 1024 - kStatic; }
 
@@ -572,7 +685,7 @@ template <bool FP8, bool PAIR, bool SPLIT, bool LOADERS>
 cudaError_t LaunchAs(const QuantParams& p, int ctas, int cluster, size_t smem, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(static_cast<unsigned>(QuantThreads<LOADERS>()));
+  cfg.blockDim = dim3(static_cast<unsigned>(kThreads<PAIR, LOADERS>));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -614,7 +727,7 @@ cudaError_t RaiseLimits() {
 int ResidentClusters(int per_sm, int cluster, int sms) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(cluster));
-  cfg.blockDim = dim3(static_cast<unsigned>(QuantThreads<false>()));
+  cfg.blockDim = dim3(static_cast<unsigned>(kThreads<false, false>));
   cfg.dynamicSmemBytes = static_cast<size_t>(SmemLimit(per_sm));
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -687,7 +800,8 @@ QuantPlan ChooseQuantPlan(const QuantCall& c) {
   return best;
 }
 
-bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& plan, cudaStream_t stream) {
+bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t stream) {
+  QuantPlan plan = asked;
   const QuantSetup* setup = nullptr;
   cudaError_t err = SetUpQuant(&setup);
   if (err != cudaSuccess) throw std::runtime_error(std::string("QuantGemm: ") + cudaGetErrorString(err));
@@ -695,6 +809,7 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& plan, cudaStream_t str
   if (plan.bm < 16 || plan.bm > 256 || plan.bm % 16 != 0 || plan.split < 1 || plan.split > kMaxSplit || plan.per_sm < 1 || plan.per_sm > 2 ||
       (plan.pair && (plan.split != 1 || plan.bm % 32 != 0 || plan.per_sm != 1 || loads)))
     throw std::runtime_error("QuantGemm: bad launch shape");
+  if (loads) plan.per_sm = 1;  // the registers of its warps, and the second ring
   QuantParams p = {};
   p.x = c.x;
   p.w = c.w;
@@ -723,18 +838,24 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& plan, cudaStream_t str
   const int64_t tiles = (c.n + width - 1) / width * p.m_tiles;
   if (tiles > INT_MAX / 16) throw std::runtime_error("QuantGemm: too many tiles");
   p.tiles = static_cast<int>(tiles);
+  p.n_tiles = p.tiles / p.m_tiles;
+  p.group = std::min(p.m_tiles, QGROUP);
   const int cluster = plan.pair ? 2 : std::min(plan.split, p.ksteps);
   const int xrows = plan.pair ? p.bm / 2 : p.bm, stage = kWBytes + xrows * kTileK;
   if (!x_loads && !EncodeRows(&p.xmap, c.x, c.m, c.k, c.ldx, xrows)) return false;
   if (!w_loads && !EncodeRows(&p.wmap, c.w, w_rows, w_cols, c.ldw, 128)) return false;
-  p.stages = std::min(kRing, (SmemLimit(plan.per_sm) - kFixed) / stage);
+  // half of the room, or less, for the rows as they are copied: they wait for memory, those behind them only for the MMA
+  const int room = SmemLimit(plan.per_sm) - Fixed(plan), raw_stage = ((w_loads ? kTileK : 0) + (x_loads ? p.bm : 0)) * kRawPitch;
+  p.raw_stages = loads ? std::max(1, std::min(kRawMost, room * 5 / 9 / raw_stage)) : 0;
+  p.stages = std::min(kRing, (room - p.raw_stages * raw_stage) / stage);
   const bool split = cluster > 1 && !plan.pair;
   const int resident = plan.pair ? setup->sms / 2 : plan.per_sm * setup->sms;
   const int walkers = split ? p.tiles : std::min(p.tiles, resident);  // clusters that walk over the tiles
   p.sets = walkers < p.tiles ? 2 : 1;
   if (p.sets * p.bm * plan.per_sm > kMostColumns) p.sets = 1;
-  size_t smem = static_cast<size_t>(kFixed) + static_cast<size_t>(p.stages) * stage;
-  if (split) smem = std::max(smem, static_cast<size_t>(1024 + p.bm * kTileN * 4));
+  p.raw_at = (Fixed(plan) - 1024 + p.stages * stage + 15) / 16 * 16;
+  size_t smem = static_cast<size_t>(1024 + p.raw_at + p.raw_stages * raw_stage);
+  if (split) smem = std::max(smem, static_cast<size_t>(1024 + (p.bm + kMaxSplit) * kTileN * 4));
   if (p.stages < 2 || smem > static_cast<size_t>(SmemLimit(1))) throw std::runtime_error("QuantGemm: bad launch shape");
   const int ctas = walkers * cluster;
   if (plan.pair) {

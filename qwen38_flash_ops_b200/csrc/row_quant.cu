@@ -15,10 +15,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "qfg_internal.h"
 #include "stream_order.cuh"
+#include "tc_ptx.cuh"
 
 namespace qfg {
 namespace {
@@ -33,6 +36,7 @@ struct RowParams {
   float* scale;
   long long ldx, ld2, rows;
   int n, warps, rows_per_block;  // warps of a row
+  int stages, stage_bytes, per_stage;  // of the ring; pieces of every thread in a stage
   bool fp8, weight_f32;
   float offset, eps, inv_n;
 };
@@ -76,108 +80,210 @@ __device__ __forceinline__ void Store(T* p, const Piece<T, C>& v) {
   }
 }
 
-// Four products f[i] * inv in eight bits.  INT8: adding 1.5 * 2^23 leaves the integer nearest to a product of at most 2^22 in the low
-// bits, rounded once; |f| <= largest and inv = top / largest to within two ulp keep it within [-127, 127].
-__device__ __forceinline__ uint32_t Quantise4(const float (&f)[4], float inv, bool fp8) {
-  if (fp8) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0] * inv, f[1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2] * inv, f[3] * inv), __NV_SATFINITE, __NV_E4M3);
-    return lo | hi << 16;
-  }
-  uint32_t v[4];
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 Add2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 Both(float v) { return make_float2(v, v); }
+
+// x + residual in their type.  In 16 bits the packed addition rounds once, as an FP32 addition rounded to 16 bits does here: a sum that is
+// inexact in FP32 has an addend below a quarter of an ulp of the other.
+__device__ __forceinline__ float Add(float a, float b) { return a + b; }
+__device__ __forceinline__ __half Add(__half a, __half b) { return __float2half_rn(__half2float(a) + __half2float(b)); }
+__device__ __forceinline__ __nv_bfloat16 Add(__nv_bfloat16 a, __nv_bfloat16 b) { return __float2bfloat16_rn(__bfloat162float(a) + __bfloat162float(b)); }
+template <typename T, int C>
+__device__ __forceinline__ Piece<T, C> AddPieces(const Piece<T, C>& a, const Piece<T, C>& b) {
+  Piece<T, C> r;
+  if constexpr (C == 1 || sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(fmaf(f[i], inv, 12582912.f));
-  return __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
+    for (int e = 0; e < C; ++e) r.v[e] = Add(a.v[e], b.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < C / 2; ++e) {
+      uint32_t &o = reinterpret_cast<uint32_t*>(&r)[e];
+      const uint32_t u = reinterpret_cast<const uint32_t*>(&a)[e], v = reinterpret_cast<const uint32_t*>(&b)[e];
+      if constexpr (std::is_same_v<T, __half>) {
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(o) : "r"(u), "r"(v));
+      } else {
+        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(o) : "r"(u), "r"(v));
+      }
+    }
+  }
+  return r;
+}
+// elements 2 e and 2 e + 1 (C = 1: the one, and nothing)
+template <typename T, int C>
+__device__ __forceinline__ float2 Two(const Piece<T, C>& p, int e) {
+  if constexpr (C == 1) {
+    return make_float2(ToFloat(p.v[0]), 0.f);
+  } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(&p)[e];
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  } else if constexpr (std::is_same_v<T, __half>) {
+    return __half22float2(reinterpret_cast<const __half2*>(&p)[e]);
+  } else {
+    return make_float2(ToFloat(p.v[2 * e]), ToFloat(p.v[2 * e + 1]));
+  }
+}
+
+template <int C>
+constexpr int kPairs = C == 1 ? 1 : C / 2;
+// The products f[i] * inv in eight bits.  INT8: adding 1.5 * 2^23 leaves the integer nearest to a product of at most 2^22 in the low
+// bits, rounded once; |f| <= largest and inv = top / largest to within two ulp keep it within [-127, 127].
+template <int C>
+__device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPairs<C>], float inv, bool fp8) {
+  uint32_t two[kPairs<C>];  // a pair in the lower 16 bits
+  if (fp8) {
+#pragma unroll
+    for (int e = 0; e < kPairs<C>; ++e) two[e] = __nv_cvt_float2_to_fp8x2(Mul2(f[e], Both(inv)), __NV_SATFINITE, __NV_E4M3);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPairs<C>; ++e) {
+      const float2 v = Fma2(f[e], Both(inv), Both(12582912.f));
+      two[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040);
+    }
+  }
+  if constexpr (C == 1) {
+    *p = static_cast<uint8_t>(two[0]);
+  } else if constexpr (C == 4) {
+    *reinterpret_cast<uint32_t*>(p) = __byte_perm(two[0], two[1], 0x5410);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(__byte_perm(two[0], two[1], 0x5410), __byte_perm(two[2], two[3], 0x5410));
+  }
 }
 template <int C>
-__device__ __forceinline__ void StoreQuantised(uint8_t* p, const float (&f)[C], float inv, bool fp8, bool bad) {
+__device__ __forceinline__ void StoreZeros(uint8_t* p) {
   if constexpr (C == 1) {
-    const float four[4] = {f[0], 0.f, 0.f, 0.f};
-    *p = bad ? 0 : static_cast<uint8_t>(Quantise4(four, inv, fp8));
+    *p = 0;
+  } else if constexpr (C == 4) {
+    *reinterpret_cast<uint32_t*>(p) = 0;
   } else {
-    uint32_t w[C / 4];
-#pragma unroll
-    for (int i = 0; i < C / 4; ++i) {
-      const float four[4] = {f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
-      w[i] = bad ? 0u : Quantise4(four, inv, fp8);
-    }
-    if constexpr (C == 8) {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    } else {
-      *reinterpret_cast<uint32_t*>(p) = w[0];
-    }
+    *reinterpret_cast<uint2*>(p) = make_uint2(0, 0);
   }
 }
 
-// a / (1 + exp(-a)), to 2^-21: exp(-a) as 2^hi (1 + lo ln 2), where hi + lo is -a log2 e to 2^-40 or so.  With the one rounded product
-// hi for the exponent, the result is off by 2^-24 |a|, 2^-18 at 60.  Past 2^127 the quotient is zero.
-__device__ __forceinline__ float Swish(float a) {
-  const float b = fminf(fmaxf(a, -200.f), 200.f), hi = b * -1.44269504f, lo = fmaf(b, -1.44269504f, -hi) + b * -1.92596299e-8f;  // log2 e in two parts
-  float e, r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  e *= fmaf(lo, 0.693147181f, 1.0f);
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return a * r;
+// a / (1 + exp(-a)), to 2^-21: exp(-a) is 2^hi (1 + lo ln 2) with hi + lo = -a log2 e.  With the rounded product alone for the exponent the
+// result would be off by 2^-24 |a|, 2^-18 at 60.  A BF16 value times the upper 16 bits of log2 e is exact, and lo the rest; else hi is the rounded
+// product and lo what the rounding left, for which values that overflow it (FP32 alone) are kept within bounds.  Results below 2^-126 are flushed to
+// zero, far below a row's least scale.
+template <typename T>
+__device__ __forceinline__ float2 Swish2(float2 a) {
+  float2 hi, t;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    hi = Mul2(a, Both(-47274.f / 32768.f));
+    t = Fma2(a, Both(-4.888495e-06f), Both(1.0f));  // 7.052608e-6 ln 2
+  } else {
+    const float2 b = std::is_same_v<T, float> ? make_float2(fmaxf(fminf(a.x, 1e38f), -200.f), fmaxf(fminf(a.y, 1e38f), -200.f)) : a;
+    hi = Mul2(b, Both(-1.44269504f));
+    const float2 lo = Fma2(b, Both(-1.92596299e-8f), Fma2(b, Both(-1.44269504f), make_float2(-hi.x, -hi.y)));
+    t = Fma2(lo, Both(0.693147181f), Both(1.0f));
+  }
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(hi.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(hi.y));
+  const float2 d = Fma2(e, t, Both(1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  return Mul2(a, r);
 }
 
-// The part of a row's values that follows from the elements themselves, and what they add to the row's sum of squares.  With
-// `keep`, the sum of the residual stream is stored to h.
+// The largest magnitude of three, or a NaN.
+__device__ __forceinline__ float MaxMagnitude(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The part of a row's values that follows from the elements themselves, what they add to the row's sum of squares, and the
+// largest magnitude so far.  The sum of the residual stream is stored to h.
 template <int KIND, typename T, int C>
-__device__ __forceinline__ void Values(float (&f)[C], const Piece<T, C>& x, const Piece<T, C>& second, const RowParams& p, const void* weight, int i, T* h,
-                                       float& squares) {
+__device__ __forceinline__ void Values(float2 (&f)[kPairs<C>], const Piece<T, C>& x, const Piece<T, C>& second, const RowParams& p, const void* weight, int i, T* h,
+                                       float2& squares, float& largest) {
+  Piece<T, C> v = x;
+  if constexpr (KIND == kNormAdd) {
+    v = AddPieces<T, C>(x, second);
+    Store<T, C>(h, v);
+  }
 #pragma unroll
-  for (int e = 0; e < C; ++e) f[e] = ToFloat(x.v[e]);
+  for (int e = 0; e < kPairs<C>; ++e) f[e] = Two<T, C>(v, e);
   if constexpr (KIND == kSwish) {
 #pragma unroll
-    for (int e = 0; e < C; ++e) f[e] = Swish(f[e]) * ToFloat(second.v[e]);
-  }
-  if constexpr (KIND == kNormAdd) {
-    Piece<T, C> sum;
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      sum.v[e] = FromFloat<T>(f[e] + ToFloat(second.v[e]));
-      f[e] = ToFloat(sum.v[e]);
-    }
-    Store<T, C>(h + i, sum);
+    for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(Swish2<T>(f[e]), Two<T, C>(second, e));
   }
   if constexpr (KIND >= kNorm) {
 #pragma unroll
-    for (int e = 0; e < C; ++e) squares = fmaf(f[e], f[e], squares);
+    for (int e = 0; e < kPairs<C>; ++e) squares = Fma2(f[e], f[e], squares);
     if (p.weight_f32) {
       const Piece<float, C> w = Load<float, C>(static_cast<const float*>(weight) + i);
 #pragma unroll
-      for (int e = 0; e < C; ++e) f[e] *= p.offset + w.v[e];
+      for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Add2(Two<float, C>(w, e), Both(p.offset)));
     } else {
       const Piece<T, C> w = Load<T, C>(static_cast<const T*>(weight) + i);
 #pragma unroll
-      for (int e = 0; e < C; ++e) f[e] *= p.offset + ToFloat(w.v[e]);
+      for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Add2(Two<T, C>(w, e), Both(p.offset)));
     }
   }
+#pragma unroll
+  for (int e = 0; e < kPairs<C>; ++e) largest = MaxMagnitude(largest, f[e].x, f[e].y);  // C = 1: y is 0
 }
 
 // The row's sum of squares and largest magnitude, for every thread of it.  Magnitudes are compared as the integers their bits are,
 // in which a NaN is larger than any number.
-__device__ __forceinline__ void Reduce(float& squares, uint32_t& largest, int warps, int warp_of_row, float* sums, uint32_t* tops, bool need_sum) {
+struct RowSums {
+  float squares;
+  uint32_t largest;
+};
+// Of up to 32 warps.  `sums` and `tops` are zero where there is no warp.
+struct Partial {
+  alignas(16) float sums[32];
+  alignas(16) uint32_t tops[32];
+};
+template <bool SUM, bool RING = false>
+__device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int warps, int warp_of_row, Partial& part) {
+  float squares = squares2.x + squares2.y;
+  uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(largest_f) & 0x7FFFFFFFu);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    if (need_sum) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+  for (int d = 16; SUM && d > 0; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+  if (warps == 1) return {squares, largest};
+  if ((threadIdx.x & 31) == 0) {
+    if (SUM) part.sums[warp_of_row] = squares;
+    part.tops[warp_of_row] = largest;
   }
-  largest = __reduce_max_sync(0xffffffffu, largest);
-  if (warps == 1) return;
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) {
-    sums[warp_of_row] = squares;
-    tops[warp_of_row] = largest;
+  if constexpr (RING) {
+    asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+  } else {
+    __syncthreads();
   }
-  __syncthreads();
-  // every warp adds the warps' sums in the same order
-  squares = lane < warps ? sums[lane] : 0.f;
-  largest = lane < warps ? tops[lane] : 0u;
+  // every thread adds the warps' sums in the same order
+  squares = 0.f;
+  largest = 0;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    if (need_sum) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+  for (int i = 0; i < 8; ++i) {
+    if (4 * i < warps) {
+      const uint4 t = reinterpret_cast<const uint4*>(part.tops)[i];
+      largest = max(max(largest, max(t.x, t.y)), max(t.z, t.w));
+      if (SUM) {
+        const float4 v = reinterpret_cast<const float4*>(part.sums)[i];
+        squares += (v.x + v.y) + (v.z + v.w);
+      }
+    }
   }
-  largest = __reduce_max_sync(0xffffffffu, largest);
+  return {squares, largest};
 }
 
 struct Scaling {
@@ -185,92 +291,199 @@ struct Scaling {
   bool bad;
 };
 template <int KIND>
-__device__ __forceinline__ Scaling ScaleOf(float squares, uint32_t largest, const RowParams& p) {
+__device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p) {
   const float top = p.fp8 ? 448.f : 127.f;
   Scaling s;
-  s.bad = largest >= 0x7F800000u;
+  s.bad = r.largest >= 0x7F800000u;
   float root = 1.f;
   if constexpr (KIND >= kNorm) {
-    s.bad = s.bad || !(squares <= 3.4028234e38f);
-    root = 1.f / sqrtf(fmaf(squares, p.inv_n, p.eps));
+    s.bad = s.bad || !(r.squares <= 3.4028234e38f);
+    root = rsqrtf(fmaf(r.squares, p.inv_n, p.eps));
   }
   // (f root) / (max(largest root, tiny) / top) without rounding f root first
-  const float most = fmaxf(__uint_as_float(largest) * root, kTiny);
+  const float most = fmaxf(__uint_as_float(r.largest) * root, kTiny);
   s.inv = root * (top / most);
-  s.scale = s.bad ? __uint_as_float(0x7FFFFFFFu) : most / top;
+  s.scale = s.bad ? __uint_as_float(0x7FFFFFFFu) : most * (p.fp8 ? 1.f / 448.f : 1.f / 127.f);
   return s;
 }
 
-// V pieces of C elements a thread.  C > 1: pieces of 16 bytes; C = 1: rows that lie anywhere.  V = 0: rows read twice.
+// Threads a block may have with so many elements of a row in each one's registers.
+constexpr int MostThreads(int elements) { return elements <= 16 ? 1024 : elements <= 24 ? 768 : elements <= 32 ? 576 : 416; }
+
+// Rows straight into registers, V pieces of C elements a thread.  C > 1: pieces of 16 bytes; C = 1: rows that lie anywhere.  V = 0: rows
+// read twice.
 template <int KIND, typename T, int C, int V>
-__global__ void __launch_bounds__(1024) RowQuantKernel(const RowParams p) {
-  __shared__ float sums[2][8][32];
-  __shared__ uint32_t tops[2][8][32];
+__global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowParams p) {
+  __shared__ Partial parts[4];
   constexpr bool kTwo = KIND == kSwish || KIND == kNormAdd;
+  for (int i = threadIdx.x; i < 4 * 32; i += blockDim.x) {
+    parts[i >> 5].sums[i & 31] = 0.f;
+    parts[i >> 5].tops[i & 31] = 0;
+  }
+  __syncthreads();
   GridDependencyWait();
   const T *const x = BehindWait(static_cast<const T*>(p.x)), *const second = BehindWait(static_cast<const T*>(p.second));
   const char* const weight = BehindWait(static_cast<const char*>(p.weight));
   const int warp = static_cast<int>(threadIdx.x) >> 5, row_of_block = warp / p.warps, warp_of_row = warp - row_of_block * p.warps;
   const int step = p.warps * 32 * C, first = (warp_of_row * 32 + (static_cast<int>(threadIdx.x) & 31)) * C;
-  int turn = 0;
-  for (long long r0 = static_cast<long long>(blockIdx.x) * p.rows_per_block; r0 < p.rows; r0 += static_cast<long long>(gridDim.x) * p.rows_per_block, turn ^= 1) {
-    const long long row = r0 + row_of_block;
-    const int n = row < p.rows ? p.n : 0;
-    const T* const xr = x + row * p.ldx;
-    const T* const sr = second + row * p.ld2;
-    T* const hr = static_cast<T*>(p.h) + row * p.n;
-    uint8_t* const qr = p.q + row * p.n;
-    float squares = 0.f;
-    uint32_t largest = 0;
-    auto look = [&](const float(&f)[C]) {
+  const long long row = static_cast<long long>(blockIdx.x) * p.rows_per_block + row_of_block;
+  const int n = row < p.rows ? p.n : 0;
+  const T* const xr = x + row * p.ldx;
+  const T* const sr = second + row * p.ld2;
+  T* const hr = static_cast<T*>(p.h) + row * p.n;
+  uint8_t* const qr = p.q + row * p.n;
+  float2 squares = make_float2(0.f, 0.f);
+  float largest = 0.f;
+  if constexpr (V > 0) {
+    Piece<T, C> a[V], b[V];
+    float2 f[V][kPairs<C>];
 #pragma unroll
-      for (int e = 0; e < C; ++e) largest = max(largest, __float_as_uint(f[e]) & 0x7FFFFFFFu);
-    };
-    if constexpr (V > 0) {
-      Piece<T, C> a[V], b[V];
-      float f[V][C];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (first + j * step < n) {
-          a[j] = Load<T, C>(xr + first + j * step);
-          if constexpr (kTwo) b[j] = Load<T, C>(sr + first + j * step);
-        }
+    for (int j = 0; j < V; ++j) {
+      if (first + j * step < n) {
+        a[j] = Load<T, C>(xr + first + j * step);
+        if constexpr (kTwo) b[j] = Load<T, C>(sr + first + j * step);
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (first + j * step < n) {
-          Values<KIND, T, C>(f[j], a[j], b[j], p, weight, first + j * step, hr, squares);
-          look(f[j]);
-        }
-      }
-      Reduce(squares, largest, p.warps, warp_of_row, sums[turn][row_of_block], tops[turn][row_of_block], KIND >= kNorm);
-      const Scaling s = ScaleOf<KIND>(squares, largest, p);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (first + j * step < n) StoreQuantised<C>(qr + first + j * step, f[j], s.inv, p.fp8, s.bad);
-      }
-      if (first < n && first == 0) p.scale[row] = s.scale;
-    } else {
-      float f[C];
-      for (int i = first; i < n; i += step) {
-        const Piece<T, C> a = Load<T, C>(xr + i);
-        Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, i, hr, squares);
-        look(f);
-      }
-      Reduce(squares, largest, p.warps, warp_of_row, sums[turn][row_of_block], tops[turn][row_of_block], KIND >= kNorm);
-      const Scaling s = ScaleOf<KIND>(squares, largest, p);
-      for (int i = first; i < n; i += step) {
-        if constexpr (KIND == kNormAdd) {  // the sums that this thread has stored
-          const Piece<T, C> a = Load<T, C>(hr + i);
-          Values<kNorm, T, C>(f, a, a, p, weight, i, hr, squares);
-        } else {
-          const Piece<T, C> a = Load<T, C>(xr + i);
-          Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, i, hr, squares);
-        }
-        StoreQuantised<C>(qr + i, f, s.inv, p.fp8, s.bad);
-      }
-      if (first < n && first == 0) p.scale[row] = s.scale;
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (first + j * step < n) Values<KIND, T, C>(f[j], a[j], b[j], p, weight, first + j * step, hr + first + j * step, squares, largest);
+    }
+    const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
+    const Scaling s = ScaleOf<KIND>(r, p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (first + j * step >= n) break;
+      if (s.bad) {
+        StoreZeros<C>(qr + first + j * step);
+      } else {
+        StoreQuantised<C>(qr + first + j * step, f[j], s.inv, p.fp8);
+      }
+    }
+    if (first == 0 && n > 0) p.scale[row] = s.scale;
+  } else {
+    float2 f[kPairs<C>];
+    for (int i = first; i < n; i += step) {
+      const Piece<T, C> a = Load<T, C>(xr + i);
+      Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, i, hr + i, squares, largest);
+    }
+    const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
+    const Scaling s = ScaleOf<KIND>(r, p);
+    for (int i = first; i < n; i += step) {
+      // of the residual stream, the sums that this thread has stored
+      const Piece<T, C> a = Load<T, C>(KIND == kNormAdd ? hr + i : xr + i);
+      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f, a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, i, hr + i, squares, largest);
+      if (s.bad) {
+        StoreZeros<C>(qr + i);
+      } else {
+        StoreQuantised<C>(qr + i, f, s.inv, p.fp8);
+      }
+    }
+    if (first == 0 && n > 0) p.scale[row] = s.scale;
+  }
+}
+
+// Many rows on 16 bytes: blocks that stay walk over them.  A warp of its own keeps a ring in shared memory full by bulk copies, of one piece
+// of every thread at a time; the others take a row's V pieces from there, give the room back at once, and hold the values as FP32 in
+// registers until the row's sums are known.
+constexpr int kMaxRowStages = 8, kRingRoom = 200 * 1024, kRingMost = 208 * 1024, kRingBlocks = 8;
+struct RowCtl {
+  unsigned long long full[kMaxRowStages], empty[kMaxRowStages];
+  volatile uint32_t fault;
+};
+template <int KIND, typename T, int V>
+__global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V), KIND < kNorm && 16 / sizeof(T) * V >= 32 ? 2 : 1) RowRingKernel(const RowParams p) {
+  constexpr int C = 16 / sizeof(T);
+  constexpr bool kTwo = KIND == kSwish || KIND == kNormAdd;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ RowCtl ctl;
+  __shared__ Partial parts[2];
+  const uint32_t full0 = Smem(ctl.full), empty0 = Smem(ctl.empty), ring0 = Smem(ring);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31, step = p.warps * 32 * C;
+  for (int i = threadIdx.x; i < 2 * 32; i += blockDim.x) {
+    parts[i >> 5].sums[i & 31] = 0.f;
+    parts[i >> 5].tops[i & 31] = 0;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      BarInit(full0 + i * 8, 1);
+      BarInit(empty0 + i * 8, p.warps);
+    }
+    ctl.fault = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  GridDependencyWait();
+  __syncthreads();
+  const T *const x = BehindWait(static_cast<const T*>(p.x)), *const second = BehindWait(static_cast<const T*>(p.second));
+  const char* const weight = BehindWait(static_cast<const char*>(p.weight));
+  const uint32_t stage_bytes = static_cast<uint32_t>(p.stage_bytes);
+  int stage = 0;
+  uint32_t parity = 0;
+  auto advance = [&]() {
+    if (++stage == p.stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  };
+  if (warp == p.warps) {
+    // ---- copies
+    bool first_round = true;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+      const T* const xr = x + row * p.ldx;
+      const T* const sr = second + row * p.ld2;
+      for (int i = 0; i < p.n; i += step * p.per_stage) {
+        if (!first_round && !BarWait(empty0 + stage * 8, parity ^ 1u, ctl)) return;
+        if (lane == 0) {
+          const uint32_t bar = full0 + stage * 8, dst = ring0 + static_cast<uint32_t>(stage) * stage_bytes;
+          const uint32_t bytes = static_cast<uint32_t>(min(step * p.per_stage, p.n - i)) * static_cast<uint32_t>(sizeof(T));
+          BarExpect(bar, kTwo ? 2 * bytes : bytes);
+          BulkLoad(dst, xr + i, bytes, bar);
+          if constexpr (kTwo) BulkLoad(dst + stage_bytes / 2, sr + i, bytes, bar);
+        }
+        advance();
+        if (stage == 0) first_round = false;
+      }
+    }
+    return;
+  }
+  const int first = static_cast<int>(threadIdx.x) * C, own = (p.n - first + step - 1) / step;  // the thread's pieces
+  const uint8_t* const from = ring + threadIdx.x * 16;
+  T* hr = static_cast<T*>(p.h) + blockIdx.x * static_cast<long long>(p.n) + first;
+  uint8_t* qr = p.q + blockIdx.x * static_cast<long long>(p.n) + first;
+  const long long stride = static_cast<long long>(gridDim.x) * p.n;
+  int turn = 0;
+#pragma unroll 1
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1, hr += stride, qr += stride) {
+    float2 f[V][kPairs<C>], squares = make_float2(0.f, 0.f);
+    float largest = 0.f;
+    int part = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (j * step < p.n) {
+        if (part == 0 && !BarWait(full0 + stage * 8, parity, ctl)) largest = __uint_as_float(0x7FFFFFFFu);
+        if (j < own) {
+          const T* const at = reinterpret_cast<const T*>(from + static_cast<uint32_t>(stage) * stage_bytes) + part * step;
+          const Piece<T, C> a = Load<T, C>(at);
+          Values<KIND, T, C>(f[j], a, kTwo ? Load<T, C>(at + stage_bytes / 2 / sizeof(T)) : a, p, weight, first + j * step, hr + j * step, squares, largest);
+        }
+        if (++part == p.per_stage || (j + 1) * step >= p.n) {
+          part = 0;
+          __syncwarp();
+          if (lane == 0) BarArrive(empty0 + stage * 8);
+          advance();
+        }
+      }
+    }
+    const RowSums r = Reduce<(KIND >= kNorm), true>(squares, largest, p.warps, warp, parts[turn]);
+    const Scaling s = ScaleOf<KIND>(r, p);
+    if (!s.bad) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (j < own) StoreQuantised<C>(qr + j * step, f[j], s.inv, p.fp8);
+      }
+    } else {
+      for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);
+    }
+    if (threadIdx.x == 0) p.scale[row] = s.scale;
   }
 }
 
@@ -287,25 +500,80 @@ cudaError_t Launch(const RowParams& p, unsigned blocks, unsigned threads, cudaSt
   return cudaLaunchKernelEx(&cfg, RowQuantKernel<KIND, T, C, V>, p);
 }
 
+// Warps of a row whose threads take `v` pieces each.
+int WarpsOf(int pieces, int v) { return (pieces + 32 * v - 1) / (32 * v); }
+
+template <int KIND, typename T, int V>
+cudaError_t LaunchRing(RowParams& p, int sms, cudaStream_t stream) {
+  constexpr int C = 16 / sizeof(T);
+  constexpr bool kTwo = KIND == kSwish || KIND == kNormAdd;
+  // set up once per device: the limit of shared memory belongs to one
+  static std::atomic<uint64_t> raised{0};
+  static std::atomic<int> registers{0};
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err == cudaSuccess && (device > 63 || !(raised.load(std::memory_order_acquire) >> device & 1))) {
+    cudaFuncAttributes attr;
+    err = cudaFuncGetAttributes(&attr, RowRingKernel<KIND, T, V>);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(RowRingKernel<KIND, T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost);
+    if (err == cudaSuccess) {
+      registers.store((attr.numRegs + 7) / 8 * 8, std::memory_order_relaxed);
+      if (device <= 63) raised.fetch_or(1ull << device, std::memory_order_release);
+    }
+  }
+  if (err != cudaSuccess) return err;
+  p.warps = WarpsOf(p.n / C, V);
+  const int threads = 32 * (p.warps + 1);
+  const int blocks = std::max(1, std::min({kRingBlocks, 65536 / (std::max(registers.load(std::memory_order_relaxed), 24) * threads), 2048 / threads}));
+  const int piece_bytes = p.warps * 32 * 16 * (kTwo ? 2 : 1), room = kRingRoom / blocks / piece_bytes;
+  p.per_stage = room >= 2 * V ? V : 1;  // whole rows where enough of them fit
+  p.stage_bytes = piece_bytes * p.per_stage;
+  p.stages = std::max(2, std::min(kMaxRowStages, room / p.per_stage));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(p.rows, static_cast<long long>(sms) * blocks)));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * p.stage_bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {OverlapAttribute()};
+  cfg.attrs = attr;
+  cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, RowRingKernel<KIND, T, V>, p);
+}
+
 template <int KIND, typename T, int C>
 cudaError_t LaunchShape(RowParams& p, cudaStream_t stream) {
-  const int sms = DeviceSmCount();
-  const int pieces = (p.n + C - 1) / C;
-  constexpr int kMost = C == 1 ? 16 : C == 4 ? 8 : 4;  // pieces that a thread holds at most
-  // Few rows: as many threads a row as it has pieces.  Many: a few pieces a thread, so that the blocks of other rows hide a row's reduction.
+  const int sms = DeviceSmCount(), pieces = (p.n + C - 1) / C;
+  constexpr int kOne = C == 1 ? 4 : 8 / C;  // pieces: four elements of a row that lies anywhere, or eight
   const bool few = p.rows <= 2 * sms;
-  int warps = few ? (pieces + 31) / 32 : (pieces + 32 * kMost - 1) / (32 * kMost);
-  warps = std::min(32, std::max(1, warps));
-  const int v = (pieces + 32 * warps - 1) / (32 * warps);
-  p.warps = warps;
-  p.rows_per_block = few ? 1 : std::max(1, 4 / warps);
-  const unsigned threads = static_cast<unsigned>(32 * warps * p.rows_per_block);
-  const long long want = (p.rows + p.rows_per_block - 1) / p.rows_per_block, most = static_cast<long long>(sms) * std::max(1u, 2048 / threads);
-  const unsigned blocks = static_cast<unsigned>(std::min(want, most));
-  if (v <= 1) return Launch<KIND, T, C, 1>(p, blocks, threads, stream);
-  if (v <= kMost / 2) return Launch<KIND, T, C, kMost / 2>(p, blocks, threads, stream);
-  if (v <= kMost) return Launch<KIND, T, C, kMost>(p, blocks, threads, stream);
-  return Launch<KIND, T, C, 0>(p, blocks, threads, stream);
+  if constexpr (C > 1) {
+    if (!few && p.n * sizeof(T) >= 1024) {
+      for (int e : {3, 4, 6}) {
+        if (WarpsOf(pieces, e * kOne) + 1 > MostThreads(C * e * kOne) / 32) continue;
+        if (e == 1) return LaunchRing<KIND, T, kOne>(p, sms, stream);
+        if (e == 2) return LaunchRing<KIND, T, 2 * kOne>(p, sms, stream);
+        if (e == 3) return LaunchRing<KIND, T, 3 * kOne>(p, sms, stream);
+        if (e == 4) return LaunchRing<KIND, T, 4 * kOne>(p, sms, stream);
+        return LaunchRing<KIND, T, 6 * kOne>(p, sms, stream);
+      }
+    }
+  }
+  // Few rows: as many threads a row as it has pieces.  Many: more pieces a thread, so that the blocks of other rows hide a row's reduction.
+  int e = few ? 1 : 2, warps = 0, most = 1;
+  for (;; ++e) {
+    warps = WarpsOf(pieces, e * kOne);
+    most = MostThreads(C * e * kOne) / 32;
+    if (warps <= most || e == 4) break;
+  }
+  p.warps = std::min(warps, most);
+  p.rows_per_block = few ? 1 : std::max(1, 4 / p.warps);
+  const unsigned threads = static_cast<unsigned>(32 * p.warps * p.rows_per_block);
+  const long long blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  if (warps > most) return Launch<KIND, T, C, 0>(p, static_cast<unsigned>(blocks), threads, stream);
+  if (e == 1) return Launch<KIND, T, C, kOne>(p, static_cast<unsigned>(blocks), threads, stream);
+  if (e == 2) return Launch<KIND, T, C, 2 * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
+  if (e == 3) return Launch<KIND, T, C, 3 * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
+  return Launch<KIND, T, C, 4 * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
 }
 
 bool On(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

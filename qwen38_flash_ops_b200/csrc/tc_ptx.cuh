@@ -79,6 +79,10 @@ __device__ __forceinline__ void TmaLoad(uint32_t dst, const CUtensorMap* map, in
                  : "memory");
   }
 }
+// bytes that lie beside one another, from and to 16-byte boundaries, a multiple of 16 of them
+__device__ __forceinline__ void BulkLoad(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 // one lane of a converged warp; unlike a test of the lane number it leaves the compiler's view of the operands uniform,
 // which the MMA's descriptors need (a lane test cost 80 cycles per MMA and 350 per wait)
 __device__ __forceinline__ bool ElectOne() {
