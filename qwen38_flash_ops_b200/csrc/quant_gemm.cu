@@ -50,6 +50,7 @@ constexpr int kPitch = 80;                // bytes of a row of 32 columns in an 
 constexpr int kWarpBuffer = 32 * kPitch + 256 * 4;  // that, and the warp's copy of its rows' scales
 constexpr int kMostColumns = 512;           // of tensor memory
 constexpr int kMaxSplit = 8;                // CTAs that share K
+constexpr int kGroup = 8;                   // row blocks that the tiles go down before the next column block
 
 struct QuantParams {
   CUtensorMap xmap, wmap;
@@ -662,9 +663,6 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
   }
 }
 
-#ifndef QGROUP
-#define QGROUP 8
-#endif
 // ------------------------------------------------------------------------------ host
 constexpr int kSmemPerSm = 233472;                                      // of an SM; a CTA takes 1 KB of it beside its own
 constexpr int kStatic = (static_cast<int>(sizeof(QuantCtl)) + 127) / 128 * 128;
@@ -779,25 +777,59 @@ cudaError_t ConfigureQuantKernels() {
   return SetUpQuant(&setup);
 }
 
+// Launch shape: rows per tile, CTAs that split K, pairs, CTAs per SM.  The cheapest by a model of a call's time in us, fitted to calls in graphs on one
+// B200: 413 random shapes (1 to 2048 rows, K 256 to 17408, N 256 to 152000), up to 50 launch shapes each; the shape chosen takes 1.6 % longer than the best one
+// on average (the worst: 197 x 13840 x 2880 27 us against 19 in other rows per tile).  Rows off 16 bytes have a fit of their own (143 shapes, 0.6 %).
+//   blocks of 128 k in turn, `waves` times; or what the CTAs fetch through L2; or memory: the longest, and a part of the shorter
+//   around that what a call takes anyway, with the last tile's epilogue, and where K is split, the ranks' exchange
+// More row tiles than needed are tried because they can fill the last wave better (509 x 5120 x 10240: three of 192 28 us, two of 256 32).
+struct QuantCost {
+  double step_least, step_row;   // of a block: at least, and for each row of the tile
+  double call, call_row, wave;   // around the blocks; of a further wave
+  double join, join_row, join_rank;
+  double memory, l2;             // bytes a us
+  double rest;                   // of the shorter of the two
+};
+constexpr double kAny = 1e30;
+constexpr QuantCost kSingle = {0.125, 0.0019, 2.6, 0.0149, 0.3, 0.565, 0.0216, 0.027, 11.5e6, 16.8e6, 0.1};
+constexpr QuantCost kPair = {0.102, 0.00134, 3.9, 0.0054, 0.73, 0, 0, 0, 11.5e6, 16.8e6, 0.1};
+constexpr QuantCost kUnaligned = {0.22, 0.00104, 0.6, 0.001, 2.6, 0.31, 0.0028, 0.027, 5.4e6, kAny, 0.41};
+constexpr double kShared = 1.17;  // a block of two CTAs on an SM, in the sum of what it takes at least and for its rows
+
 QuantPlan ChooseQuantPlan(const QuantCall& c) {
   const QuantSetup* setup = nullptr;
   if (SetUpQuant(&setup) != cudaSuccess) throw std::runtime_error("QuantGemm: the kernels could not be set up on this device");
-  QuantPlan best;
   const bool loads = !OnSixteen(c.x, c.ldx) || !OnSixteen(c.w, c.ldw);
-  const int64_t blocks = (c.k + kTileK - 1) / kTileK;
-  const int64_t n_tiles = (c.n + kTileN - 1) / kTileN;
-  if (!loads && c.m > 256) {
-    best.pair = 1;
-    best.bm = 256;
-    best.per_sm = 1;
-    return best;
-  }
-  const int64_t mt = (c.m + 255) / 256;
-  best.bm = static_cast<int>(((c.m + mt - 1) / mt + 15) / 16 * 16);
-  best.per_sm = loads || best.bm > 128 ? 1 : 2;
-  const int64_t tiles = n_tiles * mt;
-  for (int s = 2; s <= kMaxSplit && s <= blocks; ++s) {
-    if (tiles <= setup->slots[best.per_sm][s]) best.split = s;
+  const int64_t blocks = (c.k + kTileK - 1) / kTileK, least = (c.m + 255) / 256;
+  const double bytes = static_cast<double>(c.k) * c.n + static_cast<double>(c.m) * c.k + 2.0 * c.m * c.n;
+  QuantPlan best;
+  double best_cost = kAny;
+  auto consider = [&](const QuantPlan& plan) {
+    const QuantCost& q = loads ? kUnaligned : plan.pair ? kPair : kSingle;
+    const int64_t tiles = ((c.m + plan.bm - 1) / plan.bm) * ((c.n + (plan.pair ? 2 * kTileN : kTileN) - 1) / (plan.pair ? 2 * kTileN : kTileN));
+    const int64_t slots = plan.pair ? setup->sms / 2 : setup->slots[plan.per_sm][plan.split];
+    if (slots < 1) return;
+    const int64_t waves = (tiles + slots - 1) / slots, each = (blocks + plan.split - 1) / plan.split;
+    const int64_t ctas = tiles * plan.split * (plan.pair ? 2 : 1);
+    double step = std::max(q.step_least, q.step_row * plan.bm);
+    if (plan.per_sm == 2 && std::min(ctas, slots * plan.split) > setup->sms) step = std::max(step, kShared * (q.step_least + q.step_row * plan.bm));
+    const double walk = static_cast<double>(waves * each) * step + q.wave * static_cast<double>(waves - 1);
+    const double l2 = static_cast<double>(ctas * each) * (kTileN + (plan.pair ? plan.bm / 2 : plan.bm)) * kTileK / q.l2;
+    const double fetch = std::max(l2, bytes / q.memory);
+    const double join = plan.split == 1 ? 0.0 : q.join + q.join_row * plan.bm * (plan.split - 1) / plan.split + q.join_rank * (plan.split - 1);
+    const double cost = std::max(walk, fetch) + q.rest * std::min(walk, fetch) + q.call + q.call_row * plan.bm + join;
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = plan;
+    }
+  };
+  for (int64_t mt = least; mt <= 2 * least + 2 && mt <= c.m; ++mt) {
+    QuantPlan plan;
+    plan.bm = static_cast<int>(((c.m + mt - 1) / mt + 15) / 16 * 16);
+    for (plan.per_sm = 1; plan.per_sm <= (loads ? 1 : 2); ++plan.per_sm) {
+      for (plan.split = 1; plan.split <= std::min<int64_t>(kMaxSplit, blocks); ++plan.split) consider(plan);
+    }
+    if (!loads) consider({(plan.bm + 31) / 32 * 32, 1, 1, 1});
   }
   return best;
 }
@@ -841,7 +873,7 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t st
   if (tiles > INT_MAX / 16) throw std::runtime_error("QuantGemm: too many tiles");
   p.tiles = static_cast<int>(tiles);
   p.n_tiles = p.tiles / p.m_tiles;
-  p.group = std::min(p.m_tiles, QGROUP);
+  p.group = std::min(p.m_tiles, kGroup);
   const int cluster = plan.pair ? 2 : std::min(plan.split, p.ksteps);
   const int xrows = plan.pair ? p.bm / 2 : p.bm, stage = kWBytes + xrows * kTileK;
   if (!x_loads && !EncodeRows(&p.xmap, c.x, c.m, c.k, c.ldx, xrows)) return false;

@@ -36,7 +36,7 @@ struct RowParams {
   float* scale;
   long long ldx, ld2, rows;
   int n, warps, rows_per_block;  // warps of a row
-  int stages, stage_bytes, per_stage;  // of the ring; pieces of every thread in a stage
+  int stages, stage_bytes;       // of the ring
   bool fp8, weight_f32;
   float offset, eps, inv_n;
 };
@@ -212,8 +212,8 @@ __device__ __forceinline__ float MaxMagnitude(float a, float b, float c) {
 // The part of a row's values that follows from the elements themselves, what they add to the row's sum of squares, and the
 // largest magnitude so far.  The sum of the residual stream is stored to h.
 template <int KIND, typename T, int C>
-__device__ __forceinline__ void Values(float2 (&f)[kPairs<C>], const Piece<T, C>& x, const Piece<T, C>& second, const RowParams& p, const void* weight, int i, T* h,
-                                       float2& squares, float& largest) {
+__device__ __forceinline__ void Values(float2 (&f)[kPairs<C>], const Piece<T, C>& x, const Piece<T, C>& second, const RowParams& p, const void* weight,
+                                       const Piece<T, C>* held, int i, T* h, float2& squares, float& largest) {
   Piece<T, C> v = x;
   if constexpr (KIND == kNormAdd) {
     v = AddPieces<T, C>(x, second);
@@ -233,7 +233,7 @@ __device__ __forceinline__ void Values(float2 (&f)[kPairs<C>], const Piece<T, C>
 #pragma unroll
       for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Add2(Two<float, C>(w, e), Both(p.offset)));
     } else {
-      const Piece<T, C> w = Load<T, C>(static_cast<const T*>(weight) + i);
+      const Piece<T, C> w = held != nullptr ? *held : Load<T, C>(static_cast<const T*>(weight) + i);
 #pragma unroll
       for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Add2(Two<T, C>(w, e), Both(p.offset)));
     }
@@ -248,12 +248,12 @@ struct RowSums {
   float squares;
   uint32_t largest;
 };
-// Of up to 32 warps.  `sums` and `tops` are zero where there is no warp.
+// Of up to 32 warps.
 struct Partial {
-  alignas(16) float sums[32];
-  alignas(16) uint32_t tops[32];
+  float sums[32];
+  uint32_t tops[32];
 };
-template <bool SUM, bool RING = false>
+template <bool SUM>
 __device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int warps, int warp_of_row, Partial& part) {
   float squares = squares2.x + squares2.y;
   uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(largest_f) & 0x7FFFFFFFu);
@@ -264,24 +264,14 @@ __device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int 
     if (SUM) part.sums[warp_of_row] = squares;
     part.tops[warp_of_row] = largest;
   }
-  if constexpr (RING) {
-    asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
-  } else {
-    __syncthreads();
-  }
-  // every thread adds the warps' sums in the same order
-  squares = 0.f;
-  largest = 0;
+  __syncthreads();
+  // every warp adds the warps' sums in the same order
+  const int lane = threadIdx.x & 31;
+  largest = __reduce_max_sync(0xffffffffu, lane < warps ? part.tops[lane] : 0u);
+  if (SUM) {
+    squares = lane < warps ? part.sums[lane] : 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (4 * i < warps) {
-      const uint4 t = reinterpret_cast<const uint4*>(part.tops)[i];
-      largest = max(max(largest, max(t.x, t.y)), max(t.z, t.w));
-      if (SUM) {
-        const float4 v = reinterpret_cast<const float4*>(part.sums)[i];
-        squares += (v.x + v.y) + (v.z + v.w);
-      }
-    }
+    for (int d = 16; d > 0; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
   }
   return {squares, largest};
 }
@@ -316,11 +306,6 @@ template <int KIND, typename T, int C, int V>
 __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowParams p) {
   __shared__ Partial parts[4];
   constexpr bool kTwo = KIND == kSwish || KIND == kNormAdd;
-  for (int i = threadIdx.x; i < 4 * 32; i += blockDim.x) {
-    parts[i >> 5].sums[i & 31] = 0.f;
-    parts[i >> 5].tops[i & 31] = 0;
-  }
-  __syncthreads();
   GridDependencyWait();
   const T *const x = BehindWait(static_cast<const T*>(p.x)), *const second = BehindWait(static_cast<const T*>(p.second));
   const char* const weight = BehindWait(static_cast<const char*>(p.weight));
@@ -346,7 +331,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (first + j * step < n) Values<KIND, T, C>(f[j], a[j], b[j], p, weight, first + j * step, hr + first + j * step, squares, largest);
+      if (first + j * step < n) Values<KIND, T, C>(f[j], a[j], b[j], p, weight, nullptr, first + j * step, hr + first + j * step, squares, largest);
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
     const Scaling s = ScaleOf<KIND>(r, p);
@@ -364,14 +349,14 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
     float2 f[kPairs<C>];
     for (int i = first; i < n; i += step) {
       const Piece<T, C> a = Load<T, C>(xr + i);
-      Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, i, hr + i, squares, largest);
+      Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
     const Scaling s = ScaleOf<KIND>(r, p);
     for (int i = first; i < n; i += step) {
       // of the residual stream, the sums that this thread has stored
       const Piece<T, C> a = Load<T, C>(KIND == kNormAdd ? hr + i : xr + i);
-      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f, a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, i, hr + i, squares, largest);
+      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f, a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
       if (s.bad) {
         StoreZeros<C>(qr + i);
       } else {
@@ -382,32 +367,24 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
   }
 }
 
-// Many rows on 16 bytes: blocks that stay walk over them.  A warp of its own keeps a ring in shared memory full by bulk copies, of one piece
-// of every thread at a time; the others take a row's V pieces from there, give the room back at once, and hold the values as FP32 in
-// registers until the row's sums are known.
-constexpr int kMaxRowStages = 8, kRingRoom = 200 * 1024, kRingMost = 208 * 1024, kRingBlocks = 8;
+// Many rows on 16 bytes: blocks that stay walk over them, and bulk copies bring the next rows into a ring in shared memory meanwhile.  A thread
+// holds its V pieces of a row as FP32 between the row's sums and its eight bits.  Nothing but the barrier of those sums says that a row
+// has left the ring: the block's first thread then asks for the row that takes its place.  The weight waits in registers, as it is stored.
+constexpr int kMaxRowStages = 8, kRingRoom = 210 * 1024, kRingMost = 210 * 1024, kRingBlocks = 8;
 struct RowCtl {
-  unsigned long long full[kMaxRowStages], empty[kMaxRowStages];
+  unsigned long long full[kMaxRowStages];
   volatile uint32_t fault;
 };
 template <int KIND, typename T, int V>
-__global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V), KIND < kNorm && 16 / sizeof(T) * V >= 32 ? 2 : 1) RowRingKernel(const RowParams p) {
+__global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel(const RowParams p) {
   constexpr int C = 16 / sizeof(T);
   constexpr bool kTwo = KIND == kSwish || KIND == kNormAdd;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ RowCtl ctl;
   __shared__ Partial parts[2];
-  const uint32_t full0 = Smem(ctl.full), empty0 = Smem(ctl.empty), ring0 = Smem(ring);
-  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31, step = p.warps * 32 * C;
-  for (int i = threadIdx.x; i < 2 * 32; i += blockDim.x) {
-    parts[i >> 5].sums[i & 31] = 0.f;
-    parts[i >> 5].tops[i & 31] = 0;
-  }
+  const uint32_t full0 = Smem(ctl.full), ring0 = Smem(ring);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      BarInit(full0 + i * 8, 1);
-      BarInit(empty0 + i * 8, p.warps);
-    }
+    for (int i = 0; i < p.stages; ++i) BarInit(full0 + i * 8, 1);
     ctl.fault = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -415,65 +392,47 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V), KIND < kNorm 
   __syncthreads();
   const T *const x = BehindWait(static_cast<const T*>(p.x)), *const second = BehindWait(static_cast<const T*>(p.second));
   const char* const weight = BehindWait(static_cast<const char*>(p.weight));
-  const uint32_t stage_bytes = static_cast<uint32_t>(p.stage_bytes);
-  int stage = 0;
-  uint32_t parity = 0;
-  auto advance = [&]() {
-    if (++stage == p.stages) {
-      stage = 0;
-      parity ^= 1u;
-    }
+  const uint32_t row_bytes = static_cast<uint32_t>(p.n * sizeof(T)), stage_bytes = static_cast<uint32_t>(p.stage_bytes);
+  auto fetch = [&](long long row, int stage) {
+    const uint32_t bar = full0 + stage * 8, dst = ring0 + static_cast<uint32_t>(stage) * stage_bytes;
+    BarExpect(bar, kTwo ? 2 * row_bytes : row_bytes);
+    BulkLoad(dst, x + row * p.ldx, row_bytes, bar);
+    if constexpr (kTwo) BulkLoad(dst + stage_bytes / 2, second + row * p.ld2, row_bytes, bar);
   };
-  if (warp == p.warps) {
-    // ---- copies
-    bool first_round = true;
-    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-      const T* const xr = x + row * p.ldx;
-      const T* const sr = second + row * p.ld2;
-      for (int i = 0; i < p.n; i += step * p.per_stage) {
-        if (!first_round && !BarWait(empty0 + stage * 8, parity ^ 1u, ctl)) return;
-        if (lane == 0) {
-          const uint32_t bar = full0 + stage * 8, dst = ring0 + static_cast<uint32_t>(stage) * stage_bytes;
-          const uint32_t bytes = static_cast<uint32_t>(min(step * p.per_stage, p.n - i)) * static_cast<uint32_t>(sizeof(T));
-          BarExpect(bar, kTwo ? 2 * bytes : bytes);
-          BulkLoad(dst, xr + i, bytes, bar);
-          if constexpr (kTwo) BulkLoad(dst + stage_bytes / 2, sr + i, bytes, bar);
-        }
-        advance();
-        if (stage == 0) first_round = false;
-      }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      const long long row = blockIdx.x + static_cast<long long>(i) * gridDim.x;
+      if (row < p.rows) fetch(row, i);
     }
-    return;
   }
-  const int first = static_cast<int>(threadIdx.x) * C, own = (p.n - first + step - 1) / step;  // the thread's pieces
+  const int warp = static_cast<int>(threadIdx.x) >> 5, step = p.warps * 32 * C, first = static_cast<int>(threadIdx.x) * C, own = (p.n - first + step - 1) / step;
+  Piece<T, C> w[KIND >= kNorm ? V : 1];
+#pragma unroll
+  for (int j = 0; KIND >= kNorm && j < V; ++j) {
+    if (!p.weight_f32 && j < own) w[j] = Load<T, C>(reinterpret_cast<const T*>(weight) + first + j * step);
+  }
   const uint8_t* const from = ring + threadIdx.x * 16;
   T* hr = static_cast<T*>(p.h) + blockIdx.x * static_cast<long long>(p.n) + first;
   uint8_t* qr = p.q + blockIdx.x * static_cast<long long>(p.n) + first;
   const long long stride = static_cast<long long>(gridDim.x) * p.n;
-  int turn = 0;
+  int stage = 0, turn = 0;
+  uint32_t parity = 0;
 #pragma unroll 1
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1, hr += stride, qr += stride) {
     float2 f[V][kPairs<C>], squares = make_float2(0.f, 0.f);
-    float largest = 0.f;
-    int part = 0;
+    float largest = BarWait(full0 + stage * 8, parity, ctl) ? 0.f : __uint_as_float(0x7FFFFFFFu);
+    const T* const at = reinterpret_cast<const T*>(from + static_cast<uint32_t>(stage) * stage_bytes);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (j * step < p.n) {
-        if (part == 0 && !BarWait(full0 + stage * 8, parity, ctl)) largest = __uint_as_float(0x7FFFFFFFu);
-        if (j < own) {
-          const T* const at = reinterpret_cast<const T*>(from + static_cast<uint32_t>(stage) * stage_bytes) + part * step;
-          const Piece<T, C> a = Load<T, C>(at);
-          Values<KIND, T, C>(f[j], a, kTwo ? Load<T, C>(at + stage_bytes / 2 / sizeof(T)) : a, p, weight, first + j * step, hr + j * step, squares, largest);
-        }
-        if (++part == p.per_stage || (j + 1) * step >= p.n) {
-          part = 0;
-          __syncwarp();
-          if (lane == 0) BarArrive(empty0 + stage * 8);
-          advance();
-        }
+      if (j < own) {
+        const Piece<T, C> a = Load<T, C>(at + j * step);
+        Values<KIND, T, C>(f[j], a, kTwo ? Load<T, C>(at + j * step + stage_bytes / 2 / sizeof(T)) : a, p, weight, KIND >= kNorm ? &w[j] : nullptr, first + j * step, hr + j * step,
+                           squares, largest);
       }
     }
-    const RowSums r = Reduce<(KIND >= kNorm), true>(squares, largest, p.warps, warp, parts[turn]);
+    const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp, parts[turn]);
+    const long long next = row + static_cast<long long>(p.stages) * gridDim.x;
+    if (threadIdx.x == 0 && next < p.rows) fetch(next, stage);
     const Scaling s = ScaleOf<KIND>(r, p);
     if (!s.bad) {
 #pragma unroll
@@ -484,6 +443,10 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V), KIND < kNorm 
       for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);
     }
     if (threadIdx.x == 0) p.scale[row] = s.scale;
+    if (++stage == p.stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
   }
 }
 
@@ -500,6 +463,10 @@ cudaError_t Launch(const RowParams& p, unsigned blocks, unsigned threads, cudaSt
   return cudaLaunchKernelEx(&cfg, RowQuantKernel<KIND, T, C, V>, p);
 }
 
+template <int KIND, typename T>
+int RingBytes(int n) {  // of a row, or the two that it is made of
+  return (n * static_cast<int>(sizeof(T)) + 127) / 128 * 128 * (KIND == kSwish || KIND == kNormAdd ? 2 : 1);
+}
 // Warps of a row whose threads take `v` pieces each.
 int WarpsOf(int pieces, int v) { return (pieces + 32 * v - 1) / (32 * v); }
 
@@ -523,12 +490,12 @@ cudaError_t LaunchRing(RowParams& p, int sms, cudaStream_t stream) {
   }
   if (err != cudaSuccess) return err;
   p.warps = WarpsOf(p.n / C, V);
-  const int threads = 32 * (p.warps + 1);
-  const int blocks = std::max(1, std::min({kRingBlocks, 65536 / (std::max(registers.load(std::memory_order_relaxed), 24) * threads), 2048 / threads}));
-  const int piece_bytes = p.warps * 32 * 16 * (kTwo ? 2 : 1), room = kRingRoom / blocks / piece_bytes;
-  p.per_stage = room >= 2 * V ? V : 1;  // whole rows where enough of them fit
-  p.stage_bytes = piece_bytes * p.per_stage;
-  p.stages = std::max(2, std::min(kMaxRowStages, room / p.per_stage));
+  const int threads = 32 * p.warps;
+  // as many blocks as the registers allow, of three rows in flight each where a row is not too long for that
+  int blocks = std::max(1, std::min({kRingBlocks, 65536 / (std::max(registers.load(std::memory_order_relaxed), 24) * threads), 2048 / threads}));
+  p.stage_bytes = RingBytes<KIND, T>(p.n);
+  while (blocks > 1 && kRingRoom / blocks < 3 * p.stage_bytes) --blocks;
+  p.stages = std::min(kMaxRowStages, kRingRoom / blocks / p.stage_bytes);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(p.rows, static_cast<long long>(sms) * blocks)));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -546,11 +513,12 @@ cudaError_t LaunchShape(RowParams& p, cudaStream_t stream) {
   constexpr int kOne = C == 1 ? 4 : 8 / C;  // pieces: four elements of a row that lies anywhere, or eight
   const bool few = p.rows <= 2 * sms;
   if constexpr (C > 1) {
-    if (!few && p.n * sizeof(T) >= 1024) {
-      for (int e : {3, 4, 6}) {
-        if (WarpsOf(pieces, e * kOne) + 1 > MostThreads(C * e * kOne) / 32) continue;
-        if (e == 1) return LaunchRing<KIND, T, kOne>(p, sms, stream);
-        if (e == 2) return LaunchRing<KIND, T, 2 * kOne>(p, sms, stream);
+    // Many rows of a kilobyte or more, two of which fit the ring.  24 elements a thread, 32 for a norm alone, whose reduction takes the longest for
+    // what it reads; longer rows more.  Rows of 5120, 4096 of them, 16 / 24 / 32 / 48 a thread, us: norm 19.5 / 18.9 / 16.3 / 17.3, with residual 24.3 / 24.4 /
+    // 24.3 / 27.0, gated 20.5 / 20.9 / 21.3 / 21.4.
+    if (!few && p.n * sizeof(T) >= 1024 && 2 * RingBytes<KIND, T>(p.n) <= kRingMost) {
+      for (int e : {KIND == kNorm ? 4 : 3, 4, 6}) {
+        if (WarpsOf(pieces, e * kOne) > MostThreads(C * e * kOne) / 32) continue;
         if (e == 3) return LaunchRing<KIND, T, 3 * kOne>(p, sms, stream);
         if (e == 4) return LaunchRing<KIND, T, 4 * kOne>(p, sms, stream);
         return LaunchRing<KIND, T, 6 * kOne>(p, sms, stream);
