@@ -5,6 +5,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -280,6 +282,11 @@ bool ToRows(PyObject* o, Rows* r) {
   return r->ld >= r->n && (r->t->stride(1) == 1 || r->n == 1);
 }
 
+// at::empty on the current device without its way through the dispatcher: 0.3 us a tensor, of the 5 to 6 that these calls take on the host
+at::Tensor New(c10::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, c10::nullopt);
+}
+
 // rmsnorm_quant(eps, weight_offset, fp8, x, weight, residual or None) -> (q, scale) or (q, scale, h)
 PyObject* RmsNormQuant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return Guard([&]() -> PyObject* {
@@ -291,10 +298,9 @@ PyObject* RmsNormQuant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       return None();
     if (added && (!ToRows(a[5], &r) || r.t->scalar_type() != x.t->scalar_type() || r.t->sizes() != x.t->sizes())) return None();
     const bool fp8 = a[2] == Py_True;
-    const at::Tensor q = at::empty(x.t->sizes(), x.t->options().dtype(fp8 ? at::kFloat8_e4m3fn : at::kChar)),
-                     scale = at::empty(x.t->sizes().slice(0, x.t->dim() - 1), x.t->options().dtype(at::kFloat));
+    const at::Tensor q = New(x.t->sizes(), fp8 ? at::kFloat8_e4m3fn : at::kChar), scale = New(x.t->sizes().slice(0, x.t->dim() - 1), at::kFloat);
     at::Tensor h;
-    if (added) h = at::empty(x.t->sizes(), x.t->options());
+    if (added) h = New(x.t->sizes(), x.t->scalar_type());
     const int dtype = Code(x.t->scalar_type()), w_dtype = Code(w->scalar_type());
     const float offset = static_cast<float>(PyFloat_AS_DOUBLE(a[1])), eps = static_cast<float>(PyFloat_AS_DOUBLE(a[0]));
     const void *xp = x.t->data_ptr(), *rp = added ? r.t->data_ptr() : nullptr, *wp = w->data_ptr();
@@ -314,8 +320,7 @@ PyObject* RowQuant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (n_args != 3 || (a[0] != Py_True && a[0] != Py_False) || !ToRows(a[1], &x) || !Float(*x.t)) return None();
     const bool gated = a[2] != Py_None, fp8 = a[0] == Py_True;
     if (gated && (!ToRows(a[2], &u) || u.t->scalar_type() != x.t->scalar_type() || u.t->sizes() != x.t->sizes())) return None();
-    const at::Tensor q = at::empty(x.t->sizes(), x.t->options().dtype(fp8 ? at::kFloat8_e4m3fn : at::kChar)),
-                     scale = at::empty(x.t->sizes().slice(0, x.t->dim() - 1), x.t->options().dtype(at::kFloat));
+    const at::Tensor q = New(x.t->sizes(), fp8 ? at::kFloat8_e4m3fn : at::kChar), scale = New(x.t->sizes().slice(0, x.t->dim() - 1), at::kFloat);
     const int dtype = Code(x.t->scalar_type());
     const void *xp = x.t->data_ptr(), *up = gated ? u.t->data_ptr() : nullptr;
     void *const qp = q.data_ptr(), *const stream = Stream();
@@ -348,7 +353,7 @@ PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     c10::SmallVector<int64_t, 6> shape(x.t->sizes().begin(), x.t->sizes().end());
     shape.back() = n;
-    const at::Tensor out = at::empty(shape, x.t->options().dtype(out_dtype == QFG_BFLOAT16 ? at::kBFloat16 : out_dtype == QFG_FLOAT16 ? at::kHalf : at::kFloat));
+    const at::Tensor out = New(shape, out_dtype == QFG_BFLOAT16 ? at::kBFloat16 : out_dtype == QFG_FLOAT16 ? at::kHalf : at::kFloat);
     const int dtype = Code(x.t->scalar_type());
     const void *xp = x.t->data_ptr(), *wp = w->data_ptr();
     const float* const sp = xs->data_ptr<float>();

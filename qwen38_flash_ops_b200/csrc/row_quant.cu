@@ -259,7 +259,10 @@ __device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int 
   uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(largest_f) & 0x7FFFFFFFu);
 #pragma unroll
   for (int d = 16; SUM && d > 0; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
-  if (warps == 1) return {squares, largest};
+  if (warps == 1) {
+    __syncwarp();
+    return {squares, largest};
+  }
   if ((threadIdx.x & 31) == 0) {
     if (SUM) part.sums[warp_of_row] = squares;
     part.tops[warp_of_row] = largest;
@@ -287,8 +290,8 @@ __device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p)
   s.bad = r.largest >= 0x7F800000u;
   float root = 1.f;
   if constexpr (KIND >= kNorm) {
-    s.bad = s.bad || !(r.squares <= 3.4028234e38f);
     root = rsqrtf(fmaf(r.squares, p.inv_n, p.eps));
+    s.bad = s.bad || !(r.squares <= 3.4028234e38f) || !(root <= 3.4028234e38f);  // zeros without eps have no norm
   }
   // (f root) / (max(largest root, tiny) / top) without rounding f root first
   const float most = fmaxf(__uint_as_float(r.largest) * root, kTiny);

@@ -3,6 +3,10 @@
 Tolerances.  The sum of squares is added in at most 64 + 10 steps a path, so its relative error is below 80 * 2^-24 and the
 norm's factor's below half of that; the rest of a value takes fewer than eight more FP32 operations, and exp and its quotient 2^-20.
 A scale may be off by that much, and a quotient y / scale, at most 127 or 448, by twice as much before it is rounded to eight bits."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -128,6 +132,37 @@ def test_rows_that_are_not_ordinary(cuda, q_dtype, n):
     assert scale[0].item() == pytest.approx(1e25 / _TOP[q_dtype], rel=1e-6) and (q[0].float() == _TOP[q_dtype]).all()
     assert scale[1].item() == pytest.approx(2.0 ** -100 / _TOP[q_dtype], rel=1e-6)
     _check_rows(q[1:], scale[1:], x[1:].double(), 8 * 2.0 ** -24)  # 0 in INT8, 0.0059 in E4M3
+
+
+@pytest.mark.parametrize("n", [8, 31, 5120])
+def test_zeros_without_eps_have_no_norm(cuda, n):
+    """0 / 0 is not passed off as a row of zeros."""
+    x = torch.ones(2, n, device="cuda")
+    x[1] = 0.0
+    q, scale = RmsNormQuant(eps=0.0)(x, torch.ones(n, device="cuda"))
+    assert torch.isnan(scale).tolist() == [False, True] and (q[0] == 127).all() and (q[1] == 0).all()
+
+
+@pytest.mark.parametrize("rows,n", [(3, 512), (400, 512), (400, 5120)])
+def test_a_first_call_may_be_captured(cuda, rows, n):
+    """In a process that has made no call yet."""
+    code = f"""
+import torch
+from qwen38_flash_ops_b200 import QuantGemm, RmsNormQuant, RowQuant
+x, w, g = torch.randn({rows}, {n}, device="cuda").bfloat16(), torch.ones({n}, device="cuda").bfloat16(), torch.ones({n}, 64, dtype=torch.int8, device="cuda")
+norm, act, gemm, graph = RmsNormQuant(), RowQuant(), QuantGemm(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q, s, h = norm(x, w, x)
+    q2, s2 = act(h, x)
+    y = gemm(q2, s2, g)
+graph.replay()
+torch.cuda.synchronize()
+a, b, c = norm(x, w, x)
+d, e = act(c, x)
+assert torch.equal(a, q) and torch.equal(b, s) and torch.equal(c, h) and torch.equal(d, q2) and torch.equal(gemm(d, e, g), y)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
