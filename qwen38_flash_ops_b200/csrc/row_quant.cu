@@ -143,18 +143,25 @@ __device__ __forceinline__ float2 Two(const Piece<T, C>& p, int e) {
 
 template <int C>
 constexpr int kPairs = C == 1 ? 1 : C / 2;
-// The products f[i] * inv in eight bits.  INT8: adding 1.5 * 2^23 leaves the integer nearest to a product of at most 2^22 in the low
-// bits, rounded once; |f| <= largest and inv = top / largest to within two ulp keep it within [-127, 127].
-template <int C>
-__device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPairs<C>], float inv, bool fp8) {
+// What the largest value of a row gives the others: top / largest, and what that quotient's rounding left of it.
+struct Factor {
+  float hi, lo;
+};
+// The values f[i] top / largest in eight bits.  INT8: adding 1.5 * 2^23 leaves the integer nearest to a value of at most 2^22 in the low
+// bits; |f| <= largest keeps it within [-127, 127].  EXACT, where f holds its value to the last bit (a product of 16-bit inputs in FP32): the value is rounded to FP32
+// once, so that one that lies half way, as half of the largest does, is rounded to even and not as the factor was.  (A value that lands on the
+// other side is a step in one of the sums of the product that follows; with the rounded factor alone one in ten calls had such rows, 8 x 5120.)
+template <int C, bool EXACT>
+__device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPairs<C>], const Factor& by, bool fp8) {
   uint32_t two[kPairs<C>];  // a pair in the lower 16 bits
+  auto value = [&](int e) { return EXACT ? Fma2(f[e], Both(by.hi), Mul2(f[e], Both(by.lo))) : Mul2(f[e], Both(by.hi)); };
   if (fp8) {
 #pragma unroll
-    for (int e = 0; e < kPairs<C>; ++e) two[e] = __nv_cvt_float2_to_fp8x2(Mul2(f[e], Both(inv)), __NV_SATFINITE, __NV_E4M3);
+    for (int e = 0; e < kPairs<C>; ++e) two[e] = __nv_cvt_float2_to_fp8x2(value(e), __NV_SATFINITE, __NV_E4M3);
   } else {
 #pragma unroll
     for (int e = 0; e < kPairs<C>; ++e) {
-      const float2 v = Fma2(f[e], Both(inv), Both(12582912.f));
+      const float2 v = EXACT ? Add2(value(e), Both(12582912.f)) : Fma2(f[e], Both(by.hi), Both(12582912.f));
       two[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040);
     }
   }
@@ -280,7 +287,8 @@ __device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int 
 }
 
 struct Scaling {
-  float inv, scale;
+  Factor by;
+  float scale;
   bool bad;
 };
 template <int KIND>
@@ -293,10 +301,16 @@ __device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p)
     root = rsqrtf(fmaf(r.squares, p.inv_n, p.eps));
     s.bad = s.bad || !(r.squares <= 3.4028234e38f) || !(root <= 3.4028234e38f);  // zeros without eps have no norm
   }
-  // (f root) / (max(largest root, tiny) / top) without rounding f root first
-  const float most = fmaxf(__uint_as_float(r.largest) * root, kTiny);
-  s.inv = root * (top / most);
-  s.scale = s.bad ? __uint_as_float(0x7FFFFFFFu) : most * (p.fp8 ? 1.f / 448.f : 1.f / 127.f);
+  // (f root) / (max(largest root, tiny) / top): the norm's factor leaves the quotient but for rows of tiny values
+  const float largest = __uint_as_float(r.largest), most = largest * root;
+  if (most > kTiny) {
+    s.by.hi = top / largest;
+    s.by.lo = fmaf(-largest, s.by.hi, top) * (s.by.hi * (p.fp8 ? 1.f / 448.f : 1.f / 127.f));
+  } else {
+    s.by.hi = root * (top / kTiny);
+    s.by.lo = 0.f;
+  }
+  s.scale = s.bad ? __uint_as_float(0x7FFFFFFFu) : fmaxf(most, kTiny) * (p.fp8 ? 1.f / 448.f : 1.f / 127.f);
   return s;
 }
 
@@ -344,7 +358,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
       if (s.bad) {
         StoreZeros<C>(qr + first + j * step);
       } else {
-        StoreQuantised<C>(qr + first + j * step, f[j], s.inv, p.fp8);
+        StoreQuantised<C, KIND != kSwish>(qr + first + j * step, f[j], s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = s.scale;
@@ -363,7 +377,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
       if (s.bad) {
         StoreZeros<C>(qr + i);
       } else {
-        StoreQuantised<C>(qr + i, f, s.inv, p.fp8);
+        StoreQuantised<C, KIND != kSwish>(qr + i, f, s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = s.scale;
@@ -440,7 +454,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     if (!s.bad) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (j < own) StoreQuantised<C>(qr + j * step, f[j], s.inv, p.fp8);
+        if (j < own) StoreQuantised<C, KIND != kSwish>(qr + j * step, f[j], s.by, p.fp8);
       }
     } else {
       for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);
