@@ -5,13 +5,18 @@
 // 128-row operand, so that one decoded token costs 16 columns of the instruction and not 128 rows; the rows of x are the bm-column
 // operand.  Both come by tensor copies into 128-byte-swizzled shared memory, 128 bytes of k per stage, as they lie in memory: the
 // weight with its columns contiguous (order n) is read MN-major, with k contiguous (order k) K-major.  Roles by warp:
-//   0-3   epilogue: sums -> scaled -> the output
-//   4     tensor copies of every stage
+//   0-3   epilogue: sums -> scaled -> the output; pairs have four more (6-9), since theirs took 4 us behind the last tile of 256 rows and takes 2
+//   4     tensor copies of every stage; it makes the barriers too, and waits for nothing that the others set up
 //   5     tensor memory; one lane issues the MMAs
-//   6-13  LOADERS only: operands whose rows do not lie on 16 bytes, which a tensor copy cannot address, come by these warps'
-//         32-bit loads, shifted into place
+//   6-21  LOADERS only: operands whose rows do not lie on 16 bytes, which a tensor copy cannot address; see CopyRole and ShiftRole
 // SPLIT: the CTAs of a cluster share K, and add their sums through distributed shared memory in rank order.  PAIR: two CTAs work
 // on 256 columns with cta_group::2, each with its own 128 columns of w and half of the rows of x.
+//
+// What bounds it, on one B200.  Few rows: the weights' way from memory.  1 x 5120 x 34816 30.0 us, 91 % of a copy's bandwidth, 1 x 5120 x 151936 117 to 120 (all of
+// it); narrower weights have fewer CTAs than SMs hold, or ranks that meet: 8 x 5120 x 10240 12.1 us (8.0 at that bandwidth; 80 CTAs), 8 x 17408 x 5120 18.2 (13.6; 40 clusters),
+// 1 x 5120 x 5120 7.0 (4.0; start, first trip to memory and the ranks' exchange are 3).  Many rows: the tensor pipe, 94 % of cycles at 4096 x 5120 x 34816, 420 us cold and
+// 490 to 515 under the power cap (2.9 to 3.5 POP/s); fewer tiles than that the last wave, 509 x 5120 x 10240 32 us, tensor pipe 49 %.  Rows off 16 bytes: the
+// instructions that move them, 1 us a stage of 208 rows (77 x 2561 x 5117 16.7 us).
 //
 // Every wait is bounded.  A CTA that gives up on one writes NaN to the rest of its tiles and leaves.
 #include <cooperative_groups.h>
@@ -43,7 +48,7 @@ constexpr int kTileN = 128;               // columns of w per CTA
 constexpr int kTileK = 128;               // k per stage: one swizzled row of a K-major operand
 constexpr int kWBytes = kTileN * kTileK;  // of a stage
 constexpr int kRing = 12;                 // stages at most
-constexpr int kCopyWarps = 8, kShiftWarps = 8;  // LOADERS
+constexpr int kCopyWarps = 8, kShiftWarps = 8;  // LOADERS; a warp copies the ninth pieces of 32 rows, so there are eight for tiles of 256
 constexpr int kRawPitch = 144;            // bytes of a row as it is copied: 128 of them lie in nine aligned pieces of sixteen
 constexpr int kRawMost = 4;               // stages of that at most
 constexpr int kPitch = 80;                // bytes of a row of 32 columns in an epilogue warp's buffer: rows 16 bytes apart in the banks
@@ -123,9 +128,9 @@ __device__ __forceinline__ At Locate(const QuantParams& p, int tile, int rank) {
 
 // ------------------------------------------------------------------------------ operands off 16 bytes
 // Rows that tensor copies cannot address come in two steps.  Copying warps fetch the aligned pieces of sixteen bytes that hold a row's 128 into a ring of
-// their own, asynchronously, and shifting warps move the rows from there to where the MMA reads them, a word a lane.  Those have no copies of
+// their own, asynchronously, and shifting warps move the rows from there to where the MMA reads them, sixteen bytes a lane.  Those have no copies of
 // their own in flight: the proxy fence behind their stores would wait for them.  (One set of warps that loaded words and stored them took 2.8 us a
-// stage of 208 rows.)  No byte outside the tensor is read: the last piece is copied in part, and one that begins before the tensor byte by byte.
+// stage of 208 rows, the two steps 1.)  No byte outside the tensor is read: the last piece is copied in part, and one that begins before the tensor byte by byte.
 struct Unaligned {  // which rows a stage takes: the weight's, then those of x
   const uint8_t *x, *w;
   int w_rows, rows;
