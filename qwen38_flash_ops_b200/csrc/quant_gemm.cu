@@ -148,14 +148,20 @@ __device__ __forceinline__ StageRows RowsOf(const QuantParams& p, const Unaligne
   return {u.w + row * p.ldw + col, u.w, u.w + p.w_span, p.ldw, (p.order_k ? p.N : p.K) - row, min(kTileK, (p.order_k ? p.K : p.N) - col)};
 }
 
-__device__ __forceinline__ void CopyRole(const QuantParams& p, QuantCtl& ctl, int warp, int lane, int kbeg, int kcount, int first_tile, int tile_step, uint32_t raw) {
+// The first stage's copies are on their way before the barriers exist that later ones need, which `set_up` waits for.
+template <typename F>
+__device__ __forceinline__ void CopyRole(const QuantParams& p, QuantCtl& ctl, int warp, int lane, int kbeg, int kcount, int first_tile, int tile_step, uint32_t raw, F&& set_up) {
   const uint32_t full0 = Smem(&ctl.raw_full[0]), empty0 = Smem(&ctl.raw_empty[0]);
   const Unaligned u(p);
   const uint32_t slot_bytes = static_cast<uint32_t>(u.rows * kRawPitch);
-  constexpr int kPieces = kRawPitch / 16, kPass = 4 * kCopyWarps;
+  constexpr int kPass = 4 * kCopyWarps;
   const int sub = lane >> 3, piece = lane & 7, first = warp * 4 + sub;
   int slot = 0, round = 0;
-  if (p.give_up) return;
+  bool met = false;
+  if (p.give_up) {
+    set_up();
+    return;
+  }
   auto copy = [&](const StageRows& s, int stored, uint32_t to) {  // `stored`: rows that the stage has
     const int rows = min(s.rows, stored);
     const uint8_t* const last = s.row + (rows - 1) * s.ld + s.valid;
@@ -176,13 +182,13 @@ __device__ __forceinline__ void CopyRole(const QuantParams& p, QuantCtl& ctl, in
       if (r < rows && off > 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + static_cast<uint32_t>(r * kRawPitch + 128)), "l"(ninth - off + 128) : "memory");
       return;
     }
-    for (int i = warp * 32 + lane; i < rows * kPieces; i += kCopyWarps * 32) {
-      const int r = i / kPieces, c = i - r * kPieces;
+    // Ends of rows or of the tensor: the same pieces, each as far as it goes.
+    auto part = [&](int r, int c) {
       const uint8_t* const at = s.row + r * s.ld;
       const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
       const uint8_t* const src = at + (16 * c - off);
       const uint32_t dst = to + static_cast<uint32_t>(r * kRawPitch + c * 16);
-      if (16 * c >= off + s.valid) continue;
+      if (r >= rows || 16 * c >= off + s.valid) return;
       if (src >= s.begin) {
         const long long left = s.end - src;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(static_cast<int>(left < 16 ? left : 16)) : "memory");
@@ -192,7 +198,9 @@ __device__ __forceinline__ void CopyRole(const QuantParams& p, QuantCtl& ctl, in
         }
         __threadfence_block();  // the arrival below is that of the copies
       }
-    }
+    };
+    for (int r = first; r < rows; r += kPass) part(r, piece);
+    part(warp * 32 + lane, 8);
   };
   for (int tile = first_tile; tile < p.tiles; tile += tile_step) {
     const At t = Locate<false>(p, tile, 0);
@@ -201,6 +209,8 @@ __device__ __forceinline__ void CopyRole(const QuantParams& p, QuantCtl& ctl, in
       const uint32_t to = raw + static_cast<uint32_t>(slot) * slot_bytes;
       if (p.w_loads) copy(RowsOf(p, u, true, t, (kbeg + k) * kTileK), kTileK, to);
       if (p.x_loads) copy(RowsOf(p, u, false, t, (kbeg + k) * kTileK), p.bm, to + static_cast<uint32_t>(u.w_rows * kRawPitch));
+      if (!met) set_up();
+      met = true;
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full0 + slot * 8) : "memory");
       if (++slot == p.raw_stages) {
         slot = 0;
@@ -377,7 +387,10 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
     }
   }
   FenceBefore();
-  if (PAIR || warp != 4) {
+  const bool copier = LOADERS && warp >= 6 && warp < 6 + kCopyWarps;  // these come to the barrier with their first copies on their way
+  if (copier) {
+    GridDependencyWait();
+  } else if (PAIR || warp != 4) {
     GridDependencyWait();
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory");
   } else {  // this warp waits for nothing that the others set up, only they for its barriers
@@ -386,7 +399,7 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
   }
   if constexpr (PAIR) cg::this_cluster().sync();  // the leader's barriers exist before the peer arrives on them
   FenceAfter();
-  const uint32_t tmem = PAIR || warp != 4 ? ctl.tmem : 0;
+  const uint32_t tmem = PAIR || (warp != 4 && !copier) ? ctl.tmem : 0;
 
   if (warp < 4 || (PAIR && warp >= 6)) {
     // ---- epilogue; a warp reaches the 32 columns of w that its number says.  Of a pair's eight, two share them and take the rows by 32 in turn.
@@ -558,8 +571,9 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
     }
   } else if constexpr (LOADERS) {
     const uint32_t raw = smem + static_cast<uint32_t>(p.raw_at);
-    if (warp < 6 + kCopyWarps) {
-      CopyRole(p, ctl, warp - 6, lane, kbeg, kcount, first_tile, tile_step, raw);
+    if (copier) {
+      CopyRole(p, ctl, warp - 6, lane, kbeg, kcount, first_tile, tile_step, raw,
+               [] { asm volatile("bar.sync 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory"); });
     } else {
       ShiftRole(p, ctl, warp - 6 - kCopyWarps, lane, kbeg, kcount, first_tile, tile_step, smem, stage_bytes, raw);
     }
