@@ -330,6 +330,18 @@ PyObject* RowQuant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// How a weight [k, n] is stored: with its columns beside one another, or its inner dimension.
+bool Order(const at::Tensor& w, int* order, int64_t* ld) {
+  if (w.stride(1) == 1 && w.stride(0) >= w.size(1)) {
+    *order = QFG_ORDER_N, *ld = w.stride(0);
+  } else if (w.stride(0) == 1 && w.stride(1) >= w.size(0)) {
+    *order = QFG_ORDER_K, *ld = w.stride(1);
+  } else {
+    return false;
+  }
+  return true;
+}
+
 // quant_gemm(handle, output type, x, x_scale, w) -> out
 PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return Guard([&]() -> PyObject* {
@@ -344,13 +356,7 @@ PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t n = w->size(1), k = x.n;
     int order;
     int64_t ldw;
-    if (w->stride(1) == 1 && w->stride(0) >= n) {
-      order = QFG_ORDER_N, ldw = w->stride(0);
-    } else if (w->stride(0) == 1 && w->stride(1) >= k) {
-      order = QFG_ORDER_K, ldw = w->stride(1);
-    } else {
-      return None();
-    }
+    if (!Order(*w, &order, &ldw)) return None();
     c10::SmallVector<int64_t, 6> shape(x.t->sizes().begin(), x.t->sizes().end());
     shape.back() = n;
     const at::Tensor out = New(shape, out_dtype == QFG_BFLOAT16 ? at::kBFloat16 : out_dtype == QFG_FLOAT16 ? at::kHalf : at::kFloat);
@@ -361,6 +367,44 @@ PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int code =
         Call([&] { return g_lib.quant_gemm(static_cast<const qfg_quant_gemm*>(op), dtype, xp, x.ld, sp, x.rows, k, wp, ldw, order, n, yp, n, stream); });
     return code != 0 ? PyLong_FromLong(code) : THPVariable_Wrap(out);
+  });
+}
+
+// quant_mlp(eps, weight_offset, norm weight, gate and up's handle, weight, down's handle, weight, x, residual) -> (y, h).  The four calls of the block one after
+// another: from Python they take 22 us on the host, longer than small blocks take.
+PyObject* QuantMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    Rows x, r;
+    if (n_args != 9 || !PyFloat_CheckExact(a[0]) || !PyFloat_CheckExact(a[1]) || !ToRows(a[7], &x) || !ToRows(a[8], &r)) return None();
+    const void *up = PyLong_AsVoidPtr(a[3]), *down = PyLong_AsVoidPtr(a[5]);
+    const at::Tensor *g = Dense(a[2]), *w1 = Plain(a[4]), *w2 = Plain(a[6]);
+    if (PyErr_Occurred() || up == nullptr || down == nullptr || g == nullptr || w1 == nullptr || w2 == nullptr || x.t->scalar_type() != at::kBFloat16 ||
+        r.t->scalar_type() != at::kBFloat16 || r.t->sizes() != x.t->sizes() || x.rows < 1 || !Float(*g) ||
+        (g->scalar_type() != at::kBFloat16 && g->scalar_type() != at::kFloat) || g->numel() != x.n || !OnCurrent(*g) || !OnCurrent(*w1) || !OnCurrent(*w2) ||
+        w1->dim() != 2 || w2->dim() != 2 || !EightBits(*w1) || w2->scalar_type() != w1->scalar_type() || w1->size(0) != x.n || w2->size(0) < 1 ||
+        w1->size(1) != 2 * w2->size(0) || w2->size(1) != x.n)
+      return None();
+    int order1, order2;
+    int64_t ld1, ld2;
+    if (!Order(*w1, &order1, &ld1) || !Order(*w2, &order2, &ld2)) return None();
+    const int64_t m = x.rows, k = x.n, n = w2->size(0);
+    const at::ScalarType eight = w1->scalar_type();
+    const at::Tensor q1 = New({m, k}, eight), s1 = New({m}, at::kFloat), both = New({m, 2 * n}, at::kBFloat16), q2 = New({m, n}, eight), s2 = New({m}, at::kFloat),
+                     y = New(x.t->sizes(), at::kBFloat16), h = New(x.t->sizes(), at::kBFloat16);
+    const int type = Code(eight), g_type = Code(g->scalar_type());
+    const float eps = static_cast<float>(PyFloat_AS_DOUBLE(a[0])), offset = static_cast<float>(PyFloat_AS_DOUBLE(a[1]));
+    const void *xp = x.t->data_ptr(), *rp = r.t->data_ptr(), *gp = g->data_ptr(), *w1p = w1->data_ptr(), *w2p = w2->data_ptr();
+    void *const q1p = q1.data_ptr(), *const q2p = q2.data_ptr(), *const yp = y.data_ptr(), *const hp = h.data_ptr(), *const stream = Stream();
+    float *const s1p = s1.data_ptr<float>(), *const s2p = s2.data_ptr<float>();
+    uint16_t* const both_p = static_cast<uint16_t*>(both.data_ptr());
+    const int code = Call([&] {
+      int c = g_lib.rmsnorm_quant(QFG_BFLOAT16, xp, x.ld, rp, r.ld, gp, g_type, offset, eps, m, k, type, q1p, s1p, hp, stream);
+      if (c == 0) c = g_lib.quant_gemm(static_cast<const qfg_quant_gemm*>(up), type, q1p, k, s1p, m, k, w1p, ld1, order1, 2 * n, both_p, 2 * n, stream);
+      if (c == 0) c = g_lib.row_quant(QFG_BFLOAT16, both_p, 2 * n, both_p + n, 2 * n, m, n, type, q2p, s2p, stream);
+      if (c == 0) c = g_lib.quant_gemm(static_cast<const qfg_quant_gemm*>(down), type, q2p, n, s2p, m, n, w2p, ld2, order2, k, yp, k, stream);
+      return c;
+    });
+    return code != 0 ? PyLong_FromLong(code) : TupleOf({y, h});
   });
 }
 
@@ -416,6 +460,7 @@ PyMethodDef g_methods[] = {QFG_METHOD("bind", Bind),
                            QFG_METHOD("rmsnorm_quant", RmsNormQuant),
                            QFG_METHOD("row_quant", RowQuant),
                            QFG_METHOD("quant_gemm", QuantGemm),
+                           QFG_METHOD("quant_mlp", QuantMlp),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -49,7 +49,7 @@ except ImportError as e:
     _handed_back = lambda *args: None
     _calls = SimpleNamespace(bind=_handed_back, skinny_gemm=_handed_back, argmax_rows=_handed_back, dequant=_handed_back,
                              lmhead=_handed_back, shared_expert_down=_handed_back, bind_rows=_handed_back, rmsnorm_quant=_handed_back,
-                             row_quant=_handed_back, quant_gemm=_handed_back)
+                             row_quant=_handed_back, quant_gemm=_handed_back, quant_mlp=_handed_back)
 _bound = False
 
 

@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import torch
 
-from .ops import QuantGemm, RmsNormQuant, RowQuant
+from . import ops
+from .ops import QuantGemm, RmsNormQuant, RowQuant, check
 
 
 class QuantMlp:
@@ -17,7 +18,8 @@ class QuantMlp:
 
     `gate_up` [hidden, 2 * width] holds gate's columns, then up's, and `down` [width, hidden]; both torch.int8 or both
     torch.float8_e4m3fn, either dimension contiguous, with a scale per column.  Between the products the rows are quantised to the
-    same type.  The four calls follow one another on the current stream and allocate their outputs as torch does."""
+    same type.  The four calls follow one another on the current stream and allocate their outputs as torch does; BF16 rows take one
+    way through C++ for all of them."""
 
     def __init__(self, norm_weight, gate_up, gate_up_scale, down, down_scale, eps: float = 1e-6, weight_offset: float = 0.0):
         if gate_up.dtype != down.dtype or gate_up.shape[1] != 2 * down.shape[0] or gate_up.shape[0] != down.shape[1]:
@@ -30,6 +32,9 @@ class QuantMlp:
         self._down = QuantGemm(w_scale=down_scale)
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor):
+        r = ops._calls.quant_mlp(self._norm.eps, self._norm.weight_offset, self.norm_weight, self._gate_up._p, self.gate_up, self._down._p, self.down, x, residual)
+        if r is not None:
+            return r if r.__class__ is tuple else check(r)
         q, scale, h = self._norm(x, self.norm_weight, residual)
         both = self._gate_up(q, scale, self.gate_up)
         q, scale = self._act(both[..., :self.width], both[..., self.width:])

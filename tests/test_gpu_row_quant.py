@@ -10,7 +10,7 @@ import sys
 import pytest
 import torch
 
-from qwen38_flash_ops_b200 import QfgError, QuantMlp, RmsNormQuant, RowQuant, _lib
+from qwen38_flash_ops_b200 import QfgError, QuantMlp, RmsNormQuant, RowQuant, _lib, ops
 
 pytestmark = pytest.mark.gpu
 _NORM, _SWISH = 48 * 2.0 ** -24, 2.0 ** -20
@@ -255,7 +255,7 @@ def test_refusals(cuda):
 @pytest.mark.parametrize("dtype", _EIGHT)
 @pytest.mark.parametrize("order", ["n", "k"])
 @pytest.mark.parametrize("rows,hidden,width", [(1, 256, 512), (7, 640, 264), (300, 512, 384), (5, 129, 77)])
-def test_mlp(cuda, dtype, order, rows, hidden, width):
+def test_mlp(cuda, monkeypatch, dtype, order, rows, hidden, width):
     """The block against its definition, of which each eight-bit rounding moves a value by up to half a step: the products' relative
     errors add up to a few times 2^-8 (INT8) or 2^-4 (E4M3) of a row's typical value, as the sums of independent ones."""
     gen = torch.Generator(device="cuda").manual_seed(rows + hidden)
@@ -280,5 +280,23 @@ def test_mlp(cuda, dtype, order, rows, hidden, width):
     want = (a * torch.sigmoid(a) * b) @ (q2.double() * s2.double())
     bound = 0.03 if dtype == torch.int8 else 0.12
     assert ((y.double() - want).norm() / want.norm()).item() < bound
+    with monkeypatch.context() as m:  # the same four calls from Python
+        m.setattr(ops._calls, "quant_mlp", lambda *args: None)
+        assert all(torch.equal(a, b) for a, b in zip(mlp(x, r), (y, h)))
+    padded = torch.zeros(rows, hidden + 24, device="cuda").bfloat16()[:, :hidden].copy_(x)
+    assert torch.equal(mlp(padded, r)[0], y) and torch.equal(mlp(x[:1], r[:1])[1], h[:1])
     if rows > 1:
         assert torch.equal(mlp(x.view(rows, 1, hidden), r.view(rows, 1, hidden))[0].view(rows, hidden), y)
+
+
+def test_mlp_refusals(cuda):
+    w1, w2, s = torch.zeros(64, 96, dtype=torch.int8, device="cuda"), torch.zeros(48, 64, dtype=torch.int8, device="cuda"), torch.ones(96)
+    g, x = torch.ones(64, device="cuda").bfloat16(), torch.ones(3, 64, device="cuda").bfloat16()
+    mlp = QuantMlp(g, w1, s.numpy(), w2, s[:64].numpy())
+    for bad in ((x[:, :32], x[:, :32]), (x, x[:2]), (x.cpu(), x), (x, x.float()), (x.half(), x.half())):
+        with pytest.raises(QfgError):
+            mlp(*bad)
+    assert mlp(x[:0], x[:0])[0].shape == (0, 64)
+    for shapes in ((w1[:, :95], w2), (w1, w2[:, :63]), (w1, w2.float())):
+        with pytest.raises(ValueError, match="QuantMlp"):
+            QuantMlp(g, shapes[0], None, shapes[1], None)

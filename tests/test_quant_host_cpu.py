@@ -69,7 +69,7 @@ def test_nodes_that_are_refused():
 @pytest.mark.parametrize("t", [torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(2, 8, device="meta"), None, 3])
 def test_other_tensors_are_handed_back_and_refused(t):
     assert _calls.row_quant(False, t, None) is None and _calls.rmsnorm_quant(1e-6, 0.0, False, t, t, None) is None
-    assert _calls.quant_gemm(1, BF16, t, t, t) is None
+    assert _calls.quant_gemm(1, BF16, t, t, t) is None and _calls.quant_mlp(1e-6, 0.0, t, 1, t, 1, t, t, t) is None and _calls.quant_mlp() is None
     with pytest.raises(QfgError, match="CUDA"):
         RowQuant()(t)
     with pytest.raises(QfgError, match="CUDA"):
