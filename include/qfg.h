@@ -342,6 +342,17 @@ QFG_API int qfg_quant_gemm_compute(const qfg_quant_gemm* op, int dtype, const vo
 QFG_API int qfg_quant_gemm_set_option(qfg_quant_gemm* op, const char* key, const char* value);
 QFG_API void qfg_quant_gemm_destroy(qfg_quant_gemm* op);
 
+/* QuantMlp: the calls above one after another, as an MLP block: h = x + residual, kept; q1 = RmsNormQuant(h); gate, up = gate_up(q1) [rows, 2 width]; q2 =
+ * RowQuant(swish(gate) * up); y = down(q2) [rows, hidden].  Arguments as theirs; y and h contiguous, y in the type of `down`.  The same results as the four
+ * calls, but each product may fetch its first weights before the calls ahead have ended: all that was put on the stream before this call is waited for first,
+ * but nothing that writes a weight may be put on it, by another thread, while this call launches its kernels.  `workspace`: that many bytes of the GPU's
+ * memory, on 256 bytes, free again for what follows on the stream.  rows == 0 is a no-op (and needs none). */
+QFG_API size_t qfg_quant_mlp_workspace_bytes(const qfg_quant_gemm* gate_up, int64_t rows, int64_t hidden, int64_t width);
+QFG_API int qfg_quant_mlp(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* norm_weight, int weight_dtype,
+                          float weight_offset, float eps, int64_t rows, int64_t hidden, int64_t width, int q_dtype, const qfg_quant_gemm* gate_up,
+                          const void* w1, int64_t ldw1, int order1, const qfg_quant_gemm* down, const void* w2, int64_t ldw2, int order2, void* workspace,
+                          void* y, void* h, void* stream);
+
 /* Measurement aid, no counterpart in the reference: sweeps `bytes` of device memory at `buf` (16-byte aligned) with
  * 128-bit read-only loads and writes nothing (`sink`, 4 bytes of device memory or null, is never stored to on
  * real data).  Timed over a buffer several times the size of L2 it gives the read-only streaming ceiling of the

@@ -30,6 +30,7 @@ EXPORTS = (
     "qfg_shared_expert_down_destroy",
     "qfg_rmsnorm_quant", "qfg_row_quant",
     "qfg_quant_gemm_create", "qfg_quant_gemm_compute", "qfg_quant_gemm_set_option", "qfg_quant_gemm_destroy",
+    "qfg_quant_mlp_workspace_bytes", "qfg_quant_mlp",
     "qfg_lmhead_workspace_bytes", "qfg_lmhead_create", "qfg_lmhead_compute", "qfg_lmhead_static_max_rows",
     "qfg_lmhead_compute_static", "qfg_lmhead_set_option",
     "qfg_lmhead_destroy", "qfg_lmhead_combine",
@@ -111,6 +112,10 @@ def load() -> ctypes.CDLL:
     lib.qfg_quant_gemm_set_option.argtypes = [c_void_p, c_char_p, c_char_p]
     lib.qfg_quant_gemm_destroy.argtypes = [c_void_p]
     lib.qfg_quant_gemm_destroy.restype = None
+    lib.qfg_quant_mlp_workspace_bytes.argtypes = [c_void_p, c_int64, c_int64, c_int64]
+    lib.qfg_quant_mlp_workspace_bytes.restype = c_size_t
+    lib.qfg_quant_mlp.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, c_float, c_int64, c_int64, c_int64, c_int,
+                                  c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.qfg_lmhead_exchange_bytes.restype = c_size_t
     lib.qfg_lmhead_compute_sharded.argtypes = [c_void_p, c_void_p, c_int64, c_int64, POINTER(Tensor2D), c_int64, c_int64,
                                                c_void_p, POINTER(LmExchange), c_void_p, c_void_p, c_void_p, c_void_p]

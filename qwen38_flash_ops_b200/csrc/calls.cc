@@ -27,6 +27,8 @@ struct Entries {
   decltype(&qfg_rmsnorm_quant) rmsnorm_quant;
   decltype(&qfg_row_quant) row_quant;
   decltype(&qfg_quant_gemm_compute) quant_gemm;
+  decltype(&qfg_quant_mlp_workspace_bytes) quant_mlp_workspace_bytes;
+  decltype(&qfg_quant_mlp) quant_mlp;
 } g_lib;
 
 // A plain CUDA tensor, or null: no subclass, no wrapper of a transform, nothing without memory of its own.
@@ -370,39 +372,34 @@ PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
-// quant_mlp(eps, weight_offset, norm weight, gate and up's handle, weight, down's handle, weight, x, residual) -> (y, h).  The four calls of the block one after
-// another: from Python they take 22 us on the host, longer than small blocks take.
+// quant_mlp(eps, weight_offset, norm weight, gate and up's handle, its weight, down's handle, its weight, x, residual) -> (y, h); both products to BF16.
 PyObject* QuantMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return Guard([&]() -> PyObject* {
     Rows x, r;
     if (n_args != 9 || !PyFloat_CheckExact(a[0]) || !PyFloat_CheckExact(a[1]) || !ToRows(a[7], &x) || !ToRows(a[8], &r)) return None();
     const void *up = PyLong_AsVoidPtr(a[3]), *down = PyLong_AsVoidPtr(a[5]);
     const at::Tensor *g = Dense(a[2]), *w1 = Plain(a[4]), *w2 = Plain(a[6]);
-    if (PyErr_Occurred() || up == nullptr || down == nullptr || g == nullptr || w1 == nullptr || w2 == nullptr || x.t->scalar_type() != at::kBFloat16 ||
-        r.t->scalar_type() != at::kBFloat16 || r.t->sizes() != x.t->sizes() || x.rows < 1 || !Float(*g) ||
-        (g->scalar_type() != at::kBFloat16 && g->scalar_type() != at::kFloat) || g->numel() != x.n || !OnCurrent(*g) || !OnCurrent(*w1) || !OnCurrent(*w2) ||
-        w1->dim() != 2 || w2->dim() != 2 || !EightBits(*w1) || w2->scalar_type() != w1->scalar_type() || w1->size(0) != x.n || w2->size(0) < 1 ||
-        w1->size(1) != 2 * w2->size(0) || w2->size(1) != x.n)
+    if (PyErr_Occurred() || up == nullptr || down == nullptr || g == nullptr || w1 == nullptr || w2 == nullptr || !Float(*x.t) ||
+        r.t->scalar_type() != x.t->scalar_type() || r.t->sizes() != x.t->sizes() || x.rows < 1 ||
+        (g->scalar_type() != x.t->scalar_type() && g->scalar_type() != at::kFloat) || g->numel() != x.n || !OnCurrent(*g) || !OnCurrent(*w1) ||
+        !OnCurrent(*w2) || w1->dim() != 2 || w2->dim() != 2 || !EightBits(*w1) || w2->scalar_type() != w1->scalar_type() || w1->size(0) != x.n ||
+        w2->size(0) < 1 || w1->size(1) != 2 * w2->size(0) || w2->size(1) != x.n)
       return None();
     int order1, order2;
     int64_t ld1, ld2;
     if (!Order(*w1, &order1, &ld1) || !Order(*w2, &order2, &ld2)) return None();
-    const int64_t m = x.rows, k = x.n, n = w2->size(0);
-    const at::ScalarType eight = w1->scalar_type();
-    const at::Tensor q1 = New({m, k}, eight), s1 = New({m}, at::kFloat), both = New({m, 2 * n}, at::kBFloat16), q2 = New({m, n}, eight), s2 = New({m}, at::kFloat),
-                     y = New(x.t->sizes(), at::kBFloat16), h = New(x.t->sizes(), at::kBFloat16);
-    const int type = Code(eight), g_type = Code(g->scalar_type());
+    const auto *up_op = static_cast<const qfg_quant_gemm*>(up), *down_op = static_cast<const qfg_quant_gemm*>(down);
+    const int64_t width = w2->size(0);
+    const size_t bytes = g_lib.quant_mlp_workspace_bytes(up_op, x.rows, x.n, width);
+    if (bytes == 0) return None();
+    const at::Tensor workspace = New({static_cast<int64_t>(bytes)}, at::kByte), y = New(x.t->sizes(), at::kBFloat16), h = New(x.t->sizes(), x.t->scalar_type());
+    const int dtype = Code(x.t->scalar_type()), g_type = Code(g->scalar_type()), type = Code(w1->scalar_type());
     const float eps = static_cast<float>(PyFloat_AS_DOUBLE(a[0])), offset = static_cast<float>(PyFloat_AS_DOUBLE(a[1]));
     const void *xp = x.t->data_ptr(), *rp = r.t->data_ptr(), *gp = g->data_ptr(), *w1p = w1->data_ptr(), *w2p = w2->data_ptr();
-    void *const q1p = q1.data_ptr(), *const q2p = q2.data_ptr(), *const yp = y.data_ptr(), *const hp = h.data_ptr(), *const stream = Stream();
-    float *const s1p = s1.data_ptr<float>(), *const s2p = s2.data_ptr<float>();
-    uint16_t* const both_p = static_cast<uint16_t*>(both.data_ptr());
+    void *const wp = workspace.data_ptr(), *const yp = y.data_ptr(), *const hp = h.data_ptr(), *const stream = Stream();
     const int code = Call([&] {
-      int c = g_lib.rmsnorm_quant(QFG_BFLOAT16, xp, x.ld, rp, r.ld, gp, g_type, offset, eps, m, k, type, q1p, s1p, hp, stream);
-      if (c == 0) c = g_lib.quant_gemm(static_cast<const qfg_quant_gemm*>(up), type, q1p, k, s1p, m, k, w1p, ld1, order1, 2 * n, both_p, 2 * n, stream);
-      if (c == 0) c = g_lib.row_quant(QFG_BFLOAT16, both_p, 2 * n, both_p + n, 2 * n, m, n, type, q2p, s2p, stream);
-      if (c == 0) c = g_lib.quant_gemm(static_cast<const qfg_quant_gemm*>(down), type, q2p, n, s2p, m, n, w2p, ld2, order2, k, yp, k, stream);
-      return c;
+      return g_lib.quant_mlp(dtype, xp, x.ld, rp, r.ld, gp, g_type, offset, eps, x.rows, x.n, width, type, up_op, w1p, ld1, order1, down_op, w2p, ld2, order2, wp,
+                             yp, hp, stream);
     });
     return code != 0 ? PyLong_FromLong(code) : TupleOf({y, h});
   });
@@ -423,6 +420,16 @@ PyObject* BindRows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   Entries e = g_lib;
   if (!Address(a[0], &e.rmsnorm_quant) || !Address(a[1], &e.row_quant) || !Address(a[2], &e.quant_gemm)) return nullptr;
+  g_lib = e;
+  Py_RETURN_NONE;
+}
+PyObject* BindMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  if (n_args != 2) {
+    PyErr_SetString(PyExc_TypeError, "bind_mlp takes two addresses");
+    return nullptr;
+  }
+  Entries e = g_lib;
+  if (!Address(a[0], &e.quant_mlp_workspace_bytes) || !Address(a[1], &e.quant_mlp)) return nullptr;
   g_lib = e;
   Py_RETURN_NONE;
 }
@@ -457,6 +464,7 @@ PyMethodDef g_methods[] = {QFG_METHOD("bind", Bind),
                            QFG_METHOD("lmhead", LmHead),
                            QFG_METHOD("shared_expert_down", SharedExpertDown),
                            QFG_METHOD("bind_rows", BindRows),
+                           QFG_METHOD("bind_mlp", BindMlp),
                            QFG_METHOD("rmsnorm_quant", RmsNormQuant),
                            QFG_METHOD("row_quant", RowQuant),
                            QFG_METHOD("quant_gemm", QuantGemm),

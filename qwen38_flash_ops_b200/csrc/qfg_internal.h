@@ -312,6 +312,7 @@ struct QuantCall {
   void* out = nullptr;             // [m][n], rows ldo elements apart
   int64_t ldo = 0;
   int out_type = QFG_BFLOAT16;
+  bool early_weight = false;  // the weight is nothing that the call ahead writes: it may be read before that has ended
   int give_up = 0;  // testing
 };
 struct QuantPlan {
@@ -345,6 +346,7 @@ struct RowQuantCall {
   uint8_t* q = nullptr;
   float* scale = nullptr;
   void* h = nullptr;
+  bool trigger = false;  // the call behind may be placed once what ran before this one has ended
 };
 cudaError_t LaunchRowQuant(const RowQuantCall& call, cudaStream_t stream);
 

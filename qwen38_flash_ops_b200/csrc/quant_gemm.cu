@@ -16,7 +16,7 @@
 // it); narrower weights have fewer CTAs than SMs hold, or ranks that meet: 8 x 5120 x 10240 12.1 us (8.0 at that bandwidth; 80 CTAs), 8 x 17408 x 5120 18.2 (13.6; 40 clusters),
 // 1 x 5120 x 5120 7.0 (4.0; start, first trip to memory and the ranks' exchange are 3).  Many rows: the tensor pipe, 94 % of cycles at 4096 x 5120 x 34816, 420 us cold and
 // 490 to 515 under the power cap (2.9 to 3.5 POP/s); fewer tiles than that the last wave, 509 x 5120 x 10240 32 us, tensor pipe 49 %.  Rows off 16 bytes: the
-// instructions that move them, 1 us a stage of 208 rows (77 x 2561 x 5117 16.7 us).
+// instructions that move them, 1 us a stage of 208 rows (77 x 2561 x 5117 16.0 us).
 //
 // Every wait is bounded.  A CTA that gives up on one writes NaN to the rest of its tiles and leaves.
 #include <cooperative_groups.h>
@@ -70,6 +70,7 @@ struct QuantParams {
   int raw_at;            // where the rows of those are copied to, behind everything else
   int out_type;          // a qfg_dtype
   int out_vec;           // rows of the output lie on 16 bytes
+  int early_weight;      // of a QuantCall; for single CTAs and tensor copies
   int give_up;           // testing: no stage comes
 };
 
@@ -335,15 +336,15 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
   int c_tile = first_tile, c_k = 0, c_stage = 0, c_round = 0;
   At c_at = Locate<PAIR>(p, first_tile, rank);
   const uint32_t mine = static_cast<uint32_t>((load_w ? kWBytes : 0) + (load_x ? xrows * kTileK : 0));
-  auto copy_stage = [&]() {
+  auto copy_stage = [&](bool w, bool x) {
     const At t = c_at;
     const uint32_t bar = PAIR ? MapRank(full0 + c_stage * 8, 0) : full0 + c_stage * 8;
     const uint32_t dst = smem + static_cast<uint32_t>(c_stage) * stage_bytes;
     const int k0 = (kbeg + c_k) * kTileK;
     if (ElectOne()) {
-      if (rank == 0 || !PAIR) BarExpect(full0 + c_stage * 8, PAIR ? 2 * mine : mine);
-      if (load_w) TmaLoad<PAIR>(dst, &p.wmap, p.order_k ? k0 : t.n0, p.order_k ? t.n0 : k0, bar);
-      if (load_x) TmaLoad<PAIR>(dst + kWBytes, &p.xmap, k0, t.m0 + (PAIR ? rank * xrows : 0), bar);
+      if (w && (rank == 0 || !PAIR)) BarExpect(full0 + c_stage * 8, PAIR ? 2 * mine : mine);
+      if (w && load_w) TmaLoad<PAIR>(dst, &p.wmap, p.order_k ? k0 : t.n0, p.order_k ? t.n0 : k0, bar);
+      if (x && load_x) TmaLoad<PAIR>(dst + kWBytes, &p.xmap, k0, t.m0 + (PAIR ? rank * xrows : 0), bar);
     }
     __syncwarp();
     if (++c_stage == p.stages) {
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
       c_at = Locate<PAIR>(p, c_tile, rank);
     }
   };
-  const bool copies = p.give_up == 0 && (load_w || load_x);
+  const bool copies = p.give_up == 0 && (load_w || load_x), early = !PAIR && !LOADERS && p.early_weight != 0 && copies;
   if (warp == 4) {
     if (lane == 0) {
       if (load_x) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.xmap) : "memory");
@@ -395,6 +396,11 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory");
   } else {  // this warp waits for nothing that the others set up, only they for its barriers
     asm volatile("bar.arrive 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory");
+    if (early) {  // a stage is full when its rows of x have come as well
+      while (c_tile < p.tiles && c_round == 0) copy_stage(true, false);
+      c_tile = first_tile, c_k = 0, c_stage = 0, c_round = 0;
+      c_at = Locate<PAIR>(p, first_tile, rank);
+    }
     GridDependencyWait();
   }
   if constexpr (PAIR) cg::this_cluster().sync();  // the leader's barriers exist before the peer arrives on them
@@ -530,7 +536,8 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
     }
   } else if (warp == 4) {
     // ---- tensor copies
-    while (copies && c_tile < p.tiles && (c_round == 0 || BarWait(empty0 + c_stage * 8, static_cast<uint32_t>((c_round - 1) & 1), ctl))) copy_stage();
+    while (copies && c_tile < p.tiles && (c_round == 0 || BarWait(empty0 + c_stage * 8, static_cast<uint32_t>((c_round - 1) & 1), ctl)))
+      copy_stage(!early || c_round > 0, true);
   } else if (warp == 5) {
     // ---- MMAs (the leader's, for both CTAs of a pair)
     if (!PAIR || rank == 0) {
@@ -701,7 +708,7 @@ bool EncodeRows(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t col
 }
 
 template <bool FP8, bool PAIR, bool SPLIT, bool LOADERS>
-cudaError_t LaunchAs(const QuantParams& p, int ctas, int cluster, size_t smem, cudaStream_t stream) {
+cudaError_t LaunchAs(const QuantParams& p, int ctas, int cluster, size_t smem, bool overlap, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(static_cast<unsigned>(kThreads<PAIR, LOADERS>));
@@ -716,7 +723,7 @@ cudaError_t LaunchAs(const QuantParams& p, int ctas, int cluster, size_t smem, c
     attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
   }
-  if (MayOverlapPredecessor(stream)) attr[cfg.numAttrs++] = OverlapAttribute();
+  if (overlap) attr[cfg.numAttrs++] = OverlapAttribute();
   return cudaLaunchKernelEx(&cfg, QuantGemmKernel<FP8, PAIR, SPLIT, LOADERS>, p);
 }
 
@@ -882,6 +889,8 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t st
   p.N = static_cast<int>(c.n);
   p.K = static_cast<int>(c.k);
   p.give_up = c.give_up;
+  const bool overlap = MayOverlapPredecessor(stream);
+  p.early_weight = c.early_weight && overlap;  // all weights ahead of all rows of x cost 0.8 us where there is nothing to wait for
   p.x_loads = x_loads;
   p.w_loads = w_loads;
   p.bm = plan.bm;
@@ -912,15 +921,20 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t st
   if (p.stages < 2 || smem > static_cast<size_t>(SmemLimit(1))) throw std::runtime_error("QuantGemm: bad launch shape");
   const int ctas = walkers * cluster;
   if (plan.pair) {
-    err = c.fp8 ? LaunchAs<true, true, false, false>(p, ctas, 2, smem, stream) : LaunchAs<false, true, false, false>(p, ctas, 2, smem, stream);
+    err = c.fp8 ? LaunchAs<true, true, false, false>(p, ctas, 2, smem, overlap, stream)
+                : LaunchAs<false, true, false, false>(p, ctas, 2, smem, overlap, stream);
   } else if (split && loads) {
-    err = c.fp8 ? LaunchAs<true, false, true, true>(p, ctas, cluster, smem, stream) : LaunchAs<false, false, true, true>(p, ctas, cluster, smem, stream);
+    err = c.fp8 ? LaunchAs<true, false, true, true>(p, ctas, cluster, smem, overlap, stream)
+                : LaunchAs<false, false, true, true>(p, ctas, cluster, smem, overlap, stream);
   } else if (split) {
-    err = c.fp8 ? LaunchAs<true, false, true, false>(p, ctas, cluster, smem, stream) : LaunchAs<false, false, true, false>(p, ctas, cluster, smem, stream);
+    err = c.fp8 ? LaunchAs<true, false, true, false>(p, ctas, cluster, smem, overlap, stream)
+                : LaunchAs<false, false, true, false>(p, ctas, cluster, smem, overlap, stream);
   } else if (loads) {
-    err = c.fp8 ? LaunchAs<true, false, false, true>(p, ctas, 1, smem, stream) : LaunchAs<false, false, false, true>(p, ctas, 1, smem, stream);
+    err = c.fp8 ? LaunchAs<true, false, false, true>(p, ctas, 1, smem, overlap, stream)
+                : LaunchAs<false, false, false, true>(p, ctas, 1, smem, overlap, stream);
   } else {
-    err = c.fp8 ? LaunchAs<true, false, false, false>(p, ctas, 1, smem, stream) : LaunchAs<false, false, false, false>(p, ctas, 1, smem, stream);
+    err = c.fp8 ? LaunchAs<true, false, false, false>(p, ctas, 1, smem, overlap, stream)
+                : LaunchAs<false, false, false, false>(p, ctas, 1, smem, overlap, stream);
   }
   if (err == cudaSuccess) err = cudaGetLastError();
   if (err != cudaSuccess) throw std::runtime_error(std::string("QuantGemm: ") + cudaGetErrorString(err));

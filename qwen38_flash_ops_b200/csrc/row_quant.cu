@@ -42,6 +42,7 @@ struct RowParams {
   long long ldx, ld2, rows;
   int n, warps, rows_per_block;  // warps of a row
   int stages, stage_bytes;       // of the ring
+  bool trigger;                  // release the next kernel behind the wait
   bool fp8, weight_f32;
   float offset, eps, inv_n;
 };
@@ -329,6 +330,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
   __shared__ Partial parts[4];
   constexpr bool kTwo = KIND == kSwish || KIND == kNormAdd;
   GridDependencyWait();
+  if (p.trigger) GridLaunchDependents();
   const T *const x = BehindWait(static_cast<const T*>(p.x)), *const second = BehindWait(static_cast<const T*>(p.second));
   const char* const weight = BehindWait(static_cast<const char*>(p.weight));
   const int warp = static_cast<int>(threadIdx.x) >> 5, row_of_block = warp / p.warps, warp_of_row = warp - row_of_block * p.warps;
@@ -411,6 +413,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   GridDependencyWait();
+  if (p.trigger) GridLaunchDependents();
   __syncthreads();
   const T *const x = BehindWait(static_cast<const T*>(p.x)), *const second = BehindWait(static_cast<const T*>(p.second));
   const char* const weight = BehindWait(static_cast<const char*>(p.weight));
@@ -596,6 +599,7 @@ cudaError_t LaunchRowQuant(const RowQuantCall& c, cudaStream_t stream) {
   p.ld2 = p.second == nullptr ? 0 : c.norm ? c.ldr : c.ldu;
   p.weight_f32 = c.weight_dtype == QFG_FLOAT;
   p.fp8 = c.fp8;
+  p.trigger = c.trigger;
   p.rows = c.rows;
   p.n = static_cast<int>(c.n);
   p.offset = c.weight_offset;

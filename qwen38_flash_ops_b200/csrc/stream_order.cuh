@@ -15,9 +15,9 @@
 namespace qfg {
 
 // Every thread of such a kernel comes here before its first access to global memory, whatever it is launched with: the
-// predecessor may be writing anything the call reads, its weights included.  Two things are read earlier, by the few-row kernel: w_scale,
+// predecessor may be writing anything the call reads, its weights included.  Three things are read earlier: by the few-row kernel w_scale,
 // which a node uploads when it is created and no kernel writes, and with pdl_wait, which says that they may be, the first
-// weights.  Without the attribute it returns at once.
+// weights; and by a product of QuantMlp its first weights, released by a row kernel that writes none and has itself waited.  Without the attribute it returns at once.
 __device__ __forceinline__ void GridDependencyWait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void GridLaunchDependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -48,7 +48,7 @@ except ImportError as e:
                   f"`make -C {os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')}` builds it", RuntimeWarning)
     _handed_back = lambda *args: None
     _calls = SimpleNamespace(bind=_handed_back, skinny_gemm=_handed_back, argmax_rows=_handed_back, dequant=_handed_back,
-                             lmhead=_handed_back, shared_expert_down=_handed_back, bind_rows=_handed_back, rmsnorm_quant=_handed_back,
+                             lmhead=_handed_back, shared_expert_down=_handed_back, bind_rows=_handed_back, bind_mlp=_handed_back, rmsnorm_quant=_handed_back,
                              row_quant=_handed_back, quant_gemm=_handed_back, quant_mlp=_handed_back)
 _bound = False
 
@@ -63,6 +63,7 @@ def _load():
                                    "qfg_shared_expert_down_compute")])
         _calls.bind_rows(*[ctypes.cast(getattr(lib, name), c_void_p).value
                            for name in ("qfg_rmsnorm_quant", "qfg_row_quant", "qfg_quant_gemm_compute")])
+        _calls.bind_mlp(*[ctypes.cast(getattr(lib, name), c_void_p).value for name in ("qfg_quant_mlp_workspace_bytes", "qfg_quant_mlp")])
         _bound = True
     return lib
 

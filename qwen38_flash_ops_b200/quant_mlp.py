@@ -18,8 +18,10 @@ class QuantMlp:
 
     `gate_up` [hidden, 2 * width] holds gate's columns, then up's, and `down` [width, hidden]; both torch.int8 or both
     torch.float8_e4m3fn, either dimension contiguous, with a scale per column.  Between the products the rows are quantised to the
-    same type.  The four calls follow one another on the current stream and allocate their outputs as torch does; BF16 rows take one
-    way through C++ for all of them."""
+    same type.  The four calls follow one another on the current stream and allocate their outputs as torch does.
+
+    Work that other threads put on that stream during a call must not write the weights: a product may fetch its first ones before the calls
+    ahead of it have ended."""
 
     def __init__(self, norm_weight, gate_up, gate_up_scale, down, down_scale, eps: float = 1e-6, weight_offset: float = 0.0):
         if gate_up.dtype != down.dtype or gate_up.shape[1] != 2 * down.shape[0] or gate_up.shape[0] != down.shape[1]:

@@ -10,7 +10,7 @@ import sys
 import pytest
 import torch
 
-from qwen38_flash_ops_b200 import QfgError, QuantMlp, RmsNormQuant, RowQuant, _lib, ops
+from qwen38_flash_ops_b200 import QfgError, QuantGemm, QuantMlp, RmsNormQuant, RowQuant, _lib, ops
 
 pytestmark = pytest.mark.gpu
 _NORM, _SWISH = 48 * 2.0 ** -24, 2.0 ** -20
@@ -300,3 +300,75 @@ def test_mlp_refusals(cuda):
     for shapes in ((w1[:, :95], w2), (w1, w2[:, :63]), (w1, w2.float())):
         with pytest.raises(ValueError, match="QuantMlp"):
             QuantMlp(g, shapes[0], None, shapes[1], None)
+
+
+@pytest.mark.parametrize("rows,hidden,width", [(1, 256, 512), (8, 2048, 4096), (40, 1024, 2048), (200, 512, 1536), (6, 520, 1001)])
+def test_mlp_waits_for_what_ran_before(cuda, monkeypatch, rows, hidden, width):
+    """Weights, inputs and residual written right before each call, its results read right behind it."""
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    ints = lambda *s: torch.randint(-127, 128, s, generator=gen, device="cuda").to(torch.int8)
+    w1s, w2s = [ints(hidden, 2 * width) for _ in range(3)], [ints(width, hidden) for _ in range(3)]
+    xs = [torch.randn(rows, hidden, generator=gen, device="cuda").bfloat16() for _ in range(3)]
+    g = torch.ones(hidden, device="cuda").bfloat16()
+    w1, w2, x, r = w1s[0].clone(), w2s[0].clone(), xs[0].clone(), xs[0].clone()
+    mlp = QuantMlp(g, w1, torch.full((2 * width,), 1e-3).numpy(), w2, torch.full((hidden,), 1e-3).numpy())
+
+    def passes():
+        got = []
+        for i in range(24):
+            w1.copy_(w1s[i % 3]), w2.copy_(w2s[i % 3]), x.copy_(xs[i % 3]), r.copy_(xs[(i + 1) % 3])
+            y, h = mlp(x, r)
+            again, _ = mlp(y, h)  # and one call behind another
+            got += [y + 0, h + 0, again + 0]
+        return got
+
+    one = passes()
+    monkeypatch.setattr(ops._calls, "quant_mlp", lambda *args: None)
+    assert all(torch.equal(a, b) for a, b in zip(one, passes()))
+
+
+def test_mlp_on_two_streams(cuda, monkeypatch):
+    gen = torch.Generator(device="cuda").manual_seed(32)
+    ints = lambda *s: torch.randint(-127, 128, s, generator=gen, device="cuda").to(torch.int8)
+    s = torch.full((2048,), 1e-3).numpy()
+    mlps = [QuantMlp(torch.ones(512, device="cuda").bfloat16(), ints(512, 2048), s, ints(1024, 512), s[:512]) for _ in range(2)]
+    xs = [torch.randn(16, 512, generator=gen, device="cuda").bfloat16() for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(40):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(mlps[i](xs[i], xs[i])[0])
+    torch.cuda.synchronize()
+    monkeypatch.setattr(ops._calls, "quant_mlp", lambda *args: None)
+    for i in range(2):
+        want = mlps[i](xs[i], xs[i])[0]
+        assert all(torch.equal(y, want) for y in got[i])
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(workspace=None), "null argument"), (dict(workspace="odd"), "256 bytes"), (dict(residual=None), "null argument"), (dict(y=None), "null argument"),
+    (dict(rows=-1), "bad shape"), (dict(width=0), "bad shape"), (dict(hidden=0), "bad shape"), (dict(width=1 << 30), "bad shape"), (dict(ldx=63), "bad shape"),
+    (dict(ldw1=255), "bad shape"), (dict(ldw2=63), "bad shape"), (dict(q_dtype=_lib.QFG_UINT8), "INT8 or FP8"), (dict(order1=2), "bad order"),
+    (dict(weight=None), "null argument"), (dict(w1=None), "null argument"), (dict(w2=None), "null argument"), (dict(h=None), "null argument"),
+])
+def test_blocks_that_are_refused(cuda, change, message):
+    lib = _lib.load()
+    up, down = QuantGemm(), QuantGemm()
+    rows, hidden, width = 3, 64, 128
+    keep = [torch.zeros(rows, hidden, device="cuda").bfloat16() for _ in range(5)]
+    w1, w2 = torch.zeros(hidden, 2 * width, dtype=torch.int8, device="cuda"), torch.zeros(width, hidden, dtype=torch.int8, device="cuda")
+    bytes_ = lib.qfg_quant_mlp_workspace_bytes(up._p, rows, hidden, width)
+    assert bytes_ >= rows * (hidden + width + 4 * width)
+    workspace = torch.zeros(bytes_ + 16, dtype=torch.uint8, device="cuda")
+    a = dict(dtype=_lib.QFG_BFLOAT16, x=keep[0].data_ptr(), ldx=hidden, residual=keep[1].data_ptr(), ldr=hidden, weight=keep[2].data_ptr(),
+             weight_dtype=_lib.QFG_BFLOAT16, offset=0.0, eps=1e-6, rows=rows, hidden=hidden, width=width, q_dtype=_lib.QFG_INT8, up=up._p, w1=w1.data_ptr(),
+             ldw1=2 * width, order1=0, down=down._p, w2=w2.data_ptr(), ldw2=hidden, order2=0, workspace=workspace.data_ptr(), y=keep[3].data_ptr(),
+             h=keep[4].data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    assert lib.qfg_quant_mlp(*a.values()) == _lib.QFG_OK
+    a.update(change)
+    if a["workspace"] == "odd":
+        a["workspace"] = workspace.data_ptr() + 16
+    assert lib.qfg_quant_mlp(*a.values()) == _lib.QFG_INVALID_ARGUMENT and message in lib.qfg_last_error().decode()
+    torch.cuda.synchronize()

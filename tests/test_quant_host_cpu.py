@@ -54,6 +54,13 @@ def test_no_rows_are_no_call():
     assert _norm(rows=0, x=None, q=None)[0] == _lib.QFG_OK and _rows(rows=0, x=None, q=None)[0] == _lib.QFG_OK
 
 
+def test_blocks_that_are_refused():
+    lib = _lib.load()
+    assert lib.qfg_quant_mlp_workspace_bytes(None, 1, 64, 64) == 0
+    code = lib.qfg_quant_mlp(BF16, PTR, 64, PTR, 64, PTR, BF16, 0.0, 1e-6, 1, 64, 64, I8, None, PTR, 128, 0, None, PTR, 64, 0, PTR, PTR, PTR, None)
+    assert code == _lib.QFG_INVALID_ARGUMENT and lib.qfg_last_error().decode() == "QuantMlp: null node"
+
+
 def test_nodes_that_are_refused():
     lib, h = _lib.load(), ctypes.c_void_p()
     assert lib.qfg_quant_gemm_create(None, 0, I8, ctypes.byref(h)) == _lib.QFG_INVALID_ARGUMENT and not h.value
@@ -88,6 +95,13 @@ def test_bind_rows_checks_its_addresses():
         _calls.bind_rows(1, 2)
     with pytest.raises(ValueError):
         _calls.bind_rows(1, 0, 1)
+
+
+def test_bind_mlp_checks_its_addresses():
+    with pytest.raises(TypeError):
+        _calls.bind_mlp(1)
+    with pytest.raises(ValueError):
+        _calls.bind_mlp(1, 0)
 
 
 def test_lazy_names():
