@@ -312,7 +312,7 @@ QFG_API int qfg_lmhead_combine(const uint64_t* keys, int ranks, int64_t m, int64
  * kernels are fastest where bases and row distances are multiples of 16 bytes.
  *
  * RmsNormQuant: h = x + residual, rounded to its type, is kept (residual == NULL: h is x, and `h` is not written); y_i = h_i *
- * rsqrt(mean(h^2) + eps) * (weight_offset + weight_i); then as RowQuant.  `dtype` (BFLOAT16, FLOAT16, FLOAT) is that of x, residual and h,
+ * (weight_offset + weight_i) * rsqrt(mean(h^2) + eps), in this order (a product h_i w_i that FP32 flushes to zero stays zero); then as RowQuant.  `dtype` (BFLOAT16, FLOAT16, FLOAT) is that of x, residual and h,
  * `weight_dtype` the same or FLOAT, `q_dtype` INT8 or FLOAT8E4M3FN.  q is [rows, n], scale FP32 [rows], h [rows, n], all contiguous; h may be
  * the residual or x itself where that is contiguous.
  *

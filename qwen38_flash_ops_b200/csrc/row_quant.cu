@@ -1,7 +1,7 @@
 // Rows in eight bits with a scale each: of a root-mean-square norm, with the residual stream's addition; of a gated activation; of
 // the rows themselves.
 //
-//   norm    h = x + residual, rounded to its type and kept; y_i = h_i rsqrt(mean(h^2) + eps) (offset + weight_i)
+//   norm    h = x + residual, rounded to its type and kept; y_i = h_i (offset + weight_i) rsqrt(mean(h^2) + eps)
 //   act     y_i = x_i / (1 + exp(-x_i)) u_i, or x_i
 //   scale = max(max_i |y_i|, 2^-100) / top, q_i = y_i / scale rounded to the nearest (ties to even), top = 127 (INT8) or 448 (E4M3)
 //
@@ -179,6 +179,16 @@ __device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPa
     *reinterpret_cast<uint2*>(p) = make_uint2(__byte_perm(two[0], two[1], 0x5410), __byte_perm(two[2], two[3], 0x5410));
   }
 }
+// The part of a row's factor that StoreQuantised does not apply.
+template <int KIND, int C>
+__device__ __forceinline__ void TakeUp(float2 (&f)[kPairs<C>], float first) {
+  if constexpr (KIND >= kNorm) {
+    if (first != 1.f) {
+#pragma unroll
+      for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Both(first));
+    }
+  }
+}
 template <int C>
 __device__ __forceinline__ void StoreZeros(uint8_t* p) {
   if constexpr (C == 1) {
@@ -294,6 +304,7 @@ __device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int 
 
 struct Scaling {
   Factor by;
+  float first;  // a factor ahead of `by`, of rows whose one factor FP32 might not hold; else 1
   float scale;
   bool bad;
 };
@@ -307,13 +318,21 @@ __device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p)
     root = rsqrtf(fmaf(r.squares, p.inv_n, p.eps));
     s.bad = s.bad || !(r.squares <= 3.4028234e38f) || !(root <= 3.4028234e38f);  // zeros without eps have no norm
   }
-  // (f root) / (max(largest root, tiny) / top): the norm's factor leaves the quotient but for rows of tiny values
+  // (f root) / (max(largest root, tiny) / top).  The norm's factor leaves the quotient but for rows of tiny values, where f root is at most `tiny` and
+  // root (top / tiny) alone may be past FP32.  So may top / largest be where a small eps makes much of little: such values are taken up by a power of two.
   const float largest = __uint_as_float(r.largest), most = largest * root;
+  s.first = 1.f;
   if (most > kTiny) {
-    s.by.hi = top / largest;
-    s.by.lo = fmaf(-largest, s.by.hi, top) * (s.by.hi * (p.fp8 ? 1.f / 448.f : 1.f / 127.f));
+    float by = largest;
+    if (KIND >= kNorm && largest < kTiny) {
+      s.first = 1.8446744073709552e19f;  // 2^64
+      by *= s.first;
+    }
+    s.by.hi = top / by;
+    s.by.lo = fmaf(-by, s.by.hi, top) * (s.by.hi * (p.fp8 ? 1.f / 448.f : 1.f / 127.f));
   } else {
-    s.by.hi = root * (top / kTiny);
+    s.first = root;
+    s.by.hi = top / kTiny;
     s.by.lo = 0.f;
   }
   s.scale = s.bad ? __uint_as_float(0x7FFFFFFFu) : fmaxf(most, kTiny) * (p.fp8 ? 1.f / 448.f : 1.f / 127.f);
@@ -365,6 +384,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
       if (s.bad) {
         StoreZeros<C>(qr + first + j * step);
       } else {
+        TakeUp<KIND, C>(f[j], s.first);
         StoreQuantised<C, KIND != kSwish>(qr + first + j * step, f[j], s.by, p.fp8);
       }
     }
@@ -384,6 +404,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
       if (s.bad) {
         StoreZeros<C>(qr + i);
       } else {
+        TakeUp<KIND, C>(f, s.first);
         StoreQuantised<C, KIND != kSwish>(qr + i, f, s.by, p.fp8);
       }
     }
@@ -462,7 +483,10 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     if (!s.bad) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (j < own) StoreQuantised<C, KIND != kSwish>(qr + j * step, f[j], s.by, p.fp8);
+        if (j < own) {
+          TakeUp<KIND, C>(f[j], s.first);
+          StoreQuantised<C, KIND != kSwish>(qr + j * step, f[j], s.by, p.fp8);
+        }
       }
     } else {
       for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);

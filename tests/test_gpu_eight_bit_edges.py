@@ -1,0 +1,66 @@
+"""RmsNormQuant where FP32 ends.
+
+Every case goes through each form of the kernels: rows held in registers, rows read twice (longer than 18432 values), rows through the
+ring (many rows on 16 bytes); in pieces of 16 bytes, and element by element (odd lengths)."""
+import numpy as np
+import pytest
+import torch
+
+from qwen38_flash_ops_b200 import RmsNormQuant
+
+pytestmark = pytest.mark.gpu
+_TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+_EIGHT = [torch.int8, torch.float8_e4m3fn]
+_TINY = 2.0 ** -100
+_REL = 48 * 2.0 ** -24  # of a norm's values: as in test_gpu_row_quant.py
+FORMS = [(6, 512), (6, 31), (2, 40000), (2, 40001), (400, 512), (400, 5120), (700, 129)]
+
+
+def _rows(gen, rows, n):
+    return torch.randn(rows, n, generator=gen, device="cuda") * torch.exp(torch.randn(n, generator=gen, device="cuda") * 0.5)
+
+
+def _half_step(v, dtype):
+    if dtype == torch.int8:
+        return torch.full_like(v, 0.5)
+    return torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 4)
+
+
+# ---- small eps, small values, small weights
+
+
+@pytest.mark.parametrize("q_dtype", _EIGHT)
+@pytest.mark.parametrize("rows,n", FORMS)
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-14, 1e-13, 1e-12])
+@pytest.mark.parametrize("weights", ["ordinary", "zero", "1e-25", "1e-30", "1e-36"])
+def test_norms_of_little(cuda, q_dtype, rows, n, add, eps, weights):
+    """Rows of zeros, of 1e-6 and of 1e-15 among ordinary ones, by ordinary, absent and tiny weights.
+
+    Against the formula in 64 bits.  FP32 holds h_i w_i to 2^-150 where it is below 2^-126; the norm's factor takes that along, and the quotient by
+    the scale."""
+    gen = torch.Generator(device="cuda").manual_seed(n + 11)
+    size = torch.tensor([1.0, 0.0, 1e-6, 1e-15], device="cuda")[torch.arange(rows, device="cuda") % 4][:, None]
+    x = _rows(gen, rows, n) * size
+    r = _rows(gen, rows, n) * size if add else None
+    weight = (1 + 0.3 * torch.randn(n, generator=gen, device="cuda")) * (1.0 if weights == "ordinary" else 0.0 if weights == "zero" else float(weights))
+    got = RmsNormQuant(eps=eps, dtype=q_dtype)(x, weight, r)
+    q, scale = got[0].double(), got[1].double()
+    h = (x if r is None else x + r).double()
+    eps32, top = float(np.float32(eps)), _TOP[q_dtype]
+    square = (h * h).mean(-1) + eps32
+    none = square == 0  # zeros without eps have no norm
+    assert none.any().item() == (eps == 0.0)
+    root = torch.where(none, 1.0, square.rsqrt())
+    y = h * weight.double() * root[:, None]
+    s = y.abs().amax(-1).clamp(min=_TINY) / top
+    lost = 2.0 ** -150 * root
+    assert torch.equal(torch.isnan(scale), none) and (q[none] == 0).all()
+    ok = ~none
+    assert torch.isfinite(q).all()
+    assert ((scale - s).abs() <= _REL * s + lost / top)[ok].all()
+    v = y / s[:, None]
+    off = (q - v).abs() - _half_step(v, q_dtype) * (1 + 1e-9) - 2 * _REL * v.abs() - 2 * (lost / s)[:, None]
+    assert (off <= 0)[ok].all(), off[ok].max().item()
+    if weights == "zero":
+        assert (q == 0).all()
