@@ -321,6 +321,7 @@ __device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p)
   // (f root) / (max(largest root, tiny) / top).  The norm's factor leaves the quotient but for rows of tiny values, where f root is at most `tiny` and
   // root (top / tiny) alone may be past FP32.  So may top / largest be where a small eps makes much of little: such values are taken up by a power of two.
   const float largest = __uint_as_float(r.largest), most = largest * root;
+  if (KIND >= kNorm) s.bad = s.bad || !(most <= 3.4028234e38f);
   s.first = 1.f;
   if (most > kTiny) {
     float by = largest;

@@ -64,3 +64,18 @@ def test_norms_of_little(cuda, q_dtype, rows, n, add, eps, weights):
     assert (off <= 0)[ok].all(), off[ok].max().item()
     if weights == "zero":
         assert (q == 0).all()
+
+
+@pytest.mark.parametrize("q_dtype", _EIGHT)
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_norms_past_fp32(cuda, q_dtype, rows, n):
+    """A largest value that the norm's factor takes past FP32: the row is marked, and holds zeros."""
+    x = torch.zeros(rows, n, device="cuda")
+    x[:, n // 2] = 1.0  # one value, sqrt(n) behind the norm
+    x[1] = 1.0
+    weight = torch.full((n,), 3e38, device="cuda")
+    q, scale = RmsNormQuant(eps=0.0, dtype=q_dtype)(x, weight)
+    past = torch.ones(rows, dtype=torch.bool, device="cuda")
+    past[1] = False
+    assert torch.equal(torch.isnan(scale), past) and (q.float()[past] == 0).all()
+    assert abs(scale[1].item() * _TOP[q_dtype] / 3e38 - 1) < _REL and (q[1].float() == _TOP[q_dtype]).all()
