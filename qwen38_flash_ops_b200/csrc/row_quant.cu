@@ -154,20 +154,20 @@ struct Factor {
   float hi, lo;
 };
 // The values f[i] top / largest in eight bits.  INT8: adding 1.5 * 2^23 leaves the integer nearest to a value of at most 2^22 in the low
-// bits; |f| <= largest keeps it within [-127, 127].  EXACT, where f holds its value to the last bit (a product of 16-bit inputs in FP32): the value is rounded to FP32
-// once, so that one that lies half way, as half of the largest does, is rounded to even and not as the factor was.  (A value that lands on the
-// other side is a step in one of the sums of the product that follows; with the rounded factor alone one in ten calls had such rows, 8 x 5120.)
-template <int C, bool EXACT>
+// bits; |f| <= largest keeps it within [-127, 127].  The quotient is rounded to FP32 once, the factor's own rounding carried along, so that one that lies half
+// way, as half of the largest does, is rounded to even and not as the factor was.  (A value that lands on the other side is a step in one of the sums of
+// the product that follows; with the rounded factor alone one in ten calls had such rows, 8 x 5120.)
+template <int C>
 __device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPairs<C>], const Factor& by, bool fp8) {
   uint32_t two[kPairs<C>];  // a pair in the lower 16 bits
-  auto value = [&](int e) { return EXACT ? Fma2(f[e], Both(by.hi), Mul2(f[e], Both(by.lo))) : Mul2(f[e], Both(by.hi)); };
+  auto value = [&](int e) { return Fma2(f[e], Both(by.hi), Mul2(f[e], Both(by.lo))); };
   if (fp8) {
 #pragma unroll
     for (int e = 0; e < kPairs<C>; ++e) two[e] = __nv_cvt_float2_to_fp8x2(value(e), __NV_SATFINITE, __NV_E4M3);
   } else {
 #pragma unroll
     for (int e = 0; e < kPairs<C>; ++e) {
-      const float2 v = EXACT ? Add2(value(e), Both(12582912.f)) : Fma2(f[e], Both(by.hi), Both(12582912.f));
+      const float2 v = Add2(value(e), Both(12582912.f));
       two[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040);
     }
   }
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
         StoreZeros<C>(qr + first + j * step);
       } else {
         TakeUp<KIND, C>(f[j], s.first);
-        StoreQuantised<C, KIND != kSwish>(qr + first + j * step, f[j], s.by, p.fp8);
+        StoreQuantised<C>(qr + first + j * step, f[j], s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = s.scale;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
         StoreZeros<C>(qr + i);
       } else {
         TakeUp<KIND, C>(f, s.first);
-        StoreQuantised<C, KIND != kSwish>(qr + i, f, s.by, p.fp8);
+        StoreQuantised<C>(qr + i, f, s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = s.scale;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
       for (int j = 0; j < V; ++j) {
         if (j < own) {
           TakeUp<KIND, C>(f[j], s.first);
-          StoreQuantised<C, KIND != kSwish>(qr + j * step, f[j], s.by, p.fp8);
+          StoreQuantised<C>(qr + j * step, f[j], s.by, p.fp8);
         }
       }
     } else {

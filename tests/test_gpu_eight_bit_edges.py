@@ -1,4 +1,4 @@
-"""RmsNormQuant where FP32 ends.
+"""RmsNormQuant and RowQuant where FP32 ends and where values lie half way.
 
 Every case goes through each form of the kernels: rows held in registers, rows read twice (longer than 18432 values), rows through the
 ring (many rows on 16 bytes); in pieces of 16 bytes, and element by element (odd lengths)."""
@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from qwen38_flash_ops_b200 import RmsNormQuant
+from qwen38_flash_ops_b200 import RmsNormQuant, RowQuant
 
 pytestmark = pytest.mark.gpu
 _TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
@@ -79,3 +79,20 @@ def test_norms_past_fp32(cuda, q_dtype, rows, n):
     past[1] = False
     assert torch.equal(torch.isnan(scale), past) and (q.float()[past] == 0).all()
     assert abs(scale[1].item() * _TOP[q_dtype] / 3e38 - 1) < _REL and (q[1].float() == _TOP[q_dtype]).all()
+
+
+# ---- half-way values
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_gated_ties_go_to_even(cuda, dtype, rows, n):
+    """swish(96) is 96 in FP32, so the products are exact, the scale is 96 and the quotients are u: 127, and halves on either side."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    whole = torch.randint(-63, 63, (rows, n), generator=gen, device="cuda").float()
+    u = whole + 0.5
+    u[:, 0] = 127.0
+    x = torch.full((rows, n), 96.0, device="cuda")
+    q, scale = RowQuant(dtype=torch.int8)(x.to(dtype), u.to(dtype))
+    assert (scale == 96.0).all()
+    assert torch.equal(q.float(), torch.round(u))  # torch rounds halves to even
