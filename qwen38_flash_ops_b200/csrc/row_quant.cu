@@ -179,13 +179,15 @@ __device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPa
     *reinterpret_cast<uint2*>(p) = make_uint2(__byte_perm(two[0], two[1], 0x5410), __byte_perm(two[2], two[3], 0x5410));
   }
 }
-// The part of a row's factor that StoreQuantised does not apply.
-template <int KIND, int C>
-__device__ __forceinline__ void TakeUp(float2 (&f)[kPairs<C>], float first) {
+// The part of a row's factor that StoreQuantised does not apply, where there is one.
+template <int KIND, int C, int V>
+__device__ __forceinline__ void TakeUp(float2 (&f)[V][kPairs<C>], float first) {
   if constexpr (KIND >= kNorm) {
-    if (first != 1.f) {
+    if (first == 1.f) return;
 #pragma unroll
-      for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Both(first));
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+      for (int e = 0; e < kPairs<C>; ++e) f[j][e] = Mul2(f[j][e], Both(first));
     }
   }
 }
@@ -379,34 +381,34 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
     const Scaling s = ScaleOf<KIND>(r, p);
+    TakeUp<KIND, C, V>(f, s.first);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if (first + j * step >= n) break;
       if (s.bad) {
         StoreZeros<C>(qr + first + j * step);
       } else {
-        TakeUp<KIND, C>(f[j], s.first);
         StoreQuantised<C>(qr + first + j * step, f[j], s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = s.scale;
   } else {
-    float2 f[kPairs<C>];
+    float2 f[1][kPairs<C>];
     for (int i = first; i < n; i += step) {
       const Piece<T, C> a = Load<T, C>(xr + i);
-      Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
+      Values<KIND, T, C>(f[0], a, kTwo ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
     const Scaling s = ScaleOf<KIND>(r, p);
     for (int i = first; i < n; i += step) {
       // of the residual stream, the sums that this thread has stored
       const Piece<T, C> a = Load<T, C>(KIND == kNormAdd ? hr + i : xr + i);
-      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f, a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
+      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f[0], a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
       if (s.bad) {
         StoreZeros<C>(qr + i);
       } else {
-        TakeUp<KIND, C>(f, s.first);
-        StoreQuantised<C>(qr + i, f, s.by, p.fp8);
+        TakeUp<KIND, C, 1>(f, s.first);
+        StoreQuantised<C>(qr + i, f[0], s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = s.scale;
@@ -481,13 +483,11 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     const long long next = row + static_cast<long long>(p.stages) * gridDim.x;
     if (threadIdx.x == 0 && next < p.rows) fetch(next, stage);
     const Scaling s = ScaleOf<KIND>(r, p);
+    TakeUp<KIND, C, V>(f, s.first);
     if (!s.bad) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (j < own) {
-          TakeUp<KIND, C>(f[j], s.first);
-          StoreQuantised<C>(qr + j * step, f[j], s.by, p.fp8);
-        }
+        if (j < own) StoreQuantised<C>(qr + j * step, f[j], s.by, p.fp8);
       }
     } else {
       for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);
