@@ -307,11 +307,12 @@ __device__ __forceinline__ RowSums Reduce(float2 squares2, float largest_f, int 
 struct Scaling {
   Factor by;
   float first;  // a factor ahead of `by`, of rows whose one factor FP32 might not hold; else 1
-  float scale;
+  float most;   // the largest magnitude behind the norm, at least `tiny`
   bool bad;
 };
+__device__ __forceinline__ float ScaleOf(const Scaling& s, bool fp8) { return s.bad ? __uint_as_float(0x7FFFFFFFu) : s.most / (fp8 ? 448.f : 127.f); }
 template <int KIND>
-__device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p) {
+__device__ __forceinline__ Scaling ScalingOf(const RowSums& r, const RowParams& p) {
   const float top = p.fp8 ? 448.f : 127.f;
   Scaling s;
   s.bad = r.largest >= 0x7F800000u;
@@ -338,7 +339,7 @@ __device__ __forceinline__ Scaling ScaleOf(const RowSums& r, const RowParams& p)
     s.by.hi = top / kTiny;
     s.by.lo = 0.f;
   }
-  s.scale = s.bad ? __uint_as_float(0x7FFFFFFFu) : fmaxf(most, kTiny) * (p.fp8 ? 1.f / 448.f : 1.f / 127.f);
+  s.most = fmaxf(most, kTiny);
   return s;
 }
 
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
       if (first + j * step < n) Values<KIND, T, C>(f[j], a[j], b[j], p, weight, nullptr, first + j * step, hr + first + j * step, squares, largest);
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
-    const Scaling s = ScaleOf<KIND>(r, p);
+    const Scaling s = ScalingOf<KIND>(r, p);
     TakeUp<KIND, C, V>(f, s.first);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
         StoreQuantised<C>(qr + first + j * step, f[j], s.by, p.fp8);
       }
     }
-    if (first == 0 && n > 0) p.scale[row] = s.scale;
+    if (first == 0 && n > 0) p.scale[row] = ScaleOf(s, p.fp8);
   } else {
     float2 f[1][kPairs<C>];
     for (int i = first; i < n; i += step) {
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
       Values<KIND, T, C>(f[0], a, kTwo ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
-    const Scaling s = ScaleOf<KIND>(r, p);
+    const Scaling s = ScalingOf<KIND>(r, p);
     for (int i = first; i < n; i += step) {
       // of the residual stream, the sums that this thread has stored
       const Piece<T, C> a = Load<T, C>(KIND == kNormAdd ? hr + i : xr + i);
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
         StoreQuantised<C>(qr + i, f[0], s.by, p.fp8);
       }
     }
-    if (first == 0 && n > 0) p.scale[row] = s.scale;
+    if (first == 0 && n > 0) p.scale[row] = ScaleOf(s, p.fp8);
   }
 }
 
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp, parts[turn]);
     const long long next = row + static_cast<long long>(p.stages) * gridDim.x;
     if (threadIdx.x == 0 && next < p.rows) fetch(next, stage);
-    const Scaling s = ScaleOf<KIND>(r, p);
+    const Scaling s = ScalingOf<KIND>(r, p);
     TakeUp<KIND, C, V>(f, s.first);
     if (!s.bad) {
 #pragma unroll
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     } else {
       for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);
     }
-    if (threadIdx.x == 0) p.scale[row] = s.scale;
+    if (threadIdx.x == 0) p.scale[row] = ScaleOf(s, p.fp8);
     if (++stage == p.stages) {
       stage = 0;
       parity ^= 1u;

@@ -96,3 +96,17 @@ def test_gated_ties_go_to_even(cuda, dtype, rows, n):
     q, scale = RowQuant(dtype=torch.int8)(x.to(dtype), u.to(dtype))
     assert (scale == 96.0).all()
     assert torch.equal(q.float(), torch.round(u))  # torch rounds halves to even
+
+
+# ---- scales
+
+
+@pytest.mark.parametrize("q_dtype", _EIGHT)
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_scales_are_quotients(cuda, q_dtype, rows, n):
+    """scale = largest / top, rounded once."""
+    gen = torch.Generator(device="cuda").manual_seed(n + 5)
+    x = _rows(gen, rows, n) * torch.rand(rows, 1, generator=gen, device="cuda")
+    _, scale = RowQuant(dtype=q_dtype)(x)
+    want = x.abs().amax(-1).cpu().numpy() / np.float32(_TOP[q_dtype])
+    assert np.array_equal(scale.cpu().numpy(), want)
