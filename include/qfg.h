@@ -326,6 +326,9 @@ QFG_API int qfg_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void*
                               void* stream);
 QFG_API int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q,
                           float* scale, void* stream);
+/* Of both, for tests, in the whole process: "give_up" = 1, rows that go through a ring in shared memory never come, and the bounded waits
+ * for them end; such rows have scale NaN and q 0, and nothing of h is written. */
+QFG_API int qfg_row_quant_set_option(const char* key, const char* value);
 
 /* QuantGemm: out[m, n] = (sum_k x[m, k] w[k, n]) * x_scale[m] * w_scale[n].  INT8 products are summed in 32-bit integers, which is
  * exact (k <= 131071 of them cannot overflow), E4M3 products in FP32; the sum is scaled in FP32 and rounded once to `out_dtype`

@@ -28,7 +28,7 @@ EXPORTS = (
     "qfg_untile_hc_create", "qfg_untile_hc_compute", "qfg_untile_hc_destroy",
     "qfg_shared_expert_down_create", "qfg_shared_expert_down_compute", "qfg_shared_expert_down_set_option",
     "qfg_shared_expert_down_destroy",
-    "qfg_rmsnorm_quant", "qfg_row_quant",
+    "qfg_rmsnorm_quant", "qfg_row_quant", "qfg_row_quant_set_option",
     "qfg_quant_gemm_create", "qfg_quant_gemm_compute", "qfg_quant_gemm_set_option", "qfg_quant_gemm_destroy",
     "qfg_quant_mlp_workspace_bytes", "qfg_quant_mlp",
     "qfg_lmhead_workspace_bytes", "qfg_lmhead_create", "qfg_lmhead_compute", "qfg_lmhead_static_max_rows",
@@ -106,6 +106,7 @@ def load() -> ctypes.CDLL:
     lib.qfg_rmsnorm_quant.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, c_float, c_int64, c_int64, c_int,
                                       c_void_p, c_void_p, c_void_p, c_void_p]
     lib.qfg_row_quant.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]
+    lib.qfg_row_quant_set_option.argtypes = [c_char_p, c_char_p]
     lib.qfg_quant_gemm_create.argtypes = [POINTER(c_float), c_size_t, c_int, POINTER(c_void_p)]
     lib.qfg_quant_gemm_compute.argtypes = [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_int64,
                                            c_void_p, c_int64, c_void_p]

@@ -6,6 +6,7 @@
 // entry points neither allocate nor copy, so they are legal inside a stream capture.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <chrono>
 
 #include <climits>
@@ -682,6 +683,7 @@ namespace {
 size_t ElementBytes(int dtype) { return dtype == QFG_FLOAT ? 4 : dtype == QFG_BFLOAT16 || dtype == QFG_FLOAT16 ? 2 : 0; }  // 0: no type of rows
 bool Aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 bool EightBits(int dtype) { return dtype == QFG_INT8 || dtype == QFG_FLOAT8E4M3FN; }
+std::atomic<bool> g_rows_give_up{false};  // qfg_row_quant_set_option
 
 int RunRowQuant(const char* name, qfg::RowQuantCall& c, int q_dtype, void* stream) {
   const size_t elem = ElementBytes(c.dtype);
@@ -697,6 +699,7 @@ int RunRowQuant(const char* name, qfg::RowQuantCall& c, int q_dtype, void* strea
       (c.norm && !Aligned(c.weight, ElementBytes(c.weight_dtype))))
     return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": misaligned argument");
   c.fp8 = q_dtype == QFG_FLOAT8E4M3FN;
+  c.give_up = g_rows_give_up.load(std::memory_order_relaxed);
   const cudaError_t err = qfg::LaunchRowQuant(c, static_cast<cudaStream_t>(stream));
   return err == cudaSuccess ? QFG_OK : Fail(QFG_FAIL, std::string(name) + ": " + cudaGetErrorString(err));
 }
@@ -752,6 +755,13 @@ int qfg_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void* residua
 int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q, float* scale,
                   void* stream) {
   return RunAct(dtype, x, ldx, u, ldu, rows, n, q_dtype, q, scale, false, stream);
+}
+
+int qfg_row_quant_set_option(const char* key, const char* value) {
+  if (key == nullptr || value == nullptr) return Fail(QFG_INVALID_ARGUMENT, "RowQuant: null argument");
+  if (std::strcmp(key, "give_up") != 0) return Fail(QFG_INVALID_ARGUMENT, std::string("RowQuant: unknown option ") + key);
+  g_rows_give_up.store(std::atoi(value) != 0, std::memory_order_relaxed);
+  return QFG_OK;
 }
 
 int qfg_quant_gemm_create(const float* w_scale, size_t n_w_scale, int out_dtype, qfg_quant_gemm** out) {

@@ -43,6 +43,7 @@ struct RowParams {
   int n, warps, rows_per_block;  // warps of a row
   int stages, stage_bytes;       // of the ring
   bool trigger;                  // release the next kernel behind the wait
+  bool give_up;                  // testing: no row reaches the ring
   bool fp8, weight_f32;
   float offset, eps, inv_n;
 };
@@ -419,6 +420,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
 // Many rows on 16 bytes: blocks that stay walk over them, and bulk copies bring the next rows into a ring in shared memory meanwhile.  A thread
 // holds its V pieces of a row as FP32 between the row's sums and its eight bits.  Nothing but the barrier of those sums says that a row
 // has left the ring: the block's first thread then asks for the row that takes its place.  The weight waits in registers, as it is stored.
+// Every wait is bounded.  A block that gives up on one marks the rows that it has left, as rows without a finite value are, and asks for no more.
 constexpr int kMaxRowStages = 8, kRingRoom = 210 * 1024, kRingMost = 210 * 1024, kRingBlocks = 8;
 struct RowCtl {
   unsigned long long full[kMaxRowStages];
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
   const uint32_t full0 = Smem(ctl.full), ring0 = Smem(ring);
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) BarInit(full0 + i * 8, 1);
-    ctl.fault = 0;
+    ctl.fault = p.give_up ? 1u : 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   GridDependencyWait();
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     BulkLoad(dst, x + row * p.ldx, row_bytes, bar);
     if constexpr (kTwo) BulkLoad(dst + stage_bytes / 2, second + row * p.ld2, row_bytes, bar);
   };
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && !p.give_up) {
     for (int i = 0; i < p.stages; ++i) {
       const long long row = blockIdx.x + static_cast<long long>(i) * gridDim.x;
       if (row < p.rows) fetch(row, i);
@@ -467,14 +469,17 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
   const long long stride = static_cast<long long>(gridDim.x) * p.n;
   int stage = 0, turn = 0;
   uint32_t parity = 0;
+  bool good = true;  // of this thread: false from its first wait that ran out.  What it adds to the sums marks this row and all that the block has left
 #pragma unroll 1
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1, hr += stride, qr += stride) {
     float2 f[V][kPairs<C>], squares = make_float2(0.f, 0.f);
-    float largest = BarWait(full0 + stage * 8, parity, ctl) ? 0.f : __uint_as_float(0x7FFFFFFFu);
+    good &= BarWait(full0 + stage * 8, parity, ctl);
+    float largest = good ? 0.f : __uint_as_float(0x7FFFFFFFu);
+    const int come = good ? own : 0;
     const T* const at = reinterpret_cast<const T*>(from + static_cast<uint32_t>(stage) * stage_bytes);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (j < own) {
+      if (j < come) {
         const Piece<T, C> a = Load<T, C>(at + j * step);
         Values<KIND, T, C>(f[j], a, kTwo ? Load<T, C>(at + j * step + stage_bytes / 2 / sizeof(T)) : a, p, weight, KIND >= kNorm ? &w[j] : nullptr, first + j * step, hr + j * step,
                            squares, largest);
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp, parts[turn]);
     const long long next = row + static_cast<long long>(p.stages) * gridDim.x;
-    if (threadIdx.x == 0 && next < p.rows) fetch(next, stage);
+    if (threadIdx.x == 0 && good && next < p.rows) fetch(next, stage);  // what was there has come, and all have read it
     const Scaling s = ScalingOf<KIND>(r, p);
     TakeUp<KIND, C, V>(f, s.first);
     if (!s.bad) {
@@ -499,6 +504,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
       parity ^= 1u;
     }
   }
+  for (int i = 0; i < 16 && !good; ++i) __nanosleep(1000000);  // copies may still be landing in what the block leaves
 }
 
 // ------------------------------------------------------------------------------ host
@@ -626,6 +632,7 @@ cudaError_t LaunchRowQuant(const RowQuantCall& c, cudaStream_t stream) {
   p.weight_f32 = c.weight_dtype == QFG_FLOAT;
   p.fp8 = c.fp8;
   p.trigger = c.trigger;
+  p.give_up = c.give_up;
   p.rows = c.rows;
   p.n = static_cast<int>(c.n);
   p.offset = c.weight_offset;

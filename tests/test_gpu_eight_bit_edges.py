@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from qwen38_flash_ops_b200 import RmsNormQuant, RowQuant
+from qwen38_flash_ops_b200 import RmsNormQuant, RowQuant, _lib
 
 pytestmark = pytest.mark.gpu
 _TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
@@ -110,3 +110,47 @@ def test_scales_are_quotients(cuda, q_dtype, rows, n):
     _, scale = RowQuant(dtype=q_dtype)(x)
     want = x.abs().amax(-1).cpu().numpy() / np.float32(_TOP[q_dtype])
     assert np.array_equal(scale.cpu().numpy(), want)
+
+
+# ---- waits that run out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["rows", "gated", "norm", "added"])
+@pytest.mark.parametrize("rows,n", [(400, 512), (1000, 640), (400, 5120), (3000, 2560), (300, 17408)])
+def test_rows_that_never_come(cuda, dtype, kind, rows, n):
+    """Every row of such a call is marked, the residual stream stays as it was, and the next call is whole."""
+    if 2 * n * dtype.itemsize * (2 if kind in ("gated", "added") else 1) > 210 * 1024:
+        pytest.skip("two rows do not fit the ring: they go straight into registers")
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x, second = _rows(gen, rows, n).to(dtype), _rows(gen, rows, n).to(dtype)
+    weight, lib = torch.ones(n, device="cuda").to(dtype), _lib.load()
+
+    def call(h):
+        q, scale = torch.full((rows, n), 7, dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda")
+        if kind in ("rows", "gated"):
+            return RowQuant()(x, second if kind == "gated" else None, out=(q, scale))
+        return RmsNormQuant()(x, weight, h if kind == "added" else None, out=(q, scale, h) if kind == "added" else (q, scale))
+
+    want = call(second.clone())
+    assert torch.isfinite(want[1]).all()
+    stream = second.clone()
+    assert lib.qfg_row_quant_set_option(b"give_up", b"1") == _lib.QFG_OK
+    try:
+        got = call(stream)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.qfg_row_quant_set_option(b"give_up", b"0") == _lib.QFG_OK
+    assert torch.isnan(got[1]).all() and (got[0] == 0).all() and torch.equal(stream, second)
+    again = call(stream)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_only_rows_of_the_ring_wait(cuda):
+    x, lib = torch.ones(4, 512, device="cuda"), _lib.load()
+    assert lib.qfg_row_quant_set_option(b"give_up", b"1") == _lib.QFG_OK
+    try:
+        q, scale = RowQuant()(x)
+    finally:
+        assert lib.qfg_row_quant_set_option(b"give_up", b"0") == _lib.QFG_OK
+    assert (q == 127).all() and torch.isfinite(scale).all()
