@@ -685,7 +685,8 @@ bool Aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p
 bool EightBits(int dtype) { return dtype == QFG_INT8 || dtype == QFG_FLOAT8E4M3FN; }
 std::atomic<bool> g_rows_give_up{false};  // qfg_row_quant_set_option
 
-int RunRowQuant(const char* name, qfg::RowQuantCall& c, int q_dtype, void* stream) {
+// A call's arguments are checked apart from its launch, so that QuantMlp launches nothing of a call that is refused.
+int CheckRows(const char* name, qfg::RowQuantCall& c, int q_dtype) {
   const size_t elem = ElementBytes(c.dtype);
   if (elem == 0) return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": rows must be BF16/FP16/FP32");
   if (!EightBits(q_dtype)) return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": q must be INT8 or FP8 E4M3FN");
@@ -700,16 +701,20 @@ int RunRowQuant(const char* name, qfg::RowQuantCall& c, int q_dtype, void* strea
     return Fail(QFG_INVALID_ARGUMENT, std::string(name) + ": misaligned argument");
   c.fp8 = q_dtype == QFG_FLOAT8E4M3FN;
   c.give_up = g_rows_give_up.load(std::memory_order_relaxed);
+  return QFG_OK;
+}
+
+int LaunchRows(const char* name, const qfg::RowQuantCall& c, void* stream) {
   const cudaError_t err = qfg::LaunchRowQuant(c, static_cast<cudaStream_t>(stream));
   return err == cudaSuccess ? QFG_OK : Fail(QFG_FAIL, std::string(name) + ": " + cudaGetErrorString(err));
 }
 
-int RunNorm(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype, float weight_offset, float eps,
-            int64_t rows, int64_t n, int q_dtype, void* q, float* scale, void* h, bool trigger, void* stream) {
+int NormCall(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype, float weight_offset, float eps,
+             int64_t rows, int64_t n, int q_dtype, void* q, float* scale, void* h, qfg::RowQuantCall* out) {
   if (weight_dtype != dtype && weight_dtype != QFG_FLOAT)
     return Fail(QFG_INVALID_ARGUMENT, "RmsNormQuant: the weight must have the type of x, or FP32");
   if (!(eps >= 0.f)) return Fail(QFG_INVALID_ARGUMENT, "RmsNormQuant: eps must not be negative");
-  qfg::RowQuantCall c;
+  qfg::RowQuantCall& c = *out;
   c.norm = true;
   c.dtype = dtype;
   c.x = x;
@@ -725,13 +730,12 @@ int RunNorm(int dtype, const void* x, int64_t ldx, const void* residual, int64_t
   c.q = static_cast<uint8_t*>(q);
   c.scale = scale;
   c.h = residual != nullptr ? h : nullptr;
-  c.trigger = trigger;
-  return RunRowQuant("RmsNormQuant", c, q_dtype, stream);
+  return CheckRows("RmsNormQuant", c, q_dtype);
 }
 
-int RunAct(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q, float* scale, bool trigger,
-           void* stream) {
-  qfg::RowQuantCall c;
+int ActCall(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q, float* scale,
+            qfg::RowQuantCall* out) {
+  qfg::RowQuantCall& c = *out;
   c.dtype = dtype;
   c.x = x;
   c.ldx = ldx;
@@ -741,20 +745,23 @@ int RunAct(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, in
   c.n = n;
   c.q = static_cast<uint8_t*>(q);
   c.scale = scale;
-  c.trigger = trigger;
-  return RunRowQuant("RowQuant", c, q_dtype, stream);
+  return CheckRows("RowQuant", c, q_dtype);
 }
 
 }  // namespace
 
 int qfg_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype,
                       float weight_offset, float eps, int64_t rows, int64_t n, int q_dtype, void* q, float* scale, void* h, void* stream) {
-  return RunNorm(dtype, x, ldx, residual, ldr, weight, weight_dtype, weight_offset, eps, rows, n, q_dtype, q, scale, h, false, stream);
+  qfg::RowQuantCall c;
+  const int code = NormCall(dtype, x, ldx, residual, ldr, weight, weight_dtype, weight_offset, eps, rows, n, q_dtype, q, scale, h, &c);
+  return code != QFG_OK ? code : LaunchRows("RmsNormQuant", c, stream);
 }
 
 int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows, int64_t n, int q_dtype, void* q, float* scale,
                   void* stream) {
-  return RunAct(dtype, x, ldx, u, ldu, rows, n, q_dtype, q, scale, false, stream);
+  qfg::RowQuantCall c;
+  const int code = ActCall(dtype, x, ldx, u, ldu, rows, n, q_dtype, q, scale, &c);
+  return code != QFG_OK ? code : LaunchRows("RowQuant", c, stream);
 }
 
 int qfg_row_quant_set_option(const char* key, const char* value) {
@@ -788,8 +795,8 @@ int qfg_quant_gemm_create(const float* w_scale, size_t n_w_scale, int out_dtype,
 
 namespace {
 
-int RunQuantGemm(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx, const float* x_scale, int64_t m, int64_t k, const void* w, int64_t ldw,
-                 int order, int64_t n, void* out, int64_t ldo, bool early_weight, void* stream) {
+int GemmCall(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx, const float* x_scale, int64_t m, int64_t k, const void* w, int64_t ldw, int order,
+             int64_t n, void* out, int64_t ldo, bool early_weight, void* stream, qfg::QuantReady* ready) {
   if (op == nullptr) return Fail(QFG_INVALID_ARGUMENT, "QuantGemm: null node");
   try {
     if (!EightBits(dtype)) throw InvalidArgument("QuantGemm: x and the weight must be INT8 or FP8 E4M3FN");
@@ -798,7 +805,7 @@ int RunQuantGemm(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx
       throw InvalidArgument("QuantGemm: bad shape");
     if (dtype == QFG_INT8 && k > 131071) throw InvalidArgument("QuantGemm: K over 131071 can overflow a sum of INT8 products");
     if (op->w_scale_len != 0 && op->w_scale_len != static_cast<size_t>(n)) throw InvalidArgument("QuantGemm: w_scale must have one value per column");
-    if (m == 0) return QFG_OK;
+    if (m == 0) return QFG_OK;  // nothing is put in *ready
     if (x == nullptr || x_scale == nullptr || w == nullptr || out == nullptr) throw InvalidArgument("QuantGemm: null argument");
     if (!Aligned(x_scale, 4) || !Aligned(out, ElementBytes(op->out_dtype))) throw InvalidArgument("QuantGemm: misaligned argument");
     int device = -1;
@@ -822,7 +829,7 @@ int RunQuantGemm(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx
     c.early_weight = early_weight;
     c.give_up = op->give_up;
     const qfg::QuantPlan plan = op->plan.bm > 0 ? op->plan : qfg::ChooseQuantPlan(c);
-    if (!qfg::LaunchQuantGemm(c, plan, static_cast<cudaStream_t>(stream))) throw std::runtime_error("QuantGemm: a tensor map could not be made");
+    if (!qfg::PrepareQuantGemm(c, plan, static_cast<cudaStream_t>(stream), ready)) throw std::runtime_error("QuantGemm: a tensor map could not be made");
     return QFG_OK;
   } catch (const InvalidArgument& e) {
     return Fail(QFG_INVALID_ARGUMENT, e.what());
@@ -831,11 +838,18 @@ int RunQuantGemm(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx
   }
 }
 
+int LaunchGemm(const qfg::QuantReady& ready, void* stream) {
+  const cudaError_t err = qfg::LaunchQuantGemm(ready, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? QFG_OK : Fail(QFG_FAIL, std::string("QuantGemm: ") + cudaGetErrorString(err));
+}
+
 }  // namespace
 
 int qfg_quant_gemm_compute(const qfg_quant_gemm* op, int dtype, const void* x, int64_t ldx, const float* x_scale, int64_t m, int64_t k, const void* w,
                            int64_t ldw, int order, int64_t n, void* out, int64_t ldo, void* stream) {
-  return RunQuantGemm(op, dtype, x, ldx, x_scale, m, k, w, ldw, order, n, out, ldo, false, stream);
+  qfg::QuantReady ready;
+  const int code = GemmCall(op, dtype, x, ldx, x_scale, m, k, w, ldw, order, n, out, ldo, false, stream, &ready);
+  return code != QFG_OK || m == 0 ? code : LaunchGemm(ready, stream);
 }
 
 namespace {
@@ -879,12 +893,20 @@ int qfg_quant_mlp(int dtype, const void* x, int64_t ldx, const void* residual, i
   const MlpParts at = MlpLayout(rows, hidden, width, elem);
   uint8_t* const base = static_cast<uint8_t*>(workspace);
   float *const s1 = reinterpret_cast<float*>(base + at.s1), *const s2 = reinterpret_cast<float*>(base + at.s2);
-  int code = RunNorm(dtype, x, ldx, residual, ldr, weight, weight_dtype, weight_offset, eps, rows, hidden, q_dtype, base, s1, h, true, stream);
+  // all four are checked before the first of them writes anything: h may be the residual stream itself
+  qfg::RowQuantCall norm, act;
+  qfg::QuantReady first, second;
+  int code = NormCall(dtype, x, ldx, residual, ldr, weight, weight_dtype, weight_offset, eps, rows, hidden, q_dtype, base, s1, h, &norm);
   if (code == QFG_OK)
-    code = RunQuantGemm(gate_up, q_dtype, base, hidden, s1, rows, hidden, w1, ldw1, order1, 2 * width, base + at.both, 2 * width, true, stream);
+    code = GemmCall(gate_up, q_dtype, base, hidden, s1, rows, hidden, w1, ldw1, order1, 2 * width, base + at.both, 2 * width, true, stream, &first);
   if (code == QFG_OK)
-    code = RunAct(gate_up->out_dtype, base + at.both, 2 * width, base + at.both + width * elem, 2 * width, rows, width, q_dtype, base + at.q2, s2, true, stream);
-  if (code == QFG_OK) code = RunQuantGemm(down, q_dtype, base + at.q2, width, s2, rows, width, w2, ldw2, order2, hidden, y, hidden, true, stream);
+    code = ActCall(gate_up->out_dtype, base + at.both, 2 * width, base + at.both + width * elem, 2 * width, rows, width, q_dtype, base + at.q2, s2, &act);
+  if (code == QFG_OK) code = GemmCall(down, q_dtype, base + at.q2, width, s2, rows, width, w2, ldw2, order2, hidden, y, hidden, true, stream, &second);
+  norm.trigger = act.trigger = true;
+  if (code == QFG_OK) code = LaunchRows("RmsNormQuant", norm, stream);
+  if (code == QFG_OK) code = LaunchGemm(first, stream);
+  if (code == QFG_OK) code = LaunchRows("RowQuant", act, stream);
+  if (code == QFG_OK) code = LaunchGemm(second, stream);
   return code;
 }
 

@@ -323,9 +323,13 @@ struct QuantPlan {
 };
 cudaError_t ConfigureQuantKernels();  // on the current device
 QuantPlan ChooseQuantPlan(const QuantCall& call);  // throws std::runtime_error
-// false, nothing launched: a tensor map that could not be made.  Throws std::runtime_error (a launch shape that does not exist, a
-// launch that failed).
-bool LaunchQuantGemm(const QuantCall& call, const QuantPlan& plan, cudaStream_t stream);
+// A call that only needs to be launched; what it holds is quant_gemm.cu's.
+struct alignas(64) QuantReady {
+  unsigned char room[576];
+};
+// false: a tensor map that could not be made.  Throws std::runtime_error (a launch shape that does not exist).  `stream` is the one that it is launched on.
+bool PrepareQuantGemm(const QuantCall& call, const QuantPlan& plan, cudaStream_t stream, QuantReady* ready);
+cudaError_t LaunchQuantGemm(const QuantReady& ready, cudaStream_t stream);
 
 // row_quant.cu
 struct RowQuantCall {

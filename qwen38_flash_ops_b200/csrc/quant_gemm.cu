@@ -30,6 +30,7 @@
 #include <climits>
 #include <map>
 #include <mutex>
+#include <new>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -860,7 +861,16 @@ QuantPlan ChooseQuantPlan(const QuantCall& c) {
   return best;
 }
 
-bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t stream) {
+struct Ready {
+  QuantParams p;
+  cudaError_t (*launch)(const QuantParams&, int ctas, int cluster, size_t smem, bool overlap, cudaStream_t);
+  int ctas, cluster;
+  size_t smem;
+  bool overlap;
+};
+static_assert(sizeof(Ready) <= sizeof(QuantReady) && alignof(Ready) <= alignof(QuantReady) && std::is_trivially_copyable_v<Ready>, "");
+
+bool PrepareQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t stream, QuantReady* out) {
   QuantPlan plan = asked;
   const QuantSetup* setup = nullptr;
   cudaError_t err = SetUpQuant(&setup);
@@ -870,7 +880,8 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t st
       (plan.pair && (plan.split != 1 || plan.bm % 32 != 0 || plan.per_sm != 1 || loads)))
     throw std::runtime_error("QuantGemm: bad launch shape");
   if (loads) plan.per_sm = 1;  // the registers of its warps, and the second ring
-  QuantParams p = {};
+  Ready& ready = *new (out) Ready();
+  QuantParams& p = ready.p;
   p.x = c.x;
   p.w = c.w;
   p.ldx = c.ldx;
@@ -889,8 +900,8 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t st
   p.N = static_cast<int>(c.n);
   p.K = static_cast<int>(c.k);
   p.give_up = c.give_up;
-  const bool overlap = MayOverlapPredecessor(stream);
-  p.early_weight = c.early_weight && overlap;  // all weights ahead of all rows of x cost 0.8 us where there is nothing to wait for
+  ready.overlap = MayOverlapPredecessor(stream);
+  p.early_weight = c.early_weight && ready.overlap;  // all weights ahead of all rows of x cost 0.8 us where there is nothing to wait for
   p.x_loads = x_loads;
   p.w_loads = w_loads;
   p.bm = plan.bm;
@@ -919,26 +930,25 @@ bool LaunchQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t st
   size_t smem = static_cast<size_t>(1024 + p.raw_at + p.raw_stages * raw_stage);
   if (split) smem = std::max(smem, static_cast<size_t>(1024 + p.bm * kTileN * 4));
   if (p.stages < 2 || smem > static_cast<size_t>(SmemLimit(1))) throw std::runtime_error("QuantGemm: bad launch shape");
-  const int ctas = walkers * cluster;
-  if (plan.pair) {
-    err = c.fp8 ? LaunchAs<true, true, false, false>(p, ctas, 2, smem, overlap, stream)
-                : LaunchAs<false, true, false, false>(p, ctas, 2, smem, overlap, stream);
-  } else if (split && loads) {
-    err = c.fp8 ? LaunchAs<true, false, true, true>(p, ctas, cluster, smem, overlap, stream)
-                : LaunchAs<false, false, true, true>(p, ctas, cluster, smem, overlap, stream);
-  } else if (split) {
-    err = c.fp8 ? LaunchAs<true, false, true, false>(p, ctas, cluster, smem, overlap, stream)
-                : LaunchAs<false, false, true, false>(p, ctas, cluster, smem, overlap, stream);
-  } else if (loads) {
-    err = c.fp8 ? LaunchAs<true, false, false, true>(p, ctas, 1, smem, overlap, stream)
-                : LaunchAs<false, false, false, true>(p, ctas, 1, smem, overlap, stream);
-  } else {
-    err = c.fp8 ? LaunchAs<true, false, false, false>(p, ctas, 1, smem, overlap, stream)
-                : LaunchAs<false, false, false, false>(p, ctas, 1, smem, overlap, stream);
-  }
-  if (err == cudaSuccess) err = cudaGetLastError();
-  if (err != cudaSuccess) throw std::runtime_error(std::string("QuantGemm: ") + cudaGetErrorString(err));
+  ready.ctas = walkers * cluster;
+  ready.cluster = cluster;
+  ready.smem = smem;
+  auto pick = [&](auto fp8) {
+    constexpr bool FP8 = decltype(fp8)::value;
+    return plan.pair       ? LaunchAs<FP8, true, false, false>
+           : split && loads ? LaunchAs<FP8, false, true, true>
+           : split          ? LaunchAs<FP8, false, true, false>
+           : loads          ? LaunchAs<FP8, false, false, true>
+                            : LaunchAs<FP8, false, false, false>;
+  };
+  ready.launch = c.fp8 ? pick(std::true_type()) : pick(std::false_type());
   return true;
+}
+
+cudaError_t LaunchQuantGemm(const QuantReady& prepared, cudaStream_t stream) {
+  const Ready& ready = reinterpret_cast<const Ready&>(prepared);
+  const cudaError_t err = ready.launch(ready.p, ready.ctas, ready.cluster, ready.smem, ready.overlap, stream), last = cudaGetLastError();
+  return err == cudaSuccess ? last : err;
 }
 
 }  // namespace qfg
