@@ -39,6 +39,7 @@
 #include "stream_order.cuh"
 #include "tc_ptx.cuh"
 #include "tensor_map.h"
+#include "tile_walk.h"
 
 namespace qfg {
 namespace {
@@ -65,7 +66,8 @@ struct QuantParams {
   const float *x_scale, *w_scale;
   void* out;
   long long ldo;
-  int M, N, K, ksteps, bm, m_tiles, n_tiles, group, tiles, stages, sets, raw_stages;
+  int M, N, K, ksteps, bm, tiles, stages, sets, raw_stages;
+  TileGrid grid;
   int order_k;           // the weight is stored [n][k]
   int x_loads, w_loads;  // LOADERS: which operands do not come by tensor copies
   int raw_at;            // where the rows of those are copied to, behind everything else
@@ -117,15 +119,11 @@ __device__ __forceinline__ uint32_t Pack(float lo, float hi) {
 __device__ __forceinline__ void ClusterArrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void ClusterWait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-struct At {
-  int n0, m0;
-};
-// Tiles go down `group` row blocks, then on to the next column block, and through all of these before the next group: the tiles of a wave then share
-// about as many rows of x as columns of w in L2.
+// A pair shares a tile of twice the columns, and its second CTA has the upper half.
 template <bool PAIR>
 __device__ __forceinline__ At Locate(const QuantParams& p, int tile, int rank) {
-  const int g = tile / (p.group * p.n_tiles), rest = tile - g * p.group * p.n_tiles, rows = min(p.group, p.m_tiles - g * p.group), nt = rest / rows;
-  return {nt * (PAIR ? 2 * kTileN : kTileN) + (PAIR ? rank * kTileN : 0), (g * p.group + rest - nt * rows) * p.bm};
+  const At t = p.grid.Locate(tile);
+  return {t.n0 + (PAIR ? rank * kTileN : 0), t.m0};
 }
 
 // ------------------------------------------------------------------------------ operands off 16 bytes
@@ -334,29 +332,19 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
   const int my_rows = max(0, min(share, tile_rows - rank * share));
 
   // The copying warp makes the barriers itself, so that its first copies are on their way while the other warps set up.
-  int c_tile = first_tile, c_k = 0, c_stage = 0, c_round = 0;
-  At c_at = Locate<PAIR>(p, first_tile, rank);
+  StageWalk at(p.grid, first_tile);
   const uint32_t mine = static_cast<uint32_t>((load_w ? kWBytes : 0) + (load_x ? xrows * kTileK : 0));
   auto copy_stage = [&](bool w, bool x) {
-    const At t = c_at;
-    const uint32_t bar = PAIR ? MapRank(full0 + c_stage * 8, 0) : full0 + c_stage * 8;
-    const uint32_t dst = smem + static_cast<uint32_t>(c_stage) * stage_bytes;
-    const int k0 = (kbeg + c_k) * kTileK;
+    const uint32_t bar = PAIR ? MapRank(full0 + at.stage * 8, 0) : full0 + at.stage * 8;
+    const uint32_t dst = smem + static_cast<uint32_t>(at.stage) * stage_bytes;
+    const int k0 = (kbeg + at.k) * kTileK, n0 = at.at.n0 + (PAIR ? rank * kTileN : 0);
     if (ElectOne()) {
-      if (w && (rank == 0 || !PAIR)) BarExpect(full0 + c_stage * 8, PAIR ? 2 * mine : mine);
-      if (w && load_w) TmaLoad<PAIR>(dst, &p.wmap, p.order_k ? k0 : t.n0, p.order_k ? t.n0 : k0, bar);
-      if (x && load_x) TmaLoad<PAIR>(dst + kWBytes, &p.xmap, k0, t.m0 + (PAIR ? rank * xrows : 0), bar);
+      if (w && (rank == 0 || !PAIR)) BarExpect(full0 + at.stage * 8, PAIR ? 2 * mine : mine);
+      if (w && load_w) TmaLoad<PAIR>(dst, &p.wmap, p.order_k ? k0 : n0, p.order_k ? n0 : k0, bar);
+      if (x && load_x) TmaLoad<PAIR>(dst + kWBytes, &p.xmap, k0, at.at.m0 + (PAIR ? rank * xrows : 0), bar);
     }
     __syncwarp();
-    if (++c_stage == p.stages) {
-      c_stage = 0;
-      ++c_round;
-    }
-    if (++c_k == kcount) {
-      c_k = 0;
-      c_tile += tile_step;
-      c_at = Locate<PAIR>(p, c_tile, rank);
-    }
+    at.Next(p.grid, p.tiles, tile_step, kcount, p.stages);
   };
   const bool copies = p.give_up == 0 && (load_w || load_x), early = !PAIR && !LOADERS && p.early_weight != 0 && copies;
   if (warp == 4) {
@@ -398,9 +386,8 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
   } else {  // this warp waits for nothing that the others set up, only they for its barriers
     asm volatile("bar.arrive 1, %0;" ::"n"(kThreads<PAIR, LOADERS>) : "memory");
     if (early) {  // a stage is full when its rows of x have come as well
-      while (c_tile < p.tiles && c_round == 0) copy_stage(true, false);
-      c_tile = first_tile, c_k = 0, c_stage = 0, c_round = 0;
-      c_at = Locate<PAIR>(p, first_tile, rank);
+      while (at.tile < p.tiles && at.round == 0) copy_stage(true, false);
+      at = StageWalk(p.grid, first_tile);
     }
     GridDependencyWait();
   }
@@ -537,8 +524,8 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
     }
   } else if (warp == 4) {
     // ---- tensor copies
-    while (copies && c_tile < p.tiles && (c_round == 0 || BarWait(empty0 + c_stage * 8, static_cast<uint32_t>((c_round - 1) & 1), ctl)))
-      copy_stage(!early || c_round > 0, true);
+    while (copies && at.tile < p.tiles && (at.round == 0 || BarWait(empty0 + at.stage * 8, static_cast<uint32_t>((at.round - 1) & 1), ctl)))
+      copy_stage(!early || at.round > 0, true);
   } else if (warp == 5) {
     // ---- MMAs (the leader's, for both CTAs of a pair)
     if (!PAIR || rank == 0) {
@@ -906,13 +893,12 @@ bool PrepareQuantGemm(const QuantCall& c, const QuantPlan& asked, cudaStream_t s
   p.w_loads = w_loads;
   p.bm = plan.bm;
   p.ksteps = static_cast<int>((c.k + kTileK - 1) / kTileK);
-  p.m_tiles = static_cast<int>((c.m + p.bm - 1) / p.bm);
+  const int m_tiles = static_cast<int>((c.m + p.bm - 1) / p.bm);
   const int width = plan.pair ? 2 * kTileN : kTileN;
-  const int64_t tiles = (c.n + width - 1) / width * p.m_tiles;
+  const int64_t tiles = (c.n + width - 1) / width * m_tiles;
   if (tiles > INT_MAX / 16) throw std::runtime_error("QuantGemm: too many tiles");
   p.tiles = static_cast<int>(tiles);
-  p.n_tiles = p.tiles / p.m_tiles;
-  p.group = std::min(p.m_tiles, kGroup);
+  p.grid = {m_tiles, p.tiles / m_tiles, std::min(m_tiles, kGroup), p.bm, width};
   const int cluster = plan.pair ? 2 : std::min(plan.split, p.ksteps);
   const int xrows = plan.pair ? p.bm / 2 : p.bm, stage = kWBytes + xrows * kTileK;
   if (!x_loads && !EncodeRows(&p.xmap, c.x, c.m, c.k, c.ldx, xrows)) return false;
