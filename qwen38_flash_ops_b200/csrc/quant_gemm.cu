@@ -837,9 +837,11 @@ QuantPlan ChooseQuantPlan(const QuantCall& c) {
       best = plan;
     }
   };
-  for (int64_t mt = least; mt <= 2 * least + 2 && mt <= c.m; ++mt) {
+  // from the tallest tiles on, each height once: the next is that of the first count of row tiles that allows a lower one
+  for (int64_t mt = least; mt <= 2 * least + 2 && mt <= c.m;) {
     QuantPlan plan;
     plan.bm = static_cast<int>(((c.m + mt - 1) / mt + 15) / 16 * 16);
+    mt = plan.bm > 16 ? (c.m + plan.bm - 17) / (plan.bm - 16) : c.m + 1;
     for (plan.per_sm = 1; plan.per_sm <= (loads ? 1 : 2); ++plan.per_sm) {
       for (plan.split = 1; plan.split <= std::min<int64_t>(kMaxSplit, blocks); ++plan.split) consider(plan);
     }
