@@ -344,6 +344,8 @@ bool Order(const at::Tensor& w, int* order, int64_t* ld) {
   return true;
 }
 
+at::ScalarType Type(long out_dtype) { return out_dtype == QFG_BFLOAT16 ? at::kBFloat16 : out_dtype == QFG_FLOAT16 ? at::kHalf : at::kFloat; }
+
 // quant_gemm(handle, output type, x, x_scale, w) -> out
 PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return Guard([&]() -> PyObject* {
@@ -361,7 +363,7 @@ PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!Order(*w, &order, &ldw)) return None();
     c10::SmallVector<int64_t, 6> shape(x.t->sizes().begin(), x.t->sizes().end());
     shape.back() = n;
-    const at::Tensor out = New(shape, out_dtype == QFG_BFLOAT16 ? at::kBFloat16 : out_dtype == QFG_FLOAT16 ? at::kHalf : at::kFloat);
+    const at::Tensor out = New(shape, Type(out_dtype));
     const int dtype = Code(x.t->scalar_type());
     const void *xp = x.t->data_ptr(), *wp = w->data_ptr();
     const float* const sp = xs->data_ptr<float>();
@@ -372,12 +374,13 @@ PyObject* QuantGemm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
-// quant_mlp(eps, weight_offset, norm weight, gate and up's handle, its weight, down's handle, its weight, x, residual) -> (y, h); both products to BF16.
+// quant_mlp(eps, weight_offset, norm weight, gate and up's handle, its weight, down's handle, its weight, output type of both, x, residual) -> (y, h)
 PyObject* QuantMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return Guard([&]() -> PyObject* {
     Rows x, r;
-    if (n_args != 9 || !PyFloat_CheckExact(a[0]) || !PyFloat_CheckExact(a[1]) || !ToRows(a[7], &x) || !ToRows(a[8], &r)) return None();
+    if (n_args != 10 || !PyFloat_CheckExact(a[0]) || !PyFloat_CheckExact(a[1]) || !ToRows(a[8], &x) || !ToRows(a[9], &r)) return None();
     const void *up = PyLong_AsVoidPtr(a[3]), *down = PyLong_AsVoidPtr(a[5]);
+    const at::ScalarType out_type = Type(PyLong_AsLong(a[7]));
     const at::Tensor *g = Dense(a[2]), *w1 = Plain(a[4]), *w2 = Plain(a[6]);
     if (PyErr_Occurred() || up == nullptr || down == nullptr || g == nullptr || w1 == nullptr || w2 == nullptr || !Float(*x.t) ||
         r.t->scalar_type() != x.t->scalar_type() || r.t->sizes() != x.t->sizes() || x.rows < 1 ||
@@ -392,7 +395,7 @@ PyObject* QuantMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t width = w2->size(0);
     const size_t bytes = g_lib.quant_mlp_workspace_bytes(up_op, x.rows, x.n, width);
     if (bytes == 0) return None();
-    const at::Tensor workspace = New({static_cast<int64_t>(bytes)}, at::kByte), y = New(x.t->sizes(), at::kBFloat16), h = New(x.t->sizes(), x.t->scalar_type());
+    const at::Tensor workspace = New({static_cast<int64_t>(bytes)}, at::kByte), y = New(x.t->sizes(), out_type), h = New(x.t->sizes(), x.t->scalar_type());
     const int dtype = Code(x.t->scalar_type()), g_type = Code(g->scalar_type()), type = Code(w1->scalar_type());
     const float eps = static_cast<float>(PyFloat_AS_DOUBLE(a[0])), offset = static_cast<float>(PyFloat_AS_DOUBLE(a[1]));
     const void *xp = x.t->data_ptr(), *rp = r.t->data_ptr(), *gp = g->data_ptr(), *w1p = w1->data_ptr(), *w2p = w2->data_ptr();

@@ -20,21 +20,26 @@ class QuantMlp:
     torch.float8_e4m3fn, either dimension contiguous, with a scale per column.  Between the products the rows are quantised to the
     same type.  The four calls follow one another on the current stream and allocate their outputs as torch does.
 
+    x and residual are BF16, FP16 or FP32, and h is of their type.  `out_dtype` (BF16 unless given, FP16 or FP32) is the type of y, and of gate and up
+    between the products.
+
     Work that other threads put on that stream during a call must not write the weights: a product may fetch its first ones before the calls
     ahead of it have ended."""
 
-    def __init__(self, norm_weight, gate_up, gate_up_scale, down, down_scale, eps: float = 1e-6, weight_offset: float = 0.0):
+    def __init__(self, norm_weight, gate_up, gate_up_scale, down, down_scale, eps: float = 1e-6, weight_offset: float = 0.0,
+                 out_dtype: torch.dtype = torch.bfloat16):
         if gate_up.dtype != down.dtype or gate_up.shape[1] != 2 * down.shape[0] or gate_up.shape[0] != down.shape[1]:
             raise ValueError("QuantMlp: gate_up is [hidden, 2 * width] and down [width, hidden], of one type")
         self.width = down.shape[0]
         self.norm_weight, self.gate_up, self.down = norm_weight, gate_up, down
         self._norm = RmsNormQuant(eps=eps, weight_offset=weight_offset, dtype=gate_up.dtype)
         self._act = RowQuant(dtype=gate_up.dtype)
-        self._gate_up = QuantGemm(w_scale=gate_up_scale)
-        self._down = QuantGemm(w_scale=down_scale)
+        self._gate_up = QuantGemm(w_scale=gate_up_scale, out_dtype=out_dtype)
+        self._down = QuantGemm(w_scale=down_scale, out_dtype=out_dtype)
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor):
-        r = ops._calls.quant_mlp(self._norm.eps, self._norm.weight_offset, self.norm_weight, self._gate_up._p, self.gate_up, self._down._p, self.down, x, residual)
+        r = ops._calls.quant_mlp(self._norm.eps, self._norm.weight_offset, self.norm_weight, self._gate_up._p, self.gate_up, self._down._p, self.down,
+                                 self._down._code, x, residual)
         if r is not None:
             return r if r.__class__ is tuple else check(r)
         q, scale, h = self._norm(x, self.norm_weight, residual)

@@ -1,8 +1,8 @@
-"""QuantMlp: what a refused call leaves behind."""
+"""QuantMlp: its types, and what a refused call leaves behind."""
 import pytest
 import torch
 
-from qwen38_flash_ops_b200 import QuantGemm, _lib
+from qwen38_flash_ops_b200 import QfgError, QuantGemm, QuantMlp, RmsNormQuant, RowQuant, _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,43 @@ def test_a_refused_block_writes_nothing(cuda, change):
     assert lib.qfg_quant_mlp(*a.values()) != _lib.QFG_OK
     torch.cuda.synchronize()
     assert torch.equal(stream, before) and (y == 7.0).all() and torch.equal(workspace, kept)
+
+
+@pytest.mark.parametrize("eight", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,hidden,width", [(1, 256, 512), (7, 640, 264), (300, 512, 384), (5, 129, 77)])
+def test_types(cuda, monkeypatch, eight, dtype, out_dtype, rows, hidden, width):
+    """Rows and outputs of every type, against the four calls, and against the definition with the bounds of test_mlp: what eight bits move."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + hidden)
+    rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    top = 127.0 if eight == torch.int8 else 448.0
+
+    def quantised(k, n):
+        w = rand(k, n) * 0.05
+        s = w.abs().amax(0) / top
+        q = w / s
+        return (q.round() if eight == torch.int8 else q).to(eight), s
+
+    (q1, s1), (q2, s2) = quantised(hidden, 2 * width), quantised(width, hidden)
+    g, x, r = (1 + 0.2 * rand(hidden)).to(dtype), rand(rows, hidden).to(dtype), rand(rows, hidden).to(dtype)
+    mlp = QuantMlp(g, q1, s1.cpu().numpy(), q2, s2.cpu().numpy(), out_dtype=out_dtype)
+    y, h = mlp(x, r)
+    assert y.dtype == out_dtype and h.dtype == dtype and y.shape == h.shape == x.shape
+    q, scale, h4 = RmsNormQuant(dtype=eight)(x, g, r)
+    both = QuantGemm(w_scale=s1.cpu().numpy(), out_dtype=out_dtype)(q, scale, q1)
+    q, scale = RowQuant(dtype=eight)(both[:, :width], both[:, width:])
+    assert torch.equal(y, QuantGemm(w_scale=s2.cpu().numpy(), out_dtype=out_dtype)(q, scale, q2)) and torch.equal(h, h4)
+    d = (x + r).double()
+    both = d / torch.sqrt((d * d).mean(-1, keepdim=True) + 1e-6) * g.double() @ (q1.double() * s1.double())
+    a, b = both[:, :width], both[:, width:]
+    want = (a * torch.sigmoid(a) * b) @ (q2.double() * s2.double())
+    assert ((y.double() - want).norm() / want.norm()).item() < (0.03 if eight == torch.int8 else 0.12)
+    monkeypatch.setattr(ops._calls, "quant_mlp", lambda *args: None)  # the way through Python
+    assert all(torch.equal(a, b) for a, b in zip(mlp(x, r), (y, h)))
+
+
+def test_the_type_of_outputs_is_checked(cuda):
+    w1, w2 = torch.zeros(64, 96, dtype=torch.int8, device="cuda"), torch.zeros(48, 64, dtype=torch.int8, device="cuda")
+    with pytest.raises(QfgError, match="out_dtype"):
+        QuantMlp(torch.ones(64, device="cuda"), w1, None, w2, None, out_dtype=torch.int8)
