@@ -1130,11 +1130,12 @@ __global__ void __launch_bounds__(SharedThreads<MODE>(), 1) DenseSharedKernel(co
   }
   // nothing of the call is read or written before this line: a predecessor may be writing any of it
   GridDependencyWait();
-  if (q.trigger == 1) GridLaunchDependents();
   constexpr int kFirstSwish = kFirstDqWarp + (MODE == kBf16 ? 0 : kDqWarps), kSumGroups = (kFirstSwish + kSwishWarps) / 4;
   SwishRole swish(q, warp - kFirstSwish, lane, rank, t.m0);  // its first rows are on their way while the CTAs meet
   FenceBefore();
   __syncthreads();
+  // Only now that this CTA has its tensor memory: a dependent takes its own before it waits for the end of this kernel, and must not take it from under it.
+  if (q.trigger == 1) GridLaunchDependents();
   if (C > 1) cg::this_cluster().sync();  // every CTA's barriers exist
   FenceAfter();
   const uint32_t tmem = ctl.tmem;

@@ -4,7 +4,8 @@ import pytest
 import torch
 from test_gpu_stream_order import _Early, _rand
 
-from qwen38_flash_ops_b200 import QuantGemm, QuantMlp, RmsNormQuant, RowQuant
+from qwen38_flash_ops_b200 import QuantGemm, QuantMlp, RmsNormQuant, RowQuant, SharedExpertDown
+from qwen38_flash_ops_b200 import workloads as W
 
 pytestmark = pytest.mark.gpu
 ROWS = 400  # of the buffer, [ROWS, 2560] BF16: many enough for the ring of the row kernels; the predecessor writes rows 32 to 39
@@ -135,3 +136,29 @@ def test_calls_in_a_row(cuda, rows, hidden, width):
     torch.cuda.synchronize()
     for a, b in zip(alone * 3, got):
         assert all(torch.equal(_bits(p), _bits(q)) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_products_that_a_shared_expert_lets_in(cuda, mode):
+    """A many-row kernel that takes tensor memory and releases its dependents early, products that take theirs before they wait for it, and more of them on a
+    second stream."""
+    K, N, rows = 1024, 1024, 600
+    shared, gemm = SharedExpertDown(trigger=1), QuantGemm(out_dtype=torch.float32)
+    w, gs, u = W.make_weight(mode, K, N, 7)[0], [_rand(60 + i, rows, K) for i in range(2)], _rand(63, rows, K)
+    gx, gw, routed = _rand(64, rows, 256), _rand(65, 256, 1) * 0.02, _rand(66, rows, N)
+    w8, ones, other = _ints(67, 2 * N, 1024), torch.ones(rows, device="cuda"), _ints(68, rows, 2 * N)
+    step = lambda i: gemm(shared(gs[i % 2], u, w, gx, gw, routed).view(torch.int8), ones, w8)
+    alone = []
+    for i in range(2):
+        alone.append(step(i).clone())
+        torch.cuda.synchronize()
+    beside = gemm(other, ones, w8).clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got, more = [], []
+    for i in range(24):
+        got.append(step(i))
+        with torch.cuda.stream(side):
+            more.append(gemm(other, ones, w8))
+    torch.cuda.synchronize()
+    assert all(torch.equal(_bits(g), _bits(alone[i % 2])) for i, g in enumerate(got)) and all(torch.equal(m, beside) for m in more)
