@@ -331,8 +331,9 @@ QFG_API int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, 
 QFG_API int qfg_row_quant_set_option(const char* key, const char* value);
 
 /* QuantGemm: out[m, n] = (sum_k x[m, k] w[k, n]) * x_scale[m] * w_scale[n].  INT8 products are summed in 32-bit integers, which is
- * exact (k <= 131071 of them cannot overflow), E4M3 products in FP32; the sum is scaled in FP32 and rounded once to `out_dtype`
- * (BFLOAT16, FLOAT16 or FLOAT).  `w_scale` (host floats, one per column, uploaded once here; NULL: ones).
+ * exact (k <= 131071 of them cannot overflow), E4M3 products in FP32 by the tensor core, which cuts the sum off to 24 bits, toward zero, at every 32 products:
+ * measured, sums of 17408 positive products come out 1.0e-5 too small (5120: 1.7e-6), signed ones are off by 7.5e-7 of their size (1.6e-7).  That is far below
+ * a 16-bit output's rounding; FLOAT outputs show it.  The sum is scaled in FP32 and rounded once to `out_dtype` (BFLOAT16, FLOAT16 or FLOAT).  `w_scale` (host floats, one per column, uploaded once here; NULL: ones).
  * `dtype` is that of x and of w, INT8 or FLOAT8E4M3FN; x_scale FP32 [m] on the device.  The weight is [k][n] with rows ldw apart (QFG_ORDER_N: its
  * columns lie beside one another) or [n][k] (QFG_ORDER_K).  m == 0 is a no-op.  Nothing is allocated and the call may be captured. */
 typedef enum qfg_order { QFG_ORDER_N = 0, QFG_ORDER_K = 1 } qfg_order;

@@ -445,7 +445,8 @@ class RowQuant:
 
 class QuantGemm:
     """out = (x @ w) * x_scale[:, None] * w_scale: eight-bit rows by an eight-bit weight, torch.int8 summed exactly in 32-bit
-    integers (K up to 131071), torch.float8_e4m3fn in FP32; the sum is scaled in FP32 and rounded once to `out_dtype`.
+    integers (K up to 131071), torch.float8_e4m3fn in FP32 by the tensor core (cut off, not rounded, at every 32 products: up to 1e-5
+    of a sum of 17408); the sum is scaled in FP32 and rounded once to `out_dtype`.
 
     Attributes: optional `w_scale` (a value per column), `out_dtype` (BF16, FP16 or FP32).  Inputs: x [..., K] and its row scales
     x_scale [...] (FP32), as RmsNormQuant and RowQuant return them; w [K, N] of the type of x, with either dimension
