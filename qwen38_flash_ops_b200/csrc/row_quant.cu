@@ -7,7 +7,7 @@
 //
 // All of it in FP32 until the one rounding to eight bits.  One pass over memory: the largest |h_i (offset + weight_i)| is found
 // beside the sum of squares, because the norm's factor is the same for the whole row, and leaves q_i altogether, so a row needs one reduction and its
-// values wait in registers.  Rows longer than the registers of a block hold (18432 values of 16 bits, 16384 that lie anywhere) are read again.  A row whose sum of
+// values wait in registers.  Rows longer than the registers of a block hold (18432 values, 19968 of many rows through the ring, 16384 that lie anywhere) are read again.  A row whose sum of
 // squares or largest value is no finite FP32 number has scale NaN and q 0.
 //
 // What bounds it, on one B200 (a copy's 6.55 TB/s is the floor).  Few rows: the launch, one trip to memory and the reduction, 2.4 us in a graph for 1 x 5120, 3.7 for 4 x 17408
@@ -346,6 +346,7 @@ __device__ __forceinline__ Scaling ScalingOf(const RowSums& r, const RowParams& 
 
 // Threads a block may have with so many elements of a row in each one's registers.
 constexpr int MostThreads(int elements) { return elements <= 16 ? 1024 : elements <= 24 ? 768 : elements <= 32 ? 576 : 416; }
+constexpr int kMostOfRow = 24 * MostThreads(24);  // of pieces of 16 bytes: the longest row in 24 elements a thread, and in 32
 
 // Rows straight into registers, V pieces of C elements a thread.  C > 1: pieces of 16 bytes; C = 1: rows that lie anywhere.  V = 0: rows
 // read twice.
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
 // holds its V pieces of a row as FP32 between the row's sums and its eight bits.  Nothing but the barrier of those sums says that a row
 // has left the ring: the block's first thread then asks for the row that takes its place.  The weight waits in registers, as it is stored.
 // Every wait is bounded.  A block that gives up on one marks the rows that it has left, as rows without a finite value are, and asks for no more.
-constexpr int kMaxRowStages = 8, kRingRoom = 210 * 1024, kRingMost = 210 * 1024, kRingBlocks = 8;
+constexpr int kMaxRowStages = 8, kRingRoom = 210 * 1024, kRingBlocks = 8;
 struct RowCtl {
   unsigned long long full[kMaxRowStages];
   volatile uint32_t fault;
@@ -539,7 +540,7 @@ cudaError_t LaunchRing(RowParams& p, int sms, cudaStream_t stream) {
   if (err == cudaSuccess && (device > 63 || !(raised.load(std::memory_order_acquire) >> device & 1))) {
     cudaFuncAttributes attr;
     err = cudaFuncGetAttributes(&attr, RowRingKernel<KIND, T, V>);
-    if (err == cudaSuccess) err = cudaFuncSetAttribute(RowRingKernel<KIND, T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(RowRingKernel<KIND, T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingRoom);
     if (err == cudaSuccess) {
       registers.store((attr.numRegs + 7) / 8 * 8, std::memory_order_relaxed);
       if (device <= 63) raised.fetch_or(1ull << device, std::memory_order_release);
@@ -571,34 +572,37 @@ cudaError_t LaunchShape(RowParams& p, cudaStream_t stream) {
   const bool few = p.rows <= 2 * sms;
   if constexpr (C > 1) {
     // Many rows of a kilobyte or more, two of which fit the ring.  24 elements a thread, 32 for a norm alone, whose reduction takes the longest for
-    // what it reads; longer rows more.  Rows of 5120, 4096 of them, 16 / 24 / 32 / 48 a thread, us: norm 19.5 / 18.9 / 16.3 / 17.3, with residual 24.3 / 24.4 /
-    // 24.3 / 27.0, gated 20.5 / 20.9 / 21.3 / 21.4.
-    if (!few && p.n * sizeof(T) >= 1024 && 2 * RingBytes<KIND, T>(p.n) <= kRingMost) {
-      for (int e : {KIND == kNorm ? 4 : 3, 4, 6}) {
-        if (WarpsOf(pieces, e * kOne) > MostThreads(C * e * kOne) / 32) continue;
-        if (e == 3) return LaunchRing<KIND, T, 3 * kOne>(p, sms, stream);
-        if (e == 4) return LaunchRing<KIND, T, 4 * kOne>(p, sms, stream);
-        return LaunchRing<KIND, T, 6 * kOne>(p, sms, stream);
+    // what it reads: rows of up to 18432 either way.  Longer rows 48, where two of them fit at all.  Rows of 5120, 4096 of them, 16 / 24 / 32 / 48 a thread, us: norm
+    // 19.5 / 18.9 / 16.3 / 17.3, with residual 24.3 / 24.4 / 24.3 / 27.0, gated 20.5 / 20.9 / 21.3 / 21.4.
+    constexpr int kElements = KIND == kNorm ? 32 : 24, kBytes = static_cast<int>(sizeof(T)) * (KIND == kSwish || KIND == kNormAdd ? 2 : 1);
+    static_assert(kElements * MostThreads(kElements) == kMostOfRow, "");
+    if (!few && p.n * sizeof(T) >= 1024 && 2 * RingBytes<KIND, T>(p.n) <= kRingRoom) {
+      if (p.n <= kMostOfRow) return LaunchRing<KIND, T, kElements / C>(p, sms, stream);
+      if constexpr (2 * kBytes * kMostOfRow < kRingRoom) {
+        if (p.n <= 48 * MostThreads(48)) return LaunchRing<KIND, T, 48 / C>(p, sms, stream);
       }
     }
   }
-  // Few rows: as many threads a row as it has pieces.  Many: more pieces a thread, so that the blocks of other rows hide a row's reduction.
+  // Few rows: as many threads a row as it has pieces.  Many: more pieces a thread, so that the blocks of other rows hide a row's reduction.  32 elements a thread
+  // hold no longer a row than 24 do.  Rows that are read twice: 18 warps, three blocks an SM (2000 x 33000, norm alone, 69 us; of 24 warps 93).
+  constexpr int kMost = C > 1 ? 3 : 4;
   int e = few ? 1 : 2, warps = 0, most = 1;
   for (;; ++e) {
     warps = WarpsOf(pieces, e * kOne);
     most = MostThreads(C * e * kOne) / 32;
-    if (warps <= most || e == 4) break;
+    if (warps <= most || e == kMost) break;
   }
-  p.warps = std::min(warps, most);
+  const bool again = warps > most;
+  p.warps = again && C > 1 ? 18 : std::min(warps, most);
   p.rows_per_block = few ? 1 : std::max(1, 4 / p.warps);
   const unsigned threads = static_cast<unsigned>(32 * p.warps * p.rows_per_block);
   const long long blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
-  if (warps > most) return Launch<KIND, T, C, 0>(p, static_cast<unsigned>(blocks), threads, stream);
+  if (again) return Launch<KIND, T, C, 0>(p, static_cast<unsigned>(blocks), threads, stream);
   if (e == 1) return Launch<KIND, T, C, kOne>(p, static_cast<unsigned>(blocks), threads, stream);
   if (e == 2) return Launch<KIND, T, C, 2 * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
   if (e == 3) return Launch<KIND, T, C, 3 * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
-  return Launch<KIND, T, C, 4 * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
+  return Launch<KIND, T, C, kMost * kOne>(p, static_cast<unsigned>(blocks), threads, stream);
 }
 
 bool On(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

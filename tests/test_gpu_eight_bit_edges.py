@@ -5,6 +5,7 @@ ring (many rows on 16 bytes); in pieces of 16 bytes, and element by element (odd
 import numpy as np
 import pytest
 import torch
+from test_gpu_row_quant import _SWISH, _check_rows, _norm
 
 from qwen38_flash_ops_b200 import RmsNormQuant, RowQuant, _lib
 
@@ -112,6 +113,15 @@ def test_scales_are_quotients(cuda, q_dtype, rows, n):
     assert np.array_equal(scale.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("q_dtype", _EIGHT)
+@pytest.mark.parametrize("exponent", [-99, 0, 126])
+def test_scales_of_every_significand(cuda, q_dtype, exponent):
+    """The same over all 2^23 of them, one a row."""
+    x = (torch.arange(1 << 23, device="cuda", dtype=torch.int32) | ((exponent + 127) << 23)).view(torch.float32)
+    _, scale = RowQuant(dtype=q_dtype)(x[:, None])
+    assert np.array_equal(scale.cpu().numpy(), x.cpu().numpy() / np.float32(_TOP[q_dtype]))
+
+
 # ---- waits that run out
 
 
@@ -154,3 +164,26 @@ def test_only_rows_of_the_ring_wait(cuda):
     finally:
         assert lib.qfg_row_quant_set_option(b"give_up", b"0") == _lib.QFG_OK
     assert (q == 127).all() and torch.isfinite(scale).all()
+
+
+# ---- lengths at which another kernel takes over
+
+
+@pytest.mark.parametrize("q_dtype", _EIGHT)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [2, 310])
+@pytest.mark.parametrize("n", [504, 512, 8192, 8200, 12288, 12289, 13440, 13448, 16384, 16385, 16392, 18432, 18440, 19200, 19968, 19976, 26888])
+def test_lengths_around_the_kernels_limits(cuda, q_dtype, dtype, rows, n):
+    gen = torch.Generator(device="cuda").manual_seed(rows + n)
+    x, second, weight = _rows(gen, rows, n).to(dtype), (3 * _rows(gen, rows, n)).to(dtype), (1 + 0.3 * torch.randn(n, generator=gen, device="cuda")).to(dtype)
+    norm, act = RmsNormQuant(eps=1e-5, dtype=q_dtype), RowQuant(dtype=q_dtype)
+    q, scale = norm(x, weight)
+    _check_rows(q, scale, _norm(x, weight, None, 1e-5, 0.0)[0], _REL, "norm")
+    q, scale, h = norm(x, weight, second)
+    y, want = _norm(x, weight, second, 1e-5, 0.0)
+    _check_rows(q, scale, y, _REL, "norm with residual")
+    assert torch.equal(h, want)
+    q, scale = act(x)
+    _check_rows(q, scale, x.double(), 8 * 2.0 ** -24, "rows")
+    q, scale = act(x, second)
+    _check_rows(q, scale, x.double() * torch.sigmoid(x.double()) * second.double(), _SWISH + 8 * 2.0 ** -24, "gated")
