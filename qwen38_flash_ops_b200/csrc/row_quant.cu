@@ -181,14 +181,12 @@ __device__ __forceinline__ void StoreQuantised(uint8_t* p, const float2 (&f)[kPa
   }
 }
 // The part of a row's factor that StoreQuantised does not apply, where there is one.
-template <int KIND, int C, int V>
-__device__ __forceinline__ void TakeUp(float2 (&f)[V][kPairs<C>], float first) {
+template <int KIND, int C>
+__device__ __forceinline__ void TakeUp(float2 (&f)[kPairs<C>], float first) {
   if constexpr (KIND >= kNorm) {
-    if (first == 1.f) return;
+    if (first != 1.f) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-#pragma unroll
-      for (int e = 0; e < kPairs<C>; ++e) f[j][e] = Mul2(f[j][e], Both(first));
+      for (int e = 0; e < kPairs<C>; ++e) f[e] = Mul2(f[e], Both(first));
     }
   }
 }
@@ -311,21 +309,23 @@ struct Scaling {
   float most;   // the largest magnitude behind the norm, at least `tiny`
   bool bad;
 };
-__device__ __forceinline__ float ScaleOf(const Scaling& s, bool fp8) { return s.bad ? __uint_as_float(0x7FFFFFFFu) : s.most / (fp8 ? 448.f : 127.f); }
+// The quotient by the rounded reciprocal, corrected by what it leaves: rounded as a division is (Markstein's theorem, of a reciprocal rounded to nearest), without
+// the cases of a division that cannot come up here.
+__device__ __forceinline__ float ScaleOf(const Scaling& s, bool fp8) {
+  const float top = fp8 ? 448.f : 127.f, part = fp8 ? 1.f / 448.f : 1.f / 127.f, q = s.most * part;
+  return s.bad ? __uint_as_float(0x7FFFFFFFu) : fmaf(fmaf(-q, top, s.most), part, q);
+}
 template <int KIND>
 __device__ __forceinline__ Scaling ScalingOf(const RowSums& r, const RowParams& p) {
   const float top = p.fp8 ? 448.f : 127.f;
   Scaling s;
-  s.bad = r.largest >= 0x7F800000u;
   float root = 1.f;
-  if constexpr (KIND >= kNorm) {
-    root = rsqrtf(fmaf(r.squares, p.inv_n, p.eps));
-    s.bad = s.bad || !(r.squares <= 3.4028234e38f) || !(root <= 3.4028234e38f);  // zeros without eps have no norm
-  }
+  if constexpr (KIND >= kNorm) root = rsqrtf(fmaf(r.squares, p.inv_n, p.eps));
   // (f root) / (max(largest root, tiny) / top).  The norm's factor leaves the quotient but for rows of tiny values, where f root is at most `tiny` and
   // root (top / tiny) alone may be past FP32.  So may top / largest be where a small eps makes much of little: such values are taken up by a power of two.
   const float largest = __uint_as_float(r.largest), most = largest * root;
-  if (KIND >= kNorm) s.bad = s.bad || !(most <= 3.4028234e38f);
+  // An infinite root (zeros without eps have no norm) leaves an infinity or, of zeros, a NaN; a sum of squares past FP32 leaves a root of zero.
+  s.bad = !(most <= 3.4028234e38f) || (KIND >= kNorm && !(r.squares <= 3.4028234e38f));
   s.first = 1.f;
   if (most > kTiny) {
     float by = largest;
@@ -384,34 +384,34 @@ __global__ void __launch_bounds__(MostThreads(C * V)) RowQuantKernel(const RowPa
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
     const Scaling s = ScalingOf<KIND>(r, p);
-    TakeUp<KIND, C, V>(f, s.first);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if (first + j * step >= n) break;
       if (s.bad) {
         StoreZeros<C>(qr + first + j * step);
       } else {
+        TakeUp<KIND, C>(f[j], s.first);
         StoreQuantised<C>(qr + first + j * step, f[j], s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = ScaleOf(s, p.fp8);
   } else {
-    float2 f[1][kPairs<C>];
+    float2 f[kPairs<C>];
     for (int i = first; i < n; i += step) {
       const Piece<T, C> a = Load<T, C>(xr + i);
-      Values<KIND, T, C>(f[0], a, kTwo ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
+      Values<KIND, T, C>(f, a, kTwo ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
     }
     const RowSums r = Reduce<(KIND >= kNorm)>(squares, largest, p.warps, warp_of_row, parts[row_of_block]);
     const Scaling s = ScalingOf<KIND>(r, p);
     for (int i = first; i < n; i += step) {
       // of the residual stream, the sums that this thread has stored
       const Piece<T, C> a = Load<T, C>(KIND == kNormAdd ? hr + i : xr + i);
-      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f[0], a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
+      Values<KIND == kNormAdd ? kNorm : KIND, T, C>(f, a, KIND == kSwish ? Load<T, C>(sr + i) : a, p, weight, nullptr, i, hr + i, squares, largest);
       if (s.bad) {
         StoreZeros<C>(qr + i);
       } else {
-        TakeUp<KIND, C, 1>(f, s.first);
-        StoreQuantised<C>(qr + i, f[0], s.by, p.fp8);
+        TakeUp<KIND, C>(f, s.first);
+        StoreQuantised<C>(qr + i, f, s.by, p.fp8);
       }
     }
     if (first == 0 && n > 0) p.scale[row] = ScaleOf(s, p.fp8);
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     float2 f[V][kPairs<C>], squares = make_float2(0.f, 0.f);
     good &= BarWait(full0 + stage * 8, parity, ctl);
     float largest = good ? 0.f : __uint_as_float(0x7FFFFFFFu);
-    const int come = good ? own : 0;
+    const int come = KIND == kNormAdd && !good ? 0 : own;  // else what is read where nothing came goes nowhere
     const T* const at = reinterpret_cast<const T*>(from + static_cast<uint32_t>(stage) * stage_bytes);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -490,11 +490,13 @@ __global__ void __launch_bounds__(MostThreads(16 / sizeof(T) * V)) RowRingKernel
     const long long next = row + static_cast<long long>(p.stages) * gridDim.x;
     if (threadIdx.x == 0 && good && next < p.rows) fetch(next, stage);  // what was there has come, and all have read it
     const Scaling s = ScalingOf<KIND>(r, p);
-    TakeUp<KIND, C, V>(f, s.first);
     if (!s.bad) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (j < own) StoreQuantised<C>(qr + j * step, f[j], s.by, p.fp8);
+        if (j < own) {
+          TakeUp<KIND, C>(f[j], s.first);
+          StoreQuantised<C>(qr + j * step, f[j], s.by, p.fp8);
+        }
       }
     } else {
       for (int j = 0; j < own; ++j) StoreZeros<C>(qr + j * step);
