@@ -312,12 +312,13 @@ QFG_API int qfg_lmhead_combine(const uint64_t* keys, int ranks, int64_t m, int64
  * kernels are fastest where bases and row distances are multiples of 16 bytes.
  *
  * RmsNormQuant: h = x + residual, rounded to its type, is kept (residual == NULL: h is x, and `h` is not written); y_i = h_i *
- * (weight_offset + weight_i) * rsqrt(mean(h^2) + eps), in this order (a product h_i w_i that FP32 flushes to zero stays zero); then as RowQuant.  `dtype` (BFLOAT16, FLOAT16, FLOAT) is that of x, residual and h,
- * `weight_dtype` the same or FLOAT, `q_dtype` INT8 or FLOAT8E4M3FN.  q is [rows, n], scale FP32 [rows], h [rows, n], all contiguous; h may be
- * the residual or x itself where that is contiguous.
+ * (weight_offset + weight_i) * rsqrt(mean(h^2) + eps), in this order (a product h_i w_i that FP32 flushes to zero stays zero); then as
+ * RowQuant.  `dtype` (BFLOAT16, FLOAT16, FLOAT) is that of x, residual and h, `weight_dtype` the same or FLOAT, `q_dtype` INT8 or
+ * FLOAT8E4M3FN.  q is [rows, n], scale FP32 [rows], h [rows, n], all contiguous; h may be the residual or x itself where that is contiguous.
  *
- * RowQuant: y = x, or swish(x) * u in FP32 where u is given; scale = max(max_i |y_i|, 2^-100) / top with top = 127 (INT8) or 448 (E4M3); q_i = y_i /
- * scale, rounded to nearest, ties to even.  A row whose largest value, or whose sum of squares in a norm, is not a finite FP32
+ * RowQuant: y = x, or swish(x) * u in FP32 where u is given (swish within 2^-20 of itself; zero from x = -87.3 down); scale =
+ * max(max_i |y_i|, 2^-100) / top, rounded once, with top = 127 (INT8) or 448 (E4M3); q_i = y_i / scale, rounded to nearest, ties to even.
+ * A row whose largest value, or whose sum of squares in a norm, is not a finite FP32
  * number has scale NaN and q 0.
  *
  * rows == 0 is a no-op; 1 <= n <= INT_MAX / 2. */
@@ -331,11 +332,13 @@ QFG_API int qfg_row_quant(int dtype, const void* x, int64_t ldx, const void* u, 
 QFG_API int qfg_row_quant_set_option(const char* key, const char* value);
 
 /* QuantGemm: out[m, n] = (sum_k x[m, k] w[k, n]) * x_scale[m] * w_scale[n].  INT8 products are summed in 32-bit integers, which is
- * exact (k <= 131071 of them cannot overflow), E4M3 products in FP32 by the tensor core, which cuts the sum off to 24 bits, toward zero, at every 32 products:
- * measured, sums of 17408 positive products come out 1.0e-5 too small (5120: 1.7e-6), signed ones are off by 7.5e-7 of their size (1.6e-7).  That is far below
- * a 16-bit output's rounding; FLOAT outputs show it.  The sum is scaled in FP32 and rounded once to `out_dtype` (BFLOAT16, FLOAT16 or FLOAT).  `w_scale` (host floats, one per column, uploaded once here; NULL: ones).
- * `dtype` is that of x and of w, INT8 or FLOAT8E4M3FN; x_scale FP32 [m] on the device.  The weight is [k][n] with rows ldw apart (QFG_ORDER_N: its
- * columns lie beside one another) or [n][k] (QFG_ORDER_K).  m == 0 is a no-op.  Nothing is allocated and the call may be captured. */
+ * exact (k <= 131071 of them cannot overflow), E4M3 products in FP32 by the tensor core, which cuts the sum off to 24 bits, toward zero,
+ * at every 32 products: measured, sums of 17408 positive products come out 1.0e-5 too small (5120: 1.7e-6), signed ones are off by 7.5e-7
+ * of their size (1.6e-7).  That is far below a 16-bit output's rounding; FLOAT outputs show it.  The sum is scaled in FP32 and rounded
+ * once to `out_dtype` (BFLOAT16, FLOAT16 or FLOAT).  `w_scale` (host floats, one per column, uploaded once here; NULL: ones).
+ * `dtype` is that of x and of w, INT8 or FLOAT8E4M3FN; x_scale FP32 [m] on the device.  The weight is [k][n] with rows ldw apart
+ * (QFG_ORDER_N: its columns lie beside one another) or [n][k] (QFG_ORDER_K).  m == 0 is a no-op.  Nothing is allocated and the call may
+ * be captured. */
 typedef enum qfg_order { QFG_ORDER_N = 0, QFG_ORDER_K = 1 } qfg_order;
 typedef struct qfg_quant_gemm qfg_quant_gemm;
 QFG_API int qfg_quant_gemm_create(const float* w_scale, size_t n_w_scale, int out_dtype, qfg_quant_gemm** out);
@@ -346,11 +349,13 @@ QFG_API int qfg_quant_gemm_compute(const qfg_quant_gemm* op, int dtype, const vo
 QFG_API int qfg_quant_gemm_set_option(qfg_quant_gemm* op, const char* key, const char* value);
 QFG_API void qfg_quant_gemm_destroy(qfg_quant_gemm* op);
 
-/* QuantMlp: the calls above one after another, as an MLP block: h = x + residual, kept; q1 = RmsNormQuant(h); gate, up = gate_up(q1) [rows, 2 width]; q2 =
- * RowQuant(swish(gate) * up); y = down(q2) [rows, hidden].  Arguments as theirs; y and h contiguous, y in the type of `down`.  The same results as the four
- * calls, but each product may fetch its first weights before the calls ahead have ended: all that was put on the stream before this call is waited for first,
- * but nothing that writes a weight may be put on it, by another thread, while this call launches its kernels.  `workspace`: that many bytes of the GPU's
- * memory, on 256 bytes, free again for what follows on the stream.  rows == 0 is a no-op (and needs none). */
+/* QuantMlp: the calls above one after another, as an MLP block: h = x + residual, kept; q1 = RmsNormQuant(h); gate, up = gate_up(q1)
+ * [rows, 2 width]; q2 = RowQuant(swish(gate) * up); y = down(q2) [rows, hidden].  Arguments as theirs; y and h contiguous, y in the type
+ * of `down`.  The same results as the four calls, but each product may fetch its first weights before the calls ahead have ended: all
+ * that was put on the stream before this call is waited for first, but nothing that writes a weight may be put on it, by another thread,
+ * while this call launches its kernels.  All four are checked before the first is launched: a call that is refused has written nothing.
+ * `workspace`: that many bytes of the GPU's memory, on 256 bytes, free again for what follows on the stream.  rows == 0 is a no-op (and
+ * needs none). */
 QFG_API size_t qfg_quant_mlp_workspace_bytes(const qfg_quant_gemm* gate_up, int64_t rows, int64_t hidden, int64_t width);
 QFG_API int qfg_quant_mlp(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* norm_weight, int weight_dtype,
                           float weight_offset, float eps, int64_t rows, int64_t hidden, int64_t width, int q_dtype, const qfg_quant_gemm* gate_up,

@@ -459,60 +459,60 @@ __global__ void __launch_bounds__(kThreads<PAIR, LOADERS>, 1) QuantGemmKernel(co
         const uint32_t st = buf + static_cast<uint32_t>((((lane >> 4) & 1) * 8 + (lane & 7)) * kPitch + ((lane >> 3) & 1) * 16);
         const uint32_t ld = buf + static_cast<uint32_t>(row * kPitch + chunk * 16);
         auto finish = [&](auto type) {
-        for (int c = 32 * half; c < p.bm; c += PAIR ? 64 : 32) {
-          uint32_t v[2][2][8];  // [lower, upper 16 columns][16 rows][fragments]
+          for (int c = 32 * half; c < p.bm; c += PAIR ? 64 : 32) {
+            uint32_t v[2][2][8];  // [lower, upper 16 columns][16 rows][fragments]
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                if (k == 0 || c + 16 < p.bm) {
+                  uint32_t(&f)[8] = v[h][k];
+                  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                               : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]), "=r"(f[4]), "=r"(f[5]), "=r"(f[6]), "=r"(f[7])
+                               : "r"(src + (static_cast<uint32_t>(16 * h) << 16) + static_cast<uint32_t>(c + 16 * k)));
+                }
+              }
+            }
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            __syncwarp();  // the rows before have been read
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               if (k == 0 || c + 16 < p.bm) {
-                uint32_t(&f)[8] = v[h][k];
-                asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]), "=r"(f[4]), "=r"(f[5]), "=r"(f[6]), "=r"(f[7])
-                             : "r"(src + (static_cast<uint32_t>(16 * h) << 16) + static_cast<uint32_t>(c + 16 * k)));
-              }
-            }
-          }
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          __syncwarp();  // the rows before have been read
+                const float2 s0 = *reinterpret_cast<const float2*>(xs + c + 16 * k + t2), s1 = *reinterpret_cast<const float2*>(xs + c + 16 * k + 8 + t2);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (k == 0 || c + 16 < p.bm) {
-              const float2 s0 = *reinterpret_cast<const float2*>(xs + c + 16 * k + t2), s1 = *reinterpret_cast<const float2*>(xs + c + 16 * k + 8 + t2);
+                for (int h = 0; h < 2; ++h) {
+                  uint32_t w[4];
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 s = i < 2 ? s0 : s1;
-                  const float lo = Sum<FP8>(v[h][k][2 * i]) * s.x * ws[h][i & 1], hi = Sum<FP8>(v[h][k][2 * i + 1]) * s.y * ws[h][i & 1];
-                  w[i] = good ? Pack<decltype(type)::value>(lo, hi) : 0x7FFF7FFFu;
+                  for (int i = 0; i < 4; ++i) {
+                    const float2 s = i < 2 ? s0 : s1;
+                    const float lo = Sum<FP8>(v[h][k][2 * i]) * s.x * ws[h][i & 1], hi = Sum<FP8>(v[h][k][2 * i + 1]) * s.y * ws[h][i & 1];
+                    w[i] = good ? Pack<decltype(type)::value>(lo, hi) : 0x7FFF7FFFu;
+                  }
+                  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(st + k * (16 * kPitch) + h * 32), "r"(w[0]),
+                               "r"(w[1]), "r"(w[2]), "r"(w[3])
+                               : "memory");
                 }
-                asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(st + k * (16 * kPitch) + h * 32), "r"(w[0]),
-                             "r"(w[1]), "r"(w[2]), "r"(w[3])
-                             : "memory");
               }
             }
-          }
-          __syncwarp();
-          if (p.out_vec && cols >= 32) {
+            __syncwarp();
+            if (p.out_vec && cols >= 32) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = c + 8 * i + row;
-              if (r < rows) {
-                uint32_t o[4];
-                Lds128(ld + i * (8 * kPitch), o);
-                *reinterpret_cast<uint4*>(out + static_cast<long long>(r) * p.ldo + 8 * chunk) = make_uint4(o[0], o[1], o[2], o[3]);
+              for (int i = 0; i < 4; ++i) {
+                const int r = c + 8 * i + row;
+                if (r < rows) {
+                  uint32_t o[4];
+                  Lds128(ld + i * (8 * kPitch), o);
+                  *reinterpret_cast<uint4*>(out + static_cast<long long>(r) * p.ldo + 8 * chunk) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+              }
+            } else {
+              const uint16_t* const from = reinterpret_cast<const uint16_t*>(bufs) + lane;
+              const int last = min(32, rows - c);
+              for (int r = 0; r < last; ++r) {
+                if (lane < cols) out[static_cast<long long>(c + r) * p.ldo + lane] = from[r * (kPitch / 2)];
               }
             }
-          } else {
-            const uint16_t* const from = reinterpret_cast<const uint16_t*>(bufs) + lane;
-            const int last = min(32, rows - c);
-            for (int r = 0; r < last; ++r) {
-              if (lane < cols) out[static_cast<long long>(c + r) * p.ldo + lane] = from[r * (kPitch / 2)];
-            }
           }
-        }
         };
         if (p.out_type == QFG_BFLOAT16) {
           finish(std::true_type());
@@ -794,8 +794,9 @@ cudaError_t ConfigureQuantKernels() {
 }
 
 // Launch shape: rows per tile, CTAs that split K, pairs, CTAs per SM.  The cheapest by a model of a call's time in us, fitted to calls in graphs on one
-// B200: 413 random shapes (1 to 2048 rows, K 256 to 17408, N 256 to 152000), up to 50 launch shapes each; the shape chosen takes 1.6 % longer than the best one
-// on average (the worst: 197 x 13840 x 2880 27 us against 19 in other rows per tile).  Rows off 16 bytes have a fit of their own (143 shapes, 0.6 %).
+// B200: 413 random shapes (1 to 2048 rows, K 256 to 17408, N 256 to 152000), up to 131 launch shapes each, kept in profiles/quant_gemm_launch_shapes.csv; the shape
+// chosen takes 1.8 % longer than the best one on average (the worst: 197 x 13840 x 2880 27 us against 19 in other rows per tile).  Rows off 16 bytes have a fit of
+// their own (142 shapes, 0.6 %).
 //   blocks of 128 k in turn, `waves` times; or what the CTAs fetch through L2; or memory: the longest, and a part of the shorter
 //   around that what a call takes anyway, with the last tile's epilogue, and where K is split, the ranks' exchange
 // More row tiles than needed are tried because they can fill the last wave better (509 x 5120 x 10240: three of 192 28 us, two of 256 32).

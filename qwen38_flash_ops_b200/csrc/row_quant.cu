@@ -7,13 +7,14 @@
 //
 // All of it in FP32 until the one rounding to eight bits.  One pass over memory: the largest |h_i (offset + weight_i)| is found
 // beside the sum of squares, because the norm's factor is the same for the whole row, and leaves q_i altogether, so a row needs one reduction and its
-// values wait in registers.  Rows longer than the registers of a block hold (18432 values, 19968 of many rows through the ring, 16384 that lie anywhere) are read again.  A row whose sum of
-// squares or largest value is no finite FP32 number has scale NaN and q 0.
+// values wait in registers.  Rows longer than the registers of a block hold (18432 values, 19968 of many rows through the ring, 16384 that lie anywhere) are
+// read again.  A row whose sum of squares or largest value is no finite FP32 number has scale NaN and q 0.
 //
-// What bounds it, on one B200 (a copy's 6.55 TB/s is the floor).  Few rows: the launch, one trip to memory and the reduction, 2.4 us in a graph for 1 x 5120, 3.7 for 4 x 17408
-// gated; a call takes longer on the host (4.4 to 5.1).  Many rows: memory, 4096 x 5120 with residual 23.6 us (22.4); instructions, 15 an element of which four are the
-// exponential and the quotient, 2048 x 17408 gated 32 (27.2); a norm alone the latency of its two reductions, 4096 x 5120 17.4 (9.6).  Rows that lie off
-// 16 bytes go element by element, at a fifth to a third of the bandwidth: loads of two bytes and stores of one take the load unit as long as wide ones.
+// What bounds it, on one B200 (a copy's 6.55 TB/s is the floor, in brackets).  Few rows: the launch, one trip to memory and the reduction, 2.4 us in a graph for
+// 1 x 5120, 3.7 for 4 x 17408 gated; a call takes longer on the host (4.5 to 5.8).  Many rows: memory, 4096 x 5120 with residual 24 to 27 us (22.4), as they are 12
+// (9.6); instructions, 16 an element of which four are the exponential and the quotient, 2048 x 17408 gated 33 to 34 (27.2); a norm alone the latency of its two
+// reductions, 4096 x 5120 16 (9.6).  Rows that lie off 16 bytes go element by element, 4096 x 5119 67 as they are, 75 a norm, 96 with residual, 83 gated: loads of
+// two bytes and stores of one take the load unit as long as wide ones.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -203,8 +204,8 @@ __device__ __forceinline__ void StoreZeros(uint8_t* p) {
 
 // a / (1 + exp(-a)), to 2^-21: exp(-a) is 2^hi (1 + lo ln 2) with hi + lo = -a log2 e.  With the rounded product alone for the exponent the
 // result would be off by 2^-24 |a|, 2^-18 at 60.  A BF16 value times the upper 16 bits of log2 e is exact, and lo the rest; else hi is the rounded
-// product and lo what the rounding left, for which values that overflow it (FP32 alone) are kept within bounds.  Results below 2^-126 are flushed to
-// zero, far below a row's least scale.
+// product and lo what the rounding left, for which values that overflow it (FP32 alone) are kept within bounds.  A reciprocal below 2^-126 is
+// flushed, so that from a = -87.3 down, where a result is below 1.1e-36, it is zero before u multiplies it.
 template <typename T>
 __device__ __forceinline__ float2 Swish2(float2 a) {
   float2 hi, t;

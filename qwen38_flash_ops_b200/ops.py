@@ -363,10 +363,10 @@ def _given(op: str, name: str, t, shape, dtype, contiguous=True):
 class RmsNormQuant:
     """Root-mean-square norm with the residual's addition, in eight bits with a scale for each row.
 
-    h = x + residual, rounded to its type (without a residual h is x); y = h * rsqrt(mean(h^2) + eps) * (weight_offset + weight)
+    h = x + residual, rounded to its type (without a residual h is x); y = h * (weight_offset + weight) * rsqrt(mean(h^2) + eps)
     in FP32; scale = max(max|y|, 2^-100) / 127 (torch.int8) or / 448 (torch.float8_e4m3fn); q = y / scale rounded to nearest.
     x, residual: [..., n] in BF16, FP16 or FP32; weight: [n], of the same type or FP32.  Returns (q, scale), with a residual (q, scale, h).
-    A row with a value that is not finite, or whose sum of squares is not, has scale NaN and q 0."""
+    A row with a value that is not finite, of x or of y, or whose sum of squares is not, has scale NaN and q 0."""
 
     def __init__(self, eps: float = 1e-6, weight_offset: float = 0.0, dtype: torch.dtype = torch.int8):
         self._lib = _load()
