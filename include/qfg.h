@@ -362,6 +362,77 @@ QFG_API int qfg_quant_mlp(int dtype, const void* x, int64_t ldx, const void* res
                           const void* w1, int64_t ldw1, int order1, const qfg_quant_gemm* down, const void* w2, int64_t ldw2, int order2, void* workspace,
                           void* y, void* h, void* stream);
 
+/* ---------------------------------------------------------------- heads, their cache, and attention
+ * What stands between a block's q / k / v projection and its output projection; no counterpart in the part of the reference that this
+ * library replaces.  Heads have 64, 128 or 256 channels.  Rows of heads are [tokens][heads][head_dim]: the heads of a token lie beside
+ * one another, tokens `ld*` elements apart.  Nothing is allocated, and every call may be captured, the first one included.
+ *
+ * A cache of keys and values is cut into pages of `page` tokens (a multiple of 32).  A page of one head holds its tokens one after
+ * another: k and v are [pages][kv_heads][page][head_dim] FP8 E4M3FN with FP32 scales [pages][kv_heads][page], or UINT8 (block-16
+ * NVFP4) [pages][kv_heads][page][head_dim / 2], channel 2 b in the low nibble of byte b, with E4M3FN scales [pages][kv_heads][page]
+ * [head_dim / 16].  A token's slot is page * (page size) + (its place in the page).  Writing a row y of a head:
+ *   E4M3:  scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i / scale.
+ *   NVFP4: for each 16 channels scale = max(E4M3(max_i |y_i| / (6 unit)), 2^-9), at most 448, q_i = E2M1(y_i / (scale unit)).
+ * Both rounded to nearest, ties to even; `unit` is k_unit or v_unit, so that values from 2^-10 to 2688 units are held well.  A row (NVFP4:
+ * sixteen channels) that holds an infinity or a NaN has scale NaN and q 0.  All tensors begin on 16 bytes. */
+typedef struct qfg_kv_cache {
+  void *k, *k_scale, *v, *v_scale;
+  int32_t dtype; /* QFG_UINT8 or QFG_FLOAT8E4M3FN */
+  int64_t pages, kv_heads, page, head_dim;
+  float k_unit, v_unit; /* NVFP4: what a stored 1 stands for, 1e-18 to 1e18 */
+} qfg_kv_cache;
+
+/* QkNormRope: norm of each query and key head, rotation by position, and, with a cache, the write of keys and values, in one pass.
+ *   y_i = x_i rsqrt(mean(x^2) + eps) (weight_offset + weight_i)   (a weight of NULL: y = x)
+ *   (y_a, y_b) -> rotary_scale (y_a cos t - y_b sin t, y_b cos t + y_a sin t), t = positions[axis of the pair][token] * inv_freq[pair]
+ * Pair i < n_pairs is channels (i, i + n_pairs), interleaved (2 i, 2 i + 1); channels from 2 n_pairs on stay.  n_pairs is a multiple of
+ * 16.  `axis` (NULL: all 0) says which of the rows of `positions` a pair goes by: one for text, several for images and video.  Positions
+ * are integers of `position_bytes` (4 or 8), rows `ld_positions` apart; angles are exact to 2^-44 of a turn for positions of a million.
+ * All in FP32, rounded once to `dtype` (BFLOAT16, FLOAT16, FLOAT) for q_out and k_out, contiguous, and once to the cache's type.
+ * Without a cache k_out is needed and v is not looked at; with one, k_out may be NULL.  `slots` [tokens]: a token whose slot is negative
+ * or lies behind the cache is not written; slots must differ.  q_out and k_out may not overlap the inputs.  tokens == 0 is a no-op.  A node
+ * belongs to the device it was made on. */
+typedef struct qfg_qk_norm_rope qfg_qk_norm_rope;
+QFG_API int qfg_qk_norm_rope_create(const double* inv_freq, const int32_t* axis, int n_pairs, int head_dim, int interleaved, float rotary_scale,
+                                    float eps, float weight_offset, qfg_qk_norm_rope** out);
+QFG_API int qfg_qk_norm_rope_compute(const qfg_qk_norm_rope* op, int dtype, const void* q, int64_t ldq, int64_t q_heads, const void* k, int64_t ldk,
+                                     int64_t kv_heads, const void* v, int64_t ldv, const void* positions, int position_bytes, int64_t ld_positions,
+                                     int64_t axes, const void* q_weight, const void* k_weight, int weight_dtype, int64_t tokens, void* q_out,
+                                     void* k_out, const qfg_kv_cache* cache, const int64_t* slots, void* stream);
+QFG_API void qfg_qk_norm_rope_destroy(qfg_qk_norm_rope* op);
+
+/* CacheWrite: keys and values as they are into their slots.  CacheRead: rows [offsets[i], offsets[i + 1]) of k_out and v_out
+ * ([rows][kv_heads][head_dim], contiguous, rounded once to `dtype`) become the first tokens of sequence i, whose pages are table[i][0..];
+ * offsets (int32, seqs + 1) do not fall.  Rows ahead of the first and behind the last sequence are left as they were; a token past the
+ * table's width, or whose page is none of the cache's, becomes zeros. */
+QFG_API int qfg_cache_write(int dtype, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t tokens, const qfg_kv_cache* cache,
+                            const int64_t* slots, void* stream);
+QFG_API int qfg_cache_read(const qfg_kv_cache* cache, const int32_t* table, int64_t ld_table, int64_t seqs, int64_t most_pages, const int32_t* offsets,
+                           int64_t rows, int dtype, void* k_out, void* v_out, void* stream);
+
+/* CacheAttention: softmax(scale q k^T) v of the last `tokens` tokens of each sequence over its `lengths[i]` tokens in the cache, which
+ * include them: token t sees the first lengths[i] - tokens + 1 + t.  q [seqs][tokens][q_heads][head_dim] (BFLOAT16 or FLOAT16, sequences ld_seq and
+ * tokens ld_token elements apart, on 16 bytes), out the same, contiguous; `lse` (NULL, or FP32 [seqs][tokens][q_heads]) gets the natural
+ * logarithm of the sum of the exponentials.  Query head h reads key head h / (q_heads / kv_heads).  A row that sees nothing (a length of
+ * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it; tokens whose page is none of the cache's are left
+ * out.  Values that lie behind a sequence's length take no part, whatever they are.  A wait inside the kernel that runs out makes the rows concerned NaN.
+ * `workspace`: that many bytes (0 where sequences are never cut), on 16 bytes, not looked at before the call and free behind it; calls
+ * that run at once need one each. */
+QFG_API int qfg_cache_attention_workspace_bytes(const qfg_kv_cache* cache, int64_t seqs, int64_t tokens, int64_t q_heads, int64_t most_pages, size_t* bytes);
+QFG_API int qfg_cache_attention(int dtype, const void* q, int64_t ld_seq, int64_t ld_token, int64_t seqs, int64_t tokens, int64_t q_heads,
+                                const qfg_kv_cache* cache, const int32_t* table, int64_t ld_table, int64_t most_pages, const int32_t* lengths,
+                                float scale, void* workspace, void* out, float* lse, void* stream);
+
+/* PromptAttention: softmax(scale q k^T) v of packed sequences of different lengths.  Rows [q_offsets[i], q_offsets[i + 1]) of q attend to
+ * rows [k_offsets[i], k_offsets[i + 1]) of k and v; causal: the last query sees all of its keys, each one ahead of it one fewer.  Types
+ * BFLOAT16 and FLOAT16, heads of 64 or 128 channels, bases and tokens on 16 bytes; out [q_rows][q_heads][head_dim] and lse (NULL, or FP32
+ * [q_rows][q_heads]) contiguous.  A row that sees nothing is 0, its lse -inf.  Rows ahead of the first and behind the last sequence are left
+ * as they were; what lies in keys and values of other sequences takes no part, whatever it is.  Within a sequence a value that is not
+ * finite makes rows of the same head that lie up to 128 tokens ahead of it NaN as well: their weight for it is 0, and 0 times it is not. */
+QFG_API int qfg_prompt_attention(int dtype, const void* q, int64_t ldq, int64_t q_rows, int64_t q_heads, const void* k, int64_t ldk, const void* v,
+                                 int64_t ldv, int64_t k_rows, int64_t kv_heads, int64_t head_dim, const int32_t* q_offsets, const int32_t* k_offsets,
+                                 int64_t seqs, int causal, float scale, void* out, float* lse, void* stream);
+
 /* Measurement aid, no counterpart in the reference: sweeps `bytes` of device memory at `buf` (16-byte aligned) with
  * 128-bit read-only loads and writes nothing (`sink`, 4 bytes of device memory or null, is never stored to on
  * real data).  Timed over a buffer several times the size of L2 it gives the read-only streaming ceiling of the

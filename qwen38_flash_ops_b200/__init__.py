@@ -1,6 +1,7 @@
 """B200 (sm_100a) implementation of the `qwen.fused_gemm` decode weight-streaming path:
 SkinnyGemm (M <= 8 rows per pass; BF16 / FP8 E4M3FN / block-16 NVFP4 weights), ArgmaxRows,
-DequantWeightBf16 and the fused, N-shardable LM head; and blocks in eight bits (RmsNormQuant, RowQuant, QuantGemm, QuantMlp).  The compute lives in libqfg_b200.so
+DequantWeightBf16 and the fused, N-shardable LM head; and blocks in eight bits (RmsNormQuant, RowQuant, QuantGemm, QuantMlp);
+heads, their quantised cache and attention (QkNormRope, KvCache, CacheWrite, CacheRead, CacheAttention, PromptAttention).  The compute lives in libqfg_b200.so
 (C ABI in include/qfg.h); this package is the Python mirror of the operator interface."""
 from . import packing  # noqa: F401
 from ._lib import QfgError, load  # noqa: F401
@@ -13,6 +14,10 @@ def __getattr__(name):
         from . import ops
 
         return getattr(ops, name)
+    if name in ("KvCache", "QkNormRope", "CacheWrite", "CacheRead", "CacheAttention", "PromptAttention"):
+        from . import attention
+
+        return getattr(attention, name)
     if name == "ShardedLmHead":
         from .lmhead_shard import ShardedLmHead
 

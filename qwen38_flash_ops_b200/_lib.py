@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from types import SimpleNamespace
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -38,6 +38,8 @@ EXPORTS = (
     "qfg_lmhead_exchange_times",
     "qfg_peer_alloc", "qfg_peer_open", "qfg_peer_close", "qfg_peer_free",
     "qfg_lmhead_host_create", "qfg_lmhead_host_run", "qfg_lmhead_host_destroy",
+    "qfg_qk_norm_rope_create", "qfg_qk_norm_rope_compute", "qfg_qk_norm_rope_destroy",
+    "qfg_cache_write", "qfg_cache_read", "qfg_cache_attention_workspace_bytes", "qfg_cache_attention", "qfg_prompt_attention",
     "qfg_stream_read_probe",
 )
 
@@ -117,6 +119,18 @@ def load() -> ctypes.CDLL:
     lib.qfg_quant_mlp_workspace_bytes.restype = c_size_t
     lib.qfg_quant_mlp.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, c_float, c_int64, c_int64, c_int64, c_int,
                                   c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.qfg_qk_norm_rope_create.argtypes = [POINTER(c_double), POINTER(c_int32), c_int, c_int, c_int, c_float, c_float, c_float, POINTER(c_void_p)]
+    lib.qfg_qk_norm_rope_compute.argtypes = [c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64,
+                                             c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.qfg_qk_norm_rope_destroy.argtypes = [c_void_p]
+    lib.qfg_qk_norm_rope_destroy.restype = None
+    lib.qfg_cache_write.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+    lib.qfg_cache_read.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]
+    lib.qfg_cache_attention_workspace_bytes.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int64, POINTER(c_size_t)]
+    lib.qfg_cache_attention.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_float,
+                                        c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.qfg_prompt_attention.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                         c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p]
     lib.qfg_lmhead_exchange_bytes.restype = c_size_t
     lib.qfg_lmhead_compute_sharded.argtypes = [c_void_p, c_void_p, c_int64, c_int64, POINTER(Tensor2D), c_int64, c_int64,
                                                c_void_p, POINTER(LmExchange), c_void_p, c_void_p, c_void_p, c_void_p]

@@ -1,0 +1,447 @@
+// What stands between a block's q / k / v projection and its attention, a head's row of one token at a time: the norm of query and key heads
+// with the rotation by position, the write of keys and values into a cache of eight or four bits, and the read back.
+//
+//   norm      y_i = x_i rsqrt(mean(x^2) + eps) (offset + weight_i)                  (FP32 from here on)
+//   rotation  (y_a, y_b) -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t), t = position * frequency of the pair, for the pairs (i, i + R/2) or (2 i, 2 i + 1) of
+//             the first R channels; with several axes each pair has one of the positions
+//   E4M3      scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i / scale              one for each token and head
+//   NVFP4     scale = max(E4M3(max_i |y_i| / (6 unit)), 2^-9), q_i = E2M1(y_i / (scale unit))   one for each 16 channels
+//
+// An angle is a product of 64-bit integers: a pair's frequency in turns, as a fraction of 2^64, times the position, modulo 2^64, is the fraction of the turn to 2^-44
+// for positions of a million; the sine and cosine of its first 32 bits are right to 2^-23 wherever the position is.  A product in FP32 is off by 2^-8 there.
+// Quotients are rounded once: the reciprocal is carried in two parts, so that half-way values go to even.
+//
+// A row has D / 16 lanes of sixteen channels each: of a rotated part in halves, eight of the one and the eight that they are rotated with, so that nothing crosses lanes
+// but the sum of squares and the largest value.  A block's sines and cosines are made once for its tokens and wait in shared memory for all heads.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "qfg_internal.h"
+#include "stream_order.cuh"
+
+namespace qfg {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostTokens = 4;  // of a block
+
+struct Side {  // queries, keys or values
+  const void* x;
+  long long ld;  // elements from token to token
+  void* out;     // contiguous rows, or null
+  const void* weight;
+  int heads;
+  bool vec, weight_vec;  // on 16 bytes, row by row
+};
+struct HeadsParams {
+  Side side[3];
+  const void* positions;
+  long long ld_positions;
+  const RotaryPair* pairs;
+  const long long* slots;
+  KvCacheView cache;
+  int tokens, tokens_per_block, rows, rows_per_block, rotary;  // rows: heads of all sides; rotary: channels
+  float rotary_scale, eps, offset;
+  bool weight_f32, positions_64, interleaved;
+};
+
+template <typename T>
+__device__ __forceinline__ float ToFloat(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  if constexpr (std::is_same_v<T, __half>) return __half2float(v);
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T FromFloat(float v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+}
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ void LoadEight(float* f, const T* p, bool vec) {
+  Eight<T> e;
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e.v[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = ToFloat(e.v[i]);
+}
+template <typename T>
+__device__ __forceinline__ void StoreEight(T* p, const float* f) {
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e.v[i] = FromFloat<T>(f[i]);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&e)[i];
+}
+
+// The larger magnitude of all lanes of a row, as the integer that its bits are: a NaN is larger than any number.
+template <int L>
+__device__ __forceinline__ uint32_t RowMax(uint32_t v) {
+#pragma unroll
+  for (int d = L / 2; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+__device__ __forceinline__ uint32_t Magnitude(const float* f) {  // of eight
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  return m;
+}
+constexpr uint32_t kInfinity = 0x7F800000u;
+
+// 1 / scale in two parts: v / scale = v hi + v lo, rounded once by the addition
+struct Reciprocal {
+  float hi, lo;
+  __device__ explicit Reciprocal(float scale) : hi(1.f / scale) { lo = fmaf(-scale, hi, 1.f) * hi; }
+  __device__ float operator()(float v) const { return fmaf(v, hi, v * lo); }
+};
+__device__ __forceinline__ uint2 EightE4m3(const float* f, const Reciprocal& r, bool bad) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(r(f[2 * i]), r(f[2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
+  return bad ? make_uint2(0, 0) : make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+}
+__device__ __forceinline__ uint32_t EightE2m1(const float* f, const Reciprocal& r, bool bad) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(r(f[2 * i]), r(f[2 * i + 1])), __NV_E2M1, cudaRoundNearest)) << (8 * i);
+  }
+  return bad ? 0u : w;
+}
+
+__device__ __forceinline__ void Turn(float& a, float& b, float2 by) {
+  const float u = a, v = b;
+  a = u * by.x - v * by.y;
+  b = v * by.x + u * by.y;
+}
+
+// A row's sixteen values of this lane, at channels c0 and c1 of eight each, into the cache.
+template <int L>
+__device__ __forceinline__ void StoreCache(const float (&f)[16], int c0, int c1, bool blocks_shared, const KvCacheView& cache, bool values, long long row, int lane,
+                                           bool write) {
+  uint8_t* const codes = values ? cache.v : cache.k;
+  const uint32_t m0 = Magnitude(f), m1 = Magnitude(f + 8);
+  constexpr int D = 16 * L;
+  if (cache.fp4) {
+    // a block of sixteen channels is this lane's, or eight of it are and the others the neighbour's
+    const float unit = values ? cache.v_unit : cache.k_unit;
+    const uint32_t n0 = __shfl_xor_sync(0xffffffffu, m0, 1), n1 = __shfl_xor_sync(0xffffffffu, m1, 1);
+    uint32_t most[2];
+    most[0] = max(m0, blocks_shared ? n0 : m1);
+    most[1] = max(m1, blocks_shared ? n1 : m0);
+    uint8_t* const scales = static_cast<uint8_t*>(values ? cache.v_scale : cache.k_scale) + row * L;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool bad = most[h] >= kInfinity;
+      const int c = h == 0 ? c0 : c1;
+      const __nv_fp8_storage_t coded = __nv_cvt_float_to_fp8(__uint_as_float(most[h]) / (6.f * unit), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t s = bad ? 0x7Fu : max(1u, static_cast<uint32_t>(coded));
+      const float scale = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(s), __NV_E4M3))) * unit;
+      const uint32_t w = EightE2m1(f + 8 * h, Reciprocal(scale), bad);
+      if (write) {
+        *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + c / 2) = w;
+        if ((c & 15) == 0) scales[c >> 4] = static_cast<uint8_t>(s);
+      }
+    }
+  } else {
+    const uint32_t most = RowMax<L>(max(m0, m1));
+    const bool bad = most >= kInfinity;
+    const float scale = fmaxf(__uint_as_float(most) / 448.f, 9.094947017729282e-13f);  // 2^-40
+    const Reciprocal r(scale);
+    const uint2 a = EightE4m3(f, r, bad), b = EightE4m3(f + 8, r, bad);
+    if (write) {
+      *reinterpret_cast<uint2*>(codes + row * D + c0) = a;
+      *reinterpret_cast<uint2*>(codes + row * D + c1) = b;
+      if (lane == 0) static_cast<float*>(values ? cache.v_scale : cache.k_scale)[row] = bad ? __uint_as_float(0x7FFFFFFFu) : scale;
+    }
+  }
+}
+
+// L lanes a row, D = 16 L.
+template <typename T, int L>
+__global__ void __launch_bounds__(kThreads) HeadsKernel(const HeadsParams p) {
+  constexpr int D = 16 * L, kRows = kThreads / L;
+  __shared__ float2 turn[kMostTokens * D / 2];
+  __shared__ long long place[kMostTokens];  // (page, row of it) as page * kv_heads * page size + row; < 0: not written
+  GridDependencyWait();
+  const int token0 = blockIdx.x * p.tokens_per_block, tokens = min(p.tokens_per_block, p.tokens - token0), half = p.rotary / 2;
+  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+    const int t = i / half, j = i - t * half;
+    const RotaryPair pair = p.pairs[j];
+    const long long at = token0 + t + pair.axis * p.ld_positions;
+    const long long position = p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
+    const unsigned long long turns = static_cast<unsigned long long>(position) * pair.turns;
+    float s, c;
+    sincospif(static_cast<float>(static_cast<int>(turns >> 32)) * 4.656612873077393e-10f, &s, &c);  // 2^-31
+    turn[i] = make_float2(c * p.rotary_scale, s * p.rotary_scale);
+  }
+  if (p.slots != nullptr && threadIdx.x < tokens) {
+    const long long slot = p.slots[token0 + threadIdx.x], page = slot / p.cache.page;
+    place[threadIdx.x] = slot >= 0 && page < p.cache.pages ? page * p.cache.heads * p.cache.page + (slot - page * p.cache.page) : -1;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % L;
+  const int row0 = blockIdx.y * p.rows_per_block, rows = min(p.rows_per_block, p.rows - row0), items = tokens * rows;
+  // every lane of a warp makes the same number of steps: shuffles are of whole warps
+  for (int first = 0; first < items; first += kRows) {
+    const int item = first + static_cast<int>(threadIdx.x) / L;
+    const bool mine = item < items;
+    const int t = mine ? item / rows : 0;
+    int head = mine ? row0 + item - t * rows : 0;
+    const int which = head < p.side[0].heads ? 0 : head < p.side[0].heads + p.side[1].heads ? 1 : 2;
+    if (which > 0) head -= p.side[0].heads;
+    if (which > 1) head -= p.side[1].heads;
+    const Side& s = p.side[which];
+    const bool turned = which < 2 && 16 * lane < p.rotary;
+    const bool halves = turned && !p.interleaved;
+    const int c0 = halves ? 8 * lane : 16 * lane, c1 = halves ? half + 8 * lane : c0 + 8;
+    float f[16];
+    const T* const x = static_cast<const T*>(s.x) + (token0 + t) * s.ld + head * D;
+    LoadEight<T>(f, x + c0, s.vec);
+    LoadEight<T>(f + 8, x + c1, s.vec);
+    float w[16];
+    if (s.weight != nullptr) {
+      if (p.weight_f32) {
+        LoadEight<float>(w, static_cast<const float*>(s.weight) + c0, s.weight_vec);
+        LoadEight<float>(w + 8, static_cast<const float*>(s.weight) + c1, s.weight_vec);
+      } else {
+        LoadEight<T>(w, static_cast<const T*>(s.weight) + c0, s.weight_vec);
+        LoadEight<T>(w + 8, static_cast<const T*>(s.weight) + c1, s.weight_vec);
+      }
+    }
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) squares = fmaf(f[i], f[i], squares);
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+    if (s.weight != nullptr) {
+      const float root = rsqrtf(fmaf(squares, 1.f / D, p.eps));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = f[i] * root * (p.offset + w[i]);
+    }
+    if (turned) {
+      const float2* const by = turn + t * half + 8 * lane;
+      if (halves) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) Turn(f[i], f[8 + i], by[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) Turn(f[2 * i], f[2 * i + 1], by[i]);
+      }
+    }
+    if (mine && s.out != nullptr) {
+      T* const out = static_cast<T*>(s.out) + (static_cast<long long>(token0 + t) * s.heads + head) * D;
+      StoreEight<T>(out + c0, f);
+      StoreEight<T>(out + c1, f + 8);
+    }
+    if (p.slots != nullptr) {
+      const long long row = place[t] + static_cast<long long>(head) * p.cache.page;
+      StoreCache<L>(f, c0, c1, halves, p.cache, which == 2, row, lane, mine && which > 0 && place[t] >= 0);
+    }
+  }
+}
+
+template <typename T, int L>
+cudaError_t LaunchHeads(HeadsParams& p, cudaStream_t stream) {
+  // Few tokens: one a block, its heads over as many blocks as keep every lane to one row.  Many: a block's tokens share nothing but its launch and make it long enough.
+  const int sms = DeviceSmCount();
+  p.tokens_per_block = p.tokens <= 2 * sms ? 1 : kMostTokens;
+  p.rows_per_block = p.tokens <= 2 * sms ? kThreads / L : p.rows;
+  const int x = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block, y = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {OverlapAttribute()};
+  cfg.attrs = attr;
+  cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, HeadsKernel<T, L>, p);
+}
+
+template <typename T>
+cudaError_t LaunchHeadsOf(int dim, HeadsParams& p, cudaStream_t stream) {
+  switch (dim) {
+    case 64: return LaunchHeads<T, 4>(p, stream);
+    case 128: return LaunchHeads<T, 8>(p, stream);
+    case 256: return LaunchHeads<T, 16>(p, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+// ------------------------------------------------------------------------------ the way back
+struct ReadParams {
+  KvCacheView cache;
+  const int* table;
+  const int* offsets;
+  void *k_out, *v_out;
+  long long ld_table, rows;
+  int seqs, most_pages;
+};
+constexpr int kReadRows = 16;  // of a block
+
+template <typename T, int L>
+__global__ void __launch_bounds__(kThreads) CacheReadKernel(const ReadParams p) {
+  constexpr int D = 16 * L;
+  __shared__ long long place[kReadRows];  // -2: a row of no sequence; -1: one that no page holds
+  GridDependencyWait();
+  const long long row0 = static_cast<long long>(blockIdx.x) * kReadRows;
+  if (threadIdx.x < kReadRows) {
+    const long long row = row0 + threadIdx.x;
+    long long at = -2;
+    if (row < p.rows && row >= p.offsets[0] && row < p.offsets[p.seqs]) {
+      int lo = 0, hi = p.seqs;  // the last sequence that begins at this row or ahead of it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        (p.offsets[mid] <= row ? lo : hi) = mid;
+      }
+      const int in = static_cast<int>(row - p.offsets[lo]), page = in / p.cache.page;
+      at = -1;
+      if (page < p.most_pages) {
+        const int id = p.table[lo * p.ld_table + page];
+        if (id >= 0 && id < p.cache.pages) at = static_cast<long long>(id) * p.cache.heads * p.cache.page + (in - page * p.cache.page);
+      }
+    }
+    place[threadIdx.x] = at;
+  }
+  __syncthreads();
+  const int per_row = p.cache.heads * 2 * L, items = kReadRows * per_row;  // a lane's sixteen channels
+  for (int i = threadIdx.x; i < items; i += kThreads) {
+    const int r = i / per_row, rest = i - r * per_row, values = rest / (p.cache.heads * L), c = rest - values * p.cache.heads * L, head = c / L, lane = c - head * L;
+    const long long at = place[r];
+    if (at == -2) continue;
+    float f[16];
+    if (at < 0) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[e] = 0.f;
+    } else {
+      const long long row = at + static_cast<long long>(head) * p.cache.page;
+      const uint8_t* const codes = values ? p.cache.v : p.cache.k;
+      const void* const scales = values ? p.cache.v_scale : p.cache.k_scale;
+      if (p.cache.fp4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + row * (D / 2) + lane * 8);
+        const __nv_fp8_storage_t s = static_cast<const uint8_t*>(scales)[row * L + lane];
+        const float scale = __half2float(__half(__nv_cvt_fp8_to_halfraw(s, __NV_E4M3))) * (values ? p.cache.v_unit : p.cache.k_unit);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const __nv_fp4x2_storage_t two = static_cast<__nv_fp4x2_storage_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+          const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(two, __NV_E2M1);
+          const float2 v = __half22float2(__half2(h));
+          f[2 * e] = v.x * scale;
+          f[2 * e + 1] = v.y * scale;
+        }
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(codes + row * D + lane * 16);
+        const float scale = static_cast<const float*>(scales)[row];
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(words[e >> 1] >> (16 * (e & 1))), __NV_E4M3);
+          const float2 v = __half22float2(__half2(h));
+          f[2 * e] = v.x * scale;
+          f[2 * e + 1] = v.y * scale;
+        }
+      }
+    }
+    T* const out = static_cast<T*>(values ? p.v_out : p.k_out) + ((row0 + r) * p.cache.heads + head) * D + lane * 16;
+    StoreEight<T>(out, f);
+    StoreEight<T>(out + 8, f + 8);
+  }
+}
+
+template <typename T>
+cudaError_t LaunchReadOf(int dim, const ReadParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + kReadRows - 1) / kReadRows));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {OverlapAttribute()};
+  cfg.attrs = attr;
+  cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
+  switch (dim) {
+    case 64: return cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 4>, p);
+    case 128: return cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 8>, p);
+    case 256: return cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 16>, p);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+size_t BytesOf(int dtype) { return dtype == QFG_FLOAT ? 4 : 2; }
+bool Vectors(const void* x, long long ld, int dtype) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * BytesOf(dtype) % 16 == 0; }
+
+cudaError_t Ended(cudaError_t err) {
+  const cudaError_t last = cudaGetLastError();
+  return err == cudaSuccess ? last : err;
+}
+
+}  // namespace
+
+cudaError_t LaunchHeadRows(const HeadsCall& c, cudaStream_t stream) {
+  if (c.tokens == 0) return cudaSuccess;
+  HeadsParams p = {};
+  p.side[0] = {c.q, c.ldq, c.q_out, c.q_weight, c.q != nullptr ? c.q_heads : 0, Vectors(c.q, c.ldq, c.dtype), Vectors(c.q_weight, 0, c.dtype)};
+  p.side[1] = {c.k, c.ldk, c.k_out, c.k_weight, c.kv_heads, Vectors(c.k, c.ldk, c.dtype), Vectors(c.k_weight, 0, c.dtype)};
+  p.side[2] = {c.v, c.ldv, nullptr, nullptr, c.slots != nullptr ? c.kv_heads : 0, Vectors(c.v, c.ldv, c.dtype), true};
+  p.positions = c.positions;
+  p.ld_positions = c.ld_positions;
+  p.positions_64 = c.positions_64;
+  p.pairs = c.pairs;
+  p.rotary = 2 * c.n_pairs;
+  p.interleaved = c.interleaved;
+  p.rotary_scale = c.rotary_scale;
+  p.eps = c.eps;
+  p.offset = c.weight_offset;
+  p.weight_f32 = c.weight_dtype == QFG_FLOAT;
+  p.slots = reinterpret_cast<const long long*>(c.slots);
+  p.cache = c.cache;
+  p.tokens = static_cast<int>(c.tokens);
+  p.rows = p.side[0].heads + p.side[1].heads + p.side[2].heads;
+  cudaError_t err;
+  switch (c.dtype) {
+    case QFG_BFLOAT16: err = LaunchHeadsOf<__nv_bfloat16>(c.dim, p, stream); break;
+    case QFG_FLOAT16: err = LaunchHeadsOf<__half>(c.dim, p, stream); break;
+    case QFG_FLOAT: err = LaunchHeadsOf<float>(c.dim, p, stream); break;
+    default: return cudaErrorInvalidValue;
+  }
+  return Ended(err);
+}
+
+cudaError_t LaunchCacheRead(const CacheReadCall& c, cudaStream_t stream) {
+  if (c.rows == 0 || c.seqs == 0) return cudaSuccess;
+  ReadParams p = {};
+  p.cache = c.cache;
+  p.table = c.table;
+  p.ld_table = c.ld_table;
+  p.offsets = c.offsets;
+  p.seqs = c.seqs;
+  p.most_pages = c.most_pages;
+  p.rows = c.rows;
+  p.k_out = c.k_out;
+  p.v_out = c.v_out;
+  cudaError_t err;
+  switch (c.dtype) {
+    case QFG_BFLOAT16: err = LaunchReadOf<__nv_bfloat16>(c.cache.dim, p, stream); break;
+    case QFG_FLOAT16: err = LaunchReadOf<__half>(c.cache.dim, p, stream); break;
+    case QFG_FLOAT: err = LaunchReadOf<float>(c.cache.dim, p, stream); break;
+    default: return cudaErrorInvalidValue;
+  }
+  return Ended(err);
+}
+
+}  // namespace qfg

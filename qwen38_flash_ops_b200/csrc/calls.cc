@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
+#include <cmath>
 #include <vector>
 
 #include "qfg.h"
@@ -29,6 +30,12 @@ struct Entries {
   decltype(&qfg_quant_gemm_compute) quant_gemm;
   decltype(&qfg_quant_mlp_workspace_bytes) quant_mlp_workspace_bytes;
   decltype(&qfg_quant_mlp) quant_mlp;
+  decltype(&qfg_qk_norm_rope_compute) qk_norm_rope;
+  decltype(&qfg_cache_write) cache_write;
+  decltype(&qfg_cache_read) cache_read;
+  decltype(&qfg_cache_attention_workspace_bytes) cache_attention_workspace_bytes;
+  decltype(&qfg_cache_attention) cache_attention;
+  decltype(&qfg_prompt_attention) prompt_attention;
 } g_lib;
 
 // A plain CUDA tensor, or null: no subclass, no wrapper of a transform, nothing without memory of its own.
@@ -408,6 +415,180 @@ PyObject* QuantMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// ---- heads, their cache, and attention
+// [tokens, heads, channels] on the current device, the heads of a token beside one another
+struct HeadRows {
+  const at::Tensor* t = nullptr;
+  int64_t tokens = 0, heads = 0, dim = 0, ld = 0;
+  int dtype = 0;
+};
+bool ToHeads(PyObject* o, HeadRows* h) {
+  h->t = Plain(o);
+  if (h->t == nullptr || h->t->dim() != 3 || !Float(*h->t) || !OnCurrent(*h->t)) return false;
+  h->tokens = h->t->size(0), h->heads = h->t->size(1), h->dim = h->t->size(2);
+  if (h->tokens < 1 || h->heads < 1 || h->dim < 1) return false;
+  h->ld = h->tokens > 1 ? h->t->stride(0) : h->heads * h->dim;
+  h->dtype = Code(h->t->scalar_type());
+  return h->t->stride(2) == 1 && (h->heads == 1 || h->t->stride(1) == h->dim) && h->ld >= h->heads * h->dim;
+}
+bool Like(const HeadRows& a, const HeadRows& b) { return a.tokens == b.tokens && a.heads == b.heads && a.dim == b.dim && a.dtype == b.dtype; }
+struct HeldCache {  // what a KvCache keeps for its calls
+  qfg_kv_cache cache;
+  int32_t device;
+};
+const HeldCache* ToCache(PyObject* o) {
+  if (!PyLong_CheckExact(o)) return nullptr;
+  const HeldCache* c = static_cast<const HeldCache*>(PyLong_AsVoidPtr(o));
+  return c != nullptr && c->device == c10::cuda::current_device() ? c : nullptr;
+}
+const at::Tensor* Numbers(PyObject* o, at::ScalarType type, int64_t dims) {
+  const at::Tensor* t = Dense(o);
+  return t != nullptr && t->scalar_type() == type && t->dim() == dims && OnCurrent(*t) ? t : nullptr;
+}
+
+// qk_norm_rope(handle, q, k, positions, q_weight, k_weight, v, cache, slots, keys) -> q or (q, k)
+PyObject* QkNormRope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    HeadRows q, k, v;
+    if (n_args != 10 || !ToHeads(a[1], &q) || !ToHeads(a[2], &k) || k.tokens != q.tokens || k.dim != q.dim || k.dtype != q.dtype || (a[9] != Py_True && a[9] != Py_False))
+      return None();
+    const void* op = PyLong_AsVoidPtr(a[0]);
+    const at::Tensor* p = Dense(a[3]);
+    if (op == nullptr || p == nullptr || !OnCurrent(*p) || p->dim() < 1 || p->dim() > 2 || p->size(-1) != q.tokens ||
+        (p->scalar_type() != at::kLong && p->scalar_type() != at::kInt))
+      return None();
+    const void* weights[2] = {nullptr, nullptr};
+    int weight_dtype = q.dtype;
+    for (int i = 0; i < 2; ++i) {
+      if (a[4 + i] == Py_None) continue;
+      const at::Tensor* w = Dense(a[4 + i]);
+      if (w == nullptr || w->dim() != 1 || w->size(0) != q.dim || !OnCurrent(*w)) return None();
+      const int type = Code(w->scalar_type());
+      if ((type != q.dtype && type != QFG_FLOAT) || (i == 1 && weights[0] != nullptr && type != weight_dtype)) return None();
+      weights[i] = w->data_ptr();
+      weight_dtype = type;
+    }
+    const HeldCache* cache = nullptr;
+    const at::Tensor* slots = nullptr;
+    if (a[7] != Py_None) {
+      cache = ToCache(a[7]);
+      slots = Numbers(a[8], at::kLong, 1);
+      if (cache == nullptr || slots == nullptr || slots->size(0) != q.tokens || !ToHeads(a[6], &v) || !Like(v, k)) return None();
+    } else if (a[6] != Py_None || a[8] != Py_None) {
+      return None();
+    }
+    const at::ScalarType type = q.t->scalar_type();
+    const at::Tensor q_out = New({q.tokens, q.heads, q.dim}, type);
+    at::Tensor k_out;
+    if (cache == nullptr || a[9] == Py_True) k_out = New({k.tokens, k.heads, k.dim}, type);
+    const void *qp = q.t->data_ptr(), *kp = k.t->data_ptr(), *vp = cache != nullptr ? v.t->data_ptr() : nullptr, *pp = p->data_ptr();
+    void *const qo = q_out.data_ptr(), *const ko = k_out.defined() ? k_out.data_ptr() : nullptr, *const stream = Stream();
+    const int64_t* const sp = slots != nullptr ? slots->data_ptr<int64_t>() : nullptr;
+    const int bytes = static_cast<int>(p->element_size());
+    const int64_t axes = p->dim() == 2 ? p->size(0) : 1;
+    const int code = Call([&] {
+      return g_lib.qk_norm_rope(static_cast<const qfg_qk_norm_rope*>(op), q.dtype, qp, q.ld, q.heads, kp, k.ld, k.heads, vp, v.ld, pp, bytes, q.tokens, axes, weights[0],
+                                weights[1], weight_dtype, q.tokens, qo, ko, cache != nullptr ? &cache->cache : nullptr, sp, stream);
+    });
+    return code != 0 ? PyLong_FromLong(code) : k_out.defined() ? TupleOf({q_out, k_out}) : THPVariable_Wrap(q_out);
+  });
+}
+
+// cache_write(k, v, cache, slots) -> status
+PyObject* CacheWrite(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    HeadRows k, v;
+    if (n_args != 4 || !ToHeads(a[0], &k) || !ToHeads(a[1], &v) || !Like(k, v)) return None();
+    const HeldCache* cache = ToCache(a[2]);
+    const at::Tensor* slots = Numbers(a[3], at::kLong, 1);
+    if (cache == nullptr || slots == nullptr || slots->size(0) != k.tokens || cache->cache.kv_heads != k.heads || cache->cache.head_dim != k.dim) return None();
+    const void *kp = k.t->data_ptr(), *vp = v.t->data_ptr();
+    const int64_t* const sp = slots->data_ptr<int64_t>();
+    void* const stream = Stream();
+    return PyLong_FromLong(Call([&] { return g_lib.cache_write(k.dtype, kp, k.ld, vp, v.ld, k.tokens, &cache->cache, sp, stream); }));
+  });
+}
+
+// cache_read(dtype, cache, table, offsets, rows) -> (k, v)
+PyObject* CacheRead(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    if (n_args != 5 || !PyLong_CheckExact(a[0]) || !PyLong_CheckExact(a[4])) return None();
+    const HeldCache* cache = ToCache(a[1]);
+    const at::Tensor *table = Numbers(a[2], at::kInt, 2), *offsets = Numbers(a[3], at::kInt, 1);
+    const int64_t rows = PyLong_AsLongLong(a[4]);
+    const int dtype = static_cast<int>(PyLong_AsLong(a[0]));
+    if (cache == nullptr || table == nullptr || offsets == nullptr || offsets->size(0) != table->size(0) + 1 || rows < 0) return None();
+    const at::ScalarType type = dtype == QFG_FLOAT ? at::kFloat : dtype == QFG_FLOAT16 ? at::kHalf : at::kBFloat16;
+    const at::Tensor k = New({rows, cache->cache.kv_heads, cache->cache.head_dim}, type), v = New({rows, cache->cache.kv_heads, cache->cache.head_dim}, type);
+    const int32_t *tp = table->data_ptr<int32_t>(), *op = offsets->data_ptr<int32_t>();
+    const int64_t seqs = table->size(0), most = table->size(1);
+    void *const kp = k.data_ptr(), *const vp = v.data_ptr(), *const stream = Stream();
+    const int code = Call([&] { return g_lib.cache_read(&cache->cache, tp, most, seqs, most, op, rows, dtype, kp, vp, stream); });
+    return code != 0 ? PyLong_FromLong(code) : TupleOf({k, v});
+  });
+}
+
+// cache_attention(scale or 0, q, cache, table, lengths, lse) -> out or (out, lse)
+PyObject* CacheAttention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    const at::Tensor* q = n_args == 6 ? Plain(a[1]) : nullptr;
+    if (q == nullptr || !PyFloat_CheckExact(a[0]) || (a[5] != Py_True && a[5] != Py_False) || !OnCurrent(*q) || (q->dim() != 3 && q->dim() != 4)) return None();
+    const HeldCache* cache = ToCache(a[2]);
+    const at::Tensor *table = Numbers(a[3], at::kInt, 2), *lengths = Numbers(a[4], at::kInt, 1);
+    const bool four = q->dim() == 4;
+    const int64_t seqs = q->size(0), tokens = four ? q->size(1) : 1, heads = q->size(-2), dim = q->size(-1);
+    if (cache == nullptr || table == nullptr || lengths == nullptr || seqs < 1 || tokens < 1 || heads < 1 || dim != cache->cache.head_dim || table->size(0) != seqs ||
+        lengths->size(0) != seqs || q->stride(-1) != 1 || (heads > 1 && q->stride(-2) != dim) ||
+        (q->scalar_type() != at::kBFloat16 && q->scalar_type() != at::kHalf))
+      return None();
+    const int64_t ld_token = tokens > 1 ? q->stride(1) : heads * dim, ld_seq = seqs > 1 ? q->stride(0) : tokens * heads * dim, most = table->size(1);
+    size_t need = 0;
+    const int known = g_lib.cache_attention_workspace_bytes(&cache->cache, seqs, tokens, heads, most, &need);
+    if (known != 0) return PyLong_FromLong(known);
+    const at::Tensor out = New(q->sizes(), q->scalar_type());
+    at::Tensor lse, workspace;
+    if (a[5] == Py_True) lse = New(q->sizes().slice(0, q->dim() - 1), at::kFloat);
+    if (need > 0) workspace = New({static_cast<int64_t>(need)}, at::kByte);
+    const double given = PyFloat_AS_DOUBLE(a[0]);
+    const float scale = static_cast<float>(given != 0.0 ? given : 1.0 / std::sqrt(static_cast<double>(dim)));
+    const int dtype = Code(q->scalar_type());
+    const void* qp = q->data_ptr();
+    const int32_t *tp = table->data_ptr<int32_t>(), *lp = lengths->data_ptr<int32_t>();
+    void *const wp = need > 0 ? workspace.data_ptr() : nullptr, *const yp = out.data_ptr(), *const stream = Stream();
+    float* const sp = lse.defined() ? lse.data_ptr<float>() : nullptr;
+    const int code =
+        Call([&] { return g_lib.cache_attention(dtype, qp, ld_seq, ld_token, seqs, tokens, heads, &cache->cache, tp, most, most, lp, scale, wp, yp, sp, stream); });
+    return code != 0 ? PyLong_FromLong(code) : lse.defined() ? TupleOf({out, lse}) : THPVariable_Wrap(out);
+  });
+}
+
+// prompt_attention(scale or 0, causal, q, k, v, q_offsets, k_offsets or None, lse) -> out or (out, lse)
+PyObject* PromptAttention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return Guard([&]() -> PyObject* {
+    HeadRows q, k, v;
+    if (n_args != 8 || !PyFloat_CheckExact(a[0]) || (a[1] != Py_True && a[1] != Py_False) || (a[7] != Py_True && a[7] != Py_False) || !ToHeads(a[2], &q) ||
+        !ToHeads(a[3], &k) || !ToHeads(a[4], &v) || !Like(k, v) || k.dim != q.dim || k.dtype != q.dtype)
+      return None();
+    const at::Tensor *qo = Numbers(a[5], at::kInt, 1), *ko = a[6] == Py_None ? qo : Numbers(a[6], at::kInt, 1);
+    if (qo == nullptr || ko == nullptr || qo->size(0) < 1 || ko->size(0) != qo->size(0)) return None();
+    const at::Tensor out = New({q.tokens, q.heads, q.dim}, q.t->scalar_type());
+    at::Tensor lse;
+    if (a[7] == Py_True) lse = New({q.tokens, q.heads}, at::kFloat);
+    const double given = PyFloat_AS_DOUBLE(a[0]);
+    const float scale = static_cast<float>(given != 0.0 ? given : 1.0 / std::sqrt(static_cast<double>(q.dim)));
+    const int causal = a[1] == Py_True;
+    const void *qp = q.t->data_ptr(), *kp = k.t->data_ptr(), *vp = v.t->data_ptr();
+    const int32_t *qop = qo->data_ptr<int32_t>(), *kop = ko->data_ptr<int32_t>();
+    const int64_t seqs = qo->size(0) - 1;
+    void *const yp = out.data_ptr(), *const stream = Stream();
+    float* const sp = lse.defined() ? lse.data_ptr<float>() : nullptr;
+    const int code = Call([&] {
+      return g_lib.prompt_attention(q.dtype, qp, q.ld, q.tokens, q.heads, kp, k.ld, vp, v.ld, k.tokens, k.heads, q.dim, qop, kop, seqs, causal, scale, yp, sp, stream);
+    });
+    return code != 0 ? PyLong_FromLong(code) : lse.defined() ? TupleOf({out, lse}) : THPVariable_Wrap(out);
+  });
+}
+
 template <typename T>
 bool Address(PyObject* o, T* fn) {
   void* p = PyLong_AsVoidPtr(o);
@@ -433,6 +614,19 @@ PyObject* BindMlp(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   Entries e = g_lib;
   if (!Address(a[0], &e.quant_mlp_workspace_bytes) || !Address(a[1], &e.quant_mlp)) return nullptr;
+  g_lib = e;
+  Py_RETURN_NONE;
+}
+
+PyObject* BindHeads(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  if (n_args != 6) {
+    PyErr_SetString(PyExc_TypeError, "bind_heads takes six addresses");
+    return nullptr;
+  }
+  Entries e = g_lib;
+  if (!Address(a[0], &e.qk_norm_rope) || !Address(a[1], &e.cache_write) || !Address(a[2], &e.cache_read) || !Address(a[3], &e.cache_attention_workspace_bytes) ||
+      !Address(a[4], &e.cache_attention) || !Address(a[5], &e.prompt_attention))
+    return nullptr;
   g_lib = e;
   Py_RETURN_NONE;
 }
@@ -472,6 +666,12 @@ PyMethodDef g_methods[] = {QFG_METHOD("bind", Bind),
                            QFG_METHOD("row_quant", RowQuant),
                            QFG_METHOD("quant_gemm", QuantGemm),
                            QFG_METHOD("quant_mlp", QuantMlp),
+                           QFG_METHOD("bind_heads", BindHeads),
+                           QFG_METHOD("qk_norm_rope", QkNormRope),
+                           QFG_METHOD("cache_write", CacheWrite),
+                           QFG_METHOD("cache_read", CacheRead),
+                           QFG_METHOD("cache_attention", CacheAttention),
+                           QFG_METHOD("prompt_attention", PromptAttention),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,505 @@
+// Attention of whole prompts: packed sequences of different lengths, causal or not, query heads in groups over key heads.
+//
+//   s_ij = scale q_i . k_j,  j within the sequence (causal: j <= i + keys - queries);   y_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
+//
+// A block takes two tiles of 128 queries of one head and runs over the keys they see, 128 at a time.  Both products are tcgen05.mma with FP32 sums in tensor memory:
+// S = Q K^T from shared memory, and O += P V with P, in 16 bits, in tensor memory where S was.  A row of S belongs to one thread, so that the maximum and the sum of a
+// row cross no lanes.  The two tiles take turns: while the tensor core works for the one, the other's four warps are at their exponentials.
+//
+//   columns   S0 | S1 | O0 | O1 of 128, 128, D, D; P over the first half of its S
+//   warps     0-3 and 4-7 softmax and output of a tile each, 8 products, 9 copies (and zeros in the place of values past the sequence's end), 10 and 11 idle: registers
+//             are shared out by four warps
+//   ring      128 keys or 128 values a stage, by tensor copies; rows of 128 bytes, swizzled
+//
+// One pass: m is taken up only when a score passes it by 8 (in powers of two), and only then are O and the sum scaled again; weights stay below 2^8, within FP16.
+// S and the sums are FP32; P is rounded to the type of the inputs, as tensor cores take it (a relative 2^-9 or 2^-12 of each weight, before sums of many).
+//
+// Products and exponentials take the same time (a tile of 128 x 128 at D = 128: 1024 cycles of the tensor core, 1024 of the unit for exponentials at 16 a cycle), which is
+// what bounds the kernel.  No weight is made for tiles that the mask leaves out; the longest rows' blocks come first.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "qfg_internal.h"
+#include "stream_order.cuh"
+#include "tc_ptx.cuh"
+#include "tensor_map.h"
+
+namespace qfg {
+namespace {
+
+constexpr int kTile = 128, kThreads = 384;
+// Registers of a thread: the launch's 168 for all are shared out, 8 warps of 208 and 4 of 80 (together 1984 of the 2016 that a lane of twelve warps has).
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 80;
+static_assert(8 * kSoftmaxRegisters + 4 * kOtherRegisters <= 12 * 168, "");
+
+struct PromptParams {
+  CUtensorMap q, k, v;
+  const int *q_offsets, *k_offsets;
+  void* out;
+  float* lse;
+  int seqs, q_rows, k_rows, q_heads, group;
+  float scale;  // of scores, in powers of two
+  bool causal, give_up;
+};
+
+template <int D>
+struct Geometry {
+  static constexpr int kHeadTile = kTile * D * 2;  // bytes of 128 rows
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kBytes = 2 * kHeadTile + kStages * kHeadTile + 1024;
+};
+
+struct PromptCtl {
+  unsigned long long q_full[2], full[8], empty[8], s_full[2], p_ready[2], o_full[2], fixed;
+  uint32_t tmem;
+  volatile uint32_t fault;
+};
+
+__device__ __forceinline__ void TmaLoad3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void MmaTs(uint32_t d, uint32_t a, unsigned long long b, uint32_t idesc, bool add) {
+  asm volatile("{ .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+               "r"(add ? 1 : 0)
+               : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void LoadColumns(uint32_t a, float* f) {
+  uint32_t* const v = reinterpret_cast<uint32_t*>(f);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+      "%26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+        "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+        "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void StoreColumns32(uint32_t a, const float* f) {
+  const uint32_t* const v = reinterpret_cast<const uint32_t*>(f);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+      "%26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+      "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void StoreColumns16(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(a), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+               "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+__device__ __forceinline__ void WaitLoads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void WaitStores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float Exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float Log2(float v) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 Add2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t Pack(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
+  return r;
+}
+
+// Where a block's queries and keys lie; tiles < 0: a block too many.
+struct Place {
+  int q0, k0, queries, keys, first;  // first: the first of its 256 queries, within the sequence
+};
+__device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
+  const int lane = threadIdx.x & 31;
+  Place at = {0, 0, 0, 0, -1};
+  // from the last sequence on, each one's last rows, which see the most keys, ahead of its others
+  int before = 0;
+  for (int base = p.seqs - 1; base >= 0; base -= 32) {
+    const int i = base - lane;
+    int q0 = 0, q1 = 0;
+    if (i >= 0) {
+      q0 = min(max(p.q_offsets[i], 0), p.q_rows);
+      q1 = min(max(p.q_offsets[i + 1], q0), p.q_rows);
+    }
+    const int tiles = (q1 - q0 + 2 * kTile - 1) / (2 * kTile);
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    const uint32_t mine = __ballot_sync(0xffffffffu, rank < before + upto);
+    if (mine != 0) {
+      const int of = __ffs(mine) - 1;
+      const int ahead = before + __shfl_sync(0xffffffffu, upto - tiles, of), n = __shfl_sync(0xffffffffu, tiles, of);
+      at.q0 = __shfl_sync(0xffffffffu, q0, of);
+      at.queries = __shfl_sync(0xffffffffu, q1 - q0, of);
+      at.first = (n - 1 - (rank - ahead)) * 2 * kTile;
+      const int seq = base - of;
+      at.k0 = min(max(p.k_offsets[seq], 0), p.k_rows);
+      at.keys = min(max(p.k_offsets[seq + 1], at.k0), p.k_rows) - at.k0;
+      return at;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return at;
+}
+// The tiles of keys that 128 queries from `first` on look at.
+__device__ __forceinline__ int KeyTiles(const PromptParams& p, const Place& at, int first) {
+  if (first >= at.queries) return 0;
+  const int last = min(at.queries, first + kTile) - 1;
+  const int seen = p.causal ? min(at.keys, max(0, last + 1 + at.keys - at.queries)) : at.keys;
+  return (seen + kTile - 1) / kTile;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __grid_constant__ PromptParams p) {
+  using G = Geometry<D>;
+  constexpr int kBoxes = D / 64, kBox = kTile * 128;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PromptCtl ctl;
+  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  const uint32_t smem = (Smem(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * G::kHeadTile;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      BarInit(Smem(&ctl.q_full[i]), 1);
+      BarInit(Smem(&ctl.s_full[i]), 1);
+      BarInit(Smem(&ctl.p_ready[i]), 4);
+      BarInit(Smem(&ctl.o_full[i]), 1);
+    }
+    for (int i = 0; i < G::kStages; ++i) {
+      BarInit(Smem(&ctl.full[i]), 1);
+      BarInit(Smem(&ctl.empty[i]), 1);
+    }
+    BarInit(Smem(&ctl.fixed), 1);
+    ctl.fault = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Smem(&ctl.tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 9 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.v) : "memory");
+  }
+  FenceBefore();
+  GridDependencyWait();
+  const int head = static_cast<int>(blockIdx.x) % p.q_heads;
+  const Place at = FindPlace(p, static_cast<int>(blockIdx.x) / p.q_heads);
+  const int tiles[2] = {at.first < 0 ? 0 : KeyTiles(p, at, at.first), at.first < 0 ? 0 : KeyTiles(p, at, at.first + kTile)};
+  const int most = max(tiles[0], tiles[1]);
+  // the last tile of values runs past the sequence's end
+  const bool fix = most > 0 && most * kTile > at.keys;
+  __syncthreads();
+  FenceAfter();
+  const uint32_t tmem = ctl.tmem;
+
+  if (warp < 8) {
+    // ---- softmax and output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    const int t = warp >> 2, row = at.first + t * kTile + (warp & 3) * 32 + lane;  // of the sequence
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t s_at = tmem + lanes + static_cast<uint32_t>(t * kTile), o_at = tmem + lanes + static_cast<uint32_t>(2 * kTile + t * D);
+    const int count = tiles[t], sees = p.causal ? min(at.keys, row + 1 + at.keys - at.queries) : at.keys;
+    const int first_sees = p.causal ? min(at.keys, at.first + t * kTile + (warp & 3) * 32 + 1 + at.keys - at.queries) : at.keys;  // the warp's first row
+    const float step = 8.f / p.scale;
+    float reference = -INFINITY;
+    float2 sum = make_float2(0.f, 0.f);
+    bool good = true;
+    for (int j = 0; j < count; ++j) {
+      if (!BarWait(Smem(&ctl.s_full[t]), static_cast<uint32_t>(j & 1), ctl)) {
+        good = false;
+        break;
+      }
+      __syncwarp();
+      FenceAfter();
+      float s[kTile];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) LoadColumns(s_at + 32 * i, s + 32 * i);
+      WaitLoads();
+      if ((j + 1) * kTile > first_sees) {
+        const int left = sees - j * kTile;
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) s[i] = i < left ? s[i] : -INFINITY;
+      }
+      float m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] = fmaxf(s[i], s[i + 4]);
+#pragma unroll
+        for (int e = i + 8; e < kTile; e += 8) m[i] = fmaxf(fmaxf(m[i], s[e]), s[e + 4]);
+      }
+      const float highest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      if (__any_sync(0xffffffffu, highest > reference + step)) {
+        const float to = fmaxf(reference, highest);
+        const float by = to == -INFINITY ? 1.f : Exp2((reference - to) * p.scale);
+        reference = to;
+        sum.x *= by;
+        sum.y *= by;
+        if (j > 0) {  // the products of the tile ahead have ended: S, which was issued after them, has
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            LoadColumns(o_at + c, o);
+            WaitLoads();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= by;
+            StoreColumns32(o_at + c, o);
+          }
+        }
+      }
+      const float offset = reference == -INFINITY ? 0.f : -reference * p.scale;
+      const float2 scale2 = make_float2(p.scale, p.scale), offset2 = make_float2(offset, offset);
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 v = Fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), scale2, offset2);
+          v.x = Exp2(v.x);
+          v.y = Exp2(v.y);
+          sum = Add2(sum, v);
+          w[i] = Pack<BF16>(v.x, v.y);
+        }
+        StoreColumns16(s_at + c / 2, w);
+      }
+      WaitStores();
+      FenceBefore();
+      __syncwarp();
+      if (lane == 0) BarArrive(Smem(&ctl.p_ready[t]));
+    }
+    if (at.first >= 0) {
+      if (count > 0 && good) good = BarWait(Smem(&ctl.o_full[t]), 0, ctl);
+      __syncwarp();
+      FenceAfter();
+      const float total = sum.x + sum.y, by = total == 0.f ? 0.f : 1.f / total;
+      const long long to = (static_cast<long long>(at.q0) + row) * p.q_heads + head;
+      const bool mine = row < at.queries;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (count > 0) {
+          LoadColumns(o_at + c, o);
+          WaitLoads();
+        }
+        if (mine) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = !good ? 0x7FFF7FFFu : count > 0 ? Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by) : 0u;
+          uint4* const dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+      }
+      if (mine && p.lse != nullptr) p.lse[to] = !good ? __uint_as_float(0x7FFFFFFFu) : total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+  }
+  if (warp == 8) {
+    // ---- products
+    constexpr uint32_t kType = BF16 ? 1u << 7 | 1u << 10 : 0u;
+    constexpr uint32_t kScores = 0x10u | kType | static_cast<uint32_t>(kTile >> 3) << 17 | 8u << 24;
+    constexpr uint32_t kOutputs = 0x10u | kType | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;  // V: the columns of a row lie beside one another
+    const unsigned long long q_desc = SmemDesc(smem, 16, 1024), k_desc = SmemDesc(ring, 16, 1024), v_desc = SmemDesc(ring, kBox, 1024);
+    bool good = true;
+    int ready = 0;  // stages seen full so far
+    auto wait = [&](int position) {  // for the copy of that number; they are waited for in order
+      for (; ready <= position && good; ++ready) good = BarWait(Smem(&ctl.full[ready % G::kStages]), static_cast<uint32_t>(ready / G::kStages & 1), ctl);
+      __syncwarp();
+      FenceAfter();
+    };
+    auto scores = [&](int t, int j) {
+      wait(2 * j);
+      if (!good) return;
+      const unsigned long long a = q_desc + static_cast<unsigned long long>(t * G::kHeadTile >> 4), b = k_desc + static_cast<unsigned long long>(2 * j % G::kStages * G::kHeadTile >> 4);
+      if (ElectOne()) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const unsigned long long off = static_cast<unsigned long long>((i / 4 * kBox + i % 4 * 32) >> 4);
+          MmaSs<false>(tmem + static_cast<uint32_t>(t * kTile), a + off, b + off, kScores, i > 0);
+        }
+        MmaCommit<false>(Smem(&ctl.s_full[t]));
+      }
+      __syncwarp();
+    };
+    auto release = [&](int position) {
+      if (ElectOne()) MmaCommit<false>(Smem(&ctl.empty[position % G::kStages]));
+      __syncwarp();
+    };
+    for (int t = 0; t < 2 && good; ++t) {
+      if (tiles[t] == 0) continue;
+      good = BarWait(Smem(&ctl.q_full[t]), 0, ctl);
+      if (good) scores(t, 0);
+    }
+    if (most > 0 && good) release(0);
+    for (int j = 0; j < most && good; ++j) {
+      for (int t = 0; t < 2 && good; ++t) {
+        if (j >= tiles[t]) continue;
+        good = BarWait(Smem(&ctl.p_ready[t]), static_cast<uint32_t>(j & 1), ctl);
+        if (good) wait(2 * j + 1);
+        if (good && fix && j == most - 1) {
+          good = BarWait(Smem(&ctl.fixed), 0, ctl);
+          FenceAfter();
+        }
+        if (!good) break;
+        __syncwarp();
+        const unsigned long long b = v_desc + static_cast<unsigned long long>((2 * j + 1) % G::kStages * G::kHeadTile >> 4);
+        if (ElectOne()) {
+#pragma unroll
+          for (int i = 0; i < kTile / 16; ++i)
+            MmaTs(tmem + static_cast<uint32_t>(2 * kTile + t * D), tmem + static_cast<uint32_t>(t * kTile + 8 * i), b + static_cast<unsigned long long>(2048 * i >> 4), kOutputs,
+                  j > 0 || i > 0);
+          if (j + 1 == tiles[t]) MmaCommit<false>(Smem(&ctl.o_full[t]));
+        }
+        __syncwarp();
+        if (j + 1 < tiles[t]) scores(t, j + 1);
+      }
+      if (!good) break;
+      release(2 * j + 1);
+      if (j + 1 < most) release(2 * j + 2);
+    }
+    if (!good) ctl.fault = 1;
+  } else if (warp == 9) {
+    // ---- copies
+    bool good = !p.give_up;
+    auto load = [&](uint32_t dst, const CUtensorMap* map, int of, int row, uint32_t bar) {
+      if (ElectOne()) {
+        BarExpect(bar, G::kHeadTile);
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b) TmaLoad3(dst + static_cast<uint32_t>(b * kBox), map, 64 * b, of, row, bar);
+      }
+      __syncwarp();
+    };
+    const int of = head / p.group;
+    if (!good) ctl.fault = 1;
+    for (int position = 0; position < 2 * most && good; ++position) {
+      const int stage = position % G::kStages, j = position >> 1;
+      if (position >= G::kStages) good = BarWait(Smem(&ctl.empty[stage]), static_cast<uint32_t>(position / G::kStages - 1 & 1), ctl);
+      __syncwarp();
+      if (!good) break;
+      if (position == 0) {
+        for (int t = 0; t < 2; ++t) {
+          if (tiles[t] > 0) load(smem + static_cast<uint32_t>(t * G::kHeadTile), &p.q, head, at.q0 + at.first + t * kTile, Smem(&ctl.q_full[t]));
+          if (t == 0) load(ring, &p.k, of, at.k0, Smem(&ctl.full[0]));
+        }
+        continue;
+      }
+      load(ring + static_cast<uint32_t>(stage * G::kHeadTile), position & 1 ? &p.v : &p.k, of, at.k0 + j * kTile, Smem(&ctl.full[stage]));
+    }
+    if (fix && good) {
+      // what lies past the sequence's end may be no number, and a weight of zero does not undo that
+      const int position = 2 * most - 1, stage = position % G::kStages;
+      good = BarWait(Smem(&ctl.full[stage]), static_cast<uint32_t>(position / G::kStages & 1), ctl);
+      const int keep = at.keys - (most - 1) * kTile;
+      const uint32_t zero[4] = {0, 0, 0, 0};
+      for (int b = 0; b < kBoxes && good; ++b) {
+        for (int i = lane; i < (kTile - keep) * 8; i += 32) Sts128(ring + static_cast<uint32_t>(stage * G::kHeadTile + b * kBox + keep * 128 + i * 16), zero);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && good) BarArrive(Smem(&ctl.fixed));
+    }
+  }
+  if (ctl.fault != 0) {
+    for (int i = 0; i < 16; ++i) __nanosleep(1000000);  // copies and products may still be under way
+  }
+  FenceBefore();
+  __syncthreads();
+  FenceAfter();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+bool EncodeHeads(CUtensorMap* map, const void* x, int dtype, int dim, int heads, int64_t rows, int64_t ld) {
+  const TensorMapEncodeFn encode = TensorMapEncoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, static_cast<cuuint64_t>(ld) * 2};
+  const cuuint32_t box[3] = {64, 1, kTile}, one[3] = {1, 1, 1};
+  return encode(map, dtype == QFG_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(x), dims, strides, box, one,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+cudaError_t Launch(const PromptParams& p, unsigned blocks, cudaStream_t stream) {
+  using G = Geometry<D>;
+  static_assert(G::kBytes + static_cast<int>(sizeof(PromptCtl)) <= 227 * 1024 && G::kStages <= 8, "");
+  const cudaError_t set = cudaFuncSetAttribute(PromptAttentionKernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
+  if (set != cudaSuccess) return set;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = G::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {OverlapAttribute()};
+  cfg.attrs = attr;
+  cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, PromptAttentionKernel<D, BF16>, p);
+}
+
+}  // namespace
+
+cudaError_t LaunchPromptAttention(const PromptCall& c, cudaStream_t stream) {
+  PromptParams p = {};
+  // without keys nothing is copied, and any map will do
+  const bool keys = c.k_rows > 0;
+  if (!EncodeHeads(&p.q, c.q, c.dtype, c.dim, c.q_heads, c.q_rows, c.ldq) ||
+      !EncodeHeads(&p.k, keys ? c.k : c.q, c.dtype, c.dim, keys ? c.kv_heads : c.q_heads, keys ? c.k_rows : c.q_rows, keys ? c.ldk : c.ldq) ||
+      !EncodeHeads(&p.v, keys ? c.v : c.q, c.dtype, c.dim, keys ? c.kv_heads : c.q_heads, keys ? c.k_rows : c.q_rows, keys ? c.ldv : c.ldq))
+    return cudaErrorInvalidValue;
+  p.q_offsets = c.q_offsets;
+  p.k_offsets = c.k_offsets;
+  p.out = c.out;
+  p.lse = c.lse;
+  p.seqs = c.seqs;
+  p.q_rows = static_cast<int>(c.q_rows);
+  p.k_rows = static_cast<int>(c.k_rows);
+  p.q_heads = c.q_heads;
+  p.group = c.q_heads / c.kv_heads;
+  p.scale = c.scale * 1.44269504f;
+  p.causal = c.causal;
+  p.give_up = c.give_up;
+  // sequences of any lengths that add up to the rows have no more tiles than this
+  const long long blocks = (c.q_rows / (2 * kTile) + std::min<long long>(c.seqs, c.q_rows)) * c.q_heads;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  const unsigned n = static_cast<unsigned>(blocks);
+  cudaError_t err;
+  if (c.dtype == QFG_BFLOAT16) {
+    err = c.dim == 64 ? Launch<64, true>(p, n, stream) : Launch<128, true>(p, n, stream);
+  } else {
+    err = c.dim == 64 ? Launch<64, false>(p, n, stream) : Launch<128, false>(p, n, stream);
+  }
+  const cudaError_t last = cudaGetLastError();
+  return err == cudaSuccess ? last : err;
+}
+
+}  // namespace qfg

@@ -355,4 +355,84 @@ struct RowQuantCall {
 };
 cudaError_t LaunchRowQuant(const RowQuantCall& call, cudaStream_t stream);
 
+// ------------------------------------------------------------------------------ heads and their cache
+// A cache as its kernels see it: a page of one head holds its tokens one after another.
+struct KvCacheView {
+  uint8_t *k = nullptr, *v = nullptr;        // [pages][heads][page][dim], or dim / 2 in four bits
+  void *k_scale = nullptr, *v_scale = nullptr;  // FP32 [pages][heads][page], or E4M3 [pages][heads][page][dim / 16]
+  long long pages = 0;
+  int heads = 0, page = 0, dim = 0;
+  bool fp4 = false;
+  float k_unit = 1.f, v_unit = 1.f;
+};
+// cache_rows.cu
+struct RotaryPair {
+  unsigned long long turns;  // of a position, as a fraction of 2^64
+  long long axis;
+};
+struct HeadsCall {
+  int dtype = 0, dim = 0;
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // q null: keys alone; v: where slots are given
+  int64_t ldq = 0, ldk = 0, ldv = 0;                    // elements from token to token
+  int q_heads = 0, kv_heads = 0;
+  const void *q_weight = nullptr, *k_weight = nullptr;  // null: no norm
+  int weight_dtype = 0;
+  float weight_offset = 0.f, eps = 0.f;
+  const RotaryPair* pairs = nullptr;
+  int n_pairs = 0;
+  bool interleaved = false, positions_64 = true;
+  float rotary_scale = 1.f;
+  const void* positions = nullptr;
+  int64_t ld_positions = 0;
+  int64_t tokens = 0;
+  void *q_out = nullptr, *k_out = nullptr;  // contiguous
+  KvCacheView cache;
+  const int64_t* slots = nullptr;  // null: nothing goes into a cache
+};
+cudaError_t LaunchHeadRows(const HeadsCall& call, cudaStream_t stream);
+struct CacheReadCall {
+  KvCacheView cache;
+  const int* table = nullptr;
+  int64_t ld_table = 0;
+  int seqs = 0, most_pages = 0;
+  const int* offsets = nullptr;
+  int64_t rows = 0;
+  int dtype = 0;
+  void *k_out = nullptr, *v_out = nullptr;
+};
+cudaError_t LaunchCacheRead(const CacheReadCall& call, cudaStream_t stream);
+// cache_attention.cu
+struct CacheAttentionCall {
+  KvCacheView cache;
+  int dtype = 0;
+  const void* q = nullptr;
+  int64_t ld_seq = 0, ld_token = 0;  // of q, in elements
+  int seqs = 0, tokens = 0, q_heads = 0;
+  const int* table = nullptr;
+  int64_t ld_table = 0;
+  int most_pages = 0;
+  const int* lengths = nullptr;
+  float scale = 1.f;
+  void* out = nullptr;   // contiguous
+  float* lse = nullptr;  // or null
+  void* workspace = nullptr;
+  bool give_up = false;  // testing
+};
+size_t CacheAttentionWorkspace(const CacheAttentionCall& call);  // bytes
+cudaError_t LaunchCacheAttention(const CacheAttentionCall& call, cudaStream_t stream);
+// prompt_attention.cu
+struct PromptCall {
+  int dtype = 0, dim = 0, q_heads = 0, kv_heads = 0, seqs = 0;
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  int64_t ldq = 0, ldk = 0, ldv = 0;  // elements from token to token
+  int64_t q_rows = 0, k_rows = 0;
+  const int *q_offsets = nullptr, *k_offsets = nullptr;
+  bool causal = true;
+  float scale = 1.f;
+  void* out = nullptr;   // contiguous
+  float* lse = nullptr;  // or null
+  bool give_up = false;  // testing
+};
+cudaError_t LaunchPromptAttention(const PromptCall& call, cudaStream_t stream);
+
 }  // namespace qfg

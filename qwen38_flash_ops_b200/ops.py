@@ -49,7 +49,8 @@ except ImportError as e:
     _handed_back = lambda *args: None
     _calls = SimpleNamespace(bind=_handed_back, skinny_gemm=_handed_back, argmax_rows=_handed_back, dequant=_handed_back,
                              lmhead=_handed_back, shared_expert_down=_handed_back, bind_rows=_handed_back, bind_mlp=_handed_back, rmsnorm_quant=_handed_back,
-                             row_quant=_handed_back, quant_gemm=_handed_back, quant_mlp=_handed_back)
+                             row_quant=_handed_back, quant_gemm=_handed_back, quant_mlp=_handed_back, bind_heads=_handed_back, qk_norm_rope=_handed_back,
+                             cache_write=_handed_back, cache_read=_handed_back, cache_attention=_handed_back, prompt_attention=_handed_back)
 _bound = False
 
 
@@ -64,6 +65,9 @@ def _load():
         _calls.bind_rows(*[ctypes.cast(getattr(lib, name), c_void_p).value
                            for name in ("qfg_rmsnorm_quant", "qfg_row_quant", "qfg_quant_gemm_compute")])
         _calls.bind_mlp(*[ctypes.cast(getattr(lib, name), c_void_p).value for name in ("qfg_quant_mlp_workspace_bytes", "qfg_quant_mlp")])
+        _calls.bind_heads(*[ctypes.cast(getattr(lib, name), c_void_p).value
+                            for name in ("qfg_qk_norm_rope_compute", "qfg_cache_write", "qfg_cache_read", "qfg_cache_attention_workspace_bytes",
+                                         "qfg_cache_attention", "qfg_prompt_attention")])
         _bound = True
     return lib
 
