@@ -16,116 +16,168 @@
 // Softmax runs along: m is taken up only when a score passes it by 8 (in powers of two), so that sums and weights stay within 2^8 of what they would be and the outputs
 // are seldom scaled again.  Statistics and sums are FP32, weights FP16 (2^-11 of themselves, as the values are exact).
 //
-// A warp has its own ring of tiles in shared memory, which it fills by bulk copies, and its own sums; no warp waits for another before the end of a unit.  A unit is a run
-// of tiles of one sequence for one key head; sequences are cut so that units are of nearly one size, by their lengths, which only the device knows.  A second kernel joins
-// the parts of the sequences that were cut, in their order, so that results do not depend on which block is first.
+// A block runs through an equal share of all tiles (of one sequence and key head after another, in that order), its warps taking turns; each warp has its own ring of
+// tiles in shared memory, which it fills by asynchronous copies ahead of itself, across the borders of sequences and heads too.  Where a sequence and head ends the warps add up
+// their sums.  Shares begin and end anywhere; a second kernel joins those parts that share a sequence and head, in their order, so that results do not depend on which
+// block is first.  Lengths are on the device only: where the shares lie is worked out there.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <climits>
+#include <type_traits>
 
 #include "qfg_internal.h"
 #include "stream_order.cuh"
-#include "tc_ptx.cuh"
 
 namespace qfg {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kLeastTiles = kWarps;  // of a unit: a tile a warp
+constexpr int kLeastTiles = kWarps;  // of a block's share: a tile a warp
 
+// All tiles, in equal shares: share i begins at tile size i + min(i, more).
+struct Shares {
+  long long size;
+  int more, count;
+  __device__ __forceinline__ long long begin(int i) const { return size * i + min(i, more); }
+};
+struct alignas(16) ShareInfo {  // what the second kernel needs to know of a share: where it begins
+  int seq, unit, tile, tiles;
+};
 struct AttendParams {
   KvCacheView cache;
   const void* q;
   const int *table, *lengths;
-  float* partial;
+  Shares* shares;
+  ShareInfo* share;   // [blocks]
+  float* partial;     // [blocks][2][rows (D + 2)]: of a share that begins within a unit, and of its last unit where that goes on
   void* out;
   float* lse;
   long long ld_seq, ld_token, ld_table;
-  int seqs, tokens, q_heads, group, most_pages, row_blocks, target_units;
+  int seqs, tokens, q_heads, group, most_pages, row_blocks;
   float scale;  // of scores, in powers of two, with the keys' unit
-  bool bf16, give_up;
+  bool bf16;
 };
 
-template <int D, bool FP4>
+constexpr int TileOf(int dim, bool fp4) { return (fp4 ? dim / 2 + dim / 16 : dim + 4) * 64 <= 9300 && (fp4 || dim == 64) ? 32 : 16; }
+template <int D, bool FP4, int NT>
 struct Geometry {
   static constexpr int kCodes = FP4 ? D / 2 : D, kScales = FP4 ? D / 16 : 4;  // bytes of a row
-  static constexpr int kTile = (kCodes + kScales) * 64 <= 9000 ? 32 : 16;     // tokens
+  static constexpr int kTile = TileOf(D, FP4);                                // tokens
   static constexpr int kPart = kTile * (kCodes + kScales);                    // keys or values of a tile
   static constexpr int kStage = 2 * kPart;
-  static constexpr int kStages = std::min(8, 220 * 1024 / 2 / (kWarps * kStage) >= 2 ? 220 * 1024 / 2 / (kWarps * kStage) : 220 * 1024 / (kWarps * kStage));
-  static constexpr int kBytes = kWarps * kStages * kStage;
+  static constexpr int kBlocks = D * NT <= 128 ? 2 : 1;                       // of an SM
+  static constexpr int kSums = kWarps * 8 * NT * D * 4;                       // the warps' sums
+  static constexpr int kRoom = (kBlocks == 2 ? 111 : 222) * 1024 - kSums;
+  static constexpr int kStages = std::min(8, kRoom / (kWarps * kStage));
+  static constexpr int kBytes = kWarps * kStages * kStage + kSums;
 };
 
-struct AttendCtl {
-  unsigned long long full[kWarps][8];
-  float most[kWarps][16], sum[kWarps][16];
-  int scan[kWarps];
-  long long total[kWarps];
-  volatile uint32_t fault;
-};
-
-// How the sequences are cut: into pieces of `tiles` tiles; `first` is the number of pieces of the sequences ahead.
-struct Cut {
-  int seq, first, tiles, pieces;
-};
 __device__ __forceinline__ int TilesOf(const AttendParams& p, int seq, int tile, int* length) {
   const long long room = static_cast<long long>(p.most_pages) * p.cache.page;
   *length = static_cast<int>(min(static_cast<long long>(max(p.lengths[seq], 0)), room));
   return (*length + tile - 1) / tile;
 }
-// Of the sequence that holds piece `piece` (or of sequence `seq`, where it is not negative), for every thread of the block; seq is -1 where there is none.
-template <int THREADS>
-__device__ Cut FindCut(const AttendParams& p, int tile, int piece, int seq) {
-  constexpr int kW = THREADS / 32;
-  __shared__ long long total[kW];
-  __shared__ int sums[kW];
-  __shared__ Cut found;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int length;
-  long long mine = 0;
-  for (int i = threadIdx.x; i < p.seqs; i += THREADS) mine += TilesOf(p, i, tile, &length);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0) total[warp] = mine;
-  if (threadIdx.x == 0) found = {-1, 0, 0, 0};
-  __syncthreads();
+// This block's share, `from` to `to`, and the sequence that holds `from`, with the number of tiles ahead of it.  A sequence's tiles count once for each key head and
+// block of rows.
+struct Share {
+  Shares all;
+  long long from, to, ahead;
+  int seq, tiles, length;  // seq is -1 where there is no share
+};
+__device__ __forceinline__ Share FindShare(const AttendParams& p, int tile) {
+  __shared__ int sums[kWarps];
+  __shared__ long long total[kWarps];
+  __shared__ Share found;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_seq = p.cache.heads * p.row_blocks;
+  int length = 0;
   long long all = 0;
+  if (p.seqs > kThreads) {
+    for (int i = threadIdx.x; i < p.seqs; i += kThreads) all += TilesOf(p, i, tile, &length);
 #pragma unroll
-  for (int i = 0; i < kW; ++i) all += total[i];
-  const long long units = all * p.cache.heads * p.row_blocks;
-  const int most = static_cast<int>(max(static_cast<long long>(kLeastTiles), (units + p.target_units - 1) / p.target_units));
-  int before = 0;
-  for (int base = 0; base < p.seqs; base += THREADS) {
+    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    if (lane == 0) total[warp] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all += total[w];
+  }
+  Share s;
+  s.seq = -1;
+  long long before = 0;
+  for (int base = 0; base < p.seqs; base += kThreads) {
     const int i = base + static_cast<int>(threadIdx.x);
     const int tiles = i < p.seqs ? TilesOf(p, i, tile, &length) : 0;
-    const int pieces = i < p.seqs ? max(1, (tiles + most - 1) / most) : 0;
-    int upto = pieces;
+    int upto = tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += v;
     }
-    __syncthreads();
+    if (base > 0) __syncthreads();
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    int ahead = before;
+    long long ahead = before;
 #pragma unroll
-    for (int w = 0; w < kW; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) ahead += sums[w];
       before += sums[w];
     }
-    const int begin = ahead + upto - pieces;
-    // pieces of one sequence are of one size, to a tile
-    if (i < p.seqs && (seq >= 0 ? i == seq : piece >= begin && piece < begin + pieces)) found = {i, begin, (tiles + pieces - 1) / pieces, pieces};
+    if (base == 0) {
+      if (p.seqs <= kThreads) all = before;
+      all *= per_seq;
+      s.all.count = static_cast<int>(min(static_cast<long long>(gridDim.x), (all + kLeastTiles - 1) / kLeastTiles));
+      if (static_cast<int>(blockIdx.x) >= s.all.count) return s;
+      s.all.size = all >> 32 ? all / s.all.count : static_cast<uint32_t>(all) / static_cast<uint32_t>(s.all.count);
+      s.all.more = static_cast<int>(all - s.all.size * s.all.count);
+      s.from = s.all.begin(blockIdx.x);
+      s.to = s.all.begin(blockIdx.x + 1);
+    }
+    const long long begin = (ahead + upto - tiles) * per_seq, end = (ahead + upto) * per_seq;
+    if (s.from >= begin && s.from < end) {
+      found = s;
+      found.ahead = begin;
+      found.seq = i;
+      found.tiles = tiles;
+      found.length = length;
+    }
   }
   __syncthreads();
   return found;
 }
+// A run of tiles of one unit: a key head of a sequence, and a block of its rows.
+struct Segment {
+  int seq, unit, tile, tiles, length;  // tile: the first; tiles: of the whole unit
+  int begin, end;                      // in the share
+};
+__device__ __forceinline__ Segment FirstSegment(const Share& s) {
+  Segment g;
+  g.seq = s.seq;
+  g.tiles = s.tiles;
+  g.length = s.length;
+  const long long into = s.from - s.ahead;
+  const int in = static_cast<int>(into >> 32 ? into / g.tiles : static_cast<uint32_t>(into) / static_cast<uint32_t>(g.tiles));
+  g.unit = in;
+  g.tile = static_cast<int>(s.from - s.ahead - static_cast<long long>(in) * g.tiles);
+  g.begin = 0;
+  g.end = static_cast<int>(min(s.to - s.from, static_cast<long long>(g.tiles - g.tile)));
+  return g;
+}
+__device__ __forceinline__ void NextSegment(const AttendParams& p, int count, int tile, Segment* g) {  // while g->end < count
+  g->begin = g->end;
+  g->tile = 0;
+  if (++g->unit == p.cache.heads * p.row_blocks) {
+    g->unit = 0;
+    do g->tiles = TilesOf(p, ++g->seq, tile, &g->length);
+    while (g->tiles == 0);
+  }
+  g->end = g->begin + min(count - g->begin, g->tiles);
+}
 
+__device__ __forceinline__ void CopyAsync(uint32_t to, const uint8_t* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ uint32_t Smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void Mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -148,6 +200,17 @@ __device__ __forceinline__ float Log2(float v) {
 __device__ __forceinline__ uint32_t Mul16(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// a half of a pair, twice: the multiplication takes it so
+__device__ __forceinline__ uint32_t Lower(uint32_t v) {
+  uint32_t r;
+  asm("{ .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n mov.b32 %0, {l, l};\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t Upper(uint32_t v) {
+  uint32_t r;
+  asm("{ .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n mov.b32 %0, {h, h};\n}" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ uint32_t Pack16(float lo, float hi) {
@@ -184,452 +247,519 @@ __device__ __forceinline__ void LoadShared(uint32_t a, uint32_t* v) {
   }
 }
 
+template <int D>
+__device__ __forceinline__ void StoreRow(const AttendParams& p, int seq, int unit, int row, int channel, float2 y, float most, float total) {
+  const int head = unit / p.row_blocks, token = row / p.group, of = head * p.group + row - token * p.group;
+  const long long to = (static_cast<long long>(seq) * p.tokens + token) * p.q_heads + of;
+  const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
+  if (p.bf16) {
+    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + to * D + channel) = __floats2bfloat162_rn(y.x * by, y.y * by);
+  } else {
+    *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + to * D + channel) = __floats2half2_rn(y.x * by, y.y * by);
+  }
+  if (p.lse != nullptr && channel == 0) p.lse[to] = total == 0.f ? -INFINITY : (most + Log2(total)) * 0.693147181f;
+}
+
 // NT tiles of eight rows.
 template <int D, bool FP4, int NT>
-__global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 2 : 1) CacheAttentionKernel(const AttendParams p) {
-  using G = Geometry<D, FP4>;
+__global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) CacheAttentionKernel(const AttendParams p) {
+  using G = Geometry<D, FP4, NT>;
   constexpr int kRows = 8 * NT, kSteps = D / 16, kGroups = G::kTile / 16;
   constexpr int kKeyBytes = G::kCodes / 4, kValueBytes = G::kCodes / 8;  // of a lane's part of a row
   constexpr int kKeyScales = FP4 ? D / 64 : 1;                           // E4M3 scales of that part
   constexpr int kValueChannels = D / 8, kTilesOfO = D / 16;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ AttendCtl ctl;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float row_most[kWarps][kRows], row_sum[kWarps][kRows];
+  __shared__ __align__(16) uint16_t q_rows[kRows][D + 8];
+  __shared__ float q_factor[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < G::kStages; ++i) BarInit(Smem(&ctl.full[warp][i]), 1);
-    if (warp == 0) ctl.fault = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   GridDependencyWait();
-  const int heads = p.cache.heads, per_piece = heads * p.row_blocks;
-  const Cut cut = FindCut<kThreads>(p, G::kTile, static_cast<int>(blockIdx.x) / per_piece, -1);  // its barriers: the ring's exist for all
-  if (cut.seq < 0) return;
-  const int in_piece = static_cast<int>(blockIdx.x) % per_piece, head = in_piece / p.row_blocks, row0 = in_piece % p.row_blocks * kRows;
-  const int piece = static_cast<int>(blockIdx.x) / per_piece - cut.first, rows = min(kRows, p.tokens * p.group - row0);
-  int length;
-  const int tiles = TilesOf(p, cut.seq, G::kTile, &length);
-  const int tile0 = piece * cut.tiles, tile1 = min(tiles, tile0 + cut.tiles);
-
-  // q, and the factor from a row's products to its scores
-  uint32_t q[NT][kSteps][2];
-  float factor[NT][2];
-  int sees[NT][2];  // tokens that a row may look at
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int row = row0 + 8 * n + g, token = row / p.group, of = head * p.group + row - token * p.group;
-    const bool real = 8 * n + g < rows;
-    const uint16_t* const at = static_cast<const uint16_t*>(p.q) + (real ? cut.seq * p.ld_seq + token * p.ld_token + static_cast<long long>(of) * D + c * (D / 4) : 0);
-    uint32_t raw[kSteps][2];
-    float most = 0.f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint2 w = real ? *reinterpret_cast<const uint2*>(at + 4 * s) : make_uint2(0, 0);
-      raw[s][0] = w.x, raw[s][1] = w.y;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 v = p.bf16 ? make_float2(__uint_as_float(raw[s][e] << 16), __uint_as_float(raw[s][e] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<__half2*>(&raw[s][e]));
-        most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
-      }
-    }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    // 2^(9 - exponent) and its inverse; the exponent is kept where both are ordinary numbers
-    const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 20), 240);
-    const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(e - 9) << 23);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float2 v = p.bf16 ? make_float2(__uint_as_float(raw[s][h] << 16), __uint_as_float(raw[s][h] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<__half2*>(&raw[s][h]));
-        q[n][s][h] = Pack16(v.x * up, v.y * up);
-      }
-    }
-    const int see = length - p.tokens + 1 + token;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      factor[n][h] = __shfl_sync(0xffffffffu, down, (2 * c + h) * 4) * p.scale;
-      sees[n][h] = __shfl_sync(0xffffffffu, see, (2 * c + h) * 4);
+  GridLaunchDependents();  // the second kernel, which waits for all of this one
+  const Share share = FindShare(p, G::kTile);
+  for (int seq = blockIdx.x; seq < p.seqs; seq += gridDim.x) {
+    int length;
+    if (TilesOf(p, seq, G::kTile, &length) > 0) continue;
+    for (int unit = 0; unit < p.cache.heads * p.row_blocks; ++unit) {
+      const int row0 = unit % p.row_blocks * kRows, rows = min(kRows, p.tokens * p.group - row0);
+      for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) StoreRow<D>(p, seq, unit, row0 + i / (D / 2), i % (D / 2) * 2, make_float2(0.f, 0.f), 0.f, 0.f);
     }
   }
-  const int least_seen = length - p.tokens + 1;
+  if (share.seq < 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.shares != nullptr) *p.shares = {0, 0, 0};
+    return;
+  }
+  Segment at = FirstSegment(share);
+  if (threadIdx.x == 0 && p.shares != nullptr) {
+    p.share[blockIdx.x] = {at.seq, at.unit, at.tile, at.tiles};
+    if (blockIdx.x == 0) *p.shares = share.all;
+  }
+  const int count = static_cast<int>(share.to - share.from);
 
-  // ---- this warp's tiles: tile0 + warp, kWarps further, ...
-  const int count = tile0 + warp < tile1 ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;
-  const uint32_t ring = Smem(smem) + static_cast<uint32_t>(warp * G::kStages * G::kStage), bars = Smem(&ctl.full[warp][0]);
-  const int* const table = p.table + cut.seq * p.ld_table;
-  int ids = 0;              // lane i: the page of tile (i mod 32) of this warp
-  uint32_t present = 0;     // bit i mod 32: that page is one of the cache
-  bool good = !p.give_up;
-  auto issue = [&](int i) {
-    const int at = tile0 + warp + i * kWarps;  // of the sequence
-    if ((i & 31) == 0) {
-      const int mine = at + lane * kWarps;
-      ids = mine < tile1 ? table[static_cast<long long>(mine) * G::kTile / p.cache.page] : 0;
-    }
-    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
-    const bool is = id >= 0 && id < p.cache.pages;
-    present = (present & ~(1u << (i & 31))) | (is ? 1u << (i & 31) : 0u);
-    if (lane == 0) {
-      const long long row = (static_cast<long long>(is ? id : 0) * heads + head) * p.cache.page + at * G::kTile % p.cache.page;
-      const uint32_t to = ring + static_cast<uint32_t>(i % G::kStages * G::kStage), bar = bars + i % G::kStages * 8;
-      BarExpect(bar, G::kStage);
-      BulkLoad(to, p.cache.k + row * G::kCodes, G::kTile * G::kCodes, bar);
-      BulkLoad(to + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.k_scale) + row * G::kScales, G::kTile * G::kScales, bar);
-      BulkLoad(to + G::kPart, p.cache.v + row * G::kCodes, G::kTile * G::kCodes, bar);
-      BulkLoad(to + G::kPart + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.v_scale) + row * G::kScales, G::kTile * G::kScales, bar);
+  // q of a segment's rows, as FP16, for all warps: row w (and w + 8) by warp w
+  auto make_q = [&](const Segment& of) {
+    const int head = of.unit / p.row_blocks, row0 = (of.unit - head * p.row_blocks) * kRows;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = 8 * n + warp, token = (row0 + r) / p.group;
+      uint32_t w[D / 64] = {};
+      if (row0 + r < p.tokens * p.group) {
+        const uint16_t* const from = static_cast<const uint16_t*>(p.q) + of.seq * p.ld_seq + token * p.ld_token +
+                                     static_cast<long long>(head * p.group + row0 + r - token * p.group) * D + lane * (D / 32);
+        if constexpr (D == 64) w[0] = *reinterpret_cast<const uint32_t*>(from);
+        if constexpr (D == 128) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(from);
+        if constexpr (D == 256) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(from);
+      }
+      float2 v[D / 64];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        v[i] = p.bf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<__half2*>(&w[i]));
+        top = max(top, max(__float_as_uint(v[i].x) & 0x7FFFFFFFu, __float_as_uint(v[i].y) & 0x7FFFFFFFu));
+      }
+      // 2^(9 - exponent) of the largest and its inverse; the exponent is kept where both are ordinary numbers
+      const int e = min(max(static_cast<int>(__reduce_max_sync(0xffffffffu, top) >> 23), 20), 240);
+      const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) *reinterpret_cast<uint32_t*>(&q_rows[r][lane * (D / 32) + 2 * i]) = Pack16(v[i].x * up, v[i].y * up);
+      if (lane == 0) q_factor[r] = __uint_as_float(static_cast<uint32_t>(e - 9) << 23) * p.scale;
     }
   };
-  if (good) {
-    for (int i = 0; i < min(count, G::kStages); ++i) issue(i);
-  }
 
-  float o[NT][kTilesOfO][4];
-  float most[NT][2], sum[NT][2];
+  // ---- this warp's tiles: warp, warp + kWarps, ... of the share
+  const uint32_t ring = Smem(smem) + G::kSums + static_cast<uint32_t>(warp * G::kStages * G::kStage);
+  Segment ahead = at;
+  int next = warp, batch = 0, issued = 0;  // the tile that is copied next; the first one that `row` is of
+  bool known = false;
+  long long row = 0;     // lane i: where tile batch + i kWarps lies in the cache, or -1: in no page of it
+  uint32_t present = 0;  // of the stages
+  const int tiles_of_page = p.cache.page / G::kTile;
+  auto copy = [&](uint32_t to, const uint8_t* from, auto bytes) {
+    constexpr int kBytes = decltype(bytes)::value;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) most[n][h] = -INFINITY, sum[n][h] = 0.f;
-#pragma unroll
-    for (int m = 0; m < kTilesOfO; ++m) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][m][e] = 0.f;
+    for (int i = 0; i < kBytes; i += 512) {
+      if (i + 512 <= kBytes || 16 * lane < kBytes - i) CopyAsync(to + i + 16 * lane, from + i + 16 * lane);
     }
-  }
+  };
+  auto issue = [&] {
+    if (next < count) {
+      while (next >= ahead.end) {
+        NextSegment(p, count, G::kTile, &ahead);
+        known = false;
+      }
+      if (!known || next - batch >= 32 * kWarps) {
+        batch = next;
+        known = true;
+        const int mine = next + lane * kWarps;
+        row = -1;
+        if (mine < ahead.end) {
+          const int tile = ahead.tile + mine - ahead.begin, page = tile / tiles_of_page, id = p.table[ahead.seq * p.ld_table + page];
+          if (id >= 0 && id < p.cache.pages)
+            row = (static_cast<long long>(id) * p.cache.heads + ahead.unit / p.row_blocks) * p.cache.page + (tile - page * tiles_of_page) * G::kTile;
+        }
+      }
+      const long long from = __shfl_sync(0xffffffffu, row, (next - batch) / kWarps), r = max(from, 0LL);
+      present = (present & ~(1u << issued)) | (from >= 0 ? 1u << issued : 0u);
+      const uint32_t to = ring + static_cast<uint32_t>(issued * G::kStage);
+      copy(to, p.cache.k + r * G::kCodes, std::integral_constant<int, G::kTile * G::kCodes>());
+      copy(to + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.k_scale) + r * G::kScales, std::integral_constant<int, G::kTile * G::kScales>());
+      copy(to + G::kPart, p.cache.v + r * G::kCodes, std::integral_constant<int, G::kTile * G::kCodes>());
+      copy(to + G::kPart + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.v_scale) + r * G::kScales, std::integral_constant<int, G::kTile * G::kScales>());
+      issued = issued + 1 == G::kStages ? 0 : issued + 1;
+      next += kWarps;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");  // one a tile, of nothing behind the last
+  };
+#pragma unroll 1
+  for (int i = 0; i < G::kStages; ++i) issue();
+  make_q(at);
+  __syncthreads();
 
-  for (int i = 0; i < count && good; ++i) {
-    const uint32_t at = ring + static_cast<uint32_t>(i % G::kStages * G::kStage);
-    if (!BarWait(bars + i % G::kStages * 8, static_cast<uint32_t>(i / G::kStages & 1), ctl)) {
-      good = false;
-      break;
-    }
-    const int token0 = (tile0 + warp + i * kWarps) * G::kTile;
-    const bool absent = !(present >> (i & 31) & 1);
-    const bool whole = token0 + G::kTile <= least_seen && !absent;  // no row leaves any token of it out
-    // ---- scores
-    float s[kGroups][NT][4];
+  int x = warp, stage = 0;
+#pragma unroll 1
+  for (;;) {  // segments
+    const int head = at.unit / p.row_blocks, row0 = (at.unit - head * p.row_blocks) * kRows, rows = min(kRows, p.tokens * p.group - row0);
+    float o[NT][kTilesOfO][4];
+    float most[NT][2], sum[NT][2];
 #pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) most[n][h] = -INFINITY, sum[n][h] = 0.f;
+#pragma unroll
+      for (int m = 0; m < kTilesOfO; ++m) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][m][e] = 0.f;
+      }
+    }
+    const bool any = x < at.end;
+    if (any) {
+      uint32_t q[NT][kSteps][2];
+      float factor[NT][2];  // from a row's products to its scores
+      int sees[NT][2];      // tokens that a row may look at
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][n][e] = 0.f;
+        for (int i = 0; i < kSteps; ++i) {
+          const uint2 w = *reinterpret_cast<const uint2*>(&q_rows[8 * n + g][c * (D / 4) + 4 * i]);
+          q[n][i][0] = w.x, q[n][i][1] = w.y;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          factor[n][h] = q_factor[8 * n + 2 * c + h];
+          sees[n][h] = at.length - p.tokens + 1 + (row0 + 8 * n + 2 * c + h) / p.group;
+        }
       }
-      uint32_t raw[2][kKeyBytes / 4], scale[2];
+      const int least_seen = at.length - p.tokens + 1;
+
+#pragma unroll 1
+      for (; x < at.end; x += kWarps) {
+        const uint32_t tile = ring + static_cast<uint32_t>(stage * G::kStage);
+        asm volatile("cp.async.wait_group %0;" ::"n"(G::kStages - 1) : "memory");
+        __syncwarp();
+        const int token0 = (at.tile + x - at.begin) * G::kTile;
+        const bool absent = !(present >> stage & 1);
+        const bool whole = token0 + G::kTile <= least_seen && !absent;  // no row leaves any token of it out
+        // ---- scores: s[u][n][2 h + r] is token 16 u + 8 h + g, row 8 n + 2 c + r
+        float s[kGroups][NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t token = static_cast<uint32_t>(16 * u + 8 * h + g);
-        LoadShared<kKeyBytes>(at + token * G::kCodes + c * kKeyBytes, raw[h]);
-        if constexpr (FP4) LoadShared<kKeyScales>(at + G::kTile * G::kCodes + token * G::kScales + c * kKeyScales, &scale[h]);
-      }
-      if constexpr (FP4) {
-        uint32_t by[2][4];
+        for (int u = 0; u < kGroups; ++u) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) FromE4m3(scale[h], by[h]);  // pairs of scales; four at most
+          for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int j = 0; j < kKeyBytes / 4; ++j) {
-          uint32_t v[2][4];
+            for (int e = 0; e < 4; ++e) s[u][n][e] = 0.f;
+          }
+          uint32_t raw[2][kKeyBytes / 4], scale[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int b = j / 2;  // the block of sixteen channels
-            const uint32_t both = __byte_perm(by[h][b >> 1], 0, b & 1 ? 0x3232 : 0x1010);
-            FromE2m1(raw[h][j], v[h]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[h][e] = Mul16(v[h][e], both);
+            const uint32_t token = static_cast<uint32_t>(16 * u + 8 * h + g);
+            LoadShared<kKeyBytes>(tile + token * G::kCodes + c * kKeyBytes, raw[h]);
+            if constexpr (FP4) LoadShared<kKeyScales>(tile + G::kTile * G::kCodes + token * G::kScales + c * kKeyScales, &scale[h]);
           }
+          if constexpr (FP4) {
+            uint32_t by[2][2];  // pairs of scales
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t a[4] = {v[0][2 * e], v[1][2 * e], v[0][2 * e + 1], v[1][2 * e + 1]};
+            for (int h = 0; h < 2; ++h) FromE4m3(scale[h], by[h]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) Mma(s[u][n], a, q[n][2 * j + e][0], q[n][2 * j + e][1]);
+            for (int j = 0; j < kKeyBytes / 4; ++j) {
+              uint32_t v[2][4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t both = j & 2 ? Upper(by[h][j / 4]) : Lower(by[h][j / 4]);  // block j / 2 of sixteen channels
+                FromE2m1(raw[h][j], v[h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[h][e] = Mul16(v[h][e], both);
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t a[4] = {v[0][2 * e], v[1][2 * e], v[0][2 * e + 1], v[1][2 * e + 1]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) Mma(s[u][n], a, q[n][2 * j + e][0], q[n][2 * j + e][1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kKeyBytes / 4; ++j) {
+              uint32_t v[2][2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) FromE4m3(raw[h][j], v[h]);
+              const uint32_t a[4] = {v[0][0], v[1][0], v[0][1], v[1][1]};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) Mma(s[u][n], a, q[n][j][0], q[n][j][1]);
+            }
           }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kKeyBytes / 4; ++j) {
-          uint32_t v[2][2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) FromE4m3(raw[h][j], v[h]);
-          const uint32_t a[4] = {v[0][0], v[1][0], v[0][1], v[1][1]};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) Mma(s[u][n], a, q[n][j][0], q[n][j][1]);
-        }
-      }
-    }
-    // ---- weights.  s[u][n][2 h + r] is token 16 u + 8 h + g, row 8 n + 2 c + r.
-    float value_scale[kGroups][2];
-#pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t token = static_cast<uint32_t>(16 * u + 8 * h + g);
-        float key_scale = 1.f;
-        value_scale[u][h] = 1.f;
+        // eight bits: the scales of keys and values; a value's moves the point from which a weight is measured, so that the product of both stays within FP16
+        float value_scale[kGroups][2], log_scale[kGroups][2];
         if constexpr (!FP4) {
-          LoadShared<4>(at + G::kTile * G::kCodes + token * 4, reinterpret_cast<uint32_t*>(&key_scale));
-          LoadShared<4>(at + G::kPart + G::kTile * G::kCodes + token * 4, reinterpret_cast<uint32_t*>(&value_scale[u][h]));
-          if (token0 + static_cast<int>(token) >= length || absent) value_scale[u][h] = 1.f;
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t token = static_cast<uint32_t>(16 * u + 8 * h + g);
+              float key_scale;
+              LoadShared<4>(tile + G::kTile * G::kCodes + token * 4, reinterpret_cast<uint32_t*>(&key_scale));
+              LoadShared<4>(tile + G::kPart + G::kTile * G::kCodes + token * 4, reinterpret_cast<uint32_t*>(&value_scale[u][h]));
+              if (!whole && (token0 + static_cast<int>(token) >= at.length || absent)) value_scale[u][h] = 1.f;
+              log_scale[u][h] = fminf(fmaxf(Log2(value_scale[u][h]), -60.f), 60.f);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) s[u][n][2 * h + r] *= key_scale;
+              }
+            }
+          }
         }
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (token0 + 16 * u + 8 * (e >> 1) + g >= sees[n][e & 1] || absent) s[u][n][e] = -INFINITY;
+              }
+            }
+          }
+        }
+        // m is taken up where a score passes it by 8
+        bool higher = false;
+        float upto[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float& v = s[u][n][2 * h + r];
-            v *= FP4 ? factor[n][r] : factor[n][r] * key_scale;
-            if (!whole && (token0 + static_cast<int>(token) >= sees[n][r] || absent)) v = -INFINITY;
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kGroups; ++u) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) m = FP4 ? fmaxf(m, s[u][n][2 * h + r]) : fmaxf(m, fmaf(s[u][n][2 * h + r], factor[n][r], log_scale[u][h]));
+            }
+            upto[n][r] = FP4 ? m * factor[n][r] : m;
+            higher = higher || upto[n][r] > most[n][r] + 8.f;
           }
         }
+        if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float m = upto[n][r];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+              m = fmaxf(m, most[n][r]);
+              const float by = m == -INFINITY ? 1.f : Exp2(most[n][r] - m);
+              most[n][r] = m;
+              sum[n][r] *= by;
+#pragma unroll
+              for (int t = 0; t < kTilesOfO; ++t) {
+                o[n][t][r] *= by;
+                o[n][t][2 + r] *= by;
+              }
+            }
+          }
+        }
+        uint32_t weights[kGroups][NT][2];  // tokens 2 c, 2 c + 1 (and eight on) of the sixteen, row 8 n + g
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float off[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) off[r] = most[n][r] == -INFINITY ? 0.f : -most[n][r];
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = Exp2(fmaf(s[u][n][e], factor[n][e & 1], off[e & 1]));
+              sum[n][e & 1] += v;
+              w[e] = FP4 ? v : v * value_scale[u][e >> 1];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) weights[u][n][h] = Transposed(Pack16(w[2 * h], w[2 * h + 1]));
+          }
+        }
+        // ---- values
+#pragma unroll
+        for (int u = 0; u < kGroups; ++u) {
+          uint32_t raw[4][kValueBytes / 4], scale[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t token = static_cast<uint32_t>(16 * u + 8 * (t >> 1) + 2 * c + (t & 1));
+            LoadShared<kValueBytes>(tile + G::kPart + token * G::kCodes + g * kValueBytes, raw[t]);
+            if constexpr (FP4) LoadShared<(D == 256 ? 2 : 1)>(tile + G::kPart + G::kTile * G::kCodes + token * G::kScales + g * kValueChannels / 16, &scale[t]);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              if (token0 + 16 * u + 8 * (t >> 1) + 2 * c + (t & 1) >= at.length || absent) {  // nothing that may lie there takes part
+#pragma unroll
+                for (int e = 0; e < kValueBytes / 4; ++e) raw[t][e] = 0;
+                scale[t] = 0;
+              }
+            }
+          }
+          if constexpr (FP4) {
+            // codes of the same channel of two tokens side by side in a byte, and their scales in a pair
+            uint32_t by[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              FromE4m3(D == 256 ? __byte_perm(scale[2 * h], scale[2 * h + 1], 0x5140) : __byte_perm(scale[2 * h], scale[2 * h + 1], 0x0040), by[h]);
+            }
+#pragma unroll
+            for (int j = 0; j < kValueBytes / 4; ++j) {
+              uint32_t v[2][2][4];  // [tokens][even, odd channels][pairs of channels]
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t a = raw[2 * h][j], b = raw[2 * h + 1][j];
+                FromE2m1((a & 0x0F0F0F0Fu) | (b << 4 & 0xF0F0F0F0u), v[h][0]);
+                FromE2m1((a >> 4 & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u), v[h][1]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[h][e / 4][e % 4] = Mul16(v[h][e / 4][e % 4], by[h][j / 2]);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t a[4] = {v[0][0][e], v[0][1][e], v[1][0][e], v[1][1][e]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) Mma(o[n][4 * j + e], a, weights[u][n][0], weights[u][n][1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kValueBytes / 4; ++j) {
+              uint32_t v[2][2][2];  // [tokens][channels 0 and 1, 2 and 3 of four][as codes: of one channel and the next]
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                // (token, next token) of channel 0, 1 | 2, 3
+                FromE4m3(__byte_perm(raw[2 * h][j], raw[2 * h + 1][j], 0x5140), v[h][0]);
+                FromE4m3(__byte_perm(raw[2 * h][j], raw[2 * h + 1][j], 0x7362), v[h][1]);
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t a[4] = {v[0][e][0], v[0][e][1], v[1][e][0], v[1][e][1]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) Mma(o[n][2 * j + e], a, weights[u][n][0], weights[u][n][1]);
+              }
+            }
+          }
+        }
+        __syncwarp();  // every lane has read the tile
+        issue();
+        if (++stage == G::kStages) stage = 0;
       }
     }
-    // what a score may be at most without its weight, times the value's scale, passing 2^8
-    bool higher = false;
-    float upto[NT][2];
-    float log_scale[kGroups][2];
-#pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) log_scale[u][h] = FP4 ? 0.f : fminf(fmaxf(Log2(value_scale[u][h]), -60.f), 60.f);
-    }
+
+    // ---- the warps' sums.  o[n][t][2 h + r] is channel g D / 8 + 2 t + h, row 8 n + 2 c + r.
+    float* const parts = reinterpret_cast<float*>(smem);  // [warp][row][D]
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float m = s[0][n][r] + log_scale[0][0];
+        const int to_row = 8 * n + 2 * c + r;
 #pragma unroll
-        for (int u = 0; u < kGroups; ++u) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) m = fmaxf(m, s[u][n][2 * h + r] + log_scale[u][h]);
+        for (int d = 4; d < 32; d <<= 1) sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], d);
+        if (g == 0) {
+          row_most[warp][to_row] = most[n][r];
+          row_sum[warp][to_row] = sum[n][r];
         }
-        upto[n][r] = m;
-        higher = higher || m > most[n][r] + 8.f;
-      }
-    }
-    if (__any_sync(0xffffffffu, higher)) {
+        if (any) {
+          float* const to = parts + (warp * kRows + to_row) * D + g * kValueChannels;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float m = upto[n][r];
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-          m = fmaxf(m, most[n][r]);
-          const float by = m == -INFINITY ? 1.f : Exp2(most[n][r] - m);
-          most[n][r] = m;
-          sum[n][r] *= by;
-#pragma unroll
-          for (int t = 0; t < kTilesOfO; ++t) {
-            o[n][t][r] *= by;
-            o[n][t][2 + r] *= by;
-          }
+          for (int t = 0; t < kTilesOfO; ++t) *reinterpret_cast<float2*>(to + 2 * t) = make_float2(o[n][t][r], o[n][t][2 + r]);
         }
       }
     }
-    uint32_t weights[kGroups][NT][2];  // tokens 2 c, 2 c + 1 (and eight on) of the sixteen, row 8 n + g
+    __syncthreads();
+    const bool whole_unit = at.tile == 0 && at.end - at.begin == at.tiles;
+    float* const partial = p.partial + (static_cast<long long>(blockIdx.x) * 2 + (at.tile > 0 ? 0 : 1)) * kRows * (D + 2);
+    for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
+      const int of = i / (D / 2), channel = i % (D / 2) * 2;
+      float all = -INFINITY, total = 0.f;
 #pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
+      for (int w = 0; w < kWarps; ++w) all = fmaxf(all, row_most[w][of]);
+      float2 y = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float from = most[n][e & 1];
-          const float v = Exp2(s[u][n][e] - (from == -INFINITY ? 0.f : from));
-          sum[n][e & 1] += v;
-          w[e] = FP4 ? v : v * value_scale[u][e >> 1];
+      for (int w = 0; w < kWarps; ++w) {
+        const float m = row_most[w][of];
+        if (m == -INFINITY) {
+          total += row_sum[w][of];  // 0, or of a row that saw nothing but NaN
+          continue;
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) weights[u][n][h] = Transposed(Pack16(w[2 * h], w[2 * h + 1]));
+        const float by = Exp2(m - all);
+        const float2 v = *reinterpret_cast<const float2*>(parts + (w * kRows + of) * D + channel);
+        total = fmaf(by, row_sum[w][of], total);
+        y.x = fmaf(by, v.x, y.x);
+        y.y = fmaf(by, v.y, y.y);
       }
-    }
-    // ---- values
-#pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-      uint32_t raw[4][(kValueBytes + 3) / 4], scale[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t token = static_cast<uint32_t>(16 * u + 8 * (t >> 1) + 2 * c + (t & 1));
-        LoadShared<kValueBytes>(at + G::kPart + token * G::kCodes + g * kValueBytes, raw[t]);
-        if constexpr (FP4) {
-          constexpr int kScalesOfLane = D == 256 ? 2 : 1;
-          LoadShared<kScalesOfLane>(at + G::kPart + G::kTile * G::kCodes + token * G::kScales + g * kValueChannels / 16, &scale[t]);
-        }
-        if (!whole && (token0 + static_cast<int>(token) >= length || absent)) {  // nothing that may lie there takes part
-#pragma unroll
-          for (int e = 0; e < (kValueBytes + 3) / 4; ++e) raw[t][e] = 0;
-          scale[t] = 0;
-        }
-      }
-      if constexpr (FP4) {
-        uint32_t by[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          uint32_t two[2];
-          FromE4m3(scale[t], two);
-          by[t] = two[0];
-        }
-#pragma unroll
-        for (int j = 0; j < kValueBytes / 4; ++j) {
-          uint32_t v[4][4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            FromE2m1(raw[t][j], v[t]);
-            const uint32_t both = __byte_perm(by[t], 0, j / 2 ? 0x3232 : 0x1010);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[t][e] = Mul16(v[t][e], both);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t a[4] = {__byte_perm(v[0][e], v[1][e], 0x5410), __byte_perm(v[0][e], v[1][e], 0x7632), __byte_perm(v[2][e], v[3][e], 0x5410),
-                                   __byte_perm(v[2][e], v[3][e], 0x7632)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) Mma(o[n][4 * j + e], a, weights[u][n][0], weights[u][n][1]);
-          }
-        }
+      if (whole_unit) {
+        StoreRow<D>(p, at.seq, at.unit, row0 + of, channel, y, all, total);
       } else {
-#pragma unroll
-        for (int j = 0; j < kValueBytes / 4; ++j) {
-          uint32_t v[4][2];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) FromE4m3(raw[t][j], v[t]);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t a[4] = {__byte_perm(v[0][e], v[1][e], 0x5410), __byte_perm(v[0][e], v[1][e], 0x7632), __byte_perm(v[2][e], v[3][e], 0x5410),
-                                   __byte_perm(v[2][e], v[3][e], 0x7632)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) Mma(o[n][2 * j + e], a, weights[u][n][0], weights[u][n][1]);
-          }
-        }
+        *reinterpret_cast<float2*>(partial + of * D + channel) = y;
+        if (channel == 0) *reinterpret_cast<float2*>(partial + kRows * D + 2 * of) = make_float2(all, total);
       }
     }
-    __syncwarp();  // every lane has read the tile
-    if (i + G::kStages < count) issue(i + G::kStages);
-  }
-
-  // ---- the warps' sums.  o[n][t][2 h + r] is channel g D / 8 + 2 t + h, row 8 n + 2 c + r.
-  if (!good) {
-    ctl.fault = 1;
-    for (int i = 0; i < 16; ++i) __nanosleep(1000000);  // copies may still be landing
-  }
-  __syncthreads();  // no warp reads the ring any more
-  const bool failed = ctl.fault != 0;
-  float* const parts = reinterpret_cast<float*>(smem);  // [warp][row][D]
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], d);
-      const int row = 8 * n + 2 * c + r;
-      if (g == 0) {
-        ctl.most[warp][row] = most[n][r];
-        ctl.sum[warp][row] = sum[n][r];
-      }
-      float* const to = parts + (warp * kRows + row) * D + g * kValueChannels;
-#pragma unroll
-      for (int t = 0; t < kTilesOfO; ++t) *reinterpret_cast<float2*>(to + 2 * t) = make_float2(o[n][t][r], o[n][t][2 + r]);
-    }
-  }
-  __syncthreads();
-  float* const partial = p.partial + static_cast<long long>(blockIdx.x) * kRows * (D + 2);
-  for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
-    const int row = i / (D / 2), channel = i % (D / 2) * 2;
-    float all = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) all = fmaxf(all, ctl.most[w][row]);
-    float2 y = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float by = all == -INFINITY ? 0.f : Exp2(ctl.most[w][row] - all);
-      const float2 v = *reinterpret_cast<const float2*>(parts + (w * kRows + row) * D + channel);
-      total = fmaf(by, ctl.sum[w][row], total);
-      y.x = fmaf(by, v.x, y.x);
-      y.y = fmaf(by, v.y, y.y);
-    }
-    if (failed) total = __uint_as_float(0x7FFFFFFFu);
-    if (cut.pieces > 1) {
-      *reinterpret_cast<float2*>(partial + row * D + channel) = y;
-      if (channel == 0) *reinterpret_cast<float2*>(partial + kRows * D + 2 * row) = make_float2(all, total);
-    } else {
-      const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
-      const int token = (row0 + row) / p.group, of = head * p.group + (row0 + row) % p.group;
-      const long long to = (static_cast<long long>(cut.seq) * p.tokens + token) * p.q_heads + of;
-      if (p.bf16) {
-        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + to * D + channel) = __floats2bfloat162_rn(y.x * by, y.y * by);
-      } else {
-        *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + to * D + channel) = __floats2half2_rn(y.x * by, y.y * by);
-      }
-      if (p.lse != nullptr && channel == 0) p.lse[to] = total == 0.f ? -INFINITY : (all + Log2(total)) * 0.693147181f;
-    }
+    if (at.end == count) break;
+    NextSegment(p, count, G::kTile, &at);
+    make_q(at);
+    __syncthreads();  // the sums have been read, and q is there
   }
 }
 
-// The pieces of the sequences that were cut.  A block: eight or sixteen rows of one key head of one sequence.
+// The units that lie in several shares.  Block b looks after the unit that share b + 1 begins within, where no earlier share does.
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) JoinKernel(const AttendParams p, int tile) {
-  constexpr int kRows = 8 * NT;
+__global__ void __launch_bounds__(kThreads) JoinKernel(const AttendParams p) {
+  constexpr int kRows = 8 * NT, kRow = D + 2, kSlot = kRows * kRow, kBatch = 64;
+  __shared__ float2 stats[kBatch][kRows];
   GridDependencyWait();
-  const int per_seq = p.cache.heads * p.row_blocks, seq = static_cast<int>(blockIdx.x) / per_seq, unit = static_cast<int>(blockIdx.x) % per_seq;
-  const Cut cut = FindCut<kThreads>(p, tile, -1, seq);
-  if (cut.pieces < 2) return;
-  const int head = unit / p.row_blocks, row0 = unit % p.row_blocks * kRows, rows = min(kRows, p.tokens * p.group - row0);
-  const float* const first = p.partial + (static_cast<long long>(cut.first) * per_seq + unit) * kRows * (D + 2);
-  const long long step = static_cast<long long>(per_seq) * kRows * (D + 2);
-  for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
-    const int row = i / (D / 2), channel = i % (D / 2) * 2;
-    float all = -INFINITY, total = 0.f;
-    for (int k = 0; k < cut.pieces; ++k) all = fmaxf(all, first[k * step + kRows * D + 2 * row]);
-    float2 y = make_float2(0.f, 0.f);
-    for (int k = 0; k < cut.pieces; ++k) {
-      const float* const part = first + k * step;
-      const float2 ms = *reinterpret_cast<const float2*>(part + kRows * D + 2 * row), v = *reinterpret_cast<const float2*>(part + row * D + channel);
-      const float by = all == -INFINITY ? 0.f : Exp2(ms.x - all);
-      total = fmaf(by, ms.y, total);
-      y.x = fmaf(by, v.x, y.x);
-      y.y = fmaf(by, v.y, y.y);
+  const int b = static_cast<int>(blockIdx.x) + 1;
+  const Shares shares = *p.shares;
+  const ShareInfo at = p.share[b];
+  if (b >= shares.count) return;
+  const long long first = shares.begin(b) - at.tile, end = first + at.tiles;
+  if (at.tile == 0 || first < shares.begin(b - 1)) return;
+  const int row0 = at.unit % p.row_blocks * kRows, rows = min(kRows, p.tokens * p.group - row0);
+  int pieces = 2;  // of shares b - 1 (its second slot), b, ...
+  while (b - 1 + pieces < shares.count && shares.begin(b - 1 + pieces) < end) ++pieces;
+  const auto slot = [&](int k) { return p.partial + (static_cast<long long>(b - 1 + k) * 2 + (k == 0 ? 1 : 0)) * kSlot; };
+  constexpr int kMine = (kRows * D / 2 + kThreads - 1) / kThreads;
+  float most[kMine], total[kMine];
+  float2 y[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) most[j] = -INFINITY, total[j] = 0.f, y[j] = make_float2(0.f, 0.f);
+  for (int k0 = 0; k0 < pieces; k0 += kBatch) {
+    const int n = min(kBatch, pieces - k0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * kRows; i += kThreads) stats[i / kRows][i % kRows] = *reinterpret_cast<const float2*>(slot(k0 + i / kRows) + kRows * D + i % kRows * 2);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int i = static_cast<int>(threadIdx.x) + j * kThreads, of = i / (D / 2), channel = i % (D / 2) * 2;
+      if (of >= rows) continue;
+      float all = most[j];
+      for (int k = 0; k < n; ++k) all = fmaxf(all, stats[k][of].x);
+      const float again = all == -INFINITY ? 0.f : Exp2(most[j] - all);
+      total[j] *= most[j] == -INFINITY ? 1.f : again;
+      y[j].x *= again;
+      y[j].y *= again;
+      most[j] = all;
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) {
+        const float2 ms = stats[k][of], v = *reinterpret_cast<const float2*>(slot(k0 + k) + of * D + channel);
+        const float by = ms.x == -INFINITY ? 0.f : Exp2(ms.x - all);
+        total[j] += ms.x == -INFINITY ? ms.y : by * ms.y;
+        y[j].x = fmaf(by, v.x, y[j].x);
+        y[j].y = fmaf(by, v.y, y[j].y);
+      }
     }
-    const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
-    const int token = (row0 + row) / p.group, of = head * p.group + (row0 + row) % p.group;
-    const long long to = (static_cast<long long>(seq) * p.tokens + token) * p.q_heads + of;
-    if (p.bf16) {
-      *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + to * D + channel) = __floats2bfloat162_rn(y.x * by, y.y * by);
-    } else {
-      *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + to * D + channel) = __floats2half2_rn(y.x * by, y.y * by);
-    }
-    if (p.lse != nullptr && channel == 0) p.lse[to] = total == 0.f ? -INFINITY : (all + Log2(total)) * 0.693147181f;
+  }
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = static_cast<int>(threadIdx.x) + j * kThreads, of = i / (D / 2), channel = i % (D / 2) * 2;
+    if (of < rows) StoreRow<D>(p, at.seq, at.unit, row0 + of, channel, y[j], most[j], total[j]);
   }
 }
 
 struct Shape {
-  int nt, row_blocks, target, tile;
-  long long units;  // no more than that many
-  bool cuts;        // sequences may be cut
+  int nt, row_blocks, blocks;
 };
 Shape ShapeOf(const CacheAttentionCall& c) {
   Shape s;
   const int rows = c.tokens * (c.q_heads / c.cache.heads);
   s.nt = rows > 8 && c.cache.dim < 256 ? 2 : 1;
   s.row_blocks = (rows + 8 * s.nt - 1) / (8 * s.nt);
-  const int codes = c.cache.fp4 ? c.cache.dim / 2 : c.cache.dim, scales = c.cache.fp4 ? c.cache.dim / 16 : 4;
-  s.tile = (codes + scales) * 64 <= 9000 ? 32 : 16;
-  // Pieces for four rounds of two blocks an SM: enough that the last ones to end are short, few enough that a block's start is.
-  s.target = 8 * DeviceSmCount();
-  const long long per_piece = static_cast<long long>(c.cache.heads) * s.row_blocks;
-  const long long tiles = (static_cast<long long>(c.most_pages) * c.cache.page + s.tile - 1) / s.tile;
-  s.cuts = tiles > kLeastTiles;
-  const long long most_pieces = std::max(1LL, (tiles + kLeastTiles - 1) / kLeastTiles);  // of a sequence
-  s.units = per_piece * std::min(c.seqs * most_pieces, c.seqs + s.target / per_piece + 1);
+  const int tile = TileOf(c.cache.dim, c.cache.fp4);
+  const long long room = static_cast<long long>(c.most_pages) * c.cache.page, tiles = (room + tile - 1) / tile * c.seqs * c.cache.heads * s.row_blocks;
+  // as many as the GPU holds at once, and no more than have a tile for each warp
+  const long long most = static_cast<long long>(DeviceSmCount()) * (c.cache.dim * s.nt <= 128 ? 2 : 1);
+  s.blocks = static_cast<int>(std::max(1LL, std::min(most, (tiles + kLeastTiles - 1) / kLeastTiles)));
   return s;
 }
 
 template <int D, bool FP4, int NT>
 cudaError_t Launch(const AttendParams& p, const Shape& s, cudaStream_t stream) {
-  using G = Geometry<D, FP4>;
-  static_assert(G::kBytes >= kWarps * 8 * NT * D * 4, "the warps' sums take the ring's place");
-  static_assert(G::kStages >= 1 && G::kStages <= 8 && G::kBytes + 4096 <= 227 * 1024, "");
+  using G = Geometry<D, FP4, NT>;
+  static_assert(G::kStages >= 2 && G::kBlocks * (G::kBytes + 6144) <= 227 * 1024, "");
   const cudaError_t set = cudaFuncSetAttribute(CacheAttentionKernel<D, FP4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
   if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(s.units));
+  cfg.gridDim = dim3(static_cast<unsigned>(s.blocks));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = G::kBytes;
   cfg.stream = stream;
@@ -637,10 +767,10 @@ cudaError_t Launch(const AttendParams& p, const Shape& s, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
   const cudaError_t err = cudaLaunchKernelEx(&cfg, CacheAttentionKernel<D, FP4, NT>, p);
-  if (err != cudaSuccess || !s.cuts) return err;
-  cfg.gridDim = dim3(static_cast<unsigned>(p.seqs * p.cache.heads * p.row_blocks));
+  if (err != cudaSuccess || s.blocks < 2) return err;
+  cfg.gridDim = dim3(static_cast<unsigned>(s.blocks - 1));
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, JoinKernel<D, NT>, p, s.tile);
+  return cudaLaunchKernelEx(&cfg, JoinKernel<D, NT>, p);
 }
 
 template <bool FP4>
@@ -657,13 +787,12 @@ cudaError_t LaunchOf(const AttendParams& p, const Shape& s, cudaStream_t stream)
 
 size_t CacheAttentionWorkspace(const CacheAttentionCall& c) {
   const Shape s = ShapeOf(c);
-  return s.cuts ? static_cast<size_t>(s.units) * 8 * s.nt * (c.cache.dim + 2) * sizeof(float) : 0;
+  return s.blocks < 2 ? 0 : sizeof(Shares) + s.blocks * (sizeof(ShareInfo) + sizeof(float) * 2 * 8 * s.nt * (c.cache.dim + 2));
 }
 
 cudaError_t LaunchCacheAttention(const CacheAttentionCall& c, cudaStream_t stream) {
   if (c.seqs == 0 || c.tokens == 0) return cudaSuccess;
   const Shape s = ShapeOf(c);
-  if (s.units > INT_MAX) return cudaErrorInvalidValue;
   AttendParams p = {};
   p.cache = c.cache;
   p.q = c.q;
@@ -678,14 +807,16 @@ cudaError_t LaunchCacheAttention(const CacheAttentionCall& c, cudaStream_t strea
   p.q_heads = c.q_heads;
   p.group = c.q_heads / c.cache.heads;
   p.row_blocks = s.row_blocks;
-  p.target_units = s.target;
   p.scale = c.scale * 1.44269504f * (c.cache.fp4 ? c.cache.k_unit : 1.f);
   if (!c.cache.fp4) p.cache.v_unit = 1.f;
-  p.partial = static_cast<float*>(c.workspace);
+  if (s.blocks > 1) {
+    p.shares = static_cast<Shares*>(c.workspace);
+    p.share = reinterpret_cast<ShareInfo*>(p.shares + 1);
+    p.partial = reinterpret_cast<float*>(p.share + s.blocks);
+  }
   p.out = c.out;
   p.lse = c.lse;
   p.bf16 = c.dtype == QFG_BFLOAT16;
-  p.give_up = c.give_up;
   const cudaError_t err = c.cache.fp4 ? LaunchOf<true>(p, s, stream) : LaunchOf<false>(p, s, stream);
   const cudaError_t last = cudaGetLastError();
   return err == cudaSuccess ? last : err;

@@ -30,7 +30,7 @@ namespace qfg {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostTokens = 4;  // of a block
+constexpr int kMostTokens = 8;  // of a block, one for each warp
 
 struct Side {  // queries, keys or values
   const void* x;
@@ -38,7 +38,6 @@ struct Side {  // queries, keys or values
   void* out;     // contiguous rows, or null
   const void* weight;
   int heads;
-  bool vec, weight_vec;  // on 16 bytes, row by row
 };
 struct HeadsParams {
   Side side[3];
@@ -47,11 +46,27 @@ struct HeadsParams {
   const RotaryPair* pairs;
   const long long* slots;
   KvCacheView cache;
-  int tokens, tokens_per_block, rows, rows_per_block, rotary;  // rows: heads of all sides; rotary: channels
+  int tokens, log_tokens, rotary;  // 2^log_tokens tokens a block; rotary: channels
   float rotary_scale, eps, offset;
   bool weight_f32, positions_64, interleaved;
 };
 
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Eight<T> LoadEight(const T* p) {
+  Eight<T> e;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e.v[i] = p[i];
+  }
+  return e;
+}
 template <typename T>
 __device__ __forceinline__ float ToFloat(T v) {
   if constexpr (std::is_same_v<T, float>) return v;
@@ -59,33 +74,36 @@ __device__ __forceinline__ float ToFloat(T v) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
 }
 template <typename T>
-__device__ __forceinline__ T FromFloat(float v) {
-  if constexpr (std::is_same_v<T, float>) return v;
-  if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
-}
-template <typename T>
-struct alignas(16) Eight {
-  T v[8];
-};
-template <typename T>
-__device__ __forceinline__ void LoadEight(float* f, const T* p, bool vec) {
-  Eight<T> e;
-  if (vec) {
+__device__ __forceinline__ void ToFloats(float* f, const Eight<T>& e) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = p[i];
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(&e)[i];
+      f[2 * i] = __uint_as_float(w << 16);
+      f[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const float2 two = __half22float2(reinterpret_cast<const __half2*>(&e)[i]);
+      f[2 * i] = two.x;
+      f[2 * i + 1] = two.y;
+    } else {
+      f[2 * i] = e.v[2 * i];
+      f[2 * i + 1] = e.v[2 * i + 1];
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = ToFloat(e.v[i]);
 }
 template <typename T>
 __device__ __forceinline__ void StoreEight(T* p, const float* f) {
   Eight<T> e;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e.v[i] = FromFloat<T>(f[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      reinterpret_cast<__nv_bfloat162*>(&e)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      reinterpret_cast<__half2*>(&e)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    } else {
+      reinterpret_cast<float2*>(&e)[i] = make_float2(f[2 * i], f[2 * i + 1]);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&e)[i];
 }
@@ -97,11 +115,12 @@ __device__ __forceinline__ uint32_t RowMax(uint32_t v) {
   for (int d = L / 2; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
-__device__ __forceinline__ uint32_t Magnitude(const float* f) {  // of eight
-  uint32_t m = 0;
+// of eight values, the same; a NaN is kept
+__device__ __forceinline__ uint32_t Magnitude(const float* f) {
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-  return m;
+  for (int i = 0; i < 4; ++i) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+  return __float_as_uint(m) & 0x7FFFFFFFu;
 }
 constexpr uint32_t kInfinity = 0x7F800000u;
 
@@ -126,10 +145,10 @@ __device__ __forceinline__ uint32_t EightE2m1(const float* f, const Reciprocal& 
   return bad ? 0u : w;
 }
 
-__device__ __forceinline__ void Turn(float& a, float& b, float2 by) {
+__device__ __forceinline__ void Turn(float& a, float& b, float cosine, float sine) {
   const float u = a, v = b;
-  a = u * by.x - v * by.y;
-  b = v * by.x + u * by.y;
+  a = u * cosine - v * sine;
+  b = v * cosine + u * sine;
 }
 
 // A row's sixteen values of this lane, at channels c0 and c1 of eight each, into the cache.
@@ -174,113 +193,183 @@ __device__ __forceinline__ void StoreCache(const float (&f)[16], int c0, int c1,
   }
 }
 
-// L lanes a row, D = 16 L.
-template <typename T, int L>
-__global__ void __launch_bounds__(kThreads) HeadsKernel(const HeadsParams p) {
-  constexpr int D = 16 * L, kRows = kThreads / L;
-  __shared__ float2 turn[kMostTokens * D / 2];
-  __shared__ long long place[kMostTokens];  // (page, row of it) as page * kv_heads * page size + row; < 0: not written
-  GridDependencyWait();
-  const int token0 = blockIdx.x * p.tokens_per_block, tokens = min(p.tokens_per_block, p.tokens - token0), half = p.rotary / 2;
-  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
-    const int t = i / half, j = i - t * half;
-    const RotaryPair pair = p.pairs[j];
-    const long long at = token0 + t + pair.axis * p.ld_positions;
-    const long long position = p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
-    const unsigned long long turns = static_cast<unsigned long long>(position) * pair.turns;
-    float s, c;
-    sincospif(static_cast<float>(static_cast<int>(turns >> 32)) * 4.656612873077393e-10f, &s, &c);  // 2^-31
-    turn[i] = make_float2(c * p.rotary_scale, s * p.rotary_scale);
-  }
-  if (p.slots != nullptr && threadIdx.x < tokens) {
-    const long long slot = p.slots[token0 + threadIdx.x], page = slot / p.cache.page;
-    place[threadIdx.x] = slot >= 0 && page < p.cache.pages ? page * p.cache.heads * p.cache.page + (slot - page * p.cache.page) : -1;
-  }
-  __syncthreads();
+// This lane's channels of rows of a side: eight from c0 and eight from c1.
+struct Channels {
+  int c0, c1;
+  bool turned, split;  // rotated; with the channels that they are rotated with in the other eight
+};
+template <int WHICH>
+__device__ __forceinline__ Channels ChannelsOf(const HeadsParams& p, int lane) {
+  Channels c;
+  c.turned = WHICH < 2 && 16 * lane < p.rotary;
+  c.split = c.turned && !p.interleaved;
+  c.c0 = c.split ? 8 * lane : 16 * lane;
+  c.c1 = c.split ? p.rotary / 2 + 8 * lane : c.c0 + 8;
+  return c;
+}
+template <typename T>
+struct Two {
+  Eight<T> a, b;
+};
+template <typename T, int L, bool VEC>
+__device__ __forceinline__ Two<T> LoadRow(const Side& s, const Channels& c, long long token, int row) {
+  const T* const x = static_cast<const T*>(s.x) + token * s.ld + row * (16 * L);
+  return {LoadEight<T, VEC>(x + c.c0), LoadEight<T, VEC>(x + c.c1)};
+}
+
+// The rows of a token that are queries (0), keys (1) or values (2): those of this warp, every `step`-th run of kRows from row `row` on, up to row `end`.  `next` holds the
+// first; the row behind is on its way while one is worked on.  Every lane of the warp makes the same number of steps, as shuffles are of whole warps.
+template <typename T, int L, bool VEC, int WHICH>
+__device__ __forceinline__ void SideRows(const HeadsParams& p, long long token, const float2* turn, const float* weight, long long place, int row, int step, int end,
+                                         Two<T> next) {
+  constexpr int D = 16 * L, kRows = 32 / L;
+  const Side& s = p.side[WHICH];
   const int lane = threadIdx.x % L;
-  const int row0 = blockIdx.y * p.rows_per_block, rows = min(p.rows_per_block, p.rows - row0), items = tokens * rows;
-  // every lane of a warp makes the same number of steps: shuffles are of whole warps
-  for (int first = 0; first < items; first += kRows) {
-    const int item = first + static_cast<int>(threadIdx.x) / L;
-    const bool mine = item < items;
-    const int t = mine ? item / rows : 0;
-    int head = mine ? row0 + item - t * rows : 0;
-    const int which = head < p.side[0].heads ? 0 : head < p.side[0].heads + p.side[1].heads ? 1 : 2;
-    if (which > 0) head -= p.side[0].heads;
-    if (which > 1) head -= p.side[1].heads;
-    const Side& s = p.side[which];
-    const bool turned = which < 2 && 16 * lane < p.rotary;
-    const bool halves = turned && !p.interleaved;
-    const int c0 = halves ? 8 * lane : 16 * lane, c1 = halves ? half + 8 * lane : c0 + 8;
+  const Channels c = ChannelsOf<WHICH>(p, lane);
+  float cosine[8], sine[8];  // of this lane's eight pairs
+  if (c.turned) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float4 two = *reinterpret_cast<const float4*>(turn + 8 * lane + e);
+      cosine[e] = two.x, sine[e] = two.y;
+      cosine[e + 1] = two.z, sine[e + 1] = two.w;
+    }
+  }
+  const bool norm = WHICH < 2 && s.weight != nullptr;
+#pragma unroll 1
+  for (int run = row - (static_cast<int>(threadIdx.x) & 31) / L; run < end; run += step * kRows, row += step * kRows) {
     float f[16];
-    const T* const x = static_cast<const T*>(s.x) + (token0 + t) * s.ld + head * D;
-    LoadEight<T>(f, x + c0, s.vec);
-    LoadEight<T>(f + 8, x + c1, s.vec);
-    float w[16];
-    if (s.weight != nullptr) {
-      if (p.weight_f32) {
-        LoadEight<float>(w, static_cast<const float*>(s.weight) + c0, s.weight_vec);
-        LoadEight<float>(w + 8, static_cast<const float*>(s.weight) + c1, s.weight_vec);
-      } else {
-        LoadEight<T>(w, static_cast<const T*>(s.weight) + c0, s.weight_vec);
-        LoadEight<T>(w + 8, static_cast<const T*>(s.weight) + c1, s.weight_vec);
+    ToFloats(f, next.a);
+    ToFloats(f + 8, next.b);
+    if (row + step * kRows < end) next = LoadRow<T, L, VEC>(s, c, token, row + step * kRows);
+    if (norm) {
+      float squares[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) squares[e & 1] = fmaf(f[e], f[e], squares[e & 1]);
+      float all = squares[0] + squares[1];
+#pragma unroll
+      for (int d = L / 2; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+      const float root = rsqrtf(fmaf(all, 1.f / D, p.eps));
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float4 w = *reinterpret_cast<const float4*>(weight + (e < 8 ? c.c0 + e : c.c1 + e - 8));
+        f[e] *= root * w.x;
+        f[e + 1] *= root * w.y;
+        f[e + 2] *= root * w.z;
+        f[e + 3] *= root * w.w;
       }
     }
-    float squares = 0.f;
+    if (c.turned) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) squares = fmaf(f[i], f[i], squares);
-#pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
-    if (s.weight != nullptr) {
-      const float root = rsqrtf(fmaf(squares, 1.f / D, p.eps));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = f[i] * root * (p.offset + w[i]);
-    }
-    if (turned) {
-      const float2* const by = turn + t * half + 8 * lane;
-      if (halves) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) Turn(f[i], f[8 + i], by[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) Turn(f[2 * i], f[2 * i + 1], by[i]);
+      for (int e = 0; e < 8; ++e) {
+        if (c.split) {
+          Turn(f[e], f[8 + e], cosine[e], sine[e]);
+        } else {
+          Turn(f[2 * e], f[2 * e + 1], cosine[e], sine[e]);
+        }
       }
     }
-    if (mine && s.out != nullptr) {
-      T* const out = static_cast<T*>(s.out) + (static_cast<long long>(token0 + t) * s.heads + head) * D;
-      StoreEight<T>(out + c0, f);
-      StoreEight<T>(out + c1, f + 8);
+    if (WHICH < 2 && row < end && s.out != nullptr) {
+      T* const out = static_cast<T*>(s.out) + (token * s.heads + row) * D;
+      StoreEight<T>(out + c.c0, f);
+      StoreEight<T>(out + c.c1, f + 8);
+    }
+    if (WHICH > 0 && p.slots != nullptr)
+      StoreCache<L>(f, c.c0, c.c1, c.split, p.cache, WHICH == 2, place + static_cast<long long>(row) * p.cache.page, lane, row < end && place >= 0);
+  }
+}
+
+// L lanes a row, D = 16 L.
+template <typename T, int L, bool VEC>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 ? 3 : 4) HeadsKernel(const HeadsParams p) {
+  constexpr int D = 16 * L, kRows = 32 / L;
+  __shared__ __align__(16) float2 turn[kMostTokens * D / 2];
+  __shared__ __align__(16) float weight[2][D];
+  GridDependencyWait();
+  // a token's warps, a power of two, take turns at its runs of rows, from one side to the next as well; or every warp has one run, of one side
+  const int warp = static_cast<int>(threadIdx.x) / 32, warps = kThreads / 32 >> p.log_tokens, t = warp * (1 << p.log_tokens) / (kThreads / 32), sub = warp & (warps - 1);
+  const long long token = (static_cast<long long>(blockIdx.x) << p.log_tokens) + t;
+  const bool real = token < p.tokens, turns = gridDim.y == 1;
+  const int q = p.side[0].heads, k = p.side[1].heads, v = p.side[2].heads, in_run = (static_cast<int>(threadIdx.x) & 31) / L, lane = threadIdx.x % L, half = p.rotary / 2;
+  const int q_runs = (q + kRows - 1) / kRows, k_runs = (k + kRows - 1) / kRows;
+  const int run = turns ? sub : static_cast<int>(blockIdx.y) * (kThreads / 32) + warp;
+  const int first[3] = {run, turns ? (run - q_runs) & (warps - 1) : run - q_runs, turns ? (run - q_runs - k_runs) & (warps - 1) : run - q_runs - k_runs};
+  const int step = turns ? warps : 1 << 24;
+  const auto begins = [&](int side, int heads) { return real && first[side] >= 0 && first[side] * kRows + in_run < heads; };
+  Two<T> next = {};
+  if (begins(0, q)) {
+    next = LoadRow<T, L, VEC>(p.side[0], ChannelsOf<0>(p, lane), token, first[0] * kRows + in_run);
+  } else if (!turns && begins(1, k)) {
+    next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<1>(p, lane), token, first[1] * kRows + in_run);
+  } else if (!turns && begins(2, v)) {
+    next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<2>(p, lane), token, first[2] * kRows + in_run);
+  }
+
+  for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+    const void* const w = p.side[i / D].weight;
+    if (w != nullptr) weight[i / D][i % D] = p.offset + (p.weight_f32 ? static_cast<const float*>(w)[i % D] : ToFloat(static_cast<const T*>(w)[i % D]));
+  }
+  float2* const by = turn + t * half;
+  long long to = -1;  // (page, row of it) as page * kv_heads * page size + row; < 0: not written
+  if (real) {
+    for (int j = sub * 32 + (static_cast<int>(threadIdx.x) & 31); j < half; j += 32 * warps) {
+      const RotaryPair pair = p.pairs[j];
+      const long long at = token + pair.axis * p.ld_positions;
+      const long long position = p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
+      const unsigned long long part = static_cast<unsigned long long>(position) * pair.turns;
+      float s, c;
+      sincospif(static_cast<float>(static_cast<int>(part >> 32)) * 4.656612873077393e-10f, &s, &c);  // 2^-31
+      by[j] = make_float2(c * p.rotary_scale, s * p.rotary_scale);
     }
     if (p.slots != nullptr) {
-      const long long row = place[t] + static_cast<long long>(head) * p.cache.page;
-      StoreCache<L>(f, c0, c1, halves, p.cache, which == 2, row, lane, mine && which > 0 && place[t] >= 0);
+      const long long slot = p.slots[token], page = slot >> 32 ? slot / p.cache.page : static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.cache.page);
+      to = slot >= 0 && page < p.cache.pages ? page * p.cache.heads * p.cache.page + (slot - page * p.cache.page) : -1;
     }
+  }
+  __syncthreads();
+  if (!real) return;
+  if (first[0] * kRows < q) {
+    SideRows<T, L, VEC, 0>(p, token, by, weight[0], to, first[0] * kRows + in_run, step, q, next);
+    if (!turns) return;
+  }
+  if (first[1] >= 0 && first[1] * kRows < k) {
+    if (turns && begins(1, k)) next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<1>(p, lane), token, first[1] * kRows + in_run);
+    SideRows<T, L, VEC, 1>(p, token, by, weight[1], to, first[1] * kRows + in_run, step, k, next);
+    if (!turns) return;
+  }
+  if (first[2] >= 0 && first[2] * kRows < v) {
+    if (turns && begins(2, v)) next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<2>(p, lane), token, first[2] * kRows + in_run);
+    SideRows<T, L, VEC, 2>(p, token, by, nullptr, to, first[2] * kRows + in_run, step, v, next);
   }
 }
 
 template <typename T, int L>
-cudaError_t LaunchHeads(HeadsParams& p, cudaStream_t stream) {
-  // Few tokens: one a block, its heads over as many blocks as keep every lane to one row.  Many: a block's tokens share nothing but its launch and make it long enough.
+cudaError_t LaunchHeads(HeadsParams& p, bool vec, cudaStream_t stream) {
+  // Few tokens: one a block, its rows over as many blocks as leave every warp one run of them.  Many: a warp has sixteen runs or more, so that its sines and cosines
+  // are a small part of it, as long as there is a block for most SMs.
+  constexpr int kRows = 32 / L, kWarps = kThreads / 32, kLeastRuns = 16;
+  int runs = 0;
+  for (const Side& s : p.side) runs += (s.heads + kRows - 1) / kRows;
   const int sms = DeviceSmCount();
-  p.tokens_per_block = p.tokens <= 2 * sms ? 1 : kMostTokens;
-  p.rows_per_block = p.tokens <= 2 * sms ? kThreads / L : p.rows;
-  const int x = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block, y = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
+  const bool few = p.tokens <= 2 * sms;
+  p.log_tokens = 0;
+  while (1 << p.log_tokens < kMostTokens && runs << p.log_tokens < kLeastRuns * kWarps && p.tokens >> (p.log_tokens + 1) >= sms * 4 / 5) ++p.log_tokens;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.tokens + (1 << p.log_tokens) - 1) >> p.log_tokens), static_cast<unsigned>(few ? (runs + kWarps - 1) / kWarps : 1));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {OverlapAttribute()};
   cfg.attrs = attr;
   cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, HeadsKernel<T, L>, p);
+  return vec ? cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, true>, p) : cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, false>, p);
 }
 
 template <typename T>
-cudaError_t LaunchHeadsOf(int dim, HeadsParams& p, cudaStream_t stream) {
+cudaError_t LaunchHeadsOf(int dim, HeadsParams& p, bool vec, cudaStream_t stream) {
   switch (dim) {
-    case 64: return LaunchHeads<T, 4>(p, stream);
-    case 128: return LaunchHeads<T, 8>(p, stream);
-    case 256: return LaunchHeads<T, 16>(p, stream);
+    case 64: return LaunchHeads<T, 4>(p, vec, stream);
+    case 128: return LaunchHeads<T, 8>(p, vec, stream);
+    case 256: return LaunchHeads<T, 16>(p, vec, stream);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -395,9 +484,11 @@ cudaError_t Ended(cudaError_t err) {
 cudaError_t LaunchHeadRows(const HeadsCall& c, cudaStream_t stream) {
   if (c.tokens == 0) return cudaSuccess;
   HeadsParams p = {};
-  p.side[0] = {c.q, c.ldq, c.q_out, c.q_weight, c.q != nullptr ? c.q_heads : 0, Vectors(c.q, c.ldq, c.dtype), Vectors(c.q_weight, 0, c.dtype)};
-  p.side[1] = {c.k, c.ldk, c.k_out, c.k_weight, c.kv_heads, Vectors(c.k, c.ldk, c.dtype), Vectors(c.k_weight, 0, c.dtype)};
-  p.side[2] = {c.v, c.ldv, nullptr, nullptr, c.slots != nullptr ? c.kv_heads : 0, Vectors(c.v, c.ldv, c.dtype), true};
+  p.side[0] = {c.q, c.ldq, c.q_out, c.q_weight, c.q != nullptr ? c.q_heads : 0};
+  p.side[1] = {c.k, c.ldk, c.k_out, c.k_weight, c.kv_heads};
+  p.side[2] = {c.v, c.ldv, nullptr, nullptr, c.slots != nullptr ? c.kv_heads : 0};
+  bool vec = true;  // everything on 16 bytes
+  for (const Side& s : p.side) vec = vec && Vectors(s.x, s.ld, c.dtype) && Vectors(s.weight, 0, c.dtype);
   p.positions = c.positions;
   p.ld_positions = c.ld_positions;
   p.positions_64 = c.positions_64;
@@ -411,12 +502,11 @@ cudaError_t LaunchHeadRows(const HeadsCall& c, cudaStream_t stream) {
   p.slots = reinterpret_cast<const long long*>(c.slots);
   p.cache = c.cache;
   p.tokens = static_cast<int>(c.tokens);
-  p.rows = p.side[0].heads + p.side[1].heads + p.side[2].heads;
   cudaError_t err;
   switch (c.dtype) {
-    case QFG_BFLOAT16: err = LaunchHeadsOf<__nv_bfloat16>(c.dim, p, stream); break;
-    case QFG_FLOAT16: err = LaunchHeadsOf<__half>(c.dim, p, stream); break;
-    case QFG_FLOAT: err = LaunchHeadsOf<float>(c.dim, p, stream); break;
+    case QFG_BFLOAT16: err = LaunchHeadsOf<__nv_bfloat16>(c.dim, p, vec, stream); break;
+    case QFG_FLOAT16: err = LaunchHeadsOf<__half>(c.dim, p, vec, stream); break;
+    case QFG_FLOAT: err = LaunchHeadsOf<float>(c.dim, p, vec, stream); break;
     default: return cudaErrorInvalidValue;
   }
   return Ended(err);

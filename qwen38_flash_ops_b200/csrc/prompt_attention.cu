@@ -33,10 +33,11 @@ namespace qfg {
 namespace {
 
 constexpr int kTile = 128, kThreads = 384;
-// Registers of a thread: the launch's 168 for all are shared out, 8 warps of 208 and 4 of 80 (together 1984 of the 2016 that a lane of twelve warps has).
-constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 80;
+// Registers of a thread: the launch's 168 for all are shared out, 8 warps of 232 and 4 of 40 (together the 2016 that a lane of twelve warps has).
+constexpr int kSoftmaxRegisters = 232, kOtherRegisters = 40;
 static_assert(8 * kSoftmaxRegisters + 4 * kOtherRegisters <= 12 * 168, "");
 
+constexpr int kPolyOf16 = 4;
 struct PromptParams {
   CUtensorMap q, k, v;
   const int *q_offsets, *k_offsets;
@@ -55,7 +56,7 @@ struct Geometry {
 };
 
 struct PromptCtl {
-  unsigned long long q_full[2], full[8], empty[8], s_full[2], p_ready[2], o_full[2], fixed;
+  unsigned long long q_full[2], full[8], empty[8], s_full[2], p_most[2], p_ready[2], o_full[2], fixed;
   uint32_t tmem;
   volatile uint32_t fault;
 };
@@ -65,9 +66,20 @@ __device__ __forceinline__ void TmaLoad3(uint32_t dst, const CUtensorMap* map, i
                "r"(x), "r"(y), "r"(z)
                : "memory");
 }
-__device__ __forceinline__ void MmaTs(uint32_t d, uint32_t a, unsigned long long b, uint32_t idesc, bool add) {
-  asm volatile("{ .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-               "r"(add ? 1 : 0)
+// The products of one k-step, 16 wide: operands OFF bytes (of tensor memory: columns) behind those that the lower words of the descriptors name, so that what differs
+// from step to step takes no registers.  All operands in shared memory have rows of 128 bytes, swizzled, and 1024 bytes from eight rows to the next.
+constexpr uint32_t kDescUpper = static_cast<uint32_t>(((1024ull >> 4) << 32 | 1ull << 46 | 2ull << 61) >> 32);
+template <int OFF_A, int OFF_B>
+__device__ __forceinline__ void MmaSsAt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int add) {
+  asm volatile("{ .reg .pred p;\n .reg .b32 x, y;\n .reg .b64 m, n;\n setp.ne.b32 p, %4, 0;\n add.u32 x, %1, %6;\n add.u32 y, %2, %7;\n mov.b64 m, {x, %5};\n"
+               " mov.b64 n, {y, %5};\n tcgen05.mma.cta_group::1.kind::f16 [%0], m, n, %3, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kDescUpper),
+               "n"(OFF_A / 16), "n"(OFF_B / 16)
+               : "memory");
+}
+template <int OFF_A, int OFF_B>
+__device__ __forceinline__ void MmaTsAt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int add) {
+  asm volatile("{ .reg .pred p;\n .reg .b32 x, y;\n .reg .b64 n;\n setp.ne.b32 p, %4, 0;\n add.u32 x, %1, %6;\n add.u32 y, %2, %7;\n mov.b64 n, {y, %5};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [x], n, %3, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kDescUpper), "n"(OFF_A), "n"(OFF_B / 16)
                : "memory");
 }
 // 32 columns of this warp's 32 lanes
@@ -81,15 +93,12 @@ __device__ __forceinline__ void LoadColumns(uint32_t a, float* f) {
         "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(a));
 }
-__device__ __forceinline__ void StoreColumns32(uint32_t a, const float* f) {
-  const uint32_t* const v = reinterpret_cast<const uint32_t*>(f);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
-      "%26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
-      "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
-      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+__device__ __forceinline__ void LoadColumns16(uint32_t a, float* f) {
+  uint32_t* const v = reinterpret_cast<uint32_t*>(f);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                 "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(a));
 }
 __device__ __forceinline__ void StoreColumns16(uint32_t a, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(a), "r"(v[0]),
@@ -121,6 +130,26 @@ __device__ __forceinline__ float2 Add2(float2 a, float2 b) {
       : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+// 2^v for v <= 127 without the unit for exponentials: v = n + f with n whole and |f| <= 1/2, a polynomial for 2^f (the least relative error there: 7.5e-5 of degree 3, for
+// weights in BF16; 2.6e-6 of degree 4, for FP16), and n added to its exponent.  Below 2^-126 it is 2^-126, which no weight of 16 bits holds.
+template <bool BF16>
+__device__ __forceinline__ float2 PolyExp2(float2 v) {
+  const float2 round = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23
+  v = make_float2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const float2 n = Add2(v, round), whole = Add2(n, make_float2(-12582912.f, -12582912.f)), f = Fma2(whole, make_float2(-1.f, -1.f), v);
+  float2 r;
+  if constexpr (BF16) {
+    r = Fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261114f, 0.24261114f));
+    r = Fma2(r, f, make_float2(0.69326097f, 0.69326097f));
+    r = Fma2(r, f, make_float2(0.99992806f, 0.99992806f));
+  } else {
+    r = Fma2(f, make_float2(0.0095701022f, 0.0095701022f), make_float2(0.055917863f, 0.055917863f));
+    r = Fma2(r, f, make_float2(0.24024744f, 0.24024744f));
+    r = Fma2(r, f, make_float2(0.69312179f, 0.69312179f));
+    r = Fma2(r, f, make_float2(0.99999928f, 0.99999928f));
+  }
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t Pack(float lo, float hi) {
   uint32_t r;
@@ -130,6 +159,24 @@ __device__ __forceinline__ uint32_t Pack(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   }
   return r;
+}
+
+// BarWait without the pause of try_wait and in few instructions: for those that hold up the others.
+__device__ __forceinline__ bool SpinWait(uint32_t a, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+      "AGAIN:\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra.uni DONE;\n add.u32 n, n, 1;\n setp.lt.u32 p, n, %3;\n @p bra.uni AGAIN;\n"
+      " setp.ne.u32 p, n, n;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok) : "r"(a), "r"(parity), "n"(16 * kSpin) : "memory");
+  return ok != 0;
+}
+
+// A value that all lanes of the warp have, and the compiler knows it: what the instructions of the tensor core and their branches go by has to be so (else each product
+// costs its issuing thread about 90 cycles, more than the tensor core takes for it).
+template <typename T>
+__device__ __forceinline__ T Uniform(T v) {
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
 // Where a block's queries and keys lie; tiles < 0: a block too many.
@@ -185,12 +232,13 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
   constexpr int kBoxes = D / 64, kBox = kTile * 128;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PromptCtl ctl;
-  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  const int warp = Uniform(static_cast<int>(threadIdx.x) >> 5), lane = static_cast<int>(threadIdx.x) & 31;
   const uint32_t smem = (Smem(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * G::kHeadTile;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       BarInit(Smem(&ctl.q_full[i]), 1);
       BarInit(Smem(&ctl.s_full[i]), 1);
+      BarInit(Smem(&ctl.p_most[i]), 4);
       BarInit(Smem(&ctl.p_ready[i]), 4);
       BarInit(Smem(&ctl.o_full[i]), 1);
     }
@@ -202,11 +250,11 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
     ctl.fault = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Smem(&ctl.tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 9 && lane == 0) {
+  if (warp == 1 && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.v) : "memory");
@@ -216,24 +264,24 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
   const int head = static_cast<int>(blockIdx.x) % p.q_heads;
   const Place at = FindPlace(p, static_cast<int>(blockIdx.x) / p.q_heads);
   const int tiles[2] = {at.first < 0 ? 0 : KeyTiles(p, at, at.first), at.first < 0 ? 0 : KeyTiles(p, at, at.first + kTile)};
-  const int most = max(tiles[0], tiles[1]);
+  const int n0 = Uniform(tiles[0]), n1 = Uniform(tiles[1]), most = max(n0, n1);
   // the last tile of values runs past the sequence's end
-  const bool fix = most > 0 && most * kTile > at.keys;
+  const bool fix = Uniform(most > 0 && most * kTile > at.keys ? 1 : 0) != 0;
   __syncthreads();
   FenceAfter();
-  const uint32_t tmem = ctl.tmem;
+  const uint32_t tmem = Uniform(ctl.tmem);
 
-  if (warp < 8) {
+  if (warp >= 4) {
     // ---- softmax and output
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-    const int t = warp >> 2, row = at.first + t * kTile + (warp & 3) * 32 + lane;  // of the sequence
+    const int t = (warp >> 2) - 1, row = at.first + t * kTile + (warp & 3) * 32 + lane;  // of the sequence
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + static_cast<uint32_t>(t * kTile), o_at = tmem + lanes + static_cast<uint32_t>(2 * kTile + t * D);
     const int count = tiles[t], sees = p.causal ? min(at.keys, row + 1 + at.keys - at.queries) : at.keys;
     const int first_sees = p.causal ? min(at.keys, at.first + t * kTile + (warp & 3) * 32 + 1 + at.keys - at.queries) : at.keys;  // the warp's first row
     const float step = 8.f / p.scale;
     float reference = -INFINITY;
-    float2 sum = make_float2(0.f, 0.f);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     bool good = true;
     for (int j = 0; j < count; ++j) {
       if (!BarWait(Smem(&ctl.s_full[t]), static_cast<uint32_t>(j & 1), ctl)) {
@@ -263,17 +311,17 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
         const float to = fmaxf(reference, highest);
         const float by = to == -INFINITY ? 1.f : Exp2((reference - to) * p.scale);
         reference = to;
-        sum.x *= by;
-        sum.y *= by;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * by, sum[i].y * by);
         if (j > 0) {  // the products of the tile ahead have ended: S, which was issued after them, has
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            LoadColumns(o_at + c, o);
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            LoadColumns16(o_at + c, o);
             WaitLoads();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= by;
-            StoreColumns32(o_at + c, o);
+            for (int i = 0; i < 16; ++i) o[i] *= by;
+            StoreColumns16(o_at + c, reinterpret_cast<const uint32_t*>(o));
           }
         }
       }
@@ -285,23 +333,24 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float2 v = Fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), scale2, offset2);
-          v.x = Exp2(v.x);
-          v.y = Exp2(v.y);
-          sum = Add2(sum, v);
+          v = i * kPolyOf16 % 16 < kPolyOf16 ? PolyExp2<BF16>(v) : make_float2(Exp2(v.x), Exp2(v.y));
+          sum[i & 1] = Add2(sum[i & 1], v);
           w[i] = Pack<BF16>(v.x, v.y);
         }
         StoreColumns16(s_at + c / 2, w);
+        if (c >= kTile - 64) {  // three quarters of the product may begin while the last weights are made
+          WaitStores();
+          FenceBefore();
+          __syncwarp();
+          if (lane == 0) BarArrive(Smem(c == kTile - 64 ? &ctl.p_most[t] : &ctl.p_ready[t]));
+        }
       }
-      WaitStores();
-      FenceBefore();
-      __syncwarp();
-      if (lane == 0) BarArrive(Smem(&ctl.p_ready[t]));
     }
     if (at.first >= 0) {
       if (count > 0 && good) good = BarWait(Smem(&ctl.o_full[t]), 0, ctl);
       __syncwarp();
       FenceAfter();
-      const float total = sum.x + sum.y, by = total == 0.f ? 0.f : 1.f / total;
+      const float total = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), by = total == 0.f ? 0.f : 1.f / total;
       const long long to = (static_cast<long long>(at.q0) + row) * p.q_heads + head;
       const bool mine = row < at.queries;
 #pragma unroll
@@ -325,71 +374,103 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
   }
-  if (warp == 8) {
+  if (warp == 0) {
     // ---- products
     constexpr uint32_t kType = BF16 ? 1u << 7 | 1u << 10 : 0u;
     constexpr uint32_t kScores = 0x10u | kType | static_cast<uint32_t>(kTile >> 3) << 17 | 8u << 24;
     constexpr uint32_t kOutputs = 0x10u | kType | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;  // V: the columns of a row lie beside one another
-    const unsigned long long q_desc = SmemDesc(smem, 16, 1024), k_desc = SmemDesc(ring, 16, 1024), v_desc = SmemDesc(ring, kBox, 1024);
+    // descriptors' lower words: of Q, of the ring's first stage as keys and as values; they have one upper word
+    const uint32_t q_desc = static_cast<uint32_t>(SmemDesc(smem, 16, 1024)), k_desc = static_cast<uint32_t>(SmemDesc(ring, 16, 1024)),
+                   v_desc = static_cast<uint32_t>(SmemDesc(ring, kBox, 1024));
+    constexpr uint32_t kStageStep = G::kHeadTile >> 4;
     bool good = true;
-    int ready = 0;  // stages seen full so far
-    auto wait = [&](int position) {  // for the copy of that number; they are waited for in order
-      for (; ready <= position && good; ++ready) good = BarWait(Smem(&ctl.full[ready % G::kStages]), static_cast<uint32_t>(ready / G::kStages & 1), ctl);
-      __syncwarp();
+    auto wait = [&](uint32_t bar, uint32_t parity) {  // as every lane sees it: what follows is uniform to the compiler, too
+      good = __all_sync(0xffffffffu, SpinWait(bar, parity)) != 0 && good;
+    };
+    // copies are waited for in their order: keys 0, values 0, keys 1, ..., ahead of what has to be waited for longer
+    int next = 0;
+    uint32_t parity = 0;
+    auto arrived = [&] {
+      const int stage = next;
+      wait(Smem(&ctl.full[0]) + static_cast<uint32_t>(stage * 8), parity);
+      if (++next == G::kStages) {
+        next = 0;
+        parity ^= 1u;
+      }
+      return stage;
+    };
+    auto release = [&](int stage) { MmaCommit<false>(Smem(&ctl.empty[0]) + static_cast<uint32_t>(stage * 8)); };
+    auto scores = [&](auto tile, int stage) {
+      constexpr int t = decltype(tile)::value;
+      const uint32_t a = q_desc + t * kStageStep, b = k_desc + static_cast<uint32_t>(stage) * kStageStep, d = tmem + t * kTile;
+      MmaSsAt<0, 0>(d, a, b, kScores, 0);
+      MmaSsAt<32, 32>(d, a, b, kScores, 1);
+      MmaSsAt<64, 64>(d, a, b, kScores, 1);
+      MmaSsAt<96, 96>(d, a, b, kScores, 1);
+      if constexpr (D == 128) {
+        MmaSsAt<kBox, kBox>(d, a, b, kScores, 1);
+        MmaSsAt<kBox + 32, kBox + 32>(d, a, b, kScores, 1);
+        MmaSsAt<kBox + 64, kBox + 64>(d, a, b, kScores, 1);
+        MmaSsAt<kBox + 96, kBox + 96>(d, a, b, kScores, 1);
+      }
+      MmaCommit<false>(Smem(&ctl.s_full[t]));
+    };
+    auto outputs = [&](auto tile, int j, int v, int k, int count) {  // of tile t, and its next scores
+      constexpr int t = decltype(tile)::value;
+      const uint32_t b = v_desc + static_cast<uint32_t>(v) * kStageStep, d = tmem + 2 * kTile + t * D, a = tmem + t * kTile;
+      wait(Smem(&ctl.p_most[t]), static_cast<uint32_t>(j & 1));
       FenceAfter();
-    };
-    auto scores = [&](int t, int j) {
-      wait(2 * j);
-      if (!good) return;
-      const unsigned long long a = q_desc + static_cast<unsigned long long>(t * G::kHeadTile >> 4), b = k_desc + static_cast<unsigned long long>(2 * j % G::kStages * G::kHeadTile >> 4);
-      if (ElectOne()) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const unsigned long long off = static_cast<unsigned long long>((i / 4 * kBox + i % 4 * 32) >> 4);
-          MmaSs<false>(tmem + static_cast<uint32_t>(t * kTile), a + off, b + off, kScores, i > 0);
+      if (good && ElectOne()) {
+        MmaTsAt<0, 0>(d, a, b, kOutputs, j > 0);
+        MmaTsAt<8, 2048>(d, a, b, kOutputs, 1);
+        MmaTsAt<16, 4096>(d, a, b, kOutputs, 1);
+        MmaTsAt<24, 6144>(d, a, b, kOutputs, 1);
+        MmaTsAt<32, 8192>(d, a, b, kOutputs, 1);
+        MmaTsAt<40, 10240>(d, a, b, kOutputs, 1);
+      }
+      __syncwarp();
+      wait(Smem(&ctl.p_ready[t]), static_cast<uint32_t>(j & 1));
+      FenceAfter();
+      if (good && ElectOne()) {
+        MmaTsAt<48, 12288>(d, a, b, kOutputs, 1);
+        MmaTsAt<56, 14336>(d, a, b, kOutputs, 1);
+        if (j + 1 == count) {
+          MmaCommit<false>(Smem(&ctl.o_full[t]));
+        } else {
+          scores(tile, k);
         }
-        MmaCommit<false>(Smem(&ctl.s_full[t]));
       }
       __syncwarp();
     };
-    auto release = [&](int position) {
-      if (ElectOne()) MmaCommit<false>(Smem(&ctl.empty[position % G::kStages]));
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, 1> second;
+    if (most > 0) {
+      if (n0 > 0) wait(Smem(&ctl.q_full[0]), 0);
+      if (n1 > 0) wait(Smem(&ctl.q_full[1]), 0);
+      const int k0 = arrived();
+      FenceAfter();
+      if (good && ElectOne()) {
+        if (n0 > 0) scores(first, k0);
+        if (n1 > 0) scores(second, k0);
+        release(k0);
+      }
       __syncwarp();
-    };
-    for (int t = 0; t < 2 && good; ++t) {
-      if (tiles[t] == 0) continue;
-      good = BarWait(Smem(&ctl.q_full[t]), 0, ctl);
-      if (good) scores(t, 0);
     }
-    if (most > 0 && good) release(0);
+#pragma unroll 1
     for (int j = 0; j < most && good; ++j) {
-      for (int t = 0; t < 2 && good; ++t) {
-        if (j >= tiles[t]) continue;
-        good = BarWait(Smem(&ctl.p_ready[t]), static_cast<uint32_t>(j & 1), ctl);
-        if (good) wait(2 * j + 1);
-        if (good && fix && j == most - 1) {
-          good = BarWait(Smem(&ctl.fixed), 0, ctl);
-          FenceAfter();
-        }
-        if (!good) break;
-        __syncwarp();
-        const unsigned long long b = v_desc + static_cast<unsigned long long>((2 * j + 1) % G::kStages * G::kHeadTile >> 4);
-        if (ElectOne()) {
-#pragma unroll
-          for (int i = 0; i < kTile / 16; ++i)
-            MmaTs(tmem + static_cast<uint32_t>(2 * kTile + t * D), tmem + static_cast<uint32_t>(t * kTile + 8 * i), b + static_cast<unsigned long long>(2048 * i >> 4), kOutputs,
-                  j > 0 || i > 0);
-          if (j + 1 == tiles[t]) MmaCommit<false>(Smem(&ctl.o_full[t]));
-        }
-        __syncwarp();
-        if (j + 1 < tiles[t]) scores(t, j + 1);
+      const bool more = j + 1 < most;
+      const int v = arrived(), k = more ? arrived() : 0;
+      if (fix && !more) wait(Smem(&ctl.fixed), 0);
+      if (j < n0) outputs(first, j, v, k, n0);
+      if (j < n1) outputs(second, j, v, k, n1);
+      if (good && ElectOne()) {
+        release(v);
+        if (more) release(k);
       }
-      if (!good) break;
-      release(2 * j + 1);
-      if (j + 1 < most) release(2 * j + 2);
+      __syncwarp();
     }
     if (!good) ctl.fault = 1;
-  } else if (warp == 9) {
+  } else if (warp == 1) {
     // ---- copies
     bool good = !p.give_up;
     auto load = [&](uint32_t dst, const CUtensorMap* map, int of, int row, uint32_t bar) {
@@ -436,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
   FenceBefore();
   __syncthreads();
   FenceAfter();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 bool EncodeHeads(CUtensorMap* map, const void* x, int dtype, int dim, int heads, int64_t rows, int64_t ld) {

@@ -416,7 +416,6 @@ struct CacheAttentionCall {
   void* out = nullptr;   // contiguous
   float* lse = nullptr;  // or null
   void* workspace = nullptr;
-  bool give_up = false;  // testing
 };
 size_t CacheAttentionWorkspace(const CacheAttentionCall& call);  // bytes
 cudaError_t LaunchCacheAttention(const CacheAttentionCall& call, cudaStream_t stream);
