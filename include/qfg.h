@@ -371,7 +371,7 @@ QFG_API int qfg_quant_mlp(int dtype, const void* x, int64_t ldx, const void* res
  * another: k and v are [pages][kv_heads][page][head_dim] FP8 E4M3FN with FP32 scales [pages][kv_heads][page], or UINT8 (block-16
  * NVFP4) [pages][kv_heads][page][head_dim / 2], channel 2 b in the low nibble of byte b, with E4M3FN scales [pages][kv_heads][page]
  * [head_dim / 16].  A token's slot is page * (page size) + (its place in the page).  Writing a row y of a head:
- *   E4M3:  scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i / scale.
+ *   E4M3:  scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i 448 / max_i |y_i| (the quotient by the scale before that is rounded; by 2^-40 where that is larger).
  *   NVFP4: for each 16 channels scale = max(E4M3(max_i |y_i| / (6 unit)), 2^-9), at most 448, q_i = E2M1(y_i / (scale unit)).
  * Both rounded to nearest, ties to even; `unit` is k_unit or v_unit, so that values from 2^-10 to 2688 units are held well.  A row (NVFP4:
  * sixteen channels) that holds an infinity or a NaN has scale NaN and q 0.  All tensors begin on 16 bytes. */
@@ -428,7 +428,8 @@ QFG_API int qfg_cache_attention(int dtype, const void* q, int64_t ld_seq, int64_
  * BFLOAT16 and FLOAT16, heads of 64 or 128 channels, bases and tokens on 16 bytes; out [q_rows][q_heads][head_dim] and lse (NULL, or FP32
  * [q_rows][q_heads]) contiguous.  A row that sees nothing is 0, its lse -inf.  Rows ahead of the first and behind the last sequence are left
  * as they were; what lies in keys and values of other sequences takes no part, whatever it is.  Within a sequence a value that is not
- * finite makes rows of the same head that lie up to 128 tokens ahead of it NaN as well: their weight for it is 0, and 0 times it is not. */
+ * finite makes rows of the same head that lie up to 128 tokens ahead of it NaN as well: their weight for it is 0, and 0 times it is not.
+ * Scores (scale q k) have to stay below 2^28; rows with larger ones may become NaN. */
 QFG_API int qfg_prompt_attention(int dtype, const void* q, int64_t ldq, int64_t q_rows, int64_t q_heads, const void* k, int64_t ldk, const void* v,
                                  int64_t ldv, int64_t k_rows, int64_t kv_heads, int64_t head_dim, const int32_t* q_offsets, const int32_t* k_offsets,
                                  int64_t seqs, int causal, float scale, void* out, float* lse, void* stream);

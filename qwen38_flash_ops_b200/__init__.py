@@ -1,7 +1,8 @@
 """B200 (sm_100a) implementation of the `qwen.fused_gemm` decode weight-streaming path:
 SkinnyGemm (M <= 8 rows per pass; BF16 / FP8 E4M3FN / block-16 NVFP4 weights), ArgmaxRows,
 DequantWeightBf16 and the fused, N-shardable LM head; and blocks in eight bits (RmsNormQuant, RowQuant, QuantGemm, QuantMlp);
-heads, their quantised cache and attention (QkNormRope, KvCache, CacheWrite, CacheRead, CacheAttention, PromptAttention).  The compute lives in libqfg_b200.so
+heads, their quantised cache and attention (QkNormRope, KvCache, CacheWrite, CacheRead, CacheAttention, PromptAttention,
+QuantAttention).  The compute lives in libqfg_b200.so
 (C ABI in include/qfg.h); this package is the Python mirror of the operator interface."""
 from . import packing  # noqa: F401
 from ._lib import QfgError, load  # noqa: F401
@@ -26,4 +27,8 @@ def __getattr__(name):
         from .quant_mlp import QuantMlp
 
         return QuantMlp
+    if name == "QuantAttention":
+        from .quant_attention import QuantAttention
+
+        return QuantAttention
     raise AttributeError(name)

@@ -147,7 +147,7 @@ int qfg_qk_norm_rope_compute(const qfg_qk_norm_rope* op, int dtype, const void* 
   if (op->n_pairs > 0) {
     if (positions == nullptr || (position_bytes != 4 && position_bytes != 8) || !On(positions, static_cast<size_t>(position_bytes)))
       return Refuse(name, "positions must be 32-bit or 64-bit integers");
-    if (axes != op->axes || (axes > 1 && ld_positions < tokens)) return Refuse(name, "there must be positions for " + std::to_string(op->axes) + " axes");
+    if (axes != op->axes || (axes > 1 && ld_positions < tokens)) return Refuse(name, "positions must be [" + (op->axes > 1 ? std::to_string(op->axes) + ", " : std::string()) + std::to_string(tokens) + "]");
   }
   if ((q_weight != nullptr || k_weight != nullptr) && weight_dtype != dtype && weight_dtype != QFG_FLOAT)
     return Refuse(name, "the weights must have the type of the heads, or FP32");

@@ -10,7 +10,8 @@
 //   keys     S^T = K q^T.  A lane holds a quarter of the channels of two tokens; channels are taken in the order in which they lie in memory, by q as well.
 //   values   O^T = V^T P^T.  A lane holds D / 8 channels of four tokens of each sixteen; pairs of tokens are made by byte permutations.  P^T is S^T's layout transposed.
 //   scales   four bits: the product of an E2M1 value and an E4M3 scale has at most six significant bits and is exact in FP16.  Eight bits: the keys' scale multiplies the
-//            score, the values' the weight.
+//            score, the values' the weight; scores then count from where score + log2(the value's scale) is largest, so that the product is within FP16 for values of any
+//            size (of scores past 2^20 FP32 loses the logarithm, and small scales bits of their weight with it).
 //   q        as FP16, each row times the power of two that takes its largest value to 2^9, so that only what is 2^-23 of that is rounded.
 //
 // Softmax runs along: m is taken up only when a score passes it by 8 (in powers of two), so that sums and weights stay within 2^8 of what they would be and the outputs
@@ -483,8 +484,18 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) s[u][n][2 * h + r] *= key_scale;
+                for (int r = 0; r < 2; ++r) s[u][n][2 * h + r] *= key_scale * factor[n][r];
               }
+            }
+          }
+        }
+        if constexpr (FP4) {
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[u][n][e] *= factor[n][e & 1];
             }
           }
         }
@@ -511,9 +522,9 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
 #pragma unroll
             for (int u = 0; u < kGroups; ++u) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) m = FP4 ? fmaxf(m, s[u][n][2 * h + r]) : fmaxf(m, fmaf(s[u][n][2 * h + r], factor[n][r], log_scale[u][h]));
+              for (int h = 0; h < 2; ++h) m = fmaxf(m, FP4 ? s[u][n][2 * h + r] : s[u][n][2 * h + r] + log_scale[u][h]);
             }
-            upto[n][r] = FP4 ? m * factor[n][r] : m;
+            upto[n][r] = m;
             higher = higher || upto[n][r] > most[n][r] + 8.f;
           }
         }
@@ -542,13 +553,13 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
         for (int n = 0; n < NT; ++n) {
           float off[2];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) off[r] = most[n][r] == -INFINITY ? 0.f : -most[n][r];
+          for (int r = 0; r < 2; ++r) off[r] = most[n][r] == -INFINITY ? 0.f : most[n][r];
 #pragma unroll
           for (int u = 0; u < kGroups; ++u) {
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = Exp2(fmaf(s[u][n][e], factor[n][e & 1], off[e & 1]));
+              const float v = Exp2(s[u][n][e] - off[e & 1]);  // of a rounded score: 0 at the maximum, however large that is
               sum[n][e & 1] += v;
               w[e] = FP4 ? v : v * value_scale[u][e >> 1];
             }

@@ -4,12 +4,12 @@
 //   norm      y_i = x_i rsqrt(mean(x^2) + eps) (offset + weight_i)                  (FP32 from here on)
 //   rotation  (y_a, y_b) -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t), t = position * frequency of the pair, for the pairs (i, i + R/2) or (2 i, 2 i + 1) of
 //             the first R channels; with several axes each pair has one of the positions
-//   E4M3      scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i / scale              one for each token and head
+//   E4M3      scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i 448 / max_i |y_i| (where the scale is 2^-40 y_i / scale)   one for each token and head
 //   NVFP4     scale = max(E4M3(max_i |y_i| / (6 unit)), 2^-9), q_i = E2M1(y_i / (scale unit))   one for each 16 channels
 //
 // An angle is a product of 64-bit integers: a pair's frequency in turns, as a fraction of 2^64, times the position, modulo 2^64, is the fraction of the turn to 2^-44
 // for positions of a million; the sine and cosine of its first 32 bits are right to 2^-23 wherever the position is.  A product in FP32 is off by 2^-8 there.
-// Quotients are rounded once: the reciprocal is carried in two parts, so that half-way values go to even.
+// Quotients are rounded once: their factor is carried in two parts, so that half-way values go to even.
 //
 // A row has D / 16 lanes of sixteen channels each: of a rotated part in halves, eight of the one and the eight that they are rotated with, so that nothing crosses lanes
 // but the sum of squares and the largest value.  A block's sines and cosines are made once for its tokens and wait in shared memory for all heads.
@@ -123,20 +123,21 @@ __device__ __forceinline__ uint32_t Magnitude(const float* f) {
   return __float_as_uint(m) & 0x7FFFFFFFu;
 }
 constexpr uint32_t kInfinity = 0x7F800000u;
+constexpr float kLeastScale = 9.094947017729282e-13f;  // 2^-40
 
-// 1 / scale in two parts: v / scale = v hi + v lo, rounded once by the addition
-struct Reciprocal {
+// top / by in two parts: v top / by = v hi + v lo, rounded once by the addition
+struct Quotient {
   float hi, lo;
-  __device__ explicit Reciprocal(float scale) : hi(1.f / scale) { lo = fmaf(-scale, hi, 1.f) * hi; }
+  __device__ Quotient(float top, float by) : hi(top / by) { lo = fmaf(-by, hi, top) * (hi / top); }
   __device__ float operator()(float v) const { return fmaf(v, hi, v * lo); }
 };
-__device__ __forceinline__ uint2 EightE4m3(const float* f, const Reciprocal& r, bool bad) {
+__device__ __forceinline__ uint2 EightE4m3(const float* f, const Quotient& r, bool bad) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(r(f[2 * i]), r(f[2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
   return bad ? make_uint2(0, 0) : make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
 }
-__device__ __forceinline__ uint32_t EightE2m1(const float* f, const Reciprocal& r, bool bad) {
+__device__ __forceinline__ uint32_t EightE2m1(const float* f, const Quotient& r, bool bad) {
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -173,7 +174,7 @@ __device__ __forceinline__ void StoreCache(const float (&f)[16], int c0, int c1,
       const __nv_fp8_storage_t coded = __nv_cvt_float_to_fp8(__uint_as_float(most[h]) / (6.f * unit), __NV_SATFINITE, __NV_E4M3);
       const uint32_t s = bad ? 0x7Fu : max(1u, static_cast<uint32_t>(coded));
       const float scale = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(s), __NV_E4M3))) * unit;
-      const uint32_t w = EightE2m1(f + 8 * h, Reciprocal(scale), bad);
+      const uint32_t w = EightE2m1(f + 8 * h, Quotient(1.f, scale), bad);
       if (write) {
         *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + c / 2) = w;
         if ((c & 15) == 0) scales[c >> 4] = static_cast<uint8_t>(s);
@@ -182,13 +183,14 @@ __device__ __forceinline__ void StoreCache(const float (&f)[16], int c0, int c1,
   } else {
     const uint32_t most = RowMax<L>(max(m0, m1));
     const bool bad = most >= kInfinity;
-    const float scale = fmaxf(__uint_as_float(most) / 448.f, 9.094947017729282e-13f);  // 2^-40
-    const Reciprocal r(scale);
+    const float scale = __uint_as_float(most) / 448.f;
+    const bool small = scale < kLeastScale;
+    const Quotient r(small ? 1.f : 448.f, small ? kLeastScale : __uint_as_float(most));
     const uint2 a = EightE4m3(f, r, bad), b = EightE4m3(f + 8, r, bad);
     if (write) {
       *reinterpret_cast<uint2*>(codes + row * D + c0) = a;
       *reinterpret_cast<uint2*>(codes + row * D + c1) = b;
-      if (lane == 0) static_cast<float*>(values ? cache.v_scale : cache.k_scale)[row] = bad ? __uint_as_float(0x7FFFFFFFu) : scale;
+      if (lane == 0) static_cast<float*>(values ? cache.v_scale : cache.k_scale)[row] = bad ? __uint_as_float(0x7FFFFFFFu) : fmaxf(scale, kLeastScale);
     }
   }
 }

@@ -131,7 +131,8 @@ __device__ __forceinline__ float2 Add2(float2 a, float2 b) {
   return r;
 }
 // 2^v for v <= 127 without the unit for exponentials: v = n + f with n whole and |f| <= 1/2, a polynomial for 2^f (the least relative error there: 7.5e-5 of degree 3, for
-// weights in BF16; 2.6e-6 of degree 4, for FP16), and n added to its exponent.  Below 2^-126 it is 2^-126, which no weight of 16 bits holds.
+// weights in BF16; 2.6e-6 of degree 4, for FP16), and n added to its exponent.  Below 2^-126 it is 2^-126, where a masked
+// key's weight would be 0: nothing beside a sum of at least 1/2, as long as masked values stay below 2^100.
 template <bool BF16>
 __device__ __forceinline__ float2 PolyExp2(float2 v) {
   const float2 round = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23
@@ -350,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
       if (count > 0 && good) good = BarWait(Smem(&ctl.o_full[t]), 0, ctl);
       __syncwarp();
       FenceAfter();
-      const float total = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), by = total == 0.f ? 0.f : 1.f / total;
+      // a row that saw nothing has made nothing but what is left of weights that are zero
+      const float total = reference == -INFINITY && !isnan(sum[0].x + sum[1].x + sum[0].y + sum[1].y) ? 0.f : (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), by = total == 0.f ? 0.f : 1.f / total;
       const long long to = (static_cast<long long>(at.q0) + row) * p.q_heads + head;
       const bool mine = row < at.queries;
 #pragma unroll
