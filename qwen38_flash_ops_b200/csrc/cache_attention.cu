@@ -17,16 +17,17 @@
 // Softmax runs along: m is taken up only when a score passes it by 8 (in powers of two), so that sums and weights stay within 2^8 of what they would be and the outputs
 // are seldom scaled again.  Statistics and sums are FP32, weights FP16 (2^-11 of themselves, as the values are exact).
 //
-// A block runs through an equal share of all tiles (of one sequence and key head after another, in that order), its warps taking turns; each warp has its own ring of
-// tiles in shared memory, which it fills by asynchronous copies ahead of itself, across the borders of sequences and heads too.  Where a sequence and head ends the warps add up
-// their sums.  Shares begin and end anywhere; a second kernel joins those parts that share a sequence and head, in their order, so that results do not depend on which
-// block is first.  Lengths are on the device only: where the shares lie is worked out there.
+// A warp runs through an equal share of all tiles (of one sequence and key head after another, in that order) and has its own ring of tiles in shared memory, which it
+// fills by asynchronous copies ahead of itself, across the borders of sequences and heads too; no warp waits for another.  Shares begin and end anywhere; a second kernel
+// joins those parts that share a sequence and head, in their order, so that results do not depend on which warp is first.  Lengths are on the device only: where the
+// shares lie is worked out there.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "qfg_internal.h"
@@ -36,24 +37,18 @@ namespace qfg {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kLeastTiles = kWarps;  // of a block's share: a tile a warp
-
 // All tiles, in equal shares: share i begins at tile size i + min(i, more).
 struct Shares {
   long long size;
   int more, count;
   __device__ __forceinline__ long long begin(int i) const { return size * i + min(i, more); }
 };
-struct alignas(16) ShareInfo {  // what the second kernel needs to know of a share: where it begins
-  int seq, unit, tile, tiles;
-};
 struct AttendParams {
   KvCacheView cache;
   const void* q;
   const int *table, *lengths;
-  Shares* shares;
-  ShareInfo* share;   // [blocks]
-  float* partial;     // [blocks][2][rows (D + 2)]: of a share that begins within a unit, and of its last unit where that goes on
+  int2* parts;     // [seqs][key heads][row blocks]: the first share of a unit, and how many have a part of it; (0, 0) where one has all of it
+  float* partial;  // [shares][2][rows (D + 2)]: of a share that begins within a unit, and of its last unit where that goes on
   void* out;
   float* lse;
   long long ld_seq, ld_token, ld_table;
@@ -69,11 +64,15 @@ struct Geometry {
   static constexpr int kTile = TileOf(D, FP4);                                // tokens
   static constexpr int kPart = kTile * (kCodes + kScales);                    // keys or values of a tile
   static constexpr int kStage = 2 * kPart;
+  // Codes are kept with their pieces of 16 bytes exchanged within 128, by the place of those among the others, so that the lanes of a load, which read tokens that are two
+  // apart (values) or lie beside one another (keys), meet in no bank.
+  static __device__ __forceinline__ uint32_t Swizzled(uint32_t at) {
+    constexpr int kShift = kCodes == 32 ? 32 : kCodes == 64 ? 2 : 3;  // of bits 7 to 9 down to bits 4 to 6; rows of 64 bytes: bits 7 and 8 to 5 and 6
+    return kCodes == 32 ? at : at ^ (at >> kShift & (kCodes == 64 ? 0x60u : 0x70u));
+  }
   static constexpr int kBlocks = D * NT <= 128 ? 2 : 1;                       // of an SM
-  static constexpr int kSums = kWarps * 8 * NT * D * 4;                       // the warps' sums
-  static constexpr int kRoom = (kBlocks == 2 ? 111 : 222) * 1024 - kSums;
-  static constexpr int kStages = std::min(8, kRoom / (kWarps * kStage));
-  static constexpr int kBytes = kWarps * kStages * kStage + kSums;
+  static constexpr int kStages = std::min(8, (kBlocks == 2 ? 110 : 220) * 1024 / (kWarps * kStage));
+  static constexpr int kBytes = kWarps * kStages * kStage;
 };
 
 __device__ __forceinline__ int TilesOf(const AttendParams& p, int seq, int tile, int* length) {
@@ -81,7 +80,7 @@ __device__ __forceinline__ int TilesOf(const AttendParams& p, int seq, int tile,
   *length = static_cast<int>(min(static_cast<long long>(max(p.lengths[seq], 0)), room));
   return (*length + tile - 1) / tile;
 }
-// This block's share, `from` to `to`, and the sequence that holds `from`, with the number of tiles ahead of it.  A sequence's tiles count once for each key head and
+// This warp's share, `from` to `to`, and the sequence that holds `from`, with the number of tiles ahead of it.  A sequence's tiles count once for each key head and
 // block of rows.
 struct Share {
   Shares all;
@@ -91,8 +90,8 @@ struct Share {
 __device__ __forceinline__ Share FindShare(const AttendParams& p, int tile) {
   __shared__ int sums[kWarps];
   __shared__ long long total[kWarps];
-  __shared__ Share found;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_seq = p.cache.heads * p.row_blocks;
+  __shared__ Share found[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_seq = p.cache.heads * p.row_blocks, first = static_cast<int>(blockIdx.x) * kWarps;
   int length = 0;
   long long all = 0;
   if (p.seqs > kThreads) {
@@ -129,24 +128,27 @@ __device__ __forceinline__ Share FindShare(const AttendParams& p, int tile) {
     if (base == 0) {
       if (p.seqs <= kThreads) all = before;
       all *= per_seq;
-      s.all.count = static_cast<int>(min(static_cast<long long>(gridDim.x), (all + kLeastTiles - 1) / kLeastTiles));
-      if (static_cast<int>(blockIdx.x) >= s.all.count) return s;
+      s.all.count = static_cast<int>(min(static_cast<long long>(gridDim.x) * kWarps, all));
+      if (first >= s.all.count) return s;
       s.all.size = all >> 32 ? all / s.all.count : static_cast<uint32_t>(all) / static_cast<uint32_t>(s.all.count);
       s.all.more = static_cast<int>(all - s.all.size * s.all.count);
-      s.from = s.all.begin(blockIdx.x);
-      s.to = s.all.begin(blockIdx.x + 1);
     }
     const long long begin = (ahead + upto - tiles) * per_seq, end = (ahead + upto) * per_seq;
-    if (s.from >= begin && s.from < end) {
-      found = s;
-      found.ahead = begin;
-      found.seq = i;
-      found.tiles = tiles;
-      found.length = length;
+#pragma unroll 1
+    for (int w = 0; w < kWarps && first + w < s.all.count; ++w) {
+      const long long from = s.all.begin(first + w);
+      if (from >= begin && from < end) found[w] = {s.all, from, s.all.begin(first + w + 1), begin, i, tiles, length};
     }
   }
   __syncthreads();
-  return found;
+  if (first + warp < s.all.count) s = found[warp];
+  return s;
+}
+// The share that holds a tile.
+__device__ __forceinline__ int ShareOf(const Shares& s, long long tile) {
+  const long long larger = (s.size + 1) * s.more;  // tiles of the shares that have one more
+  if (tile < larger) return static_cast<int>(tile >> 32 ? tile / (s.size + 1) : static_cast<uint32_t>(tile) / static_cast<uint32_t>(s.size + 1));
+  return s.more + static_cast<int>((tile - larger) >> 32 ? (tile - larger) / s.size : static_cast<uint32_t>(tile - larger) / static_cast<uint32_t>(s.size));
 }
 // A run of tiles of one unit: a key head of a sequence, and a block of its rows.
 struct Segment {
@@ -248,18 +250,21 @@ __device__ __forceinline__ void LoadShared(uint32_t a, uint32_t* v) {
   }
 }
 
-template <int D>
-__device__ __forceinline__ void StoreRow(const AttendParams& p, int seq, int unit, int row, int channel, float2 y, float most, float total) {
+// Where a row of a unit lies among the outputs.
+__device__ __forceinline__ long long RowOf(const AttendParams& p, int seq, int unit, int row) {
   const int head = unit / p.row_blocks, token = row / p.group, of = head * p.group + row - token * p.group;
-  const long long to = (static_cast<long long>(seq) * p.tokens + token) * p.q_heads + of;
-  const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
-  if (p.bf16) {
-    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + to * D + channel) = __floats2bfloat162_rn(y.x * by, y.y * by);
-  } else {
-    *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + to * D + channel) = __floats2half2_rn(y.x * by, y.y * by);
-  }
-  if (p.lse != nullptr && channel == 0) p.lse[to] = total == 0.f ? -INFINITY : (most + Log2(total)) * 0.693147181f;
+  return (static_cast<long long>(seq) * p.tokens + token) * p.q_heads + of;
 }
+__device__ __forceinline__ uint32_t Packed(bool bf16, float lo, float hi) {
+  uint32_t r;
+  if (bf16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    r = Pack16(lo, hi);
+  }
+  return r;
+}
+__device__ __forceinline__ float LogOfSum(float most, float total) { return total == 0.f ? -INFINITY : (most + Log2(total)) * 0.693147181f; }
 
 // NT tiles of eight rows.
 template <int D, bool FP4, int NT>
@@ -270,75 +275,38 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
   constexpr int kKeyScales = FP4 ? D / 64 : 1;                           // E4M3 scales of that part
   constexpr int kValueChannels = D / 8, kTilesOfO = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_most[kWarps][kRows], row_sum[kWarps][kRows];
-  __shared__ __align__(16) uint16_t q_rows[kRows][D + 8];
-  __shared__ float q_factor[kRows];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, worker = static_cast<int>(blockIdx.x) * kWarps + warp;
   GridDependencyWait();
   GridLaunchDependents();  // the second kernel, which waits for all of this one
   const Share share = FindShare(p, G::kTile);
+  const int units = p.cache.heads * p.row_blocks;
   for (int seq = blockIdx.x; seq < p.seqs; seq += gridDim.x) {
     int length;
     if (TilesOf(p, seq, G::kTile, &length) > 0) continue;
-    for (int unit = 0; unit < p.cache.heads * p.row_blocks; ++unit) {
-      const int row0 = unit % p.row_blocks * kRows, rows = min(kRows, p.tokens * p.group - row0);
-      for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) StoreRow<D>(p, seq, unit, row0 + i / (D / 2), i % (D / 2) * 2, make_float2(0.f, 0.f), 0.f, 0.f);
-    }
+    const long long rows = static_cast<long long>(p.tokens) * p.q_heads;
+    uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + seq * rows * D);
+    for (long long i = threadIdx.x; i < rows * (D / 8); i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
+    for (long long i = threadIdx.x; p.lse != nullptr && i < rows; i += kThreads) p.lse[seq * rows + i] = -INFINITY;
+    for (int i = threadIdx.x; p.parts != nullptr && i < units; i += kThreads) p.parts[static_cast<long long>(seq) * units + i] = make_int2(0, 0);
   }
-  if (share.seq < 0) {
-    if (blockIdx.x == 0 && threadIdx.x == 0 && p.shares != nullptr) *p.shares = {0, 0, 0};
-    return;
-  }
+  if (share.seq < 0) return;
   Segment at = FirstSegment(share);
-  if (threadIdx.x == 0 && p.shares != nullptr) {
-    p.share[blockIdx.x] = {at.seq, at.unit, at.tile, at.tiles};
-    if (blockIdx.x == 0) *p.shares = share.all;
-  }
   const int count = static_cast<int>(share.to - share.from);
 
-  // q of a segment's rows, as FP16, for all warps: row w (and w + 8) by warp w
-  auto make_q = [&](const Segment& of) {
-    const int head = of.unit / p.row_blocks, row0 = (of.unit - head * p.row_blocks) * kRows;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = 8 * n + warp, token = (row0 + r) / p.group;
-      uint32_t w[D / 64] = {};
-      if (row0 + r < p.tokens * p.group) {
-        const uint16_t* const from = static_cast<const uint16_t*>(p.q) + of.seq * p.ld_seq + token * p.ld_token +
-                                     static_cast<long long>(head * p.group + row0 + r - token * p.group) * D + lane * (D / 32);
-        if constexpr (D == 64) w[0] = *reinterpret_cast<const uint32_t*>(from);
-        if constexpr (D == 128) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(from);
-        if constexpr (D == 256) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(from);
-      }
-      float2 v[D / 64];
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        v[i] = p.bf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<__half2*>(&w[i]));
-        top = max(top, max(__float_as_uint(v[i].x) & 0x7FFFFFFFu, __float_as_uint(v[i].y) & 0x7FFFFFFFu));
-      }
-      // 2^(9 - exponent) of the largest and its inverse; the exponent is kept where both are ordinary numbers
-      const int e = min(max(static_cast<int>(__reduce_max_sync(0xffffffffu, top) >> 23), 20), 240);
-      const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23);
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) *reinterpret_cast<uint32_t*>(&q_rows[r][lane * (D / 32) + 2 * i]) = Pack16(v[i].x * up, v[i].y * up);
-      if (lane == 0) q_factor[r] = __uint_as_float(static_cast<uint32_t>(e - 9) << 23) * p.scale;
-    }
-  };
-
-  // ---- this warp's tiles: warp, warp + kWarps, ... of the share
-  const uint32_t ring = Smem(smem) + G::kSums + static_cast<uint32_t>(warp * G::kStages * G::kStage);
+  // ---- this warp's tiles
+  const uint32_t ring = Smem(smem) + static_cast<uint32_t>(warp * G::kStages * G::kStage);
   Segment ahead = at;
-  int next = warp, batch = 0, issued = 0;  // the tile that is copied next; the first one that `row` is of
+  int next = 0, batch = 0, issued = 0;  // the tile that is copied next; the first one that `row` is of
   bool known = false;
-  long long row = 0;     // lane i: where tile batch + i kWarps lies in the cache, or -1: in no page of it
+  long long row = 0;     // lane i: where tile batch + i lies in the cache, or -1: in no page of it
   uint32_t present = 0;  // of the stages
   const int tiles_of_page = p.cache.page / G::kTile;
-  auto copy = [&](uint32_t to, const uint8_t* from, auto bytes) {
+  auto copy = [&](uint32_t to, const uint8_t* from, auto bytes, auto swizzled) {
     constexpr int kBytes = decltype(bytes)::value;
 #pragma unroll
     for (int i = 0; i < kBytes; i += 512) {
-      if (i + 512 <= kBytes || 16 * lane < kBytes - i) CopyAsync(to + i + 16 * lane, from + i + 16 * lane);
+      const uint32_t at = static_cast<uint32_t>(i + 16 * lane);
+      if (i + 512 <= kBytes || 16 * lane < kBytes - i) CopyAsync(to + (decltype(swizzled)::value ? G::Swizzled(at) : at), from + at);
     }
   };
   auto issue = [&] {
@@ -347,10 +315,10 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
         NextSegment(p, count, G::kTile, &ahead);
         known = false;
       }
-      if (!known || next - batch >= 32 * kWarps) {
+      if (!known || next - batch >= 32) {
         batch = next;
         known = true;
-        const int mine = next + lane * kWarps;
+        const int mine = next + lane;
         row = -1;
         if (mine < ahead.end) {
           const int tile = ahead.tile + mine - ahead.begin, page = tile / tiles_of_page, id = p.table[ahead.seq * p.ld_table + page];
@@ -358,24 +326,36 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
             row = (static_cast<long long>(id) * p.cache.heads + ahead.unit / p.row_blocks) * p.cache.page + (tile - page * tiles_of_page) * G::kTile;
         }
       }
-      const long long from = __shfl_sync(0xffffffffu, row, (next - batch) / kWarps), r = max(from, 0LL);
+      const long long from = __shfl_sync(0xffffffffu, row, next - batch), r = max(from, 0LL);
       present = (present & ~(1u << issued)) | (from >= 0 ? 1u << issued : 0u);
       const uint32_t to = ring + static_cast<uint32_t>(issued * G::kStage);
-      copy(to, p.cache.k + r * G::kCodes, std::integral_constant<int, G::kTile * G::kCodes>());
-      copy(to + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.k_scale) + r * G::kScales, std::integral_constant<int, G::kTile * G::kScales>());
-      copy(to + G::kPart, p.cache.v + r * G::kCodes, std::integral_constant<int, G::kTile * G::kCodes>());
-      copy(to + G::kPart + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.v_scale) + r * G::kScales, std::integral_constant<int, G::kTile * G::kScales>());
+      copy(to, p.cache.k + r * G::kCodes, std::integral_constant<int, G::kTile * G::kCodes>(), std::true_type());
+      copy(to + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.k_scale) + r * G::kScales, std::integral_constant<int, G::kTile * G::kScales>(), std::false_type());
+      copy(to + G::kPart, p.cache.v + r * G::kCodes, std::integral_constant<int, G::kTile * G::kCodes>(), std::true_type());
+      copy(to + G::kPart + G::kTile * G::kCodes, static_cast<const uint8_t*>(p.cache.v_scale) + r * G::kScales, std::integral_constant<int, G::kTile * G::kScales>(), std::false_type());
       issued = issued + 1 == G::kStages ? 0 : issued + 1;
-      next += kWarps;
+      ++next;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");  // one a tile, of nothing behind the last
   };
 #pragma unroll 1
   for (int i = 0; i < G::kStages; ++i) issue();
-  make_q(at);
-  __syncthreads();
 
-  int x = warp, stage = 0;
+  // where this lane's parts of the tile's first tokens lie; sixteen, and eight, tokens on it is the same place
+  constexpr int kKeyPieces = (kKeyBytes + 15) / 16, kValuePieces = (kValueBytes + 15) / 16;
+  uint32_t key_at[kKeyPieces], value_at[2][kValuePieces];
+#pragma unroll
+  for (int i = 0; i < kKeyPieces; ++i) key_at[i] = G::Swizzled(static_cast<uint32_t>(g * G::kCodes + c * kKeyBytes + 16 * i));
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int i = 0; i < kValuePieces; ++i) {
+      const uint32_t at_lane = static_cast<uint32_t>((2 * c + t) * G::kCodes + g * kValueBytes + 16 * i);
+      value_at[t][i] = static_cast<uint32_t>(G::kPart) + (G::Swizzled(at_lane & ~15u) | (at_lane & 15u));
+    }
+  }
+
+  int x = 0, stage = 0;
 #pragma unroll 1
   for (;;) {  // segments
     const int head = at.unit / p.row_blocks, row0 = (at.unit - head * p.row_blocks) * kRows, rows = min(kRows, p.tokens * p.group - row0);
@@ -391,28 +371,45 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
         for (int e = 0; e < 4; ++e) o[n][m][e] = 0.f;
       }
     }
-    const bool any = x < at.end;
-    if (any) {
+    {
+      // q as FP16, and the factor from a row's products to its scores
       uint32_t q[NT][kSteps][2];
-      float factor[NT][2];  // from a row's products to its scores
-      int sees[NT][2];      // tokens that a row may look at
+      float factor[NT][2];
+      int sees[NT][2];  // tokens that a row may look at
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        const int r = row0 + 8 * n + g, token = r / p.group;
+        const uint16_t* const from = static_cast<const uint16_t*>(p.q) + at.seq * p.ld_seq + token * p.ld_token + static_cast<long long>(head * p.group + r - token * p.group) * D;
+        constexpr int kPieces = D / 32;  // of eight channels, this lane's part of the row
+        uint4 raw[kPieces];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const uint2 w = *reinterpret_cast<const uint2*>(&q_rows[8 * n + g][c * (D / 4) + 4 * i]);
-          q[n][i][0] = w.x, q[n][i][1] = w.y;
+        for (int i = 0; i < kPieces; ++i) raw[i] = 8 * n + g < rows ? *reinterpret_cast<const uint4*>(from + c * (D / 4) + 8 * i) : make_uint4(0, 0, 0, 0);
+        float v[D / 4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(raw)[i];
+          const float2 two = p.bf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
+          v[2 * i] = two.x, v[2 * i + 1] = two.y;
+          top = max(top, max(__float_as_uint(two.x) & 0x7FFFFFFFu, __float_as_uint(two.y) & 0x7FFFFFFFu));
         }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(9 - exponent) of the largest and its inverse; the exponent is kept where both are ordinary numbers
+        const int e = min(max(static_cast<int>(top >> 23), 20), 240);
+        const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(e - 9) << 23) * p.scale;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) q[n][i / 2][i % 2] = Pack16(v[2 * i] * up, v[2 * i + 1] * up);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          factor[n][h] = q_factor[8 * n + 2 * c + h];
+          factor[n][h] = __shfl_sync(0xffffffffu, down, (2 * c + h) * 4);
           sees[n][h] = at.length - p.tokens + 1 + (row0 + 8 * n + 2 * c + h) / p.group;
         }
       }
       const int least_seen = at.length - p.tokens + 1;
 
 #pragma unroll 1
-      for (; x < at.end; x += kWarps) {
+      for (; x < at.end; ++x) {
         const uint32_t tile = ring + static_cast<uint32_t>(stage * G::kStage);
         asm volatile("cp.async.wait_group %0;" ::"n"(G::kStages - 1) : "memory");
         __syncwarp();
@@ -432,7 +429,8 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t token = static_cast<uint32_t>(16 * u + 8 * h + g);
-            LoadShared<kKeyBytes>(tile + token * G::kCodes + c * kKeyBytes, raw[h]);
+#pragma unroll
+            for (int i = 0; i < kKeyPieces; ++i) LoadShared<(kKeyBytes < 16 ? kKeyBytes : 16)>(tile + key_at[i] + static_cast<uint32_t>((16 * u + 8 * h) * G::kCodes), raw[h] + 4 * i);
             if constexpr (FP4) LoadShared<kKeyScales>(tile + G::kTile * G::kCodes + token * G::kScales + c * kKeyScales, &scale[h]);
           }
           if constexpr (FP4) {
@@ -574,7 +572,9 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const uint32_t token = static_cast<uint32_t>(16 * u + 8 * (t >> 1) + 2 * c + (t & 1));
-            LoadShared<kValueBytes>(tile + G::kPart + token * G::kCodes + g * kValueBytes, raw[t]);
+#pragma unroll
+            for (int i = 0; i < kValuePieces; ++i)
+              LoadShared<(kValueBytes < 16 ? kValueBytes : 16)>(tile + value_at[t & 1][i] + static_cast<uint32_t>((16 * u + 8 * (t >> 1)) * G::kCodes), raw[t] + 4 * i);
             if constexpr (FP4) LoadShared<(D == 256 ? 2 : 1)>(tile + G::kPart + G::kTile * G::kCodes + token * G::kScales + g * kValueChannels / 16, &scale[t]);
           }
           if (!whole) {
@@ -637,118 +637,135 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
       }
     }
 
-    // ---- the warps' sums.  o[n][t][2 h + r] is channel g D / 8 + 2 t + h, row 8 n + 2 c + r.
-    float* const parts = reinterpret_cast<float*>(smem);  // [warp][row][D]
+    // ---- the sums.  o[n][t][2 h + r] is channel g D / 8 + 2 t + h, row 8 n + 2 c + r.
+    const bool whole_unit = at.tile == 0 && at.end - at.begin == at.tiles;
+    float* const partial = p.partial + (static_cast<long long>(worker) * 2 + (at.tile > 0 ? 0 : 1)) * kRows * (D + 2);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int to_row = 8 * n + 2 * c + r;
+        float total = sum[n][r];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], d);
-        if (g == 0) {
-          row_most[warp][to_row] = most[n][r];
-          row_sum[warp][to_row] = sum[n][r];
-        }
-        if (any) {
-          float* const to = parts + (warp * kRows + to_row) * D + g * kValueChannels;
+        for (int d = 4; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        const int of = 8 * n + 2 * c + r;
+        if (of >= rows) continue;
+        if (whole_unit) {
+          const long long to = RowOf(p, at.seq, at.unit, row0 + of);
+          const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
+          uint32_t w[kTilesOfO];
 #pragma unroll
-          for (int t = 0; t < kTilesOfO; ++t) *reinterpret_cast<float2*>(to + 2 * t) = make_float2(o[n][t][r], o[n][t][2 + r]);
+          for (int t = 0; t < kTilesOfO; ++t) w[t] = Packed(p.bf16, o[n][t][r] * by, o[n][t][2 + r] * by);
+          uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D + g * kValueChannels);
+#pragma unroll
+          for (int t = 0; t < kTilesOfO / 4; ++t) out[t] = make_uint4(w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]);
+          if (p.lse != nullptr && g == 0) p.lse[to] = LogOfSum(most[n][r], total);
+        } else {
+          float4* const out = reinterpret_cast<float4*>(partial + of * D + g * kValueChannels);
+#pragma unroll
+          for (int t = 0; t < kTilesOfO / 2; ++t) out[t] = make_float4(o[n][2 * t][r], o[n][2 * t][2 + r], o[n][2 * t + 1][r], o[n][2 * t + 1][2 + r]);
+          if (g == 0) *reinterpret_cast<float2*>(partial + kRows * D + 2 * of) = make_float2(most[n][r], total);
         }
       }
     }
-    __syncthreads();
-    const bool whole_unit = at.tile == 0 && at.end - at.begin == at.tiles;
-    float* const partial = p.partial + (static_cast<long long>(blockIdx.x) * 2 + (at.tile > 0 ? 0 : 1)) * kRows * (D + 2);
-    for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
-      const int of = i / (D / 2), channel = i % (D / 2) * 2;
-      float all = -INFINITY, total = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) all = fmaxf(all, row_most[w][of]);
-      float2 y = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float m = row_most[w][of];
-        if (m == -INFINITY) {
-          total += row_sum[w][of];  // 0, or of a row that saw nothing but NaN
-          continue;
-        }
-        const float by = Exp2(m - all);
-        const float2 v = *reinterpret_cast<const float2*>(parts + (w * kRows + of) * D + channel);
-        total = fmaf(by, row_sum[w][of], total);
-        y.x = fmaf(by, v.x, y.x);
-        y.y = fmaf(by, v.y, y.y);
-      }
-      if (whole_unit) {
-        StoreRow<D>(p, at.seq, at.unit, row0 + of, channel, y, all, total);
-      } else {
-        *reinterpret_cast<float2*>(partial + of * D + channel) = y;
-        if (channel == 0) *reinterpret_cast<float2*>(partial + kRows * D + 2 * of) = make_float2(all, total);
-      }
+    if (at.tile == 0 && lane == 0 && p.parts != nullptr) {  // the first share of the unit says where the others are
+      const long long last = share.from + at.begin + at.tiles - 1;
+      p.parts[static_cast<long long>(at.seq) * units + at.unit] = whole_unit ? make_int2(0, 0) : make_int2(worker, ShareOf(share.all, last) - worker + 1);
     }
     if (at.end == count) break;
     NextSegment(p, count, G::kTile, &at);
-    make_q(at);
-    __syncthreads();  // the sums have been read, and q is there
   }
 }
 
-// The units that lie in several shares.  Block b looks after the unit that share b + 1 begins within, where no earlier share does.
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) JoinKernel(const AttendParams p) {
-  constexpr int kRows = 8 * NT, kRow = D + 2, kSlot = kRows * kRow, kBatch = 64;
-  __shared__ float2 stats[kBatch][kRows];
+// The units that lie in several shares.  Of few parts, a row is a warp's; of many, a block's, whose warps each take every eighth.  Which of the two goes by the parts
+// alone, so that the order of the sums does, too.
+constexpr int kManyParts = 24;
+template <int D>
+__global__ void __launch_bounds__(kThreads) JoinKernel(const AttendParams p, int rows_of_unit) {
+  constexpr int kMine = D / 32;  // channels of a lane
+  __shared__ float sums[kWarps][D + 2];
   GridDependencyWait();
-  const int b = static_cast<int>(blockIdx.x) + 1;
-  const Shares shares = *p.shares;
-  const ShareInfo at = p.share[b];
-  if (b >= shares.count) return;
-  const long long first = shares.begin(b) - at.tile, end = first + at.tiles;
-  if (at.tile == 0 || first < shares.begin(b - 1)) return;
-  const int row0 = at.unit % p.row_blocks * kRows, rows = min(kRows, p.tokens * p.group - row0);
-  int pieces = 2;  // of shares b - 1 (its second slot), b, ...
-  while (b - 1 + pieces < shares.count && shares.begin(b - 1 + pieces) < end) ++pieces;
-  const auto slot = [&](int k) { return p.partial + (static_cast<long long>(b - 1 + k) * 2 + (k == 0 ? 1 : 0)) * kSlot; };
-  constexpr int kMine = (kRows * D / 2 + kThreads - 1) / kThreads;
-  float most[kMine], total[kMine];
-  float2 y[kMine];
+  const int units = p.cache.heads * p.row_blocks, warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  const int2 parts = p.parts[blockIdx.x];
+  const bool many = parts.y >= kManyParts;
+  if (parts.y == 0) return;
+  const int seq = static_cast<int>(blockIdx.x) / units, unit = static_cast<int>(blockIdx.x) - seq * units, row0 = unit % p.row_blocks * rows_of_unit;
+  const int rows = min(rows_of_unit, p.tokens * p.group - row0);
+  const long long slot = static_cast<long long>(rows_of_unit) * (D + 2);
+  // the first part is of a share that goes on behind its unit's beginning, the others of shares that begin within the unit
+  const auto part = [&](int k) { return p.partial + (static_cast<long long>(parts.x + k) * 2 + (k == 0 ? 1 : 0)) * slot; };
+  const int rows_at_once = static_cast<int>(gridDim.y) * (many ? 1 : kWarps);
+  for (int of = many ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * kWarps + warp; of < rows; of += rows_at_once) {
+    // kAhead parts at a time, all of whose loads are on their way together
+    constexpr int kAhead = D == 256 ? 4 : 8;
+    const int step = many ? kWarps : 1;
+    float all = -INFINITY, y[kMine] = {}, total = 0.f;
+    for (int k0 = many ? warp : 0; k0 < parts.y; k0 += kAhead * step) {
+      float2 ms[kAhead], v[kAhead][kMine / 2];
 #pragma unroll
-  for (int j = 0; j < kMine; ++j) most[j] = -INFINITY, total[j] = 0.f, y[j] = make_float2(0.f, 0.f);
-  for (int k0 = 0; k0 < pieces; k0 += kBatch) {
-    const int n = min(kBatch, pieces - k0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * kRows; i += kThreads) stats[i / kRows][i % kRows] = *reinterpret_cast<const float2*>(slot(k0 + i / kRows) + kRows * D + i % kRows * 2);
-    __syncthreads();
+      for (int i = 0; i < kAhead; ++i) {
+        const int k = k0 + i * step;
+        ms[i] = make_float2(-INFINITY, 0.f);
+        if (k < parts.y) {
+          ms[i] = *reinterpret_cast<const float2*>(part(k) + rows_of_unit * D + 2 * of);
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int i = static_cast<int>(threadIdx.x) + j * kThreads, of = i / (D / 2), channel = i % (D / 2) * 2;
-      if (of >= rows) continue;
-      float all = most[j];
-      for (int k = 0; k < n; ++k) all = fmaxf(all, stats[k][of].x);
-      const float again = all == -INFINITY ? 0.f : Exp2(most[j] - all);
-      total[j] *= most[j] == -INFINITY ? 1.f : again;
-      y[j].x *= again;
-      y[j].y *= again;
-      most[j] = all;
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float2 ms = stats[k][of], v = *reinterpret_cast<const float2*>(slot(k0 + k) + of * D + channel);
-        const float by = ms.x == -INFINITY ? 0.f : Exp2(ms.x - all);
-        total[j] += ms.x == -INFINITY ? ms.y : by * ms.y;
-        y[j].x = fmaf(by, v.x, y[j].x);
-        y[j].y = fmaf(by, v.y, y[j].y);
+          for (int e = 0; e < kMine / 2; ++e) v[i][e] = *reinterpret_cast<const float2*>(part(k) + of * D + lane * kMine + 2 * e);
+        }
+      }
+      float to = all;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) to = fmaxf(to, ms[i].x);
+      const float again = to == -INFINITY ? 1.f : Exp2(all - to);
+      total *= again;
+#pragma unroll
+      for (int e = 0; e < kMine; ++e) y[e] *= again;
+      all = to;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (ms[i].x == -INFINITY) {
+          total += ms[i].y;  // 0, or of a row that saw nothing but NaN
+          continue;
+        }
+        const float by = Exp2(ms[i].x - all);
+        total = fmaf(by, ms[i].y, total);
+#pragma unroll
+        for (int e = 0; e < kMine / 2; ++e) {
+          y[2 * e] = fmaf(by, v[i][e].x, y[2 * e]);
+          y[2 * e + 1] = fmaf(by, v[i][e].y, y[2 * e + 1]);
+        }
       }
     }
-  }
+    if (many) {
+      __syncthreads();  // the row ahead has been read
 #pragma unroll
-  for (int j = 0; j < kMine; ++j) {
-    const int i = static_cast<int>(threadIdx.x) + j * kThreads, of = i / (D / 2), channel = i % (D / 2) * 2;
-    if (of < rows) StoreRow<D>(p, at.seq, at.unit, row0 + of, channel, y[j], most[j], total[j]);
+      for (int e = 0; e < kMine; ++e) sums[warp][lane * kMine + e] = y[e];
+      if (lane == 0) sums[warp][D] = total, sums[warp][D + 1] = all;
+      __syncthreads();
+      if (warp > 0) continue;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) all = fmaxf(all, sums[w][D + 1]);
+#pragma unroll
+      for (int e = 0; e < kMine; ++e) y[e] = 0.f;
+      total = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float most = sums[w][D + 1], by = most == -INFINITY ? 1.f : Exp2(most - all);
+        total = fmaf(by, sums[w][D], total);
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) y[e] = fmaf(by, sums[w][lane * kMine + e], y[e]);
+      }
+    }
+    const long long to = RowOf(p, seq, unit, row0 + of);
+    const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
+    uint32_t* const out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to * D + lane * kMine);
+#pragma unroll
+    for (int e = 0; e < kMine / 2; ++e) out[e] = Packed(p.bf16, y[2 * e] * by, y[2 * e + 1] * by);
+    if (p.lse != nullptr && lane == 0) p.lse[to] = LogOfSum(all, total);
   }
 }
 
 struct Shape {
   int nt, row_blocks, blocks;
+  bool cuts;  // shares may begin within a unit
 };
 Shape ShapeOf(const CacheAttentionCall& c) {
   Shape s;
@@ -759,14 +776,15 @@ Shape ShapeOf(const CacheAttentionCall& c) {
   const long long room = static_cast<long long>(c.most_pages) * c.cache.page, tiles = (room + tile - 1) / tile * c.seqs * c.cache.heads * s.row_blocks;
   // as many as the GPU holds at once, and no more than have a tile for each warp
   const long long most = static_cast<long long>(DeviceSmCount()) * (c.cache.dim * s.nt <= 128 ? 2 : 1);
-  s.blocks = static_cast<int>(std::max(1LL, std::min(most, (tiles + kLeastTiles - 1) / kLeastTiles)));
+  s.blocks = static_cast<int>(std::max(1LL, std::min(most, (tiles + kWarps - 1) / kWarps)));
+  s.cuts = tiles > static_cast<long long>(c.seqs) * c.cache.heads * s.row_blocks;  // a unit may have more than one
   return s;
 }
 
 template <int D, bool FP4, int NT>
 cudaError_t Launch(const AttendParams& p, const Shape& s, cudaStream_t stream) {
   using G = Geometry<D, FP4, NT>;
-  static_assert(G::kStages >= 2 && G::kBlocks * (G::kBytes + 6144) <= 227 * 1024, "");
+  static_assert(G::kStages >= 2 && G::kBlocks * (G::kBytes + 2048) <= 227 * 1024, "");
   const cudaError_t set = cudaFuncSetAttribute(CacheAttentionKernel<D, FP4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
   if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
@@ -778,10 +796,12 @@ cudaError_t Launch(const AttendParams& p, const Shape& s, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
   const cudaError_t err = cudaLaunchKernelEx(&cfg, CacheAttentionKernel<D, FP4, NT>, p);
-  if (err != cudaSuccess || s.blocks < 2) return err;
-  cfg.gridDim = dim3(static_cast<unsigned>(s.blocks - 1));
+  if (err != cudaSuccess || !s.cuts) return err;
+  // a block for each row where some units can be expected to have many parts: the longest sequence may be four times the mean
+  const int units = p.seqs * p.cache.heads * p.row_blocks, rows = std::min(8 * NT, p.tokens * p.group);
+  cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(4 * s.blocks * kWarps / units >= kManyParts ? rows : (rows + kWarps - 1) / kWarps));
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, JoinKernel<D, NT>, p);
+  return cudaLaunchKernelEx(&cfg, JoinKernel<D>, p, 8 * NT);
 }
 
 template <bool FP4>
@@ -796,9 +816,11 @@ cudaError_t LaunchOf(const AttendParams& p, const Shape& s, cudaStream_t stream)
 
 }  // namespace
 
+// The parts of the units come first, on 16 bytes.
+size_t PartsBytes(const CacheAttentionCall& c, const Shape& s) { return (sizeof(int2) * c.seqs * c.cache.heads * s.row_blocks + 15) / 16 * 16; }
 size_t CacheAttentionWorkspace(const CacheAttentionCall& c) {
   const Shape s = ShapeOf(c);
-  return s.blocks < 2 ? 0 : sizeof(Shares) + s.blocks * (sizeof(ShareInfo) + sizeof(float) * 2 * 8 * s.nt * (c.cache.dim + 2));
+  return !s.cuts ? 0 : PartsBytes(c, s) + sizeof(float) * s.blocks * kWarps * 2 * 8 * s.nt * (c.cache.dim + 2);
 }
 
 cudaError_t LaunchCacheAttention(const CacheAttentionCall& c, cudaStream_t stream) {
@@ -820,10 +842,10 @@ cudaError_t LaunchCacheAttention(const CacheAttentionCall& c, cudaStream_t strea
   p.row_blocks = s.row_blocks;
   p.scale = c.scale * 1.44269504f * (c.cache.fp4 ? c.cache.k_unit : 1.f);
   if (!c.cache.fp4) p.cache.v_unit = 1.f;
-  if (s.blocks > 1) {
-    p.shares = static_cast<Shares*>(c.workspace);
-    p.share = reinterpret_cast<ShareInfo*>(p.shares + 1);
-    p.partial = reinterpret_cast<float*>(p.share + s.blocks);
+  if (static_cast<long long>(c.seqs) * c.cache.heads * s.row_blocks > INT_MAX) return cudaErrorInvalidValue;
+  if (s.cuts) {
+    p.parts = static_cast<int2*>(c.workspace);
+    p.partial = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + PartsBytes(c, s));
   }
   p.out = c.out;
   p.lse = c.lse;
