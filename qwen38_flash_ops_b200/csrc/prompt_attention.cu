@@ -32,11 +32,9 @@
 namespace qfg {
 namespace {
 
-constexpr int kTile = 128, kThreads = 384;
-// Registers of a thread: the launch's 168 for all are shared out, 8 warps of 232 and 4 of 40 (together the 2016 that a lane of twelve warps has).
-constexpr int kSoftmaxRegisters = 232, kOtherRegisters = 40;
-static_assert(8 * kSoftmaxRegisters + 4 * kOtherRegisters <= 12 * 168, "");
-
+constexpr int kTile = 128;
+// Of sixteen pairs of weights those that the FMA units make, so that less waits for the unit for exponentials, which is an eighth as wide.  8192 tokens of 64 heads of 128, us:
+// none 1019, two 1006, four 1002, six 998; packed prompts of 24 heads of 64 54.4, 54.4, 53.3, 52.4.
 constexpr int kPolyOf16 = 4;
 struct PromptParams {
   CUtensorMap q, k, v;
@@ -48,11 +46,18 @@ struct PromptParams {
   bool causal, give_up;
 };
 
-template <int D>
+// TILES: of queries, for a block.
+template <int D, int TILES>
 struct Geometry {
-  static constexpr int kHeadTile = kTile * D * 2;  // bytes of 128 rows
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kBytes = 2 * kHeadTile + kStages * kHeadTile + 1024;
+  static constexpr int kThreads = 128 + 128 * TILES, kBlocks = TILES == 1 ? 2 : 1;
+  // Registers of a thread: the launch's for all are shared out, by four warps.  Two tiles: 168, 8 warps of 232 and 4 of 40 (together the 2016 that a lane of twelve warps
+  // has).  One tile, two blocks an SM: 128, 4 warps of 208 and 4 of 48 (the 1024 of eight warps).
+  static constexpr int kSoftmaxRegisters = TILES == 2 ? 232 : 208, kOtherRegisters = TILES == 2 ? 40 : 48;
+  static_assert(TILES * 4 * kSoftmaxRegisters + 4 * kOtherRegisters <= (TILES == 2 ? 12 * 168 : 8 * 128), "");
+  static constexpr int kColumns = TILES == 2 ? 512 : 256, kOutput = TILES * kTile;  // of tensor memory; where O begins
+  static constexpr int kHeadTile = kTile * D * 2;                                   // bytes of 128 rows
+  static constexpr int kStages = 5;
+  static constexpr int kBytes = (TILES + kStages) * kHeadTile + 1024;
 };
 
 struct PromptCtl {
@@ -182,8 +187,9 @@ __device__ __forceinline__ T Uniform(T v) {
 
 // Where a block's queries and keys lie; tiles < 0: a block too many.
 struct Place {
-  int q0, k0, queries, keys, first;  // first: the first of its 256 queries, within the sequence
+  int q0, k0, queries, keys, first;  // first: the first of its queries, within the sequence
 };
+template <int ROWS>  // of a block
 __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
   const int lane = threadIdx.x & 31;
   Place at = {0, 0, 0, 0, -1};
@@ -196,7 +202,7 @@ __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
       q0 = min(max(p.q_offsets[i], 0), p.q_rows);
       q1 = min(max(p.q_offsets[i + 1], q0), p.q_rows);
     }
-    const int tiles = (q1 - q0 + 2 * kTile - 1) / (2 * kTile);
+    const int tiles = (q1 - q0 + ROWS - 1) / ROWS;
     int upto = tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -209,7 +215,7 @@ __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
       const int ahead = before + __shfl_sync(0xffffffffu, upto - tiles, of), n = __shfl_sync(0xffffffffu, tiles, of);
       at.q0 = __shfl_sync(0xffffffffu, q0, of);
       at.queries = __shfl_sync(0xffffffffu, q1 - q0, of);
-      at.first = (n - 1 - (rank - ahead)) * 2 * kTile;
+      at.first = (n - 1 - (rank - ahead)) * ROWS;
       const int seq = base - of;
       at.k0 = min(max(p.k_offsets[seq], 0), p.k_rows);
       at.keys = min(max(p.k_offsets[seq + 1], at.k0), p.k_rows) - at.k0;
@@ -227,16 +233,16 @@ __device__ __forceinline__ int KeyTiles(const PromptParams& p, const Place& at, 
   return (seen + kTile - 1) / kTile;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __grid_constant__ PromptParams p) {
-  using G = Geometry<D>;
+template <int D, bool BF16, int TILES>
+__global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILES>::kBlocks) PromptAttentionKernel(const __grid_constant__ PromptParams p) {
+  using G = Geometry<D, TILES>;
   constexpr int kBoxes = D / 64, kBox = kTile * 128;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PromptCtl ctl;
   const int warp = Uniform(static_cast<int>(threadIdx.x) >> 5), lane = static_cast<int>(threadIdx.x) & 31;
-  const uint32_t smem = (Smem(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * G::kHeadTile;
+  const uint32_t smem = (Smem(smem_raw) + 1023u) & ~1023u, ring = smem + TILES * G::kHeadTile;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < TILES; ++i) {
       BarInit(Smem(&ctl.q_full[i]), 1);
       BarInit(Smem(&ctl.s_full[i]), 1);
       BarInit(Smem(&ctl.p_most[i]), 4);
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Smem(&ctl.tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Smem(&ctl.tmem)), "r"(G::kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (warp == 1 && lane == 0) {
@@ -263,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
   FenceBefore();
   GridDependencyWait();
   const int head = static_cast<int>(blockIdx.x) % p.q_heads;
-  const Place at = FindPlace(p, static_cast<int>(blockIdx.x) / p.q_heads);
-  const int tiles[2] = {at.first < 0 ? 0 : KeyTiles(p, at, at.first), at.first < 0 ? 0 : KeyTiles(p, at, at.first + kTile)};
+  const Place at = FindPlace<TILES * kTile>(p, static_cast<int>(blockIdx.x) / p.q_heads);
+  const int tiles[2] = {at.first < 0 ? 0 : KeyTiles(p, at, at.first), at.first < 0 || TILES == 1 ? 0 : KeyTiles(p, at, at.first + kTile)};
   const int n0 = Uniform(tiles[0]), n1 = Uniform(tiles[1]), most = max(n0, n1);
   // the last tile of values runs past the sequence's end
   const bool fix = Uniform(most > 0 && most * kTile > at.keys ? 1 : 0) != 0;
@@ -274,10 +280,10 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
 
   if (warp >= 4) {
     // ---- softmax and output
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kSoftmaxRegisters));
     const int t = (warp >> 2) - 1, row = at.first + t * kTile + (warp & 3) * 32 + lane;  // of the sequence
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_at = tmem + lanes + static_cast<uint32_t>(t * kTile), o_at = tmem + lanes + static_cast<uint32_t>(2 * kTile + t * D);
+    const uint32_t s_at = tmem + lanes + static_cast<uint32_t>(t * kTile), o_at = tmem + lanes + static_cast<uint32_t>(G::kOutput + t * D);
     const int count = tiles[t], sees = p.causal ? min(at.keys, row + 1 + at.keys - at.queries) : at.keys;
     const int first_sees = p.causal ? min(at.keys, at.first + t * kTile + (warp & 3) * 32 + 1 + at.keys - at.queries) : at.keys;  // the warp's first row
     const float step = 8.f / p.scale;
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
       if (mine && p.lse != nullptr) p.lse[to] = !good ? __uint_as_float(0x7FFFFFFFu) : total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegisters));
   }
   if (warp == 0) {
     // ---- products
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
     };
     auto outputs = [&](auto tile, int j, int v, int k, int count) {  // of tile t, and its next scores
       constexpr int t = decltype(tile)::value;
-      const uint32_t b = v_desc + static_cast<uint32_t>(v) * kStageStep, d = tmem + 2 * kTile + t * D, a = tmem + t * kTile;
+      const uint32_t b = v_desc + static_cast<uint32_t>(v) * kStageStep, d = tmem + G::kOutput + t * D, a = tmem + t * kTile;
       wait(Smem(&ctl.p_most[t]), static_cast<uint32_t>(j & 1));
       FenceAfter();
       if (good && ElectOne()) {
@@ -448,12 +454,14 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
     const std::integral_constant<int, 1> second;
     if (most > 0) {
       if (n0 > 0) wait(Smem(&ctl.q_full[0]), 0);
-      if (n1 > 0) wait(Smem(&ctl.q_full[1]), 0);
+      if (TILES > 1 && n1 > 0) wait(Smem(&ctl.q_full[1]), 0);
       const int k0 = arrived();
       FenceAfter();
       if (good && ElectOne()) {
         if (n0 > 0) scores(first, k0);
-        if (n1 > 0) scores(second, k0);
+        if constexpr (TILES > 1) {
+          if (n1 > 0) scores(second, k0);
+        }
         release(k0);
       }
       __syncwarp();
@@ -464,7 +472,9 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
       const int v = arrived(), k = more ? arrived() : 0;
       if (fix && !more) wait(Smem(&ctl.fixed), 0);
       if (j < n0) outputs(first, j, v, k, n0);
-      if (j < n1) outputs(second, j, v, k, n1);
+      if constexpr (TILES > 1) {
+        if (j < n1) outputs(second, j, v, k, n1);
+      }
       if (good && ElectOne()) {
         release(v);
         if (more) release(k);
@@ -491,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
       __syncwarp();
       if (!good) break;
       if (position == 0) {
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < TILES; ++t) {
           if (tiles[t] > 0) load(smem + static_cast<uint32_t>(t * G::kHeadTile), &p.q, head, at.q0 + at.first + t * kTile, Smem(&ctl.q_full[t]));
           if (t == 0) load(ring, &p.k, of, at.k0, Smem(&ctl.full[0]));
         }
@@ -519,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) PromptAttentionKernel(const __gri
   FenceBefore();
   __syncthreads();
   FenceAfter();
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kColumns) : "memory");
 }
 
 bool EncodeHeads(CUtensorMap* map, const void* x, int dtype, int dim, int heads, int64_t rows, int64_t ld) {
@@ -532,21 +542,24 @@ bool EncodeHeads(CUtensorMap* map, const void* x, int dtype, int dim, int heads,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool BF16>
-cudaError_t Launch(const PromptParams& p, unsigned blocks, cudaStream_t stream) {
-  using G = Geometry<D>;
-  static_assert(G::kBytes + static_cast<int>(sizeof(PromptCtl)) <= 227 * 1024 && G::kStages <= 8, "");
-  const cudaError_t set = cudaFuncSetAttribute(PromptAttentionKernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
+template <int D, bool BF16, int TILES>
+cudaError_t Launch(const PromptParams& p, cudaStream_t stream) {
+  using G = Geometry<D, TILES>;
+  static_assert(G::kBlocks * (G::kBytes + static_cast<int>(sizeof(PromptCtl)) + 1024) <= 228 * 1024, "");
+  // sequences of any lengths that add up to the rows have no more tiles than this
+  const long long blocks = (static_cast<long long>(p.q_rows) / (TILES * kTile) + std::min(p.seqs, p.q_rows)) * p.q_heads;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  const cudaError_t set = cudaFuncSetAttribute(PromptAttentionKernel<D, BF16, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
   if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(G::kThreads);
   cfg.dynamicSmemBytes = G::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {OverlapAttribute()};
   cfg.attrs = attr;
   cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, PromptAttentionKernel<D, BF16>, p);
+  return cudaLaunchKernelEx(&cfg, PromptAttentionKernel<D, BF16, TILES>, p);
 }
 
 }  // namespace
@@ -571,15 +584,11 @@ cudaError_t LaunchPromptAttention(const PromptCall& c, cudaStream_t stream) {
   p.scale = c.scale * 1.44269504f;
   p.causal = c.causal;
   p.give_up = c.give_up;
-  // sequences of any lengths that add up to the rows have no more tiles than this
-  const long long blocks = (c.q_rows / (2 * kTile) + std::min<long long>(c.seqs, c.q_rows)) * c.q_heads;
-  if (blocks > INT_MAX) return cudaErrorInvalidValue;
-  const unsigned n = static_cast<unsigned>(blocks);
   cudaError_t err;
   if (c.dtype == QFG_BFLOAT16) {
-    err = c.dim == 64 ? Launch<64, true>(p, n, stream) : Launch<128, true>(p, n, stream);
+    err = c.dim == 64 ? Launch<64, true, 1>(p, stream) : Launch<128, true, 2>(p, stream);
   } else {
-    err = c.dim == 64 ? Launch<64, false>(p, n, stream) : Launch<128, false>(p, n, stream);
+    err = c.dim == 64 ? Launch<64, false, 1>(p, stream) : Launch<128, false, 2>(p, stream);
   }
   const cudaError_t last = cudaGetLastError();
   return err == cudaSuccess ? last : err;
