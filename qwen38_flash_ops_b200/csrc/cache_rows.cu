@@ -195,18 +195,19 @@ __device__ __forceinline__ void StoreCache(const float (&f)[16], int c0, int c1,
   }
 }
 
-// This lane's channels of rows of a side: eight from c0 and eight from c1.
+// This lane's channels of rows of a side: eight from c0 and eight from c1.  Where it may be, those are eight of either half of what is rotated or of the row, so that
+// the lanes of a load or a store take whole sectors.
 struct Channels {
   int c0, c1;
-  bool turned, split;  // rotated; with the channels that they are rotated with in the other eight
+  bool turned, split;  // rotated; eight of either half
 };
-template <int WHICH>
+template <int L, int WHICH>  // 0: queries, 1: keys, 2: values, 3: keys as they are
 __device__ __forceinline__ Channels ChannelsOf(const HeadsParams& p, int lane) {
   Channels c;
   c.turned = WHICH < 2 && 16 * lane < p.rotary;
-  c.split = c.turned && !p.interleaved;
+  c.split = WHICH >= 2 || (c.turned && !p.interleaved);
   c.c0 = c.split ? 8 * lane : 16 * lane;
-  c.c1 = c.split ? p.rotary / 2 + 8 * lane : c.c0 + 8;
+  c.c1 = c.split ? (WHICH < 2 ? p.rotary / 2 : 8 * L) + 8 * lane : c.c0 + 8;
   return c;
 }
 template <typename T>
@@ -219,15 +220,15 @@ __device__ __forceinline__ Two<T> LoadRow(const Side& s, const Channels& c, long
   return {LoadEight<T, VEC>(x + c.c0), LoadEight<T, VEC>(x + c.c1)};
 }
 
-// The rows of a token that are queries (0), keys (1) or values (2): those of this warp, every `step`-th run of kRows from row `row` on, up to row `end`.  `next` holds the
+// The rows of a token that are queries (0), keys (1), values (2) or keys as they are (3): those of this warp, every `step`-th run of kRows from row `row` on, up to row `end`.  `next` holds the
 // first; the row behind is on its way while one is worked on.  Every lane of the warp makes the same number of steps, as shuffles are of whole warps.
 template <typename T, int L, bool VEC, int WHICH>
 __device__ __forceinline__ void SideRows(const HeadsParams& p, long long token, const float2* turn, const float* weight, long long place, int row, int step, int end,
                                          Two<T> next) {
   constexpr int D = 16 * L, kRows = 32 / L;
-  const Side& s = p.side[WHICH];
+  const Side& s = p.side[WHICH == 3 ? 1 : WHICH];
   const int lane = threadIdx.x % L;
-  const Channels c = ChannelsOf<WHICH>(p, lane);
+  const Channels c = ChannelsOf<L, WHICH>(p, lane);
   float cosine[8], sine[8];  // of this lane's eight pairs
   if (c.turned) {
 #pragma unroll
@@ -281,9 +282,9 @@ __device__ __forceinline__ void SideRows(const HeadsParams& p, long long token, 
   }
 }
 
-// L lanes a row, D = 16 L.
-template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 ? 3 : 4) HeadsKernel(const HeadsParams p) {
+// L lanes a row, D = 16 L.  QUERIES: false where keys and values alone are written, without a norm or a rotation.
+template <typename T, int L, bool VEC, bool QUERIES>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 || !QUERIES ? 3 : 4) HeadsKernel(const HeadsParams p) {
   constexpr int D = 16 * L, kRows = 32 / L;
   __shared__ __align__(16) float2 turn[kMostTokens * D / 2];
   __shared__ __align__(16) float weight[2][D];
@@ -299,22 +300,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 ? 3 : 4) H
   const int step = turns ? warps : 1 << 24;
   const auto begins = [&](int side, int heads) { return real && first[side] >= 0 && first[side] * kRows + in_run < heads; };
   Two<T> next = {};
-  if (begins(0, q)) {
-    next = LoadRow<T, L, VEC>(p.side[0], ChannelsOf<0>(p, lane), token, first[0] * kRows + in_run);
+  if (QUERIES && begins(0, q)) {
+    next = LoadRow<T, L, VEC>(p.side[0], ChannelsOf<L, 0>(p, lane), token, first[0] * kRows + in_run);
   } else if (!turns && begins(1, k)) {
-    next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<1>(p, lane), token, first[1] * kRows + in_run);
+    next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<L, QUERIES ? 1 : 3>(p, lane), token, first[1] * kRows + in_run);
   } else if (!turns && begins(2, v)) {
-    next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<2>(p, lane), token, first[2] * kRows + in_run);
+    next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<L, 2>(p, lane), token, first[2] * kRows + in_run);
   }
 
-  for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+  for (int i = threadIdx.x; QUERIES && i < 2 * D; i += kThreads) {
     const void* const w = p.side[i / D].weight;
     if (w != nullptr) weight[i / D][i % D] = p.offset + (p.weight_f32 ? static_cast<const float*>(w)[i % D] : ToFloat(static_cast<const T*>(w)[i % D]));
   }
   float2* const by = turn + t * half;
   long long to = -1;  // (page, row of it) as page * kv_heads * page size + row; < 0: not written
   if (real) {
-    for (int j = sub * 32 + (static_cast<int>(threadIdx.x) & 31); j < half; j += 32 * warps) {
+    for (int j = sub * 32 + (static_cast<int>(threadIdx.x) & 31); QUERIES && j < half; j += 32 * warps) {
       const RotaryPair pair = p.pairs[j];
       const long long at = token + pair.axis * p.ld_positions;
       const long long position = p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
@@ -328,19 +329,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 ? 3 : 4) H
       to = slot >= 0 && page < p.cache.pages ? page * p.cache.heads * p.cache.page + (slot - page * p.cache.page) : -1;
     }
   }
-  __syncthreads();
+  if constexpr (QUERIES) __syncthreads();
   if (!real) return;
-  if (first[0] * kRows < q) {
+  if (QUERIES && first[0] * kRows < q) {
     SideRows<T, L, VEC, 0>(p, token, by, weight[0], to, first[0] * kRows + in_run, step, q, next);
     if (!turns) return;
   }
   if (first[1] >= 0 && first[1] * kRows < k) {
-    if (turns && begins(1, k)) next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<1>(p, lane), token, first[1] * kRows + in_run);
-    SideRows<T, L, VEC, 1>(p, token, by, weight[1], to, first[1] * kRows + in_run, step, k, next);
+    if (turns && begins(1, k)) next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<L, QUERIES ? 1 : 3>(p, lane), token, first[1] * kRows + in_run);
+    SideRows<T, L, VEC, QUERIES ? 1 : 3>(p, token, by, weight[1], to, first[1] * kRows + in_run, step, k, next);
     if (!turns) return;
   }
   if (first[2] >= 0 && first[2] * kRows < v) {
-    if (turns && begins(2, v)) next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<2>(p, lane), token, first[2] * kRows + in_run);
+    if (turns && begins(2, v)) next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<L, 2>(p, lane), token, first[2] * kRows + in_run);
     SideRows<T, L, VEC, 2>(p, token, by, nullptr, to, first[2] * kRows + in_run, step, v, next);
   }
 }
@@ -349,13 +350,13 @@ template <typename T, int L>
 cudaError_t LaunchHeads(HeadsParams& p, bool vec, cudaStream_t stream) {
   // Few tokens: one a block, its rows over as many blocks as leave every warp one run of them.  Many: a warp has sixteen runs or more, so that its sines and cosines
   // are a small part of it, as long as there is a block for most SMs.
-  constexpr int kRows = 32 / L, kWarps = kThreads / 32, kLeastRuns = 16;
+  constexpr int kRows = 32 / L, kWarps = kThreads / 32;
   int runs = 0;
   for (const Side& s : p.side) runs += (s.heads + kRows - 1) / kRows;
   const int sms = DeviceSmCount();
   const bool few = p.tokens <= 2 * sms;
   p.log_tokens = 0;
-  while (1 << p.log_tokens < kMostTokens && runs << p.log_tokens < kLeastRuns * kWarps && p.tokens >> (p.log_tokens + 1) >= sms * 4 / 5) ++p.log_tokens;
+  while (1 << p.log_tokens < kMostTokens && runs << p.log_tokens < 16 * kWarps && p.tokens >> (p.log_tokens + 1) >= sms * 4 / 5) ++p.log_tokens;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.tokens + (1 << p.log_tokens) - 1) >> p.log_tokens), static_cast<unsigned>(few ? (runs + kWarps - 1) / kWarps : 1));
   cfg.blockDim = dim3(kThreads);
@@ -363,7 +364,8 @@ cudaError_t LaunchHeads(HeadsParams& p, bool vec, cudaStream_t stream) {
   cudaLaunchAttribute attr[1] = {OverlapAttribute()};
   cfg.attrs = attr;
   cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
-  return vec ? cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, true>, p) : cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, false>, p);
+  if (p.side[0].heads > 0) return vec ? cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, true, true>, p) : cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, false, true>, p);
+  return vec ? cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, true, false>, p) : cudaLaunchKernelEx(&cfg, HeadsKernel<T, L, false, false>, p);
 }
 
 template <typename T>
@@ -387,7 +389,7 @@ struct ReadParams {
 };
 constexpr int kReadRows = 16;  // of a block
 
-template <typename T, int L>
+template <typename T, int L, bool FP4>
 __global__ void __launch_bounds__(kThreads) CacheReadKernel(const ReadParams p) {
   constexpr int D = 16 * L;
   __shared__ long long place[kReadRows];  // -2: a row of no sequence; -1: one that no page holds
@@ -412,47 +414,67 @@ __global__ void __launch_bounds__(kThreads) CacheReadKernel(const ReadParams p) 
     place[threadIdx.x] = at;
   }
   __syncthreads();
-  const int per_row = p.cache.heads * 2 * L, items = kReadRows * per_row;  // a lane's sixteen channels
-  for (int i = threadIdx.x; i < items; i += kThreads) {
-    const int r = i / per_row, rest = i - r * per_row, values = rest / (p.cache.heads * L), c = rest - values * p.cache.heads * L, head = c / L, lane = c - head * L;
-    const long long at = place[r];
-    if (at == -2) continue;
-    float f[16];
-    if (at < 0) {
+  // A warp takes a head's keys, or values: rows that lie beside one another in the cache, L lanes each, all of whose codes are on their way together.
+  constexpr int kAtOnce = 32 / L, kSteps = kReadRows / kAtOnce, kAhead = kSteps < 4 ? kSteps : 4;
+  const int warp = static_cast<int>(threadIdx.x) / 32, in_warp = static_cast<int>(threadIdx.x) & 31, lane = in_warp % L;
+  for (int side = warp; side < 2 * p.cache.heads; side += kThreads / 32) {
+    const bool values = side >= p.cache.heads;
+    const int head = values ? side - p.cache.heads : side;
+    const long long base = static_cast<long long>(head) * p.cache.page;
+    const uint8_t* const codes = values ? p.cache.v : p.cache.k;
+    const uint8_t* const scales = static_cast<const uint8_t*>(values ? p.cache.v_scale : p.cache.k_scale);
+    const float unit = values ? p.cache.v_unit : p.cache.k_unit;
+    // eight channels of either half of the row, so that the lanes of a store fill whole sectors
+    T* const out = static_cast<T*>(values ? p.v_out : p.k_out) + (row0 * p.cache.heads + head) * D + lane * 8;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] = 0.f;
-    } else {
-      const long long row = at + static_cast<long long>(head) * p.cache.page;
-      const uint8_t* const codes = values ? p.cache.v : p.cache.k;
-      const void* const scales = values ? p.cache.v_scale : p.cache.k_scale;
-      if (p.cache.fp4) {
-        const uint2 w = *reinterpret_cast<const uint2*>(codes + row * (D / 2) + lane * 8);
-        const __nv_fp8_storage_t s = static_cast<const uint8_t*>(scales)[row * L + lane];
-        const float scale = __half2float(__half(__nv_cvt_fp8_to_halfraw(s, __NV_E4M3))) * (values ? p.cache.v_unit : p.cache.k_unit);
+    for (int first = 0; first < kSteps; first += kAhead) {
+      uint4 w[kAhead];
+      float scale[kAhead][2];
+      long long at[kAhead];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const __nv_fp4x2_storage_t two = static_cast<__nv_fp4x2_storage_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
-          const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(two, __NV_E2M1);
-          const float2 v = __half22float2(__half2(h));
-          f[2 * e] = v.x * scale;
-          f[2 * e + 1] = v.y * scale;
-        }
-      } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(codes + row * D + lane * 16);
-        const float scale = static_cast<const float*>(scales)[row];
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+      for (int i = 0; i < kAhead; ++i) {
+        at[i] = place[(first + i) * kAtOnce + in_warp / L];
+        w[i] = make_uint4(0, 0, 0, 0);
+        scale[i][0] = scale[i][1] = 0.f;
+        if (at[i] < 0) continue;
+        const long long row = at[i] + base;
+        if constexpr (FP4) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(words[e >> 1] >> (16 * (e & 1))), __NV_E4M3);
-          const float2 v = __half22float2(__half2(h));
-          f[2 * e] = v.x * scale;
-          f[2 * e + 1] = v.y * scale;
+          for (int h = 0; h < 2; ++h) {
+            (h == 0 ? w[i].x : w[i].z) = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + h * (D / 4) + lane * 4);
+            scale[i][h] = __half2float(__half(__nv_cvt_fp8_to_halfraw(scales[row * L + h * (L / 2) + lane / 2], __NV_E4M3))) * unit;
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint2 two = *reinterpret_cast<const uint2*>(codes + row * D + h * (D / 2) + lane * 8);
+            (h == 0 ? w[i].x : w[i].z) = two.x, (h == 0 ? w[i].y : w[i].w) = two.y;
+          }
+          scale[i][0] = scale[i][1] = reinterpret_cast<const float*>(scales)[row];
         }
       }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (at[i] == -2) continue;
+        float f[16];
+        const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          __half2_raw h;
+          if constexpr (FP4) {
+            h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(words[e >> 2 << 1] >> (8 * (e & 3))), __NV_E2M1);
+          } else {
+            h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(words[e >> 1] >> (16 * (e & 1))), __NV_E4M3);
+          }
+          const float2 v = __half22float2(__half2(h));
+          f[2 * e] = v.x * scale[i][e >> 2];
+          f[2 * e + 1] = v.y * scale[i][e >> 2];
+        }
+        T* const to = out + static_cast<long long>((first + i) * kAtOnce + in_warp / L) * p.cache.heads * D;
+        StoreEight<T>(to, f);
+        StoreEight<T>(to + D / 2, f + 8);
+      }
     }
-    T* const out = static_cast<T*>(values ? p.v_out : p.k_out) + ((row0 + r) * p.cache.heads + head) * D + lane * 16;
-    StoreEight<T>(out, f);
-    StoreEight<T>(out + 8, f + 8);
   }
 }
 
@@ -466,9 +488,9 @@ cudaError_t LaunchReadOf(int dim, const ReadParams& p, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = MayOverlapPredecessor(stream) ? 1 : 0;
   switch (dim) {
-    case 64: return cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 4>, p);
-    case 128: return cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 8>, p);
-    case 256: return cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 16>, p);
+    case 64: return p.cache.fp4 ? cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 4, true>, p) : cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 4, false>, p);
+    case 128: return p.cache.fp4 ? cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 8, true>, p) : cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 8, false>, p);
+    case 256: return p.cache.fp4 ? cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 16, true>, p) : cudaLaunchKernelEx(&cfg, CacheReadKernel<T, 16, false>, p);
     default: return cudaErrorInvalidValue;
   }
 }
