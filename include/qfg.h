@@ -414,8 +414,8 @@ QFG_API int qfg_cache_read(const qfg_kv_cache* cache, const int32_t* table, int6
  * include them: token t sees the first lengths[i] - tokens + 1 + t.  q [seqs][tokens][q_heads][head_dim] (BFLOAT16 or FLOAT16, sequences ld_seq and
  * tokens ld_token elements apart, on 16 bytes), out the same, contiguous; `lse` (NULL, or FP32 [seqs][tokens][q_heads]) gets the natural
  * logarithm of the sum of the exponentials.  Query head h reads key head h / (q_heads / kv_heads).  A row that sees nothing (a length of
- * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it; tokens whose page is none of the cache's are left
- * out.  Values that lie behind a sequence's length take no part, whatever they are.  A wait inside the kernel that runs out makes the rows concerned NaN.
+ * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it (a table is for 2^34 tokens at most); tokens whose page is none of the cache's are left
+ * out.  Values that lie behind a sequence's length take no part, whatever they are. 
  * `workspace`: that many bytes (0 where sequences are never cut), on 16 bytes, not looked at before the call and free behind it; calls
  * that run at once need one each. */
 QFG_API int qfg_cache_attention_workspace_bytes(const qfg_kv_cache* cache, int64_t seqs, int64_t tokens, int64_t q_heads, int64_t most_pages, size_t* bytes);
@@ -433,6 +433,9 @@ QFG_API int qfg_cache_attention(int dtype, const void* q, int64_t ld_seq, int64_
 QFG_API int qfg_prompt_attention(int dtype, const void* q, int64_t ldq, int64_t q_rows, int64_t q_heads, const void* k, int64_t ldk, const void* v,
                                  int64_t ldv, int64_t k_rows, int64_t kv_heads, int64_t head_dim, const int32_t* q_offsets, const int32_t* k_offsets,
                                  int64_t seqs, int causal, float scale, void* out, float* lse, void* stream);
+/* Every wait inside the kernel is bounded; rows of a block whose wait ran out are NaN, and the next call is whole.  For tests, in the whole process: "give_up" = 1, no
+ * operand comes, and what waits for it gives up. */
+QFG_API int qfg_prompt_attention_set_option(const char* key, const char* value);
 
 /* Measurement aid, no counterpart in the reference: sweeps `bytes` of device memory at `buf` (16-byte aligned) with
  * 128-bit read-only loads and writes nothing (`sink`, 4 bytes of device memory or null, is never stored to on

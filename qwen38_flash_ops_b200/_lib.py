@@ -40,6 +40,7 @@ EXPORTS = (
     "qfg_lmhead_host_create", "qfg_lmhead_host_run", "qfg_lmhead_host_destroy",
     "qfg_qk_norm_rope_create", "qfg_qk_norm_rope_compute", "qfg_qk_norm_rope_destroy",
     "qfg_cache_write", "qfg_cache_read", "qfg_cache_attention_workspace_bytes", "qfg_cache_attention", "qfg_prompt_attention",
+    "qfg_prompt_attention_set_option",
     "qfg_stream_read_probe",
 )
 
@@ -131,6 +132,7 @@ def load() -> ctypes.CDLL:
                                         c_void_p, c_void_p, c_void_p, c_void_p]
     lib.qfg_prompt_attention.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                          c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p]
+    lib.qfg_prompt_attention_set_option.argtypes = [c_char_p, c_char_p]
     lib.qfg_lmhead_exchange_bytes.restype = c_size_t
     lib.qfg_lmhead_compute_sharded.argtypes = [c_void_p, c_void_p, c_int64, c_int64, POINTER(Tensor2D), c_int64, c_int64,
                                                c_void_p, POINTER(LmExchange), c_void_p, c_void_p, c_void_p, c_void_p]

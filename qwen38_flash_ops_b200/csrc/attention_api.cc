@@ -1,6 +1,9 @@
 // The C ABI of heads, their cache and attention: checks of arguments, and the calls into their kernels.
+#include <atomic>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 #include <exception>
 #include <stdexcept>
 #include <string>
@@ -62,6 +65,7 @@ int CheckHeads(const char* name, const char* what, const void* x, int64_t ld, in
   return QFG_OK;
 }
 bool Scale(float s) { return s > 0.f && s <= 1e18f; }
+std::atomic<bool> g_prompt_give_up{false};  // qfg_prompt_attention_set_option
 
 }  // namespace
 
@@ -251,6 +255,9 @@ int AttentionCall(const qfg_kv_cache* cache, int64_t seqs, int64_t tokens, int64
   if (tokens < 0 || tokens > 1024) return Refuse(name, "at most 1024 tokens of a sequence attend in one call");
   if (q_heads < 1 || q_heads > kMostHeads || q_heads % c->cache.heads != 0) return Refuse(name, "the query heads must be a multiple of the cache's, up to 4096");
   if (most_pages < 0 || most_pages > INT_MAX / c->cache.page) return Refuse(name, "a sequence may have at most 2147483647 tokens");
+  // what shares of it are counted in
+  const int64_t room = seqs * most_pages * c->cache.page, rows = tokens * (q_heads / c->cache.heads);
+  if (room > int64_t{1} << 34 || room > (int64_t{1} << 42) / (c->cache.heads * (rows / 8 + 1))) return Refuse(name, "the table is too large");
   c->seqs = static_cast<int>(seqs);
   c->tokens = static_cast<int>(tokens);
   c->q_heads = static_cast<int>(q_heads);
@@ -337,5 +344,13 @@ int qfg_prompt_attention(int dtype, const void* q, int64_t ldq, int64_t q_rows, 
   c.scale = scale;
   c.out = out;
   c.lse = lse;
+  c.give_up = g_prompt_give_up.load(std::memory_order_relaxed);
   return Launched(name, qfg::LaunchPromptAttention(c, static_cast<cudaStream_t>(stream)));
+}
+
+int qfg_prompt_attention_set_option(const char* key, const char* value) {
+  if (key == nullptr || value == nullptr) return Refuse("PromptAttention", "null argument");
+  if (std::strcmp(key, "give_up") != 0) return Refuse("PromptAttention", std::string("unknown option ") + key);
+  g_prompt_give_up.store(std::atoi(value) != 0, std::memory_order_relaxed);
+  return QFG_OK;
 }

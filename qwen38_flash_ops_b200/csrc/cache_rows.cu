@@ -356,7 +356,7 @@ cudaError_t LaunchHeads(HeadsParams& p, bool vec, cudaStream_t stream) {
   const int sms = DeviceSmCount();
   const bool few = p.tokens <= 2 * sms;
   p.log_tokens = 0;
-  while (1 << p.log_tokens < kMostTokens && runs << p.log_tokens < 16 * kWarps && p.tokens >> (p.log_tokens + 1) >= sms * 4 / 5) ++p.log_tokens;
+  while (!few && 1 << p.log_tokens < kMostTokens && runs << p.log_tokens < 16 * kWarps && p.tokens >> (p.log_tokens + 1) >= sms * 4 / 5) ++p.log_tokens;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.tokens + (1 << p.log_tokens) - 1) >> p.log_tokens), static_cast<unsigned>(few ? (runs + kWarps - 1) / kWarps : 1));
   cfg.blockDim = dim3(kThreads);

@@ -74,7 +74,8 @@ def test_caches_that_are_refused(other, message):
     (lambda: attend(cache(), ld_seq=512), "overlap"), (lambda: attend(cache(), tokens=2, ld_token=512, ld_seq=4096), "overlap"), (lambda: attend(cache(), scale=0.0), "scale"),
     (lambda: attend(cache(), scale=NAN), "scale"), (lambda: attend(cache(), scale=INF), "scale"), (lambda: attend(cache(), scale=-1.0), "scale"),
     (lambda: attend(cache(), lengths=None), "null or misaligned"), (lambda: attend(cache(), out=None), "null or misaligned"), (lambda: attend(cache(), lse=P + 2), "null or misaligned"),
-    (lambda: attend(cache(), most=1 << 26, ldt=1 << 26), "2147483647 tokens"),
+    (lambda: attend(cache(), most=1 << 26, ldt=1 << 26), "2147483647 tokens"), (lambda: attend(cache(), seqs=60000, most=1 << 16, ldt=1 << 16), "too large"),
+    (lambda: attend(cache(kv_heads=2000), heads=4000, ld_seq=1 << 30, ld_token=1 << 20, tokens=1024, seqs=16, most=1 << 20, ldt=1 << 20), "too large"),
     (lambda: prompt(dtype=_lib.QFG_FLOAT), "BF16/FP16"), (lambda: prompt(dim=256), "64 or 128"), (lambda: prompt(heads=3), "multiple of the key heads"),
     (lambda: prompt(kv_heads=0), "multiple of the key heads"), (lambda: prompt(seqs=-1), "65536"), (lambda: prompt(q_rows=-1), "number of rows"),
     (lambda: prompt(q=P + 8), "misaligned"), (lambda: prompt(ldq=516), "16 bytes"), (lambda: prompt(ldk=128), "overlap"), (lambda: prompt(v=None), "null v"),
@@ -82,6 +83,13 @@ def test_caches_that_are_refused(other, message):
 ])
 def test_calls_that_are_refused(call, message):
     refused(call(), message)
+
+
+def test_options():
+    lib = _lib.load()
+    refused(lib.qfg_prompt_attention_set_option(b"give_ups", b"1"), "unknown option give_ups")
+    refused(lib.qfg_prompt_attention_set_option(None, b"1"), "null argument")
+    assert lib.qfg_prompt_attention_set_option(b"give_up", b"0") == _lib.QFG_OK
 
 
 def test_calls_of_nothing_are_no_calls():

@@ -36,7 +36,7 @@ def close(got, want, dtype):
 CASES = [(128, None, False, 1), (128, 64, True, 1), (64, 32, False, 3), (64, 64, True, 2), (256, 64, False, 1), (256, 256, True, 3), (128, 0, False, 1)]
 
 
-@pytest.mark.parametrize("tokens,q_heads,kv_heads", [(1, 1, 1), (5, 8, 2), (300, 3, 3), (700, 12, 4)])
+@pytest.mark.parametrize("tokens,q_heads,kv_heads", [(1, 1, 1), (5, 8, 2), (240, 40, 4), (296, 64, 8), (300, 3, 3), (700, 12, 4)])
 @pytest.mark.parametrize("dim,rotary,interleaved,n_axes", CASES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_norm_and_rotation(cuda, dtype, dim, rotary, interleaved, n_axes, tokens, q_heads, kv_heads):
@@ -87,7 +87,7 @@ def test_strided_rows_of_one_projection(cuda, tokens, shift):
 
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dim,rotary,interleaved", [(128, 128, False), (64, 32, False), (64, 64, True), (256, 128, False), (256, 96, False)])
-@pytest.mark.parametrize("tokens", [3, 330])
+@pytest.mark.parametrize("tokens", [3, 270, 330])
 def test_the_cache_holds_the_rotated_keys(cuda, form, dim, rotary, interleaved, tokens):
     gen = torch.Generator().manual_seed(4)
     channel = torch.exp(torch.randn(dim, generator=gen))

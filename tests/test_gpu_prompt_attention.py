@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from _attention import attention, half_step
-from qwen38_flash_ops_b200 import PromptAttention, QfgError
+from qwen38_flash_ops_b200 import PromptAttention, QfgError, _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -145,6 +145,23 @@ def test_offsets_that_are_none(cuda):
     for qo, ko in (([0, 100, 50, 200], [0, 100, 50, 200]), ([-5, 90, 1000, 2000], [-5, 90, 1000, 2000]), ([0, 200, 200, 200], [150, 400, 3, -9])):
         PromptAttention()(q, k, v, torch.tensor(qo, dtype=torch.int32).cuda(), torch.tensor(ko, dtype=torch.int32).cuda())
     torch.cuda.synchronize()
+
+
+def test_waits_that_run_out(cuda):
+    """No operand comes: the block's waits end, its rows are NaN, and the next call is whole."""
+    lib = _lib.load()
+    for dim in (64, 128):
+        q, k, v = a_case([200], [200], 2, 1, dim, torch.bfloat16)
+        at, op = offsets([200]), PromptAttention()
+        want = op(q, k, v, at)
+        assert lib.qfg_prompt_attention_set_option(b"give_up", b"1") == 0
+        try:
+            got, lse = op(q, k, v, at, lse=True)
+            torch.cuda.synchronize()
+        finally:
+            assert lib.qfg_prompt_attention_set_option(b"give_up", b"0") == 0
+        assert torch.isnan(got.float()).all() and torch.isnan(lse).all()
+        assert torch.equal(op(q, k, v, at), want)
 
 
 def test_calls_that_are_refused(cuda):
