@@ -371,7 +371,8 @@ QFG_API int qfg_quant_mlp(int dtype, const void* x, int64_t ldx, const void* res
  * another: k and v are [pages][kv_heads][page][head_dim] FP8 E4M3FN with FP32 scales [pages][kv_heads][page], or UINT8 (block-16
  * NVFP4) [pages][kv_heads][page][head_dim / 2], channel 2 b in the low nibble of byte b, with E4M3FN scales [pages][kv_heads][page]
  * [head_dim / 16].  A token's slot is page * (page size) + (its place in the page).  Writing a row y of a head:
- *   E4M3:  scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i 448 / max_i |y_i| (the quotient by the scale before that is rounded; by 2^-40 where that is larger).
+ *   E4M3:  scale = max(max_i |y_i| / 448, 2^-40), q_i = y_i 448 / max_i |y_i| (the quotient by the scale before that is rounded; by 2^-40
+ *          where that is larger).
  *   NVFP4: for each 16 channels scale = max(E4M3(max_i |y_i| / (6 unit)), 2^-9), at most 448, q_i = E2M1(y_i / (scale unit)).
  * Both rounded to nearest, ties to even; `unit` is k_unit or v_unit, so that values from 2^-10 to 2688 units are held well.  A row (NVFP4:
  * sixteen channels) that holds an infinity or a NaN has scale NaN and q 0.  All tensors begin on 16 bytes. */
@@ -414,8 +415,9 @@ QFG_API int qfg_cache_read(const qfg_kv_cache* cache, const int32_t* table, int6
  * include them: token t sees the first lengths[i] - tokens + 1 + t.  q [seqs][tokens][q_heads][head_dim] (BFLOAT16 or FLOAT16, sequences ld_seq and
  * tokens ld_token elements apart, on 16 bytes), out the same, contiguous; `lse` (NULL, or FP32 [seqs][tokens][q_heads]) gets the natural
  * logarithm of the sum of the exponentials.  Query head h reads key head h / (q_heads / kv_heads).  A row that sees nothing (a length of
- * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it (a table is for 2^34 tokens at most); tokens whose page is none of the cache's are left
- * out.  Values that lie behind a sequence's length take no part, whatever they are. 
+ * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it (a table is for 2^34 tokens at most); tokens whose
+ * page is none of the cache's are left out.  What lies behind a sequence's length takes no part, whatever it is.  A value within it that is
+ * not finite makes all rows of its key head NaN, those of earlier tokens too: their weight for it is 0, and 0 times it is not.
  * `workspace`: that many bytes (0 where sequences are never cut), on 16 bytes, not looked at before the call and free behind it; calls
  * that run at once need one each. */
 QFG_API int qfg_cache_attention_workspace_bytes(const qfg_kv_cache* cache, int64_t seqs, int64_t tokens, int64_t q_heads, int64_t most_pages, size_t* bytes);

@@ -288,7 +288,8 @@ class CacheAttention:
 
     q [sequences, tokens, heads, head_dim] (or, of one token each, [sequences, heads, head_dim]) in BF16 or FP16; table int32 [sequences, most pages]: each
     sequence's pages; lengths int32 [sequences]: its tokens in the cache, those of q among them.  Token t sees the first lengths - tokens + 1 + t of them;
-    a row that sees nothing is 0.  Query head h reads key head h // (heads // kv_heads).  `scale`: 1 / sqrt(head_dim) unless given.  Returns a tensor like q; with
+    a row that sees nothing is 0; a value within a sequence that is not finite makes the rows of its key head NaN.  Query head h reads key head
+    h // (heads // kv_heads).  `scale`: 1 / sqrt(head_dim) unless given.  Returns a tensor like q; with
     lse=True also the logarithm of each row's sum of exponentials, FP32, by which attention over several caches can be joined.  A call allocates its own workspace."""
 
     def __init__(self, scale: float | None = None):

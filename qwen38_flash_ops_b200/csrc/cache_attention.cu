@@ -21,6 +21,11 @@
 // fills by asynchronous copies ahead of itself, across the borders of sequences and heads too; no warp waits for another.  Shares begin and end anywhere; a second kernel
 // joins those parts that share a sequence and head, in their order, so that results do not depend on which warp is first.  Lengths are on the device only: where the
 // shares lie is worked out there.
+//
+// Measured, 8 key heads of 128 channels.  Two sequences of up to 131072 tokens, E4M3, 64 query heads: 83 us for 400 MB, 4.8 TB/s, of which the join has 8.  64 of up to 8192,
+// NVFP4: 85 us for 335 MB, 3.9 TB/s; 63 % of the issue slots are taken, by conversions, multiplications by scales and the order of the values' codes, one warp in four
+// waits for the result of the instruction ahead, one in five for the unit of its own.  Few tiles for each warp (16 of up to 4001 tokens, four tokens each: 7): 31.7 us where the
+// bytes take 7; three trips to memory before the first tile, two warps a scheduler, and the join.  One sequence of 1000 tokens: 9.5 us, trips to memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -36,6 +41,9 @@
 namespace qfg {
 namespace {
 
+// Warps of a block.  One tile of eight rows leaves room for two blocks an SM, sixteen warps of 128 registers; two tiles, or heads of 256 channels, for one, eight warps of up to
+// 255.  Twelve warps of 168 are slower there: 16 sequences of up to 4001 tokens, four tokens of 32 / 8 heads of 128 each, 31.7 -> 39.8 us; 32 of up to 8192, 24 / 4 heads of
+// 256, NVFP4 50.7 -> 62.7, E4M3 69.3 -> 85.9.
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 // All tiles, in equal shares: share i begins at tile size i + min(i, more).
 struct Shares {

@@ -12,7 +12,13 @@
 // Quotients are rounded once: their factor is carried in two parts, so that half-way values go to even.
 //
 // A row has D / 16 lanes of sixteen channels each: of a rotated part in halves, eight of the one and the eight that they are rotated with, so that nothing crosses lanes
-// but the sum of squares and the largest value.  A block's sines and cosines are made once for its tokens and wait in shared memory for all heads.
+// but the sum of squares and the largest value, and the lanes of a load or a store fill whole sectors (with sixteen beside one another, the write of 2048 tokens of 8 heads
+// and the reading of 10007 took 23.7 us instead of 18.6).  A token's sines and cosines are made once and wait in shared memory for all of its heads; weights do, too.
+//
+// What bounds them: one read and one write of every head.  4096 tokens of 64 + 8 + 8 heads of 128, BF16, with an E4M3 cache: 40 us for 160 MB, 4.0 TB/s; of the issue slots
+// two thirds are taken (the quotients in two parts, the norm's and the rotation's FP32), of the DRAM's cycles one half.  Four blocks an SM of 64 registers hold as many
+// rows in flight as fit: three of 80, which have room for the weights, take 44 to 47 us, sines and cosines read from shared memory at every row 46.  Eight tokens: 4.8 us, the
+// launch and one trip to memory: a row for each warp.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp4.h>
@@ -220,8 +226,8 @@ __device__ __forceinline__ Two<T> LoadRow(const Side& s, const Channels& c, long
   return {LoadEight<T, VEC>(x + c.c0), LoadEight<T, VEC>(x + c.c1)};
 }
 
-// The rows of a token that are queries (0), keys (1), values (2) or keys as they are (3): those of this warp, every `step`-th run of kRows from row `row` on, up to row `end`.  `next` holds the
-// first; the row behind is on its way while one is worked on.  Every lane of the warp makes the same number of steps, as shuffles are of whole warps.
+// The rows of a token that are queries (0), keys (1), values (2) or keys as they are (3): those of this warp, every `step`-th run of kRows from row `row` on, up to row
+// `end`.  `next` holds the first; the row behind is on its way while one is worked on.  Every lane of the warp makes the same number of steps, as shuffles are of whole warps.
 template <typename T, int L, bool VEC, int WHICH>
 __device__ __forceinline__ void SideRows(const HeadsParams& p, long long token, const float2* turn, const float* weight, long long place, int row, int step, int end,
                                          Two<T> next) {
@@ -387,7 +393,8 @@ struct ReadParams {
   long long ld_table, rows;
   int seqs, most_pages;
 };
-constexpr int kReadRows = 16;  // of a block
+// Tokens of a block.  10007 tokens of 8 heads of 128, NVFP4 to BF16 (53 MB, a floor of 8.1 us): 10 us behind a write that takes the other 8.6; of 32 tokens 13.
+constexpr int kReadRows = 16;
 
 template <typename T, int L, bool FP4>
 __global__ void __launch_bounds__(kThreads) CacheReadKernel(const ReadParams p) {

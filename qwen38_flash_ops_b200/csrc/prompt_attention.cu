@@ -2,20 +2,23 @@
 //
 //   s_ij = scale q_i . k_j,  j within the sequence (causal: j <= i + keys - queries);   y_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
 //
-// A block takes two tiles of 128 queries of one head and runs over the keys they see, 128 at a time.  Both products are tcgen05.mma with FP32 sums in tensor memory:
-// S = Q K^T from shared memory, and O += P V with P, in 16 bits, in tensor memory where S was.  A row of S belongs to one thread, so that the maximum and the sum of a
-// row cross no lanes.  The two tiles take turns: while the tensor core works for the one, the other's four warps are at their exponentials.
+// A block takes tiles of 128 queries of one head and runs over the keys they see, 128 at a time: two tiles of heads of 128 channels, with the SM to itself, or one tile of
+// heads of 64, two blocks an SM (a packed batch of short prompts: 53 -> 44 us).  Both products are tcgen05.mma with FP32 sums in tensor memory: S = Q K^T from shared
+// memory, and O += P V with P, in 16 bits, in tensor memory where S was.  A row of S belongs to one thread, so that the maximum and the sum of a row cross no lanes.  Two
+// tiles take turns: while the tensor core works for the one, the other's four warps are at their exponentials.  Three quarters of the second product begin while the last
+// quarter of P is made.
 //
-//   columns   S0 | S1 | O0 | O1 of 128, 128, D, D; P over the first half of its S
-//   warps     0-3 and 4-7 softmax and output of a tile each, 8 products, 9 copies (and zeros in the place of values past the sequence's end), 10 and 11 idle: registers
-//             are shared out by four warps
+//   columns   S (of each tile) | O (of each), of 128 and D; P over the first half of its S
+//   warps     0 products, 1 copies (and zeros in the place of values past the sequence's end), 2 and 3 idle, 4-7 softmax and output of the first tile, 8-11 of the second:
+//             registers are shared out by four warps.  Two warpgroups for a tile, each half of a row's columns, were slower (1.1 to 1.4 ms), two warps for products no faster
 //   ring      128 keys or 128 values a stage, by tensor copies; rows of 128 bytes, swizzled
 //
 // One pass: m is taken up only when a score passes it by 8 (in powers of two), and only then are O and the sum scaled again; weights stay below 2^8, within FP16.
-// S and the sums are FP32; P is rounded to the type of the inputs, as tensor cores take it (a relative 2^-9 or 2^-12 of each weight, before sums of many).
+// S and the sums are FP32; P is rounded to the type of the inputs, as tensor cores take it (2^-8 or 2^-11 of each weight, before sums of many).
 //
 // Products and exponentials take the same time (a tile of 128 x 128 at D = 128: 1024 cycles of the tensor core, 1024 of the unit for exponentials at 16 a cycle), which is
-// what bounds the kernel.  No weight is made for tiles that the mask leaves out; the longest rows' blocks come first.
+// what bounds the kernel; a quarter of the exponentials goes to the FMA units for that reason.  No weight is made for tiles that the mask leaves out.  Causal, 8192 tokens of
+// 64 / 8 heads of 128: 870 us by itself, 1.26 PFLOP/s, the tensor pipe busy for 66 % of the cycles; 930 to 1000 back to back, under the power cap.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -185,9 +188,9 @@ __device__ __forceinline__ T Uniform(T v) {
   return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// Where a block's queries and keys lie; tiles < 0: a block too many.
+// Where a block's queries and keys lie.
 struct Place {
-  int q0, k0, queries, keys, first;  // first: the first of its queries, within the sequence
+  int q0, k0, queries, keys, first;  // first: the first of its queries, within the sequence; < 0: a block too many
 };
 template <int ROWS>  // of a block
 __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
