@@ -46,7 +46,7 @@ struct PromptParams {
   float* lse;
   int seqs, q_rows, k_rows, q_heads, group;
   float scale;  // of scores, in powers of two
-  bool causal, give_up;
+  bool causal, waves, give_up;  // waves: there are more blocks than the GPU holds at once
 };
 
 // TILES: of queries, for a block.
@@ -63,8 +63,21 @@ struct Geometry {
   static constexpr int kBytes = (TILES + kStages) * kHeadTile + 1024;
 };
 
+// Where a block's queries and keys lie.
+struct Place {
+  int q0, k0, queries, keys, first;  // first: the first of its queries, within the sequence; < 0: a block too many
+};
+// Work for all warps: a place, the head, and the tiles of keys that its tiles of queries look at.
+struct Item {
+  Place at;
+  int head, tiles[2];
+};
+constexpr int kItems = 4;  // that the copies may be ahead
 struct PromptCtl {
-  unsigned long long q_full[2], full[8], empty[8], s_full[2], p_most[2], p_ready[2], o_full[2], fixed;
+  uint4 next;  // the answer to this block's asking for another one's work
+  unsigned long long q_full[2], q_empty[2], full[8], empty[8], fixed[8], s_full[2], p_most[2], p_ready[2], o_full[2], o_empty[2], item_full[kItems], item_empty[kItems], next_full;
+  Item item[kItems];
+  int claimed;  // a block whose work is this one's, but not in `item` yet; -1: none
   uint32_t tmem;
   volatile uint32_t fault;
 };
@@ -181,6 +194,30 @@ __device__ __forceinline__ bool SpinWait(uint32_t a, uint32_t parity) {
   return ok != 0;
 }
 
+// The same, until some warp of the block has given up.
+__device__ __forceinline__ bool SpinWait(uint32_t a, uint32_t parity, const PromptCtl& c) {
+  for (int i = 0; i < 16 * kSpin; ++i) {
+    if (BarTest(a, parity)) return true;
+    if ((i & 255) == 255 && c.fault) return false;
+  }
+  return false;
+}
+
+// Four pieces of 16 bytes of each lane's row: lane i of four gets piece i of their four rows instead, so that a store takes 64 bytes of a row and not 16.
+__device__ __forceinline__ void Exchange(uint32_t (&w)[16], int lane) {
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    const bool upper = (lane & d) != 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i & 4 * d) continue;
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[i] : w[i + 4 * d], d);
+      w[i] = upper ? got : w[i];
+      w[i + 4 * d] = upper ? w[i + 4 * d] : got;
+    }
+  }
+}
+
 // A value that all lanes of the warp have, and the compiler knows it: what the instructions of the tensor core and their branches go by has to be so (else each product
 // costs its issuing thread about 90 cycles, more than the tensor core takes for it).
 template <typename T>
@@ -188,10 +225,21 @@ __device__ __forceinline__ T Uniform(T v) {
   return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// Where a block's queries and keys lie.
-struct Place {
-  int q0, k0, queries, keys, first;  // first: the first of its queries, within the sequence; < 0: a block too many
-};
+// Asks for a block of the grid that has not begun: it never will, and its work is this block's.  One asking at a time, and none behind the first that got nothing.
+__device__ __forceinline__ void AskForBlock(uint4* answer, uint32_t bar) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  BarExpect(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(Smem(answer)), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int BlockGot(const uint4* answer) {  // -1: none
+  uint32_t block;
+  asm volatile(
+      "{ .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%1];\n clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n mov.u32 %0, -1;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n}"
+      : "=r"(block) : "r"(Smem(answer)) : "memory");
+  return static_cast<int>(block);
+}
+
 template <int ROWS>  // of a block
 __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
   const int lane = threadIdx.x & 31;
@@ -247,6 +295,8 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
   if (threadIdx.x == 0) {
     for (int i = 0; i < TILES; ++i) {
       BarInit(Smem(&ctl.q_full[i]), 1);
+      BarInit(Smem(&ctl.q_empty[i]), 1);
+      BarInit(Smem(&ctl.o_empty[i]), 4);
       BarInit(Smem(&ctl.s_full[i]), 1);
       BarInit(Smem(&ctl.p_most[i]), 4);
       BarInit(Smem(&ctl.p_ready[i]), 4);
@@ -255,8 +305,15 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     for (int i = 0; i < G::kStages; ++i) {
       BarInit(Smem(&ctl.full[i]), 1);
       BarInit(Smem(&ctl.empty[i]), 1);
+      BarInit(Smem(&ctl.fixed[i]), 1);
     }
-    BarInit(Smem(&ctl.fixed), 1);
+    for (int i = 0; i < kItems; ++i) {
+      BarInit(Smem(&ctl.item_full[i]), 1);
+      BarInit(Smem(&ctl.item_empty[i]), 4 * TILES + 1);
+    }
+    BarInit(Smem(&ctl.next_full), 1);
+    for (Item& item : ctl.item) item.at.first = -1;
+    ctl.claimed = -1;
     ctl.fault = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -271,34 +328,43 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
   }
   FenceBefore();
   GridDependencyWait();
-  const int head = static_cast<int>(blockIdx.x) % p.q_heads;
-  const Place at = FindPlace<TILES * kTile>(p, static_cast<int>(blockIdx.x) / p.q_heads);
-  const int tiles[2] = {at.first < 0 ? 0 : KeyTiles(p, at, at.first), at.first < 0 || TILES == 1 ? 0 : KeyTiles(p, at, at.first + kTile)};
-  const int n0 = Uniform(tiles[0]), n1 = Uniform(tiles[1]), most = max(n0, n1);
-  // the last tile of values runs past the sequence's end
-  const bool fix = Uniform(most > 0 && most * kTile > at.keys ? 1 : 0) != 0;
+  Place at = {0, 0, 0, 0, -1};
+  if (warp == 1) at = FindPlace<TILES * kTile>(p, static_cast<int>(blockIdx.x) / p.q_heads);
   __syncthreads();
   FenceAfter();
   const uint32_t tmem = Uniform(ctl.tmem);
+  // whether there is an n-th item, which is in `item` until this warp has done with it; a wait that runs out shows in `good`, which is the same for all lanes
+  bool good = true;
+  auto there = [&](int n) {
+    good = __all_sync(0xffffffffu, SpinWait(Smem(&ctl.item_full[n % kItems]), static_cast<uint32_t>(n / kItems & 1), ctl)) != 0;
+    return good && Uniform(ctl.item[n % kItems].at.first) >= 0;
+  };
+  auto done = [&](int n) {
+    __syncwarp();
+    if (lane == 0) BarArrive(Smem(&ctl.item_empty[n % kItems]));
+  };
 
   if (warp >= 4) {
     // ---- softmax and output
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kSoftmaxRegisters));
-    const int t = (warp >> 2) - 1, row = at.first + t * kTile + (warp & 3) * 32 + lane;  // of the sequence
+    const int t = (warp >> 2) - 1;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + static_cast<uint32_t>(t * kTile), o_at = tmem + lanes + static_cast<uint32_t>(G::kOutput + t * D);
-    const int count = tiles[t], sees = p.causal ? min(at.keys, row + 1 + at.keys - at.queries) : at.keys;
-    const int first_sees = p.causal ? min(at.keys, at.first + t * kTile + (warp & 3) * 32 + 1 + at.keys - at.queries) : at.keys;  // the warp's first row
     const float step = 8.f / p.scale;
+    uint32_t s_parity = 0, o_parity = 0;
+    const int in_block = t * kTile + (warp & 3) * 32 + lane;
+#pragma unroll 1
+    for (int n = 0; there(n); ++n) {
+    const Item& item = ctl.item[n % kItems];
+    const int keys = item.at.keys, count = item.tiles[t], over = keys - item.at.queries + 1 + item.at.first + in_block;  // over: the keys that a causal row sees, if there are as many
+    const int sees = p.causal ? min(keys, over) : keys, first_sees = p.causal ? min(keys, over - lane) : keys;          // first_sees: the warp's first row
     float reference = -INFINITY;
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    bool good = true;
+#pragma unroll 1
     for (int j = 0; j < count; ++j) {
-      if (!BarWait(Smem(&ctl.s_full[t]), static_cast<uint32_t>(j & 1), ctl)) {
-        good = false;
-        break;
-      }
-      __syncwarp();
+      good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.s_full[t]), s_parity, ctl)) != 0;
+      if (!good) break;
+      s_parity ^= 1u;
       FenceAfter();
       float s[kTile];
 #pragma unroll
@@ -356,31 +422,39 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
         }
       }
     }
-    if (at.first >= 0) {
-      if (count > 0 && good) good = BarWait(Smem(&ctl.o_full[t]), 0, ctl);
-      __syncwarp();
-      FenceAfter();
-      // a row that saw nothing has made nothing but what is left of weights that are zero
-      const float total = reference == -INFINITY && !isnan(sum[0].x + sum[1].x + sum[0].y + sum[1].y) ? 0.f : (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), by = total == 0.f ? 0.f : 1.f / total;
-      const long long to = (static_cast<long long>(at.q0) + row) * p.q_heads + head;
-      const bool mine = row < at.queries;
+    if (count > 0 && good) good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.o_full[t]), o_parity, ctl)) != 0;
+    if (!good) break;
+    FenceAfter();
+    // a row that saw nothing has made nothing but what is left of weights that are zero
+    const float all = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), total = reference == -INFINITY && !isnan(all) ? 0.f : all, by = total == 0.f ? 0.f : 1.f / total;
+    const int row = item.at.first + in_block;  // of the sequence
+    const int rows = item.at.queries - (row & ~3);  // from the first of four lanes' on
+    const long long to = (static_cast<long long>(item.at.q0) + row) * p.q_heads + item.head, step_of_row = static_cast<long long>(p.q_heads) * D;
+    uint16_t* const out = static_cast<uint16_t*>(p.out) + to * D - (lane & 3) * step_of_row + (lane & 3) * 8;
+    done(n);
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+    for (int c = 0; c < D; c += 32) {
+      uint32_t w[16] = {};
+      if (count > 0) {
         float o[32];
-        if (count > 0) {
-          LoadColumns(o_at + c, o);
-          WaitLoads();
-        }
-        if (mine) {
-          uint32_t w[16];
+        LoadColumns(o_at + c, o);
+        WaitLoads();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = !good ? 0x7FFF7FFFu : count > 0 ? Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by) : 0u;
-          uint4* const dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        }
+        for (int i = 0; i < 16; ++i) w[i] = Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by);
+        Exchange(w, lane);
       }
-      if (mine && p.lse != nullptr) p.lse[to] = !good ? __uint_as_float(0x7FFFFFFFu) : total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < rows) *reinterpret_cast<uint4*>(out + i * step_of_row + c) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      }
+    }
+    if (count > 0) {
+      o_parity ^= 1u;
+      FenceBefore();
+      __syncwarp();
+      if (lane == 0) BarArrive(Smem(&ctl.o_empty[t]));
+    }
+    if ((lane & 3) < rows && p.lse != nullptr) p.lse[to] = total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegisters));
@@ -394,7 +468,6 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     const uint32_t q_desc = static_cast<uint32_t>(SmemDesc(smem, 16, 1024)), k_desc = static_cast<uint32_t>(SmemDesc(ring, 16, 1024)),
                    v_desc = static_cast<uint32_t>(SmemDesc(ring, kBox, 1024));
     constexpr uint32_t kStageStep = G::kHeadTile >> 4;
-    bool good = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {  // as every lane sees it: what follows is uniform to the compiler, too
       good = __all_sync(0xffffffffu, SpinWait(bar, parity)) != 0 && good;
     };
@@ -411,7 +484,8 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
       return stage;
     };
     auto release = [&](int stage) { MmaCommit<false>(Smem(&ctl.empty[0]) + static_cast<uint32_t>(stage * 8)); };
-    auto scores = [&](auto tile, int stage) {
+    uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0}, o_uses[2] = {0, 0}, fixes = 0;
+    auto scores = [&](auto tile, int stage, bool last) {
       constexpr int t = decltype(tile)::value;
       const uint32_t a = q_desc + t * kStageStep, b = k_desc + static_cast<uint32_t>(stage) * kStageStep, d = tmem + t * kTile;
       MmaSsAt<0, 0>(d, a, b, kScores, 0);
@@ -425,11 +499,13 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
         MmaSsAt<kBox + 96, kBox + 96>(d, a, b, kScores, 1);
       }
       MmaCommit<false>(Smem(&ctl.s_full[t]));
+      if (last) MmaCommit<false>(Smem(&ctl.q_empty[t]));
     };
     auto outputs = [&](auto tile, int j, int v, int k, int count) {  // of tile t, and its next scores
       constexpr int t = decltype(tile)::value;
       const uint32_t b = v_desc + static_cast<uint32_t>(v) * kStageStep, d = tmem + G::kOutput + t * D, a = tmem + t * kTile;
-      wait(Smem(&ctl.p_most[t]), static_cast<uint32_t>(j & 1));
+      if (j == 0 && o_uses[t]++ > 0) wait(Smem(&ctl.o_empty[t]), o_uses[t] & 1);  // the item ahead has been read
+      wait(Smem(&ctl.p_most[t]), p_parity[t]);
       FenceAfter();
       if (good && ElectOne()) {
         MmaTsAt<0, 0>(d, a, b, kOutputs, j > 0);
@@ -440,7 +516,8 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
         MmaTsAt<40, 10240>(d, a, b, kOutputs, 1);
       }
       __syncwarp();
-      wait(Smem(&ctl.p_ready[t]), static_cast<uint32_t>(j & 1));
+      wait(Smem(&ctl.p_ready[t]), p_parity[t]);
+      p_parity[t] ^= 1u;
       FenceAfter();
       if (good && ElectOne()) {
         MmaTsAt<48, 12288>(d, a, b, kOutputs, 1);
@@ -448,46 +525,54 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
         if (j + 1 == count) {
           MmaCommit<false>(Smem(&ctl.o_full[t]));
         } else {
-          scores(tile, k);
+          scores(tile, k, j + 2 == count);
         }
       }
       __syncwarp();
     };
     const std::integral_constant<int, 0> first;
     const std::integral_constant<int, 1> second;
-    if (most > 0) {
-      if (n0 > 0) wait(Smem(&ctl.q_full[0]), 0);
-      if (TILES > 1 && n1 > 0) wait(Smem(&ctl.q_full[1]), 0);
+#pragma unroll 1
+    for (int n = 0; good && there(n); ++n) {
+      const Item& item = ctl.item[n % kItems];
+      const int n0 = Uniform(item.tiles[0]), n1 = Uniform(item.tiles[1]), most = max(n0, n1);
+      const bool fix = most * kTile > Uniform(item.at.keys);  // the last tile of values runs past the sequence's end
+      done(n);
+      if (most == 0) continue;
+      if (n0 > 0) wait(Smem(&ctl.q_full[0]), q_parity[0]), q_parity[0] ^= 1u;
+      if (TILES > 1 && n1 > 0) wait(Smem(&ctl.q_full[1]), q_parity[1]), q_parity[1] ^= 1u;
       const int k0 = arrived();
       FenceAfter();
       if (good && ElectOne()) {
-        if (n0 > 0) scores(first, k0);
+        if (n0 > 0) scores(first, k0, n0 == 1);
         if constexpr (TILES > 1) {
-          if (n1 > 0) scores(second, k0);
+          if (n1 > 0) scores(second, k0, n1 == 1);
         }
         release(k0);
       }
       __syncwarp();
-    }
 #pragma unroll 1
-    for (int j = 0; j < most && good; ++j) {
-      const bool more = j + 1 < most;
-      const int v = arrived(), k = more ? arrived() : 0;
-      if (fix && !more) wait(Smem(&ctl.fixed), 0);
-      if (j < n0) outputs(first, j, v, k, n0);
-      if constexpr (TILES > 1) {
-        if (j < n1) outputs(second, j, v, k, n1);
+      for (int j = 0; j < most && good; ++j) {
+        const bool more = j + 1 < most;
+        const int v = arrived(), k = more ? arrived() : 0;
+        if (fix && !more) {
+          wait(Smem(&ctl.fixed[0]) + static_cast<uint32_t>(v * 8), fixes >> v & 1);
+          fixes ^= 1u << v;
+        }
+        if (j < n0) outputs(first, j, v, k, n0);
+        if constexpr (TILES > 1) {
+          if (j < n1) outputs(second, j, v, k, n1);
+        }
+        if (good && ElectOne()) {
+          release(v);
+          if (more) release(k);
+        }
+        __syncwarp();
       }
-      if (good && ElectOne()) {
-        release(v);
-        if (more) release(k);
-      }
-      __syncwarp();
     }
     if (!good) ctl.fault = 1;
   } else if (warp == 1) {
     // ---- copies
-    bool good = !p.give_up;
     auto load = [&](uint32_t dst, const CUtensorMap* map, int of, int row, uint32_t bar) {
       if (ElectOne()) {
         BarExpect(bar, G::kHeadTile);
@@ -496,35 +581,70 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
       }
       __syncwarp();
     };
-    const int of = head / p.group;
-    if (!good) ctl.fault = 1;
-    for (int position = 0; position < 2 * most && good; ++position) {
-      const int stage = position % G::kStages, j = position >> 1;
-      if (position >= G::kStages) good = BarWait(Smem(&ctl.empty[stage]), static_cast<uint32_t>(position / G::kStages - 1 & 1), ctl);
+    int stage = 0, items = 0, block = static_cast<int>(blockIdx.x);
+    uint32_t parity = 1, q_uses[2] = {0, 0};  // a ring's first round waits for nothing: the phase ahead of the first has ended
+    auto wait = [&](unsigned long long* bar, uint32_t of) { good = good && __all_sync(0xffffffffu, BarWait(Smem(bar), of, ctl)) != 0; };
+    auto tell = [&](const Item& item) {  // all warps
+      const int slot = items % kItems;
+      wait(&ctl.item_empty[slot], static_cast<uint32_t>(items / kItems & 1) ^ 1u);
+      if (lane == 0 && good) {
+        ctl.item[slot] = item;
+        ctl.claimed = -1;
+        BarArrive(Smem(&ctl.item_full[slot]));
+      }
+      if (good) ++items;
       __syncwarp();
-      if (!good) break;
-      if (position == 0) {
-        for (int t = 0; t < TILES; ++t) {
-          if (tiles[t] > 0) load(smem + static_cast<uint32_t>(t * G::kHeadTile), &p.q, head, at.q0 + at.first + t * kTile, Smem(&ctl.q_full[t]));
-          if (t == 0) load(ring, &p.k, of, at.k0, Smem(&ctl.full[0]));
+    };
+    if (lane == 0) ctl.claimed = block;
+    good = !p.give_up;
+#pragma unroll 1
+    for (uint32_t asked = 0; good; asked ^= 1u) {
+      if (at.first >= 0) {
+        const Item item = {at, block % p.q_heads, {KeyTiles(p, at, at.first), TILES == 1 ? 0 : KeyTiles(p, at, at.first + kTile)}};
+        tell(item);
+        const int most = max(item.tiles[0], item.tiles[1]), of = item.head / p.group, keep = at.keys - (most - 1) * kTile;
+        for (int position = 0; position < 2 * most && good; ++position) {
+          wait(&ctl.empty[stage], parity);
+          if (!good) break;
+          const uint32_t to = ring + static_cast<uint32_t>(stage * G::kHeadTile);
+          load(to, position & 1 ? &p.v : &p.k, of, at.k0 + (position >> 1) * kTile, Smem(&ctl.full[stage]));
+          for (int t = 0; position == 0 && t < TILES; ++t) {
+            if (item.tiles[t] == 0) continue;
+            wait(&ctl.q_empty[t], ++q_uses[t] & 1);
+            if (good) load(smem + static_cast<uint32_t>(t * G::kHeadTile), &p.q, item.head, at.q0 + at.first + t * kTile, Smem(&ctl.q_full[t]));
+          }
+          if (position + 1 == 2 * most && keep < kTile) {
+            // what lies past the sequence's end may be no number, and a weight of zero does not undo that
+            wait(&ctl.full[stage], parity ^ 1u);
+            const uint32_t zero[4] = {0, 0, 0, 0};
+            for (int b = 0; b < kBoxes && good; ++b) {
+              for (int i = lane; i < (kTile - keep) * 8; i += 32) Sts128(to + static_cast<uint32_t>(b * kBox + keep * 128 + i * 16), zero);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && good) BarArrive(Smem(&ctl.fixed[stage]));
+          }
+          if (++stage == G::kStages) {
+            stage = 0;
+            parity ^= 1u;
+          }
         }
-        continue;
       }
-      load(ring + static_cast<uint32_t>(stage * G::kHeadTile), position & 1 ? &p.v : &p.k, of, at.k0 + j * kTile, Smem(&ctl.full[stage]));
-    }
-    if (fix && good) {
-      // what lies past the sequence's end may be no number, and a weight of zero does not undo that
-      const int position = 2 * most - 1, stage = position % G::kStages;
-      good = BarWait(Smem(&ctl.full[stage]), static_cast<uint32_t>(position / G::kStages & 1), ctl);
-      const int keep = at.keys - (most - 1) * kTile;
-      const uint32_t zero[4] = {0, 0, 0, 0};
-      for (int b = 0; b < kBoxes && good; ++b) {
-        for (int i = lane; i < (kTile - keep) * 8; i += 32) Sts128(ring + static_cast<uint32_t>(stage * G::kHeadTile + b * kBox + keep * 128 + i * 16), zero);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (!good || !p.waves) break;
+      if (lane == 0) AskForBlock(&ctl.next, Smem(&ctl.next_full));
       __syncwarp();
-      if (lane == 0 && good) BarArrive(Smem(&ctl.fixed));
+      // the answer comes in any case, and what it gives is this block's
+      bool answered = false;
+      for (int i = 0; i < kSpin && !answered; ++i) answered = BarTry(Smem(&ctl.next_full), asked);
+      good = __all_sync(0xffffffffu, answered) != 0;
+      block = answered ? BlockGot(&ctl.next) : -1;
+      __syncwarp();
+      if (block < 0) break;
+      if (lane == 0) ctl.claimed = block;
+      at = FindPlace<TILES * kTile>(p, block / p.q_heads);
     }
+    if (good) tell({{0, 0, 0, 0, -1}, 0, {0, 0}});
+    if (!good) ctl.fault = 1;
   }
   if (ctl.fault != 0) {
     for (int i = 0; i < 16; ++i) __nanosleep(1000000);  // copies and products may still be under way
@@ -533,6 +653,19 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
   __syncthreads();
   FenceAfter();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kColumns) : "memory");
+  if (ctl.fault != 0 && warp >= 4) {  // all rows of the last items, and of one that no warp has heard of
+    const int thread = static_cast<int>(threadIdx.x) - 128;
+    for (int i = 0; i <= kItems; ++i) {
+      const int block = i < kItems ? -1 : ctl.claimed;
+      const Place from = i < kItems ? ctl.item[i].at : block < 0 ? Place{0, 0, 0, 0, -1} : FindPlace<TILES * kTile>(p, block / p.q_heads);
+      const int head = i < kItems ? ctl.item[i].head : block % p.q_heads, rows = from.first < 0 ? 0 : min(TILES * kTile, from.queries - from.first);
+      for (int e = thread; e < rows * (D / 8); e += 128 * TILES) {
+        const long long to = (static_cast<long long>(from.q0) + from.first + e / (D / 8)) * p.q_heads + head;
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D)[e % (D / 8)] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+        if (p.lse != nullptr && e % (D / 8) == 0) p.lse[to] = __uint_as_float(0x7FFFFFFFu);
+      }
+    }
+  }
 }
 
 bool EncodeHeads(CUtensorMap* map, const void* x, int dtype, int dim, int heads, int64_t rows, int64_t ld) {
@@ -546,12 +679,13 @@ bool EncodeHeads(CUtensorMap* map, const void* x, int dtype, int dim, int heads,
 }
 
 template <int D, bool BF16, int TILES>
-cudaError_t Launch(const PromptParams& p, cudaStream_t stream) {
+cudaError_t Launch(PromptParams p, cudaStream_t stream) {
   using G = Geometry<D, TILES>;
   static_assert(G::kBlocks * (G::kBytes + static_cast<int>(sizeof(PromptCtl)) + 1024) <= 228 * 1024, "");
   // sequences of any lengths that add up to the rows have no more tiles than this
   const long long blocks = (static_cast<long long>(p.q_rows) / (TILES * kTile) + std::min(p.seqs, p.q_rows)) * p.q_heads;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  p.waves = blocks > G::kBlocks * DeviceSmCount();
   const cudaError_t set = cudaFuncSetAttribute(PromptAttentionKernel<D, BF16, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
   if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
