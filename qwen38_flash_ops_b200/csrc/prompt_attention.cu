@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstddef>
 #include <type_traits>
 
 #include "qfg_internal.h"
@@ -75,7 +76,9 @@ struct Item {
 constexpr int kItems = 4;  // that the copies may be ahead
 struct PromptCtl {
   uint4 next;  // the answer to this block's asking for another one's work
-  unsigned long long q_full[2], q_empty[2], full[8], empty[8], fixed[8], s_full[2], p_most[2], p_ready[2], o_full[2], o_empty[2], item_full[kItems], item_empty[kItems], next_full;
+  unsigned long long q_full[2], q_empty[2], full[8], empty[8], fixed[8], s_full[2], o_full[2], item_full[kItems], next_full;  // of one arrival,
+  unsigned long long p_most[2], p_ready[2], o_empty[2];                                                                      // of four warps',
+  unsigned long long item_empty[kItems];                                                                                     // of all that take items
   Item item[kItems];
   int claimed;  // a block whose work is this one's, but not in `item` yet; -1: none
   uint32_t tmem;
@@ -248,10 +251,11 @@ __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
   int before = 0;
   for (int base = p.seqs - 1; base >= 0; base -= 32) {
     const int i = base - lane;
-    int q0 = 0, q1 = 0;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
     if (i >= 0) {
-      q0 = min(max(p.q_offsets[i], 0), p.q_rows);
-      q1 = min(max(p.q_offsets[i + 1], q0), p.q_rows);
+      q0 = p.q_offsets[i], q1 = p.q_offsets[i + 1], k0 = p.k_offsets[i], k1 = p.k_offsets[i + 1];
+      q0 = min(max(q0, 0), p.q_rows), q1 = min(max(q1, q0), p.q_rows);
+      k0 = min(max(k0, 0), p.k_rows), k1 = min(max(k1, k0), p.k_rows);
     }
     const int tiles = (q1 - q0 + ROWS - 1) / ROWS;
     int upto = tiles;
@@ -267,9 +271,8 @@ __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
       at.q0 = __shfl_sync(0xffffffffu, q0, of);
       at.queries = __shfl_sync(0xffffffffu, q1 - q0, of);
       at.first = (n - 1 - (rank - ahead)) * ROWS;
-      const int seq = base - of;
-      at.k0 = min(max(p.k_offsets[seq], 0), p.k_rows);
-      at.keys = min(max(p.k_offsets[seq + 1], at.k0), p.k_rows) - at.k0;
+      at.k0 = __shfl_sync(0xffffffffu, k0, of);
+      at.keys = __shfl_sync(0xffffffffu, k1 - k0, of);
       return at;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -292,29 +295,16 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
   __shared__ PromptCtl ctl;
   const int warp = Uniform(static_cast<int>(threadIdx.x) >> 5), lane = static_cast<int>(threadIdx.x) & 31;
   const uint32_t smem = (Smem(smem_raw) + 1023u) & ~1023u, ring = smem + TILES * G::kHeadTile;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < TILES; ++i) {
-      BarInit(Smem(&ctl.q_full[i]), 1);
-      BarInit(Smem(&ctl.q_empty[i]), 1);
-      BarInit(Smem(&ctl.o_empty[i]), 4);
-      BarInit(Smem(&ctl.s_full[i]), 1);
-      BarInit(Smem(&ctl.p_most[i]), 4);
-      BarInit(Smem(&ctl.p_ready[i]), 4);
-      BarInit(Smem(&ctl.o_full[i]), 1);
+  if (warp == 2) {
+    constexpr int kFours = offsetof(PromptCtl, p_most), kItemEmpty = offsetof(PromptCtl, item_empty), kFirst = offsetof(PromptCtl, q_full);
+    for (int at = kFirst + 8 * lane; at < kItemEmpty + 8 * kItems; at += 8 * 32) {
+      BarInit(Smem(&ctl) + static_cast<uint32_t>(at), at < kFours ? 1 : at < kItemEmpty ? 4 : 4 * TILES + 1);
     }
-    for (int i = 0; i < G::kStages; ++i) {
-      BarInit(Smem(&ctl.full[i]), 1);
-      BarInit(Smem(&ctl.empty[i]), 1);
-      BarInit(Smem(&ctl.fixed[i]), 1);
+    if (lane < kItems) ctl.item[lane].at.first = -1;
+    if (lane == 0) {
+      ctl.claimed = -1;
+      ctl.fault = 0;
     }
-    for (int i = 0; i < kItems; ++i) {
-      BarInit(Smem(&ctl.item_full[i]), 1);
-      BarInit(Smem(&ctl.item_empty[i]), 4 * TILES + 1);
-    }
-    BarInit(Smem(&ctl.next_full), 1);
-    for (Item& item : ctl.item) item.at.first = -1;
-    ctl.claimed = -1;
-    ctl.fault = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
@@ -432,7 +422,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     const long long to = (static_cast<long long>(item.at.q0) + row) * p.q_heads + item.head, step_of_row = static_cast<long long>(p.q_heads) * D;
     uint16_t* const out = static_cast<uint16_t*>(p.out) + to * D - (lane & 3) * step_of_row + (lane & 3) * 8;
     done(n);
-#pragma unroll
+#pragma unroll 1  // cold code
     for (int c = 0; c < D; c += 32) {
       uint32_t w[16] = {};
       if (count > 0) {
@@ -601,17 +591,21 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     for (uint32_t asked = 0; good; asked ^= 1u) {
       if (at.first >= 0) {
         const Item item = {at, block % p.q_heads, {KeyTiles(p, at, at.first), TILES == 1 ? 0 : KeyTiles(p, at, at.first + kTile)}};
-        tell(item);
         const int most = max(item.tiles[0], item.tiles[1]), of = item.head / p.group, keep = at.keys - (most - 1) * kTile;
+        if (most == 0) tell(item);
         for (int position = 0; position < 2 * most && good; ++position) {
           wait(&ctl.empty[stage], parity);
           if (!good) break;
           const uint32_t to = ring + static_cast<uint32_t>(stage * G::kHeadTile);
           load(to, position & 1 ? &p.v : &p.k, of, at.k0 + (position >> 1) * kTile, Smem(&ctl.full[stage]));
-          for (int t = 0; position == 0 && t < TILES; ++t) {
-            if (item.tiles[t] == 0) continue;
-            wait(&ctl.q_empty[t], ++q_uses[t] & 1);
-            if (good) load(smem + static_cast<uint32_t>(t * G::kHeadTile), &p.q, item.head, at.q0 + at.first + t * kTile, Smem(&ctl.q_full[t]));
+          if (position == 0) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+              if (item.tiles[t] == 0) continue;
+              wait(&ctl.q_empty[t], ++q_uses[t] & 1);
+              if (good) load(smem + static_cast<uint32_t>(t * G::kHeadTile), &p.q, item.head, at.q0 + at.first + t * kTile, Smem(&ctl.q_full[t]));
+            }
+            tell(item);
           }
           if (position + 1 == 2 * most && keep < kTile) {
             // what lies past the sequence's end may be no number, and a weight of zero does not undo that
