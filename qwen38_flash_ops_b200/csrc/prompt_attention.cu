@@ -243,41 +243,69 @@ __device__ __forceinline__ int BlockGot(const uint4* answer) {  // -1: none
   return static_cast<int>(block);
 }
 
-template <int ROWS>  // of a block
+// A sequence, and its blocks of ROWS queries.
+template <int ROWS>
+struct Sequence {
+  int q0 = 0, queries = 0, k0 = 0, keys = 0, blocks = 0;
+  __device__ __forceinline__ Sequence(const PromptParams& p, int i) {
+    if (i < 0 || i >= p.seqs) return;
+    const int q1 = p.q_offsets[i + 1], k1 = p.k_offsets[i + 1];
+    q0 = min(max(p.q_offsets[i], 0), p.q_rows), k0 = min(max(p.k_offsets[i], 0), p.k_rows);
+    queries = min(max(q1, q0), p.q_rows) - q0, keys = min(max(k1, k0), p.k_rows) - k0;
+    blocks = (queries + ROWS - 1) / ROWS;
+  }
+  // its blocks whose last row sees more than `seen` keys: the last ones
+  __device__ __forceinline__ int seeing(const PromptParams& p, int seen) const {
+    if (seen < 0) return blocks;
+    if (!p.causal) return keys > seen ? blocks : 0;
+    // block i < blocks - 1 sees (i + 1) ROWS + keys - queries, the last one all
+    return (keys > seen && blocks > 0 ? 1 : 0) + max(0, blocks - max(1, (seen + 1 - keys + queries + ROWS - 1) / ROWS));
+  }
+};
+__device__ __forceinline__ int UpTo(int v, int lane) {  // the sum of this lane's and those ahead of it
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+// The place of a block of the grid, by its rank among those of its head.
+template <int ROWS>
 __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
   const int lane = threadIdx.x & 31;
-  Place at = {0, 0, 0, 0, -1};
-  // from the last sequence on, each one's last rows, which see the most keys, ahead of its others
+  // Where the GPU holds fewer blocks than there are, those with the most keys come first, so that none of them is the last to end; of up to 32 sequences, that is, which
+  // a warp has at hand.  Of more, each one's last rows, which see the most keys, come ahead of its others.
+  const bool sorted = p.waves && p.seqs > 1 && p.seqs <= 32;
   int before = 0;
   for (int base = p.seqs - 1; base >= 0; base -= 32) {
-    const int i = base - lane;
-    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-    if (i >= 0) {
-      q0 = p.q_offsets[i], q1 = p.q_offsets[i + 1], k0 = p.k_offsets[i], k1 = p.k_offsets[i + 1];
-      q0 = min(max(q0, 0), p.q_rows), q1 = min(max(q1, q0), p.q_rows);
-      k0 = min(max(k0, 0), p.k_rows), k1 = min(max(k1, k0), p.k_rows);
+    const Sequence<ROWS> s(p, base - lane);
+    int mine = s.blocks, from = 0;  // of this sequence's blocks, from its last: those that are counted
+    if (sorted) {
+      int lo = -1, hi = __reduce_max_sync(0xffffffffu, s.keys / kTile);  // the most tiles of keys that this block and those ahead of it look at are lo + 1
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (static_cast<int>(__reduce_add_sync(0xffffffffu, s.seeing(p, mid * kTile))) > rank) {
+          lo = mid;
+        } else {
+          hi = mid - 1;
+        }
+      }
+      from = s.seeing(p, (lo + 1) * kTile);
+      mine = s.seeing(p, lo < 0 ? -1 : lo * kTile) - from;
+      before = __reduce_add_sync(0xffffffffu, from);
     }
-    const int tiles = (q1 - q0 + ROWS - 1) / ROWS;
-    int upto = tiles;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += v;
-    }
-    const uint32_t mine = __ballot_sync(0xffffffffu, rank < before + upto);
-    if (mine != 0) {
-      const int of = __ffs(mine) - 1;
-      const int ahead = before + __shfl_sync(0xffffffffu, upto - tiles, of), n = __shfl_sync(0xffffffffu, tiles, of);
-      at.q0 = __shfl_sync(0xffffffffu, q0, of);
-      at.queries = __shfl_sync(0xffffffffu, q1 - q0, of);
-      at.first = (n - 1 - (rank - ahead)) * ROWS;
-      at.k0 = __shfl_sync(0xffffffffu, k0, of);
-      at.keys = __shfl_sync(0xffffffffu, k1 - k0, of);
-      return at;
+    const int upto = UpTo(mine, lane);
+    const uint32_t there = __ballot_sync(0xffffffffu, rank < before + upto);
+    if (there != 0) {
+      const int of = __ffs(there) - 1;
+      const int back = from + rank - before - (upto - mine);  // blocks of the sequence behind this one
+      return {__shfl_sync(0xffffffffu, s.q0, of), __shfl_sync(0xffffffffu, s.k0, of), __shfl_sync(0xffffffffu, s.queries, of), __shfl_sync(0xffffffffu, s.keys, of),
+              __shfl_sync(0xffffffffu, (s.blocks - 1 - back) * ROWS, of)};
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  return at;
+  return {0, 0, 0, 0, -1};
 }
 // The tiles of keys that 128 queries from `first` on look at.
 __device__ __forceinline__ int KeyTiles(const PromptParams& p, const Place& at, int first) {

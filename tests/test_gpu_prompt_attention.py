@@ -147,6 +147,47 @@ def test_offsets_that_are_none(cuda):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("seqs", [2, 31, 32, 33, 70])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_more_blocks_than_the_gpu_holds(cuda, causal, dim, seqs):
+    """Blocks take on the work of others, the longest first (of more than 32 sequences in the order of their rows): every row is written once, whatever its turn."""
+    gen = torch.Generator().manual_seed(seqs)
+    most = 9000 // seqs
+    queries = [int(n) for n in torch.randint(0, most, (seqs,), generator=gen)]
+    keys = [max(0, n + int(d)) for n, d in zip(queries, torch.randint(-40, 400, (seqs,), generator=gen))]
+    q, k, v = a_case(queries, keys, 24, 8, dim, torch.bfloat16, seed=seqs)
+    out = torch.full_like(q, float("nan"))
+    op = PromptAttention(causal=causal)
+    op(q, k, v, offsets(queries), offsets(keys), out=out)
+    assert torch.isfinite(out).all() and torch.equal(out, op(q, k, v, offsets(queries), offsets(keys)))
+    # each sequence by itself, where no block waits for a place
+    a = b = 0
+    for n, m in zip(queries, keys):
+        for h in range(0, 24, 12):
+            alone = op(q[a:a + n, h:h + 12], k[b:b + m, h // 3:h // 3 + 4], v[b:b + m, h // 3:h // 3 + 4], offsets([n]), offsets([m]))
+            assert torch.equal(out[a:a + n, h:h + 12], alone)
+        a, b = a + n, b + m
+    few = max(range(seqs), key=lambda i: queries[i] if queries[i] < 300 else 0)
+    a, b, n, m = sum(queries[:few]), sum(keys[:few]), queries[few], keys[few]
+    check(out[a:a + n], None, q[a:a + n], k[b:b + m], v[b:b + m], [n], [m], causal, 1 / math.sqrt(dim))
+
+
+def test_waits_that_run_out_of_many_blocks(cuda):
+    lib = _lib.load()
+    q, k, v = a_case([200] * 30, [200] * 30, 24, 8, 64, torch.bfloat16)
+    at, op = offsets([200] * 30), PromptAttention()
+    want = op(q, k, v, at)
+    assert lib.qfg_prompt_attention_set_option(b"give_up", b"1") == 0
+    try:
+        got, lse = op(q, k, v, at, lse=True)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.qfg_prompt_attention_set_option(b"give_up", b"0") == 0
+    assert torch.isnan(got.float()).all() and torch.isnan(lse).all()
+    assert torch.equal(op(q, k, v, at), want)
+
+
 def test_waits_that_run_out(cuda):
     """No operand comes: the block's waits end, its rows are NaN, and the next call is whole."""
     lib = _lib.load()
