@@ -157,6 +157,19 @@ __device__ __forceinline__ void Turn(float& a, float& b, float cosine, float sin
   a = u * cosine - v * sine;
   b = v * cosine + u * sine;
 }
+// two at a time
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 
 // A row's sixteen values of this lane, at channels c0 and c1 of eight each, into the cache.
 template <int L>
@@ -252,29 +265,36 @@ __device__ __forceinline__ void SideRows(const HeadsParams& p, long long token, 
     ToFloats(f + 8, next.b);
     if (row + step * kRows < end) next = LoadRow<T, L, VEC>(s, c, token, row + step * kRows);
     if (norm) {
-      float squares[2] = {0.f, 0.f};
+      float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) squares[e & 1] = fmaf(f[e], f[e], squares[e & 1]);
-      float all = squares[0] + squares[1];
+      for (int e = 0; e < 16; e += 2) squares = Fma2(make_float2(f[e], f[e + 1]), make_float2(f[e], f[e + 1]), squares);
+      float all = squares.x + squares.y;
 #pragma unroll
       for (int d = L / 2; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
       const float root = rsqrtf(fmaf(all, 1.f / D, p.eps));
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const float4 w = *reinterpret_cast<const float4*>(weight + (e < 8 ? c.c0 + e : c.c1 + e - 8));
-        f[e] *= root * w.x;
-        f[e + 1] *= root * w.y;
-        f[e + 2] *= root * w.z;
-        f[e + 3] *= root * w.w;
+        const float2 by[2] = {Mul2(make_float2(root, root), make_float2(w.x, w.y)), Mul2(make_float2(root, root), make_float2(w.z, w.w))};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 y = Mul2(make_float2(f[e + 2 * i], f[e + 2 * i + 1]), by[i]);
+          f[e + 2 * i] = y.x;
+          f[e + 2 * i + 1] = y.y;
+        }
       }
     }
     if (c.turned) {
+      if (p.interleaved) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (c.split) {
-          Turn(f[e], f[8 + e], cosine[e], sine[e]);
-        } else {
-          Turn(f[2 * e], f[2 * e + 1], cosine[e], sine[e]);
+        for (int e = 0; e < 8; ++e) Turn(f[2 * e], f[2 * e + 1], cosine[e], sine[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 a = make_float2(f[e], f[e + 1]), b = make_float2(f[8 + e], f[9 + e]), by = make_float2(cosine[e], cosine[e + 1]), in = make_float2(sine[e], sine[e + 1]);
+          const float2 u = Fma2(make_float2(-b.x, -b.y), in, Mul2(a, by)), v = Fma2(a, in, Mul2(b, by));
+          f[e] = u.x, f[e + 1] = u.y;
+          f[8 + e] = v.x, f[9 + e] = v.y;
         }
       }
     }
