@@ -229,110 +229,127 @@ __device__ __forceinline__ Channels ChannelsOf(const HeadsParams& p, int lane) {
   c.c1 = c.split ? (WHICH < 2 ? p.rotary / 2 : 8 * L) + 8 * lane : c.c0 + 8;
   return c;
 }
+// Rows on their way: of each warp kStages runs, a lane's two pieces where only it looks for them.
 template <typename T>
-struct Two {
-  Eight<T> a, b;
+struct Ring {
+  static constexpr int kStages = sizeof(T) == 4 ? 2 : 4, kLane = 16 * sizeof(T), kBytes = kStages * kLane * 32;  // of a warp
 };
-template <typename T, int L, bool VEC>
-__device__ __forceinline__ Two<T> LoadRow(const Side& s, const Channels& c, long long token, int row) {
-  const T* const x = static_cast<const T*>(s.x) + token * s.ld + row * (16 * L);
-  return {LoadEight<T, VEC>(x + c.c0), LoadEight<T, VEC>(x + c.c1)};
+template <typename T, bool VEC>
+__device__ __forceinline__ void Fetch(uint8_t* slot, const T* a, const T* b) {  // the k-th 16 bytes of a lane's part 512 k bytes on
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const T* const from = h == 0 ? a : b;
+    constexpr int kPieces = sizeof(T) / 2;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot + 512 * (kPieces * h + i)))),
+                     "l"(from + 16 / sizeof(T) * i)
+                     : "memory");
+    } else {
+      const Eight<T> e = LoadEight<T, false>(from);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) *reinterpret_cast<uint4*>(slot + 512 * (kPieces * h + i)) = reinterpret_cast<const uint4*>(&e)[i];
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void Fetched(float (&f)[16], const uint8_t* slot) {
+  constexpr int kPieces = sizeof(T) / 2;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    Eight<T> e;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      uint4& to = reinterpret_cast<uint4*>(&e)[i];
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to.x), "=r"(to.y), "=r"(to.z), "=r"(to.w)
+                   : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot + 512 * (kPieces * h + i))))
+                   : "memory");
+    }
+    ToFloats(f + 8 * h, e);
+  }
 }
 
-// The rows of a token that are queries (0), keys (1), values (2) or keys as they are (3): those of this warp, every `step`-th run of kRows from row `row` on, up to row
-// `end`.  `next` holds the first; the row behind is on its way while one is worked on.  Every lane of the warp makes the same number of steps, as shuffles are of whole warps.
-template <typename T, int L, bool VEC, int WHICH>
-__device__ __forceinline__ void SideRows(const HeadsParams& p, long long token, const float2* turn, const float* weight, long long place, int row, int step, int end,
-                                         Two<T> next) {
-  constexpr int D = 16 * L, kRows = 32 / L;
+// A row of the queries (0), keys (1), values (2) or keys as they are (3).  Every lane of the warp is here, as shuffles are of whole warps; rows from `heads` on are not written.
+template <typename T, int L, int WHICH>
+__device__ __forceinline__ void Row(const HeadsParams& p, float (&f)[16], const Channels& c, const float (&cosine)[8], const float (&sine)[8], const float* weight,
+                                    long long token, long long place, int row) {
+  constexpr int D = 16 * L;
   const Side& s = p.side[WHICH == 3 ? 1 : WHICH];
-  const int lane = threadIdx.x % L;
-  const Channels c = ChannelsOf<L, WHICH>(p, lane);
-  float cosine[8], sine[8];  // of this lane's eight pairs
-  if (c.turned) {
+  if (WHICH < 2 && s.weight != nullptr) {
+    float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float4 two = *reinterpret_cast<const float4*>(turn + 8 * lane + e);
-      cosine[e] = two.x, sine[e] = two.y;
-      cosine[e + 1] = two.z, sine[e + 1] = two.w;
-    }
-  }
-  const bool norm = WHICH < 2 && s.weight != nullptr;
-#pragma unroll 1
-  for (int run = row - (static_cast<int>(threadIdx.x) & 31) / L; run < end; run += step * kRows, row += step * kRows) {
-    float f[16];
-    ToFloats(f, next.a);
-    ToFloats(f + 8, next.b);
-    if (row + step * kRows < end) next = LoadRow<T, L, VEC>(s, c, token, row + step * kRows);
-    if (norm) {
-      float2 squares = make_float2(0.f, 0.f);
+    for (int e = 0; e < 16; e += 2) squares = Fma2(make_float2(f[e], f[e + 1]), make_float2(f[e], f[e + 1]), squares);
+    float all = squares.x + squares.y;
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) squares = Fma2(make_float2(f[e], f[e + 1]), make_float2(f[e], f[e + 1]), squares);
-      float all = squares.x + squares.y;
+    for (int d = L / 2; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    const float root = rsqrtf(fmaf(all, 1.f / D, p.eps));
 #pragma unroll
-      for (int d = L / 2; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-      const float root = rsqrtf(fmaf(all, 1.f / D, p.eps));
+    for (int e = 0; e < 16; e += 4) {
+      const float4 w = *reinterpret_cast<const float4*>(weight + (e < 8 ? c.c0 + e : c.c1 + e - 8));
+      const float2 by[2] = {Mul2(make_float2(root, root), make_float2(w.x, w.y)), Mul2(make_float2(root, root), make_float2(w.z, w.w))};
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const float4 w = *reinterpret_cast<const float4*>(weight + (e < 8 ? c.c0 + e : c.c1 + e - 8));
-        const float2 by[2] = {Mul2(make_float2(root, root), make_float2(w.x, w.y)), Mul2(make_float2(root, root), make_float2(w.z, w.w))};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 y = Mul2(make_float2(f[e + 2 * i], f[e + 2 * i + 1]), by[i]);
-          f[e + 2 * i] = y.x;
-          f[e + 2 * i + 1] = y.y;
-        }
+      for (int i = 0; i < 2; ++i) {
+        const float2 y = Mul2(make_float2(f[e + 2 * i], f[e + 2 * i + 1]), by[i]);
+        f[e + 2 * i] = y.x;
+        f[e + 2 * i + 1] = y.y;
       }
     }
-    if (c.turned) {
-      if (p.interleaved) {
+  }
+  if (WHICH < 2 && c.turned) {
+    if (p.interleaved) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) Turn(f[2 * e], f[2 * e + 1], cosine[e], sine[e]);
-      } else {
+      for (int e = 0; e < 8; ++e) Turn(f[2 * e], f[2 * e + 1], cosine[e], sine[e]);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float2 a = make_float2(f[e], f[e + 1]), b = make_float2(f[8 + e], f[9 + e]), by = make_float2(cosine[e], cosine[e + 1]), in = make_float2(sine[e], sine[e + 1]);
-          const float2 u = Fma2(make_float2(-b.x, -b.y), in, Mul2(a, by)), v = Fma2(a, in, Mul2(b, by));
-          f[e] = u.x, f[e + 1] = u.y;
-          f[8 + e] = v.x, f[9 + e] = v.y;
-        }
+      for (int e = 0; e < 8; e += 2) {
+        const float2 a = make_float2(f[e], f[e + 1]), b = make_float2(f[8 + e], f[9 + e]), by = make_float2(cosine[e], cosine[e + 1]), in = make_float2(sine[e], sine[e + 1]);
+        const float2 u = Fma2(make_float2(-b.x, -b.y), in, Mul2(a, by)), v = Fma2(a, in, Mul2(b, by));
+        f[e] = u.x, f[e + 1] = u.y;
+        f[8 + e] = v.x, f[9 + e] = v.y;
       }
     }
-    if (WHICH < 2 && row < end && s.out != nullptr) {
-      T* const out = static_cast<T*>(s.out) + (token * s.heads + row) * D;
-      StoreEight<T>(out + c.c0, f);
-      StoreEight<T>(out + c.c1, f + 8);
-    }
-    if (WHICH > 0 && p.slots != nullptr)
-      StoreCache<L>(f, c.c0, c.c1, c.split, p.cache, WHICH == 2, place + static_cast<long long>(row) * p.cache.page, lane, row < end && place >= 0);
   }
+  if (WHICH < 2 && row < s.heads && s.out != nullptr) {
+    T* const out = static_cast<T*>(s.out) + (token * s.heads + row) * D;
+    StoreEight<T>(out + c.c0, f);
+    StoreEight<T>(out + c.c1, f + 8);
+  }
+  if (WHICH > 0 && p.slots != nullptr)
+    StoreCache<L>(f, c.c0, c.c1, c.split, p.cache, WHICH == 2, place + static_cast<long long>(row) * p.cache.page, static_cast<int>(threadIdx.x) % L, row < s.heads && place >= 0);
 }
 
 // L lanes a row, D = 16 L.  QUERIES: false where keys and values alone are written, without a norm or a rotation.
 template <typename T, int L, bool VEC, bool QUERIES>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 || !QUERIES ? 3 : 4) HeadsKernel(const HeadsParams p) {
-  constexpr int D = 16 * L, kRows = 32 / L;
-  __shared__ __align__(16) float2 turn[kMostTokens * D / 2];
+__global__ void __launch_bounds__(kThreads, QUERIES && (sizeof(T) == 4 || L == 16) ? 3 : 4) HeadsKernel(const HeadsParams p) {
+  using R = Ring<T>;
+  constexpr int D = 16 * L, kRows = 32 / L, kKeys = QUERIES ? 1 : 3;
+  __shared__ __align__(16) uint8_t rings[kThreads / 32 * R::kBytes];
+  __shared__ __align__(16) float2 turn[QUERIES ? kMostTokens * D / 2 : 1];
   __shared__ __align__(16) float weight[2][D];
   GridDependencyWait();
-  // a token's warps, a power of two, take turns at its runs of rows, from one side to the next as well; or every warp has one run, of one side
+  // a token's warps, a power of two, take turns at its runs of rows, of queries, keys and values one after another; or every warp has one run
   const int warp = static_cast<int>(threadIdx.x) / 32, warps = kThreads / 32 >> p.log_tokens, t = warp * (1 << p.log_tokens) / (kThreads / 32), sub = warp & (warps - 1);
   const long long token = (static_cast<long long>(blockIdx.x) << p.log_tokens) + t;
   const bool real = token < p.tokens, turns = gridDim.y == 1;
-  const int q = p.side[0].heads, k = p.side[1].heads, v = p.side[2].heads, in_run = (static_cast<int>(threadIdx.x) & 31) / L, lane = threadIdx.x % L, half = p.rotary / 2;
-  const int q_runs = (q + kRows - 1) / kRows, k_runs = (k + kRows - 1) / kRows;
-  const int run = turns ? sub : static_cast<int>(blockIdx.y) * (kThreads / 32) + warp;
-  const int first[3] = {run, turns ? (run - q_runs) & (warps - 1) : run - q_runs, turns ? (run - q_runs - k_runs) & (warps - 1) : run - q_runs - k_runs};
+  const int in_warp = static_cast<int>(threadIdx.x) & 31, in_run = in_warp / L, lane = in_warp % L, half = p.rotary / 2;
+  const int q_runs = (p.side[0].heads + kRows - 1) / kRows, k_runs = q_runs + (p.side[1].heads + kRows - 1) / kRows, runs = k_runs + (p.side[2].heads + kRows - 1) / kRows;
   const int step = turns ? warps : 1 << 24;
-  const auto begins = [&](int side, int heads) { return real && first[side] >= 0 && first[side] * kRows + in_run < heads; };
-  Two<T> next = {};
-  if (QUERIES && begins(0, q)) {
-    next = LoadRow<T, L, VEC>(p.side[0], ChannelsOf<L, 0>(p, lane), token, first[0] * kRows + in_run);
-  } else if (!turns && begins(1, k)) {
-    next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<L, QUERIES ? 1 : 3>(p, lane), token, first[1] * kRows + in_run);
-  } else if (!turns && begins(2, v)) {
-    next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<L, 2>(p, lane), token, first[2] * kRows + in_run);
-  }
+  int run = turns ? sub : static_cast<int>(blockIdx.y) * (kThreads / 32) + warp;
+  const Channels c = ChannelsOf<L, kKeys>(p, lane), as_they_are = ChannelsOf<L, 2>(p, lane);
+  uint8_t* const ring = rings + warp * R::kBytes + in_warp * 16;
+  const auto issue = [&](int of, int stage) {
+    if (of < runs && real) {
+      const int which = of < q_runs ? 0 : of < k_runs ? 1 : 2, row = (of - (which == 0 ? 0 : which == 1 ? q_runs : k_runs)) * kRows + in_run;
+      const Side& s = p.side[which];
+      const Channels& at = which == 2 ? as_they_are : c;
+      const T* const x = static_cast<const T*>(s.x) + token * s.ld + row * D;
+      if (row < s.heads) Fetch<T, VEC>(ring + stage * (R::kLane * 32), x + at.c0, x + at.c1);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < R::kStages; ++i) issue(run + i * step, i);
 
   for (int i = threadIdx.x; QUERIES && i < 2 * D; i += kThreads) {
     const void* const w = p.side[i / D].weight;
@@ -341,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 || !QUERIE
   float2* const by = turn + t * half;
   long long to = -1;  // (page, row of it) as page * kv_heads * page size + row; < 0: not written
   if (real) {
-    for (int j = sub * 32 + (static_cast<int>(threadIdx.x) & 31); QUERIES && j < half; j += 32 * warps) {
+    for (int j = sub * 32 + in_warp; QUERIES && j < half; j += 32 * warps) {
       const RotaryPair pair = p.pairs[j];
       const long long at = token + pair.axis * p.ld_positions;
       const long long position = p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
@@ -357,18 +374,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || L == 16 || !QUERIE
   }
   if constexpr (QUERIES) __syncthreads();
   if (!real) return;
-  if (QUERIES && first[0] * kRows < q) {
-    SideRows<T, L, VEC, 0>(p, token, by, weight[0], to, first[0] * kRows + in_run, step, q, next);
-    if (!turns) return;
+  float cosine[8], sine[8];  // of this lane's eight pairs
+  if (c.turned) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float4 two = *reinterpret_cast<const float4*>(by + 8 * lane + e);
+      cosine[e] = two.x, sine[e] = two.y;
+      cosine[e + 1] = two.z, sine[e + 1] = two.w;
+    }
   }
-  if (first[1] >= 0 && first[1] * kRows < k) {
-    if (turns && begins(1, k)) next = LoadRow<T, L, VEC>(p.side[1], ChannelsOf<L, QUERIES ? 1 : 3>(p, lane), token, first[1] * kRows + in_run);
-    SideRows<T, L, VEC, QUERIES ? 1 : 3>(p, token, by, weight[1], to, first[1] * kRows + in_run, step, k, next);
-    if (!turns) return;
-  }
-  if (first[2] >= 0 && first[2] * kRows < v) {
-    if (turns && begins(2, v)) next = LoadRow<T, L, VEC>(p.side[2], ChannelsOf<L, 2>(p, lane), token, first[2] * kRows + in_run);
-    SideRows<T, L, VEC, 2>(p, token, by, nullptr, to, first[2] * kRows + in_run, step, v, next);
+  int stage = 0;
+#pragma unroll 1
+  for (; run < runs; run += step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(R::kStages - 1) : "memory");
+    float f[16];
+    Fetched<T>(f, ring + stage * (R::kLane * 32));
+    issue(run + R::kStages * step, stage);
+    if (++stage == R::kStages) stage = 0;
+    if (QUERIES && run < q_runs) {
+      Row<T, L, 0>(p, f, c, cosine, sine, weight[0], token, to, run * kRows + in_run);
+    } else if (run < k_runs) {
+      Row<T, L, kKeys>(p, f, c, cosine, sine, weight[1], token, to, (run - q_runs) * kRows + in_run);
+    } else {
+      Row<T, L, 2>(p, f, as_they_are, cosine, sine, nullptr, token, to, (run - k_runs) * kRows + in_run);
+    }
   }
 }
 
