@@ -320,8 +320,10 @@ __device__ __forceinline__ void Row(const HeadsParams& p, float (&f)[16], const 
 }
 
 // L lanes a row, D = 16 L.  QUERIES: false where keys and values alone are written, without a norm or a rotation.
+template <typename T, int L, bool QUERIES>
+constexpr int kHeadsBlocks = QUERIES && (sizeof(T) == 4 || L == 16) ? 3 : 4;  // of an SM
 template <typename T, int L, bool VEC, bool QUERIES>
-__global__ void __launch_bounds__(kThreads, QUERIES && (sizeof(T) == 4 || L == 16) ? 3 : 4) HeadsKernel(const HeadsParams p) {
+__global__ void __launch_bounds__(kThreads, kHeadsBlocks<T, L, QUERIES>) HeadsKernel(const HeadsParams p) {
   using R = Ring<T>;
   constexpr int D = 16 * L, kRows = 32 / L, kKeys = QUERIES ? 1 : 3;
   __shared__ __align__(16) uint8_t rings[kThreads / 32 * R::kBytes];
@@ -403,17 +405,23 @@ __global__ void __launch_bounds__(kThreads, QUERIES && (sizeof(T) == 4 || L == 1
 
 template <typename T, int L>
 cudaError_t LaunchHeads(HeadsParams& p, bool vec, cudaStream_t stream) {
-  // Few tokens: one a block, its rows over as many blocks as leave every warp one run of them.  Many: a warp has sixteen runs or more, so that its sines and cosines
-  // are a small part of it, as long as there is a block for most SMs.
+  // Few tokens: one a block, its rows over as many blocks as leave every warp one run of them.  More: as few tokens a block as let the GPU hold all blocks at once, but two
+  // where warps would have nothing else; of more tokens than that up to eight, as long as a warp has no more than sixteen runs.  64 + 8 + 8 heads of 128, us of 1, 2, 4, 8
+  // tokens a block: 1024 of them - / 12.5 / 12.8 / 16.8, 2048 - / - / 20.2 / 21.5; 24 + 4 + 4 of 256, 1024 of them - / 13.3 / 11.2 / 13.6.
   constexpr int kRows = 32 / L, kWarps = kThreads / 32;
   int runs = 0;
   for (const Side& s : p.side) runs += (s.heads + kRows - 1) / kRows;
   const int sms = DeviceSmCount();
   const bool few = p.tokens <= 2 * sms;
   p.log_tokens = 0;
-  while (!few && 1 << p.log_tokens < kMostTokens && runs << p.log_tokens < 16 * kWarps && p.tokens >> (p.log_tokens + 1) >= sms * 4 / 5) ++p.log_tokens;
+  const int slots = sms * (p.side[0].heads > 0 ? kHeadsBlocks<T, L, true> : kHeadsBlocks<T, L, false>);
+  const auto blocks = [&](int log) { return (p.tokens - 1 >> log) + 1; };
+  while (!few && 1 << p.log_tokens < kMostTokens &&
+         ((blocks(p.log_tokens) > slots && runs << p.log_tokens < 16 * kWarps) || (runs << p.log_tokens < kWarps && blocks(p.log_tokens + 1) >= sms))) {
+    ++p.log_tokens;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.tokens + (1 << p.log_tokens) - 1) >> p.log_tokens), static_cast<unsigned>(few ? (runs + kWarps - 1) / kWarps : 1));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks(p.log_tokens)), static_cast<unsigned>(few ? (runs + kWarps - 1) / kWarps : 1));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {OverlapAttribute()};
