@@ -22,10 +22,10 @@
 // joins those parts that share a sequence and head, in their order, so that results do not depend on which warp is first.  Lengths are on the device only: where the
 // shares lie is worked out there.
 //
-// Measured, 8 key heads of 128 channels.  Two sequences of up to 131072 tokens, E4M3, 64 query heads: 83 us for 400 MB, 4.8 TB/s, of which the join has 8.  64 of up to 8192,
-// NVFP4: 85 us for 335 MB, 3.9 TB/s; 63 % of the issue slots are taken, by conversions, multiplications by scales and the order of the values' codes, one warp in four
-// waits for the result of the instruction ahead, one in five for the unit of its own.  Few tiles for each warp (16 of up to 4001 tokens, four tokens each: 7): 31.7 us where the
-// bytes take 7; three trips to memory before the first tile, two warps a scheduler, and the join.  One sequence of 1000 tokens: 9.5 us, trips to memory.
+// Measured, 8 key heads of 128 channels.  Two sequences of up to 131072 tokens, E4M3, 64 query heads: 83 us for 400 MB, 4.8 TB/s; the first kernel takes 72 to 75 of them.  64 of up
+// to 8192, NVFP4: 85 us for 335 MB, 3.9 TB/s; 61 % of the issue slots are taken, by conversions, multiplications by scales and the order of the values' codes, one warp in four
+// waits for the result of the instruction ahead, one in five for the unit of its own.  Few tiles for each warp (16 of up to 4001 tokens, four tokens each: 7): 29.6 us where the
+// bytes take 7; three trips to memory before the first tile, two warps a scheduler, and the join.  One sequence of 1000 tokens: 9.8 us, trips to memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -136,7 +136,11 @@ __device__ __forceinline__ Share FindShare(const AttendParams& p, int tile) {
     if (base == 0) {
       if (p.seqs <= kThreads) all = before;
       all *= per_seq;
-      s.all.count = static_cast<int>(min(static_cast<long long>(gridDim.x) * kWarps, all));
+      // Few units: a part more costs the join about 9 ns, a tile more a share 1.5 us, so that of a unit of n tiles shares are best sqrt(n / 160) tiles or longer.  One sequence
+      // of 131072 tokens and one key head, NVFP4: 47 us with shares of one or two tiles, 29 of five; 20000 tokens 17.9 and
+      // 15.0 of two.
+      const int least = static_cast<int>(sqrtf(static_cast<float>(all) / (160.f * p.seqs * per_seq)) + 0.5f);
+      s.all.count = static_cast<int>(min(static_cast<long long>(gridDim.x) * kWarps, least > 1 ? (all + least - 1) / least : all));
       if (first >= s.all.count) return s;
       s.all.size = all >> 32 ? all / s.all.count : static_cast<uint32_t>(all) / static_cast<uint32_t>(s.all.count);
       s.all.more = static_cast<int>(all - s.all.size * s.all.count);

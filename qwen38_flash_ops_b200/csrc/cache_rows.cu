@@ -15,10 +15,12 @@
 // but the sum of squares and the largest value, and the lanes of a load or a store fill whole sectors (with sixteen beside one another, the write of 2048 tokens of 8 heads
 // and the reading of 10007 took 23.7 us instead of 18.6).  A token's sines and cosines are made once and wait in shared memory for all of its heads; weights do, too.
 //
-// What bounds them: one read and one write of every head.  4096 tokens of 64 + 8 + 8 heads of 128, BF16, with an E4M3 cache: 40 us for 160 MB, 4.0 TB/s; of the issue slots
-// two thirds are taken (the quotients in two parts, the norm's and the rotation's FP32), of the DRAM's cycles one half.  Four blocks an SM of 64 registers hold as many
-// rows in flight as fit: three of 80, which have room for the weights, take 44 to 47 us, sines and cosines read from shared memory at every row 46.  Eight tokens: 4.8 us, the
-// launch and one trip to memory: a row for each warp.
+// Rows are fetched by asynchronous copies into a ring of each warp's own, four of its runs at a time: no register waits for them, and they are on their way while the angles
+// are made (from registers, one run ahead, 38.5 us for the 35.4 below, and 286 bytes of them spilt).
+//
+// What bounds them: one read and one write of every head.  4096 tokens of 64 + 8 + 8 heads of 128, BF16, with an E4M3 cache: 35.4 us for 160 MB, 4.5 TB/s; of the issue slots
+// two thirds are taken (the quotients in two parts, the norm's and the rotation's FP32).  Four blocks an SM of 64 registers hide more than five with shorter rings (47 us), and than
+// three of 80 did.  Sines and cosines read from shared memory at every row: 46.  Eight tokens: 4.8 us, the launch and one trip to memory: a row for each warp.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp4.h>
@@ -450,7 +452,7 @@ struct ReadParams {
   long long ld_table, rows;
   int seqs, most_pages;
 };
-// Tokens of a block.  10007 tokens of 8 heads of 128, NVFP4 to BF16 (53 MB, a floor of 8.1 us): 10 us behind a write that takes the other 8.6; of 32 tokens 13.
+// Tokens of a block.  10007 tokens of 8 heads of 128, NVFP4 to BF16 (53 MB, a floor of 8.1 us): 10 of the 17.4 us with a write ahead of it; with blocks of 32 tokens 3 more.
 constexpr int kReadRows = 16;
 
 template <typename T, int L, bool FP4>

@@ -2,8 +2,8 @@
 //
 //   s_ij = scale q_i . k_j,  j within the sequence (causal: j <= i + keys - queries);   y_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
 //
-// A block takes tiles of 128 queries of one head and runs over the keys they see, 128 at a time: two tiles of heads of 128 channels, with the SM to itself, or one tile of
-// heads of 64, two blocks an SM (a packed batch of short prompts: 53 -> 44 us).  Both products are tcgen05.mma with FP32 sums in tensor memory: S = Q K^T from shared
+// A block's item of work is one head's tiles of 128 queries, and the keys they see, 128 at a time: two tiles of heads of 128 channels, the block having the SM to itself, or one
+// tile of heads of 64, two blocks an SM (packed prompts, one against two: 53 -> 44 us).  Both products are tcgen05.mma with FP32 sums in tensor memory: S = Q K^T from shared
 // memory, and O += P V with P, in 16 bits, in tensor memory where S was.  A row of S belongs to one thread, so that the maximum and the sum of a row cross no lanes.  Two
 // tiles take turns: while the tensor core works for the one, the other's four warps are at their exponentials.  Three quarters of the second product begin while the last
 // quarter of P is made.
@@ -13,12 +13,18 @@
 //             registers are shared out by four warps.  Two warpgroups for a tile, each half of a row's columns, were slower (1.1 to 1.4 ms), two warps for products no faster
 //   ring      128 keys or 128 values a stage, by tensor copies; rows of 128 bytes, swizzled
 //
+// Where there are more blocks than the GPU holds, a block that is done takes on one that has not begun, and never will: the copies go on to its queries and keys while the last
+// ones are worked on, and its first S is made while the rows ahead are written.  Rows are written in runs of 64 bytes: a warp's 16 bytes of 32 rows at a time fill the queue of
+// loads and stores, and waits and the next item's reading stand behind them.  Both together: 8192 tokens of 64 heads 930 -> 829 us, 48 prompts of 256 tokens of 24 heads of 128
+// 102 -> 51.
+//
 // One pass: m is taken up only when a score passes it by 8 (in powers of two), and only then are O and the sum scaled again; weights stay below 2^8, within FP16.
 // S and the sums are FP32; P is rounded to the type of the inputs, as tensor cores take it (2^-8 or 2^-11 of each weight, before sums of many).
 //
 // Products and exponentials take the same time (a tile of 128 x 128 at D = 128: 1024 cycles of the tensor core, 1024 of the unit for exponentials at 16 a cycle), which is
 // what bounds the kernel; a quarter of the exponentials goes to the FMA units for that reason.  No weight is made for tiles that the mask leaves out.  Causal, 8192 tokens of
-// 64 / 8 heads of 128: 870 us by itself, 1.26 PFLOP/s, the tensor pipe busy for 66 % of the cycles; 930 to 1000 back to back, under the power cap.
+// 64 / 8 heads of 128: 802 us by itself, 1.37 PFLOP/s, the tensor pipe busy for 73 % of the cycles; 925 back to back, under the power cap.  Heads of 64: the softmax warps, two a
+// scheduler, 650 instructions a tile each (S apart from P, so that the next is made meanwhile, changed nothing; 8192 tokens of 24 heads 263 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,8 +43,8 @@ namespace qfg {
 namespace {
 
 constexpr int kTile = 128;
-// Of sixteen pairs of weights those that the FMA units make, so that less waits for the unit for exponentials, which is an eighth as wide.  8192 tokens of 64 heads of 128, us:
-// none 1019, two 1006, four 1002, six 998; packed prompts of 24 heads of 64 54.4, 54.4, 53.3, 52.4.
+// Of sixteen pairs of weights those that the FMA units make, so that less waits for the unit for exponentials, which is an eighth as wide.  8192 tokens of 24 heads of 64,
+// us: none 280, two 267, four 263, six 277; of 64 heads of 128 830 to 870 whatever the share.
 constexpr int kPolyOf16 = 4;
 struct PromptParams {
   CUtensorMap q, k, v;
