@@ -71,6 +71,15 @@ def test_shapes_of_a_server(cuda, form, dim, heads, group, tokens, lengths, page
 
 
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim,group,tokens,lengths", [(64, 8, 1, [30011]), (128, 4, 2, [14000, 100]), (128, 16, 1, [12001]), (256, 2, 1, [13000, 0, 25000])])
+def test_few_heads_of_long_sequences(cuda, form, dim, group, tokens, lengths):
+    """Shares of several tiles where there could be one for each warp."""
+    cache, table, q, n = a_case(form, dim, 1, group, tokens, lengths, torch.bfloat16, page=64)
+    got, lse = CacheAttention()(q, cache, table, n, lse=True)
+    check(got, lse, cache, table, q, n, 1 / math.sqrt(dim))
+
+
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_nothing_behind_a_length_takes_part(cuda, form, dim):
     lengths = [45, 1, 0, 130]

@@ -85,6 +85,23 @@ def test_strided_rows_of_one_projection(cuda, tokens, shift):
     assert all(same_bits(getattr(a, n), getattr(b, n)) for n in ("k", "k_scale", "v", "v_scale"))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim", [(297, 1, 1, 64), (593, 3, 1, 64), (700, 24, 8, 128), (1185, 8, 2, 128), (1337, 24, 4, 256), (2369, 5, 5, 128), (4097, 16, 2, 64), (9600, 2, 1, 256)])
+def test_rows_do_not_depend_on_the_call_they_are_in(cuda, tokens, q_heads, kv_heads, dim, dtype):
+    """Tokens go one to eight to a block, by their number: the same bits as in calls of a hundred, each of whose rows is a warp's."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    q, k, v = (torch.randn(tokens, h, dim, generator=gen, device="cuda").to(dtype) for h in (q_heads, kv_heads, kv_heads))
+    w, positions, slots, op = torch.rand(dim, generator=gen, device="cuda"), torch.arange(tokens, device="cuda") * 37, torch.arange(tokens, device="cuda"), QkNormRope(dim)
+    caches = [new_cache("e4m3", -(-tokens // 32), kv_heads, dim) for _ in range(3)]
+    got = op(q, k, positions, w, w, v=v, cache=caches[0], slots=slots, keys=True)
+    CacheWrite()(got[1], v, caches[2], slots)
+    for i in range(0, tokens, 100):
+        part = op(q[i:i + 100], k[i:i + 100], positions[i:i + 100], w, w, v=v[i:i + 100], cache=caches[1], slots=slots[i:i + 100], keys=True)
+        assert all(torch.equal(a[i:i + 100], b) for a, b in zip(got, part))
+    assert all(same_bits(getattr(caches[0], name), getattr(caches[1], name)) for name in ("k", "v", "k_scale", "v_scale"))
+    assert all(same_bits(getattr(caches[0], name), getattr(caches[2], name)) for name in (("k", "v", "k_scale", "v_scale") if dtype == torch.float32 else ("v", "v_scale")))
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dim,rotary,interleaved", [(128, 128, False), (64, 32, False), (64, 64, True), (256, 128, False), (256, 96, False)])
 @pytest.mark.parametrize("tokens", [3, 270, 330])

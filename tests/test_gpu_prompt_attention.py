@@ -173,6 +173,26 @@ def test_more_blocks_than_the_gpu_holds(cuda, causal, dim, seqs):
     check(out[a:a + n], None, q[a:a + n], k[b:b + m], v[b:b + m], [n], [m], causal, 1 / math.sqrt(dim))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_blocks_captured_and_at_once(cuda, dim):
+    """Each call takes on blocks of its own alone, in a graph and beside another call as well."""
+    lengths = [300, 200, 1, 700, 64] * 4
+    cases = [a_case(lengths, lengths, 24, 8, dim, torch.bfloat16, seed=i) for i in range(2)]
+    at, op, graph = offsets(lengths), PromptAttention(), torch.cuda.CUDAGraph()
+    want = [op(*c, at) for c in cases]
+    with torch.cuda.graph(graph):
+        captured = op(*cases[0], at)
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(op(*cases[i % 2], at))
+        if i % 4 == 3:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs)) and torch.equal(captured, want[0])
+
+
 def test_waits_that_run_out_of_many_blocks(cuda):
     lib = _lib.load()
     q, k, v = a_case([200] * 30, [200] * 30, 24, 8, 64, torch.bfloat16)
