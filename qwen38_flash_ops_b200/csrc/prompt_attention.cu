@@ -379,106 +379,106 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     const int in_block = t * kTile + (warp & 3) * 32 + lane;
 #pragma unroll 1
     for (int n = 0; there(n); ++n) {
-    const Item& item = ctl.item[n % kItems];
-    const int keys = item.at.keys, count = item.tiles[t], over = keys - item.at.queries + 1 + item.at.first + in_block;  // over: the keys that a causal row sees, if there are as many
-    const int sees = p.causal ? min(keys, over) : keys, first_sees = p.causal ? min(keys, over - lane) : keys;          // first_sees: the warp's first row
-    float reference = -INFINITY;
-    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const Item& item = ctl.item[n % kItems];
+      const int keys = item.at.keys, count = item.tiles[t], over = keys - item.at.queries + 1 + item.at.first + in_block;  // what a causal row sees, if there is as much
+      const int sees = p.causal ? min(keys, over) : keys, first_sees = p.causal ? min(keys, over - lane) : keys;          // first_sees: the warp's first row
+      float reference = -INFINITY;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-    for (int j = 0; j < count; ++j) {
-      good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.s_full[t]), s_parity, ctl)) != 0;
-      if (!good) break;
-      s_parity ^= 1u;
-      FenceAfter();
-      float s[kTile];
+      for (int j = 0; j < count; ++j) {
+        good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.s_full[t]), s_parity, ctl)) != 0;
+        if (!good) break;
+        s_parity ^= 1u;
+        FenceAfter();
+        float s[kTile];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) LoadColumns(s_at + 32 * i, s + 32 * i);
-      WaitLoads();
-      if ((j + 1) * kTile > first_sees) {
-        const int left = sees - j * kTile;
+        for (int i = 0; i < 4; ++i) LoadColumns(s_at + 32 * i, s + 32 * i);
+        WaitLoads();
+        if ((j + 1) * kTile > first_sees) {
+          const int left = sees - j * kTile;
 #pragma unroll
-        for (int i = 0; i < kTile; ++i) s[i] = i < left ? s[i] : -INFINITY;
-      }
-      float m[4];
+          for (int i = 0; i < kTile; ++i) s[i] = i < left ? s[i] : -INFINITY;
+        }
+        float m[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = fmaxf(s[i], s[i + 4]);
+        for (int i = 0; i < 4; ++i) {
+          m[i] = fmaxf(s[i], s[i + 4]);
 #pragma unroll
-        for (int e = i + 8; e < kTile; e += 8) m[i] = fmaxf(fmaxf(m[i], s[e]), s[e + 4]);
-      }
-      const float highest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      if (__any_sync(0xffffffffu, highest > reference + step)) {
-        const float to = fmaxf(reference, highest);
-        const float by = to == -INFINITY ? 1.f : Exp2((reference - to) * p.scale);
-        reference = to;
+          for (int e = i + 8; e < kTile; e += 8) m[i] = fmaxf(fmaxf(m[i], s[e]), s[e + 4]);
+        }
+        const float highest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        if (__any_sync(0xffffffffu, highest > reference + step)) {
+          const float to = fmaxf(reference, highest);
+          const float by = to == -INFINITY ? 1.f : Exp2((reference - to) * p.scale);
+          reference = to;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * by, sum[i].y * by);
-        if (j > 0) {  // the products of the tile ahead have ended: S, which was issued after them, has
+          for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * by, sum[i].y * by);
+          if (j > 0) {  // the products of the tile ahead have ended: S, which was issued after them, has
 #pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            float o[16];
-            LoadColumns16(o_at + c, o);
-            WaitLoads();
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              LoadColumns16(o_at + c, o);
+              WaitLoads();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= by;
-            StoreColumns16(o_at + c, reinterpret_cast<const uint32_t*>(o));
+              for (int i = 0; i < 16; ++i) o[i] *= by;
+              StoreColumns16(o_at + c, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+        }
+        const float offset = reference == -INFINITY ? 0.f : -reference * p.scale;
+        const float2 scale2 = make_float2(p.scale, p.scale), offset2 = make_float2(offset, offset);
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 v = Fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), scale2, offset2);
+            v = i * kPolyOf16 % 16 < kPolyOf16 ? PolyExp2<BF16>(v) : make_float2(Exp2(v.x), Exp2(v.y));
+            sum[i & 1] = Add2(sum[i & 1], v);
+            w[i] = Pack<BF16>(v.x, v.y);
+          }
+          StoreColumns16(s_at + c / 2, w);
+          if (c >= kTile - 64) {  // three quarters of the product may begin while the last weights are made
+            WaitStores();
+            FenceBefore();
+            __syncwarp();
+            if (lane == 0) BarArrive(Smem(c == kTile - 64 ? &ctl.p_most[t] : &ctl.p_ready[t]));
           }
         }
       }
-      const float offset = reference == -INFINITY ? 0.f : -reference * p.scale;
-      const float2 scale2 = make_float2(p.scale, p.scale), offset2 = make_float2(offset, offset);
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 v = Fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), scale2, offset2);
-          v = i * kPolyOf16 % 16 < kPolyOf16 ? PolyExp2<BF16>(v) : make_float2(Exp2(v.x), Exp2(v.y));
-          sum[i & 1] = Add2(sum[i & 1], v);
-          w[i] = Pack<BF16>(v.x, v.y);
-        }
-        StoreColumns16(s_at + c / 2, w);
-        if (c >= kTile - 64) {  // three quarters of the product may begin while the last weights are made
-          WaitStores();
-          FenceBefore();
-          __syncwarp();
-          if (lane == 0) BarArrive(Smem(c == kTile - 64 ? &ctl.p_most[t] : &ctl.p_ready[t]));
-        }
-      }
-    }
-    if (count > 0 && good) good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.o_full[t]), o_parity, ctl)) != 0;
-    if (!good) break;
-    FenceAfter();
-    // a row that saw nothing has made nothing but what is left of weights that are zero
-    const float all = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), total = reference == -INFINITY && !isnan(all) ? 0.f : all, by = total == 0.f ? 0.f : 1.f / total;
-    const int row = item.at.first + in_block;  // of the sequence
-    const int rows = item.at.queries - (row & ~3);  // from the first of four lanes' on
-    const long long to = (static_cast<long long>(item.at.q0) + row) * p.q_heads + item.head, step_of_row = static_cast<long long>(p.q_heads) * D;
-    uint16_t* const out = static_cast<uint16_t*>(p.out) + to * D - (lane & 3) * step_of_row + (lane & 3) * 8;
-    done(n);
+      if (count > 0 && good) good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.o_full[t]), o_parity, ctl)) != 0;
+      if (!good) break;
+      FenceAfter();
+      // a row that saw nothing has made nothing but what is left of weights that are zero
+      const float all = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), total = reference == -INFINITY && !isnan(all) ? 0.f : all, by = total == 0.f ? 0.f : 1.f / total;
+      const int row = item.at.first + in_block;  // of the sequence
+      const int rows = item.at.queries - (row & ~3);  // from the first of four lanes' on
+      const long long to = (static_cast<long long>(item.at.q0) + row) * p.q_heads + item.head, step_of_row = static_cast<long long>(p.q_heads) * D;
+      uint16_t* const out = static_cast<uint16_t*>(p.out) + to * D - (lane & 3) * step_of_row + (lane & 3) * 8;
+      done(n);
 #pragma unroll 1  // cold code
-    for (int c = 0; c < D; c += 32) {
-      uint32_t w[16] = {};
+      for (int c = 0; c < D; c += 32) {
+        uint32_t w[16] = {};
+        if (count > 0) {
+          float o[32];
+          LoadColumns(o_at + c, o);
+          WaitLoads();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by);
+          Exchange(w, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i < rows) *reinterpret_cast<uint4*>(out + i * step_of_row + c) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+      }
       if (count > 0) {
-        float o[32];
-        LoadColumns(o_at + c, o);
-        WaitLoads();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by);
-        Exchange(w, lane);
+        o_parity ^= 1u;
+        FenceBefore();
+        __syncwarp();
+        if (lane == 0) BarArrive(Smem(&ctl.o_empty[t]));
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i < rows) *reinterpret_cast<uint4*>(out + i * step_of_row + c) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      }
-    }
-    if (count > 0) {
-      o_parity ^= 1u;
-      FenceBefore();
-      __syncwarp();
-      if (lane == 0) BarArrive(Smem(&ctl.o_empty[t]));
-    }
-    if ((lane & 3) < rows && p.lse != nullptr) p.lse[to] = total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
+      if ((lane & 3) < rows && p.lse != nullptr) p.lse[to] = total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegisters));
