@@ -276,17 +276,22 @@ __device__ __forceinline__ int UpTo(int v, int lane) {  // the sum of this lane'
   }
   return v;
 }
-// The place of a block of the grid, by its rank among those of its head.
+// The place of a block of the grid, by its rank among those of its head.  `from` is where the last search of many sequences ended, which is where the next one begins: ranks
+// mostly rise (the last of 32 sequences, and the blocks ahead of them).  512 prompts of up to 300 tokens, 24 / 8 heads of 128: 815 -> 502 us, 2000 of up to 30 3.0 -> 0.73 ms.
+struct Cursor {
+  int base, before;
+};
 template <int ROWS>
-__device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
+__device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank, Cursor* from) {
   const int lane = threadIdx.x & 31;
   // Where the GPU holds fewer blocks than there are, those with the most keys come first, so that none of them is the last to end; of up to 32 sequences, that is, which
   // a warp has at hand.  Of more, each one's last rows, which see the most keys, come ahead of its others.
   const bool sorted = p.waves && p.seqs > 1 && p.seqs <= 32;
-  int before = 0;
-  for (int base = p.seqs - 1; base >= 0; base -= 32) {
+  if (rank < from->before) *from = {p.seqs - 1, 0};
+  int before = from->before;
+  for (int base = from->base; base >= 0; base -= 32) {
     const Sequence<ROWS> s(p, base - lane);
-    int mine = s.blocks, from = 0;  // of this sequence's blocks, from its last: those that are counted
+    int mine = s.blocks, behind = 0;  // of this sequence's blocks: those that are counted, and those behind them, which come ahead of all that are
     if (sorted) {
       int lo = -1, hi = __reduce_max_sync(0xffffffffu, s.keys / kTile);  // the most tiles of keys that this block and those ahead of it look at are lo + 1
       while (lo < hi) {
@@ -297,15 +302,16 @@ __device__ __forceinline__ Place FindPlace(const PromptParams& p, int rank) {
           hi = mid - 1;
         }
       }
-      from = s.seeing(p, (lo + 1) * kTile);
-      mine = s.seeing(p, lo < 0 ? -1 : lo * kTile) - from;
-      before = __reduce_add_sync(0xffffffffu, from);
+      behind = s.seeing(p, (lo + 1) * kTile);
+      mine = s.seeing(p, lo < 0 ? -1 : lo * kTile) - behind;
+      before = __reduce_add_sync(0xffffffffu, behind);
     }
     const int upto = UpTo(mine, lane);
     const uint32_t there = __ballot_sync(0xffffffffu, rank < before + upto);
     if (there != 0) {
       const int of = __ffs(there) - 1;
-      const int back = from + rank - before - (upto - mine);  // blocks of the sequence behind this one
+      const int back = behind + rank - before - (upto - mine);  // blocks of the sequence behind this one
+      if (!sorted) *from = {base, before};
       return {__shfl_sync(0xffffffffu, s.q0, of), __shfl_sync(0xffffffffu, s.k0, of), __shfl_sync(0xffffffffu, s.queries, of), __shfl_sync(0xffffffffu, s.keys, of),
               __shfl_sync(0xffffffffu, (s.blocks - 1 - back) * ROWS, of)};
     }
@@ -353,7 +359,8 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
   FenceBefore();
   GridDependencyWait();
   Place at = {0, 0, 0, 0, -1};
-  if (warp == 1) at = FindPlace<TILES * kTile>(p, static_cast<int>(blockIdx.x) / p.q_heads);
+  Cursor cursor = {p.seqs - 1, 0};
+  if (warp == 1) at = FindPlace<TILES * kTile>(p, static_cast<int>(blockIdx.x) / p.q_heads, &cursor);
   __syncthreads();
   FenceAfter();
   const uint32_t tmem = Uniform(ctl.tmem);
@@ -669,7 +676,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
       __syncwarp();
       if (block < 0) break;
       if (lane == 0) ctl.claimed = block;
-      at = FindPlace<TILES * kTile>(p, block / p.q_heads);
+      at = FindPlace<TILES * kTile>(p, block / p.q_heads, &cursor);
     }
     if (good) tell({{0, 0, 0, 0, -1}, 0, {0, 0}});
     if (!good) ctl.fault = 1;
@@ -685,7 +692,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     const int thread = static_cast<int>(threadIdx.x) - 128;
     for (int i = 0; i <= kItems; ++i) {
       const int block = i < kItems ? -1 : ctl.claimed;
-      const Place from = i < kItems ? ctl.item[i].at : block < 0 ? Place{0, 0, 0, 0, -1} : FindPlace<TILES * kTile>(p, block / p.q_heads);
+      const Place from = i < kItems ? ctl.item[i].at : block < 0 ? Place{0, 0, 0, 0, -1} : FindPlace<TILES * kTile>(p, block / p.q_heads, &cursor);
       const int head = i < kItems ? ctl.item[i].head : block % p.q_heads, rows = from.first < 0 ? 0 : min(TILES * kTile, from.queries - from.first);
       for (int e = thread; e < rows * (D / 8); e += 128 * TILES) {
         const long long to = (static_cast<long long>(from.q0) + from.first + e / (D / 8)) * p.q_heads + head;

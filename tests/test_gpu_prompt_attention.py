@@ -147,7 +147,7 @@ def test_offsets_that_are_none(cuda):
     torch.cuda.synchronize()
 
 
-@pytest.mark.parametrize("seqs", [2, 31, 32, 33, 70])
+@pytest.mark.parametrize("seqs", [2, 31, 32, 33, 70, 500])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
 def test_more_blocks_than_the_gpu_holds(cuda, causal, dim, seqs):
