@@ -160,13 +160,25 @@ __device__ __forceinline__ float2 Add2(float2 a, float2 b) {
       : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float MaxOrNan(float a, float b) {  // the larger one; NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // 2^v for v <= 127 without the unit for exponentials: v = n + f with n whole and |f| <= 1/2, a polynomial for 2^f (the least relative error there: 7.5e-5 of degree 3, for
-// weights in BF16; 2.6e-6 of degree 4, for FP16), and n added to its exponent.  Below 2^-126 it is 2^-126, where a masked
+// weights in BF16; 2.6e-6 of degree 4, for FP16), and 2^n, whose exponent n is.  What is no number stays none: 2^n is a product's
+// factor, as n added to the polynomial's exponent makes a number of a NaN.  Below 2^-126 it is 2^-126, where a masked
 // key's weight would be 0: nothing beside a sum of at least 1/2, as long as masked values stay below 2^100.
 template <bool BF16>
 __device__ __forceinline__ float2 PolyExp2(float2 v) {
   const float2 round = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23
-  v = make_float2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  v = make_float2(MaxOrNan(v.x, -126.f), MaxOrNan(v.y, -126.f));
   const float2 n = Add2(v, round), whole = Add2(n, make_float2(-12582912.f, -12582912.f)), f = Fma2(whole, make_float2(-1.f, -1.f), v);
   float2 r;
   if constexpr (BF16) {
@@ -179,7 +191,8 @@ __device__ __forceinline__ float2 PolyExp2(float2 v) {
     r = Fma2(r, f, make_float2(0.69312179f, 0.69312179f));
     r = Fma2(r, f, make_float2(0.99999928f, 0.99999928f));
   }
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
+  const auto power = [](float whole) { return __int_as_float((__float_as_int(whole) << 23) + (127 << 23)); };
+  return Mul2(r, make_float2(power(n.x), power(n.y)));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t Pack(float lo, float hi) {

@@ -1,0 +1,62 @@
+"""PromptAttention of values that are no numbers, that are as large as their type has them, or whose weights are tiny."""
+import math
+
+import pytest
+import torch
+
+from _attention import half_step
+from qwen38_flash_ops_b200 import PromptAttention
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+
+
+def offsets(*lengths):
+    return torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32).cuda()
+
+
+def a_case(n, heads, kv_heads, dim, dtype, seed=1):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(n, h, dim, generator=gen).to(dtype).cuda() for h in (heads, kv_heads, kv_heads)]
+
+
+def alike(got, want, v):
+    """The same rows, but that the rows of a warp take up their maxima together, so that weights may be rounded at other points."""
+    bound = 2 * half_step(got.dtype) * (want.abs() + v[torch.isfinite(v)].abs().amax()).double()
+    return torch.isfinite(got).all() and ((got.double() - want.double()).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 130])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_query_that_is_no_number(cuda, dtype, dim, causal, n):
+    """Its row alone is NaN, however few keys it sees."""
+    op = PromptAttention(causal=causal)
+    for bad in (row for row in (0, 1, 2, 64, 129) if row < n):
+        q, k, v = a_case(n, 2, 1, dim, dtype)
+        want, log = op(q, k, v, offsets(n), lse=True)
+        q[bad, 1, 3] = NAN
+        got, also = op(q, k, v, offsets(n), lse=True)
+        assert torch.isnan(got[bad, 1].float()).all() and torch.isnan(also[bad, 1]), (bad, got[bad, 1], also[bad, 1])
+        got[bad, 1], also[bad, 1] = want[bad, 1], log[bad, 1]
+        assert alike(got, want, v) and torch.allclose(also, log, atol=1e-3)
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_key_that_is_no_number(cuda, dtype, dim, causal, value):
+    """At every place of a tile's eight, of the first tile and of a later one: the rows that see it are NaN, the others as they were."""
+    n, op = 200, PromptAttention(causal=causal)
+    for key in (*range(16), *range(136, 144)):
+        q, k, v = a_case(n, 2, 1, dim, dtype)
+        q[:, :, 5] = 1.0  # a score of infinity, not of its negative
+        want, log = op(q, k, v, offsets(n), lse=True)
+        k[key, 0, 5] = value
+        got, also = op(q, k, v, offsets(n), lse=True)
+        first = key if causal else 0
+        assert torch.isnan(got[first:].float()).all() and torch.isnan(also[first:]).all(), (key, torch.isfinite(got.float()).all(-1).nonzero().tolist()[:4])
+        assert alike(got[:first], want[:first], v) and torch.isfinite(also[:first]).all()
