@@ -173,12 +173,12 @@ __device__ __forceinline__ float MaxOrNan(float a, float b) {  // the larger one
 }
 // 2^v for v <= 127 without the unit for exponentials: v = n + f with n whole and |f| <= 1/2, a polynomial for 2^f (the least relative error there: 7.5e-5 of degree 3, for
 // weights in BF16; 2.6e-6 of degree 4, for FP16), and 2^n, whose exponent n is.  What is no number stays none: 2^n is a product's
-// factor, as n added to the polynomial's exponent makes a number of a NaN.  Below 2^-126 it is 2^-126, where a masked
-// key's weight would be 0: nothing beside a sum of at least 1/2, as long as masked values stay below 2^100.
+// factor, as n added to the polynomial's exponent makes a number of a NaN.  From v = -126.5 down n is -127, for which the factor's bits are those of 0: a masked key weighs
+// nothing, whatever its value.
 template <bool BF16>
 __device__ __forceinline__ float2 PolyExp2(float2 v) {
   const float2 round = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23
-  v = make_float2(MaxOrNan(v.x, -126.f), MaxOrNan(v.y, -126.f));
+  v = make_float2(MaxOrNan(v.x, -127.f), MaxOrNan(v.y, -127.f));
   const float2 n = Add2(v, round), whole = Add2(n, make_float2(-12582912.f, -12582912.f)), f = Fma2(whole, make_float2(-1.f, -1.f), v);
   float2 r;
   if constexpr (BF16) {
@@ -469,8 +469,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
       if (count > 0 && good) good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.o_full[t]), o_parity, ctl)) != 0;
       if (!good) break;
       FenceAfter();
-      // a row that saw nothing has made nothing but what is left of weights that are zero
-      const float all = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), total = reference == -INFINITY && !isnan(all) ? 0.f : all, by = total == 0.f ? 0.f : 1.f / total;
+      const float total = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), by = total == 0.f ? 0.f : 1.f / total;  // 0: of a row that saw nothing
       const int row = item.at.first + in_block;  // of the sequence
       const int rows = item.at.queries - (row & ~3);  // from the first of four lanes' on
       const long long to = (static_cast<long long>(item.at.q0) + row) * p.q_heads + item.head, step_of_row = static_cast<long long>(p.q_heads) * D;

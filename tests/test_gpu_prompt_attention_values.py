@@ -60,3 +60,26 @@ def test_a_key_that_is_no_number(cuda, dtype, dim, causal, value):
         first = key if causal else 0
         assert torch.isnan(got[first:].float()).all() and torch.isnan(also[first:]).all(), (key, torch.isfinite(got.float()).all(-1).nonzero().tolist()[:4])
         assert alike(got[:first], want[:first], v) and torch.isfinite(also[:first]).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_masked_values_may_be_as_large_as_there_are(cuda, dtype, dim, sign):
+    """The type's largest and lowest value in keys and values of a token that causal rows do not see yet: those rows are as they were, to the bit where they see one key."""
+    n, op = 200, PromptAttention()
+    for token in (*range(1, 17), *range(136, 144)):
+        q, k, v = a_case(n, 2, 1, dim, dtype)
+        want = op(q, k, v, offsets(n))
+        v[token] = sign * torch.finfo(dtype).max
+        got = op(q, k, v, offsets(n))
+        assert torch.equal(got[0], want[0]) and alike(got[:token], want[:token], v[:token]), (token, (got[:token].float() - want[:token].float()).abs().max())
+
+
+def test_rows_that_see_nothing_beside_masked_values(cuda):
+    """More queries than keys: the first ones see none, and are 0 whatever the keys' finite values are."""
+    for dtype in (torch.bfloat16, torch.float16):
+        q, k, v = a_case(90, 2, 1, 64, dtype)
+        v[:] = torch.finfo(dtype).max
+        got, lse = PromptAttention()(q, k[:40], v[:40], offsets(90), offsets(40), lse=True)
+        assert (got[:50] == 0).all() and (lse[:50] == -math.inf).all() and torch.isfinite(lse[50:]).all()
