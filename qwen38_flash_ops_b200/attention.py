@@ -20,6 +20,10 @@ from .ops import _DTYPES, _FLOATS, _given, _load, _refuse, _stream_ptr
 _HALVES = (torch.bfloat16, torch.float16)
 _PACK_CACHE = struct.Struct("PPPPi4xqqqqffi4x")  # qfg_kv_cache, and the device that it lies on
 _IDS = {torch.int32: 4, torch.int64: 8}
+# What says in C++ that an object is a cache: a capsule, which nothing but a KvCache makes, of the address of its qfg_kv_cache.
+_CAPSULE = b"qfg_kv_cache"
+_new_capsule = ctypes.pythonapi.PyCapsule_New
+_new_capsule.restype, _new_capsule.argtypes = ctypes.py_object, (c_void_p, ctypes.c_char_p, c_void_p)
 
 
 def _on_current(t) -> bool:
@@ -115,6 +119,7 @@ class KvCache:
         self._packed = ctypes.create_string_buffer(_PACK_CACHE.pack(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), _DTYPES[k.dtype],
                                                                     self.pages, self.kv_heads, self.page, dim, self.k_unit, self.v_unit, k.get_device()))
         self._at = ctypes.addressof(self._packed)
+        self._capsule = _new_capsule(self._at, _CAPSULE, None)
 
     k = property(lambda self: self._k)
     k_scale = property(lambda self: self._k_scale)
@@ -171,7 +176,7 @@ class QkNormRope:
     def __call__(self, q, k, positions=None, q_weight=None, k_weight=None, v=None, cache: KvCache | None = None, slots=None, keys: bool = False):
         """positions [tokens], or [axes, tokens] of as many as `sections` has, int64 or int32; slots [tokens] int64: a token whose slot is negative or lies
         behind the cache is not written; slots must differ."""
-        r = ops._calls.qk_norm_rope(self._p, q, k, positions, q_weight, k_weight, v, cache._at if cache.__class__ is KvCache else cache, slots, keys)
+        r = ops._calls.qk_norm_rope(self._p, q, k, positions, q_weight, k_weight, v, cache._capsule if cache.__class__ is KvCache else cache, slots, keys)
         if r is not None:
             return r if r.__class__ is not int else check(r)
         op = "QkNormRope"
@@ -232,7 +237,7 @@ class CacheWrite:
         self._lib = _load()
 
     def __call__(self, k, v, cache: KvCache, slots) -> None:
-        r = ops._calls.cache_write(k, v, cache._at if cache.__class__ is KvCache else cache, slots)
+        r = ops._calls.cache_write(k, v, cache._capsule if cache.__class__ is KvCache else cache, slots)
         if r is not None:
             return check(r)
         op = "CacheWrite"
@@ -258,7 +263,7 @@ class CacheRead:
 
     def __call__(self, cache: KvCache, table, offsets, rows: int, out=None):
         if out is None:
-            r = ops._calls.cache_read(self._code, cache._at if cache.__class__ is KvCache else cache, table, offsets, rows)
+            r = ops._calls.cache_read(self._code, cache._capsule if cache.__class__ is KvCache else cache, table, offsets, rows)
             if r is not None:
                 return r if r.__class__ is tuple else check(r)
         op = "CacheRead"
@@ -298,7 +303,7 @@ class CacheAttention:
 
     def __call__(self, q, cache: KvCache, table, lengths, out=None, lse: bool = False):
         if out is None:
-            r = ops._calls.cache_attention(self.scale, q, cache._at if cache.__class__ is KvCache else cache, table, lengths, lse)
+            r = ops._calls.cache_attention(self.scale, q, cache._capsule if cache.__class__ is KvCache else cache, table, lengths, lse)
             if r is not None:
                 return r if r.__class__ is not int else check(r)
         op = "CacheAttention"

@@ -436,10 +436,11 @@ struct HeldCache {  // what a KvCache keeps for its calls
   qfg_kv_cache cache;
   int32_t device;
 };
+// from the capsule that only a KvCache makes: an integer in its place is some caller's mistake, and no address
 const HeldCache* ToCache(PyObject* o) {
-  if (!PyLong_CheckExact(o)) return nullptr;
-  const HeldCache* c = static_cast<const HeldCache*>(PyLong_AsVoidPtr(o));
-  return c != nullptr && c->device == c10::cuda::current_device() ? c : nullptr;
+  if (!PyCapsule_IsValid(o, "qfg_kv_cache")) return nullptr;
+  const HeldCache* c = static_cast<const HeldCache*>(PyCapsule_GetPointer(o, "qfg_kv_cache"));
+  return c->device == c10::cuda::current_device() ? c : nullptr;
 }
 const at::Tensor* Numbers(PyObject* o, at::ScalarType type, int64_t dims) {
   const at::Tensor* t = Dense(o);
