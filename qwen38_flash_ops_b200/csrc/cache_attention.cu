@@ -10,8 +10,8 @@
 //   keys     S^T = K q^T.  A lane holds a quarter of the channels of two tokens; channels are taken in the order in which they lie in memory, by q as well.
 //   values   O^T = V^T P^T.  A lane holds D / 8 channels of four tokens of each sixteen; pairs of tokens are made by byte permutations.  P^T is S^T's layout transposed.
 //   scales   four bits: the product of an E2M1 value and an E4M3 scale has at most six significant bits and is exact in FP16.  Eight bits: the keys' scale multiplies the
-//            score, the values' the weight; scores then count from where score + log2(the value's scale) is largest, so that the product is within FP16 for values of any
-//            size (of scores past 2^20 FP32 loses the logarithm, and small scales bits of their weight with it).
+//            score, the values' the weight; scores then count from where score + log2(the value's scale) is largest, so that the product is within FP16 for scales up
+//            to 2^107 (of scores past 2^20 FP32 loses the logarithm, and small scales bits of their weight with it).
 //   q        as FP16, each row times the power of two that takes its largest value to 2^9, so that only what is 2^-23 of that is rounded.
 //
 // Softmax runs along: m is taken up only when a score passes it by 8 (in powers of two), so that sums and weights stay within 2^8 of what they would be and the outputs
@@ -45,6 +45,9 @@ namespace {
 // 255.  Twelve warps of 168 are slower there: 16 sequences of up to 4001 tokens, four tokens of 32 / 8 heads of 128 each, 31.7 -> 39.8 us; 32 of up to 8192, 24 / 4 heads of
 // 256, NVFP4 50.7 -> 62.7, E4M3 69.3 -> 85.9.
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
+// Eight bits: of a value's scale, 2^this is the most that moves the point from which weights are measured.  FP32 still holds the exponentials of 2^-26 of the largest there; FP16
+// holds a weight's product with a scale of 2^7 more.
+constexpr float kMostLogScale = 100.f;
 // All tiles, in equal shares: share i begins at tile size i + min(i, more).
 struct Shares {
   long long size;
@@ -490,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
               LoadShared<4>(tile + G::kTile * G::kCodes + token * 4, reinterpret_cast<uint32_t*>(&key_scale));
               LoadShared<4>(tile + G::kPart + G::kTile * G::kCodes + token * 4, reinterpret_cast<uint32_t*>(&value_scale[u][h]));
               if (!whole && (token0 + static_cast<int>(token) >= at.length || absent)) value_scale[u][h] = 1.f;
-              log_scale[u][h] = fminf(fmaxf(Log2(value_scale[u][h]), -60.f), 60.f);
+              log_scale[u][h] = fminf(fmaxf(Log2(value_scale[u][h]), -60.f), kMostLogScale);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
 #pragma unroll
