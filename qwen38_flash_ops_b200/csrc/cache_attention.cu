@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // 2^(9 - exponent) of the largest and its inverse; the exponent is kept where both are ordinary numbers
-        const int e = min(max(static_cast<int>(top >> 23), 20), 240);
+        const int e = min(max(static_cast<int>(top >> 23), 20), 254);  // 254: of the largest number there is
         const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(e - 9) << 23) * p.scale;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) q[n][i / 2][i % 2] = Pack16(v[2 * i] * up, v[2 * i + 1] * up);

@@ -21,3 +21,14 @@ def test_large_values(cuda, some, power, dim, group, tokens):
     flat[::some] = (flat[::some] * 2.0 ** power).clamp(max=2.0 ** 107)
     got, lse = CacheAttention()(q, cache, table, n, lse=True)
     check(got, lse, cache, table, q, n, 1 / math.sqrt(dim))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [112, 122, 125])
+def test_large_queries(cuda, form, power):
+    """Queries up to BF16's largest exponent, with a scale that makes ordinary scores of them."""
+    cache, table, q, n = a_case(form, 128, 2, 4, 2, [300, 65], torch.bfloat16)
+    q[0] *= 2.0 ** power
+    assert torch.isfinite(q).all()
+    got, lse = CacheAttention(scale=2.0 ** -power)(q, cache, table, n, lse=True)
+    check(got, lse, cache, table, q, n, 2.0 ** -power)
