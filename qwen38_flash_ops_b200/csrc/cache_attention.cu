@@ -14,8 +14,9 @@
 //            to 2^107 (of scores past 2^20 FP32 loses the logarithm, and small scales bits of their weight with it).
 //   q        as FP16, each row times the power of two that takes its largest value to 2^9, so that only what is 2^-23 of that is rounded.
 //
-// Softmax runs along: m is taken up only when a score passes it by 8 (in powers of two), so that sums and weights stay within 2^8 of what they would be and the outputs
-// are seldom scaled again.  Statistics and sums are FP32, weights FP16 (2^-11 of themselves, as the values are exact).
+// Softmax runs along: m is taken up only when a score has gone past it by some powers of two, so that the outputs are seldom scaled again.  Statistics and sums are FP32, weights
+// FP16: off by 2^-11 of themselves, as the values are exact, and by 2^-25 below 2^-14.  So that long sequences whose weights are all small beside one do not lose them, in four
+// bits m lies 7 below the largest score when it is taken up: FP16's smallest number is 2^-31 of that one's weight.  In eight bits it is 2^-24 of the largest product with a scale.
 //
 // A warp runs through an equal share of all tiles (of one sequence and key head after another, in that order) and has its own ring of tiles in shared memory, which it
 // fills by asynchronous copies ahead of itself, across the borders of sequences and heads too; no warp waits for another.  Shares begin and end anywhere; a second kernel
@@ -524,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
             }
           }
         }
-        // m is taken up where a score passes it by 8
+        // m is taken up where a weight is past 2^15, near FP16's largest (eight bits: past 2^8, as the sums of scores past 2^24 and logarithms are off by up to 2^8 themselves)
+        constexpr float kBelow = FP4 ? 7.f : 0.f, kRoom = FP4 ? 15.f : 8.f;
         bool higher = false;
         float upto[NT][2];
 #pragma unroll
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
               for (int h = 0; h < 2; ++h) m = fmaxf(m, FP4 ? s[u][n][2 * h + r] : s[u][n][2 * h + r] + log_scale[u][h]);
             }
             upto[n][r] = m;
-            higher = higher || upto[n][r] > most[n][r] + 8.f;
+            higher = higher || upto[n][r] - most[n][r] > kRoom;  // the difference is exact, however large they are
           }
         }
         if (__any_sync(0xffffffffu, higher)) {
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
               float m = upto[n][r];
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-              m = fmaxf(m, most[n][r]);
+              m = fmaxf(m - kBelow, most[n][r]);
               const float by = m == -INFINITY ? 1.f : Exp2(most[n][r] - m);
               most[n][r] = m;
               sum[n][r] *= by;

@@ -4,8 +4,8 @@ import math
 import pytest
 import torch
 
-from _attention import FORMS
-from qwen38_flash_ops_b200 import CacheAttention
+from _attention import FORMS, attention, half_step, held, new_cache
+from qwen38_flash_ops_b200 import CacheAttention, CacheWrite
 from test_gpu_cache_attention import a_case, check
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +32,27 @@ def test_large_queries(cuda, form, power):
     assert torch.isfinite(q).all()
     got, lse = CacheAttention(scale=2.0 ** -power)(q, cache, table, n, lse=True)
     check(got, lse, cache, table, q, n, 2.0 ** -power)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_weights_that_are_tiny_beside_one(cuda, dim, form):
+    """A first token whose score is 18 above those of 120000 others: each weighs 2^-26 of it and all of them a 500th, which is all there is, as the first value is 0.  As many
+    sequences, of the same pages, that a warp has a whole one to itself."""
+    count, seqs, gen = 120000, 2400, torch.Generator().manual_seed(1)
+    cache = new_cache(form, -(-count // 64), 1, dim, page=64)
+    k, v = torch.zeros(count, 1, dim), 1 + 0.25 * torch.rand(count, 1, dim, generator=gen)
+    k[0, 0, 0], v[0] = 4.5, 0.0
+    CacheWrite()(k.half().cuda(), v.half().cuda(), cache, torch.arange(count).cuda())
+    table, n = torch.arange(cache.pages).int().repeat(seqs, 1).cuda(), torch.full((seqs,), count, dtype=torch.int32).cuda()
+    q = torch.zeros(seqs, 2, dim)
+    q[..., 0] = 4.0
+    got, lse = CacheAttention(scale=1.0)(q.half().cuda(), cache, table, n, lse=True)
+    ki, vi = (held(c, s, u)[:, 0].flatten(0, 1)[:count] for c, s, u in ((cache.k, cache.k_scale, cache.k_unit), (cache.v, cache.v_scale, cache.v_unit)))
+    y, size, log = attention(q[0].double(), ki, vi, torch.tensor([count, count]), 1.0)
+    # A weight is off by 2^-11 of itself and, below 2^-14, by 2^-25 where the largest is 2^7 or more (in eight bits the zero row's scale of 2^-40 makes it small).  An eighth of a
+    # row's weights are added one after another in FP32, each sum off by up to 2^-24 of itself; the products, sixteen tokens at a time, are cut off at up to 2^-23.
+    tiny, sums = count * 2.0 ** -32 * vi.abs().amax(), count / 8 * 2.0 ** -24
+    tol = (half_step(torch.float16) + sums + count / 16 * 2.0 ** -23) * y.abs() + 2.0 ** -11 * size + tiny + 2.0 ** -25
+    assert ((got.cpu().double() - y).abs() <= tol).all(), ((got.cpu().double() - y).abs() / tol).max()
+    assert ((lse.cpu().double() - log).abs() <= 2.0 ** -18 * (1 + log) + sums).all()
