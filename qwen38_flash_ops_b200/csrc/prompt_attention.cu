@@ -18,8 +18,9 @@
 // loads and stores, and waits and the next item's reading stand behind them.  Both together: 8192 tokens of 64 heads 930 -> 829 us, 48 prompts of 256 tokens of 24 heads of 128
 // 102 -> 51.
 //
-// One pass: m is taken up only when a score passes it by 8 (in powers of two), and only then are O and the sum scaled again; weights stay below 2^8, within FP16.
-// S and the sums are FP32; P is rounded to the type of the inputs, as tensor cores take it (2^-8 or 2^-11 of each weight, before sums of many).
+// One pass: m is taken up only when a score passes it by 8 (in powers of two), and only then are O and the sum scaled again.  In FP16 weights are 2^7 times as large, up to 2^15: its
+// smallest number is 2^-31 of the largest weight then, which keeps those of long sequences that are all small beside one.  S and the sums are FP32; P is rounded to the type of
+// the inputs, as tensor cores take it (2^-8 or 2^-11 of each weight, before sums of many).
 //
 // Products and exponentials take the same time (a tile of 128 x 128 at D = 128: 1024 cycles of the tensor core, 1024 of the unit for exponentials at 16 a cycle), which is
 // what bounds the kernel; a quarter of the exponentials goes to the FMA units for that reason.  No weight is made for tiles that the mask leaves out.  Causal, 8192 tokens of
@@ -52,7 +53,7 @@ struct PromptParams {
   void* out;
   float* lse;
   int seqs, q_rows, k_rows, q_heads, group;
-  float scale;  // of scores, in powers of two
+  float scale, step;  // of scores, in powers of two; how far, before that, one may pass the highest ahead of it
   bool causal, waves, give_up;  // waves: there are more blocks than the GPU holds at once
 };
 
@@ -394,7 +395,6 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
     const int t = (warp >> 2) - 1;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + static_cast<uint32_t>(t * kTile), o_at = tmem + lanes + static_cast<uint32_t>(G::kOutput + t * D);
-    const float step = 8.f / p.scale;
     uint32_t s_parity = 0, o_parity = 0;
     const int in_block = t * kTile + (warp & 3) * 32 + lane;
 #pragma unroll 1
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
       const Item& item = ctl.item[n % kItems];
       const int keys = item.at.keys, count = item.tiles[t], over = keys - item.at.queries + 1 + item.at.first + in_block;  // what a causal row sees, if there is as much
       const int sees = p.causal ? min(keys, over) : keys, first_sees = p.causal ? min(keys, over - lane) : keys;          // first_sees: the warp's first row
-      float reference = -INFINITY;
+      float limit = -INFINITY, offset = 0.f;  // a weight is 2^(scale s + offset), as long as no s is above the limit
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
       for (int j = 0; j < count; ++j) {
@@ -427,10 +427,15 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
           for (int e = i + 8; e < kTile; e += 8) m[i] = fmaxf(fmaxf(m[i], s[e]), s[e + 4]);
         }
         const float highest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        if (__any_sync(0xffffffffu, highest > reference + step)) {
-          const float to = fmaxf(reference, highest);
-          const float by = to == -INFINITY ? 1.f : Exp2((reference - to) * p.scale);
-          reference = to;
+        if (__any_sync(0xffffffffu, highest > limit)) {
+          float by = 1.f;
+          if (highest + p.step > limit) {
+            // of scores past 2^23 the offset's rounding leaves FP16 no room for the 2^7
+            const float most = highest * p.scale, to = (BF16 || !(fabsf(most) < 8388608.f) ? 0.f : 7.f) - most;
+            by = limit == -INFINITY ? 0.f : Exp2(to - offset);
+            limit = highest + p.step;
+            offset = to;
+          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * by, sum[i].y * by);
           if (j > 0) {  // the products of the tile ahead have ended: S, which was issued after them, has
@@ -445,7 +450,6 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
             }
           }
         }
-        const float offset = reference == -INFINITY ? 0.f : -reference * p.scale;
         const float2 scale2 = make_float2(p.scale, p.scale), offset2 = make_float2(offset, offset);
 #pragma unroll
         for (int c = 0; c < kTile; c += 32) {
@@ -497,7 +501,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
         __syncwarp();
         if (lane == 0) BarArrive(Smem(&ctl.o_empty[t]));
       }
-      if ((lane & 3) < rows && p.lse != nullptr) p.lse[to] = total == 0.f ? -INFINITY : (reference * p.scale + Log2(total)) * 0.693147181f;
+      if ((lane & 3) < rows && p.lse != nullptr) p.lse[to] = total == 0.f ? -INFINITY : (Log2(total) - offset) * 0.693147181f;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegisters));
@@ -766,6 +770,7 @@ cudaError_t LaunchPromptAttention(const PromptCall& c, cudaStream_t stream) {
   p.q_heads = c.q_heads;
   p.group = c.q_heads / c.kv_heads;
   p.scale = c.scale * 1.44269504f;
+  p.step = 8.f / p.scale;
   p.causal = c.causal;
   p.give_up = c.give_up;
   cudaError_t err;

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _attention import half_step
+from _attention import attention, half_step
 from qwen38_flash_ops_b200 import PromptAttention
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +83,19 @@ def test_rows_that_see_nothing_beside_masked_values(cuda):
         v[:] = torch.finfo(dtype).max
         got, lse = PromptAttention()(q, k[:40], v[:40], offsets(90), offsets(40), lse=True)
         assert (got[:50] == 0).all() and (lse[:50] == -math.inf).all() and torch.isfinite(lse[50:]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_weights_that_are_tiny_beside_one(cuda, dim):
+    """A first key whose score is 18 above those of 120000 others: each weighs 2^-26 of it and all of them a 500th, which is all there is, as the first value is 0."""
+    count, gen = 120000, torch.Generator().manual_seed(1)
+    q, k, v = torch.zeros(3, 2, dim), torch.zeros(count, 1, dim), 1 + 0.25 * torch.rand(count, 1, dim, generator=gen)
+    q[..., 0], k[0, 0, 0], v[0] = 4.0, 4.5, 0.0
+    got, lse = PromptAttention(scale=1.0, causal=False)(q.half().cuda(), k.half().cuda(), v.half().cuda(), offsets(3), offsets(count), lse=True)
+    y, size, log = attention(q[0].half().double(), k[:, 0].half().double(), v[:, 0].half().double(), torch.tensor([count, count]), 1.0)
+    # A weight is off by 2^-11 of itself and, below 2^-14, by 2^-25 where the largest is 2^7 or more.  A quarter of a row's weights are added one after another in FP32, each sum
+    # off by up to 2^-24 of itself; the products, sixteen keys at a time, are cut off at up to 2^-23.
+    sums = count / 4 * 2.0 ** -24
+    tol = (half_step(torch.float16) + sums + count / 16 * 2.0 ** -23) * y.abs() + (2.0 ** -11 + 1e-5) * size + count * 2.0 ** -32 * v.abs().amax() + 2.0 ** -25
+    assert ((got.cpu().double() - y).abs() <= tol).all(), ((got.cpu().double() - y).abs() / tol).max()
+    assert ((lse.cpu().double() - log).abs() <= 2.0 ** -18 * (1 + log) + sums).all()
