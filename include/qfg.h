@@ -432,8 +432,9 @@ QFG_API int qfg_cache_attention(int dtype, const void* q, int64_t ld_seq, int64_
  * [q_rows][q_heads]) contiguous.  A row that sees nothing is 0, its lse -inf.  Rows ahead of the first and behind the last sequence are left
  * as they were; what lies in keys and values of other sequences takes no part, whatever it is.  Within a sequence a value that is not
  * finite makes rows of the same head that lie up to 128 tokens ahead of it NaN as well: their weight for it is 0, and 0 times it is not;
- * a finite one, however large, takes no part in them.  A row that has a score of NaN or +infinity is NaN, its lse as well; one of -infinity is a weight of 0.
- * Scores (scale q k) have to stay below 2^28; rows with larger ones may become NaN. */
+ * a finite one, however large, takes no part in them.  A row that has a score of NaN or +infinity is NaN, its lse as well; one of -infinity
+ * is a weight of 0, and a row of none but those NaN.  Scores (scale q k) have to stay below 2^28: a row whose largest is further from 0 than
+ * that may become NaN, and does where FP32 cannot tell what it is. */
 QFG_API int qfg_prompt_attention(int dtype, const void* q, int64_t ldq, int64_t q_rows, int64_t q_heads, const void* k, int64_t ldk, const void* v,
                                  int64_t ldv, int64_t k_rows, int64_t kv_heads, int64_t head_dim, const int32_t* q_offsets, const int32_t* k_offsets,
                                  int64_t seqs, int causal, float scale, void* out, float* lse, void* stream);

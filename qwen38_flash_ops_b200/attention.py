@@ -342,8 +342,8 @@ class PromptAttention:
     there).  `scale`: 1 / sqrt(head_dim) unless given.  Returns [rows, heads, head_dim]; with lse=True also the logarithm of each row's sum of exponentials, FP32.
 
     What lies in the keys and values of other sequences takes no part, whatever it is.  Within a sequence, a value that is not finite makes rows of its head
-    up to 128 tokens ahead of it NaN as well.  A row that has a score of NaN or +infinity is NaN.  Scores (scale q k) have to stay below 2^28; rows with larger
-    ones may become NaN."""
+    up to 128 tokens ahead of it NaN as well.  A row that has a score of NaN or +infinity is NaN.  Scores (scale q k) have to stay below 2^28: a row whose
+    largest is further from 0 than that may become NaN."""
 
     def __init__(self, scale: float | None = None, causal: bool = True):
         self._lib = _load()

@@ -430,8 +430,9 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
         if (__any_sync(0xffffffffu, highest > limit)) {
           float by = 1.f;
           if (highest + p.step > limit) {
-            // of scores past 2^23 the offset's rounding leaves FP16 no room for the 2^7
-            const float most = highest * p.scale, to = (BF16 || !(fabsf(most) < 8388608.f) ? 0.f : 7.f) - most;
+            // of scores past 2^23 the offset's rounding leaves FP16 no room for the 2^7; past 2^28 (BF16: 2^31) it may be that all weights are 0: the row is NaN
+            const float most = highest * p.scale, bias = BF16 || !(fabsf(most) < 8388608.f) ? 0.f : 7.f;
+            const float to = fabsf(most) < (BF16 ? 2147483648.f : 268435456.f) ? bias - most : __int_as_float(0x7FFFFFFF);
             by = limit == -INFINITY ? 0.f : Exp2(to - offset);
             limit = highest + p.step;
             offset = to;
@@ -473,7 +474,9 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
       if (count > 0 && good) good = __all_sync(0xffffffffu, BarWait(Smem(&ctl.o_full[t]), o_parity, ctl)) != 0;
       if (!good) break;
       FenceAfter();
-      const float total = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), by = total == 0.f ? 0.f : 1.f / total;  // 0: of a row that saw nothing
+      // 0: of a row that saw nothing; of keys whose scores are all -infinity nothing can be said
+      const float all = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y), total = limit == -INFINITY && sees > 0 ? __int_as_float(0x7FFFFFFF) : all;
+      const float by = total == 0.f ? 0.f : 1.f / total;
       const int row = item.at.first + in_block;  // of the sequence
       const int rows = item.at.queries - (row & ~3);  // from the first of four lanes' on
       const long long to = (static_cast<long long>(item.at.q0) + row) * p.q_heads + item.head, step_of_row = static_cast<long long>(p.q_heads) * D;

@@ -99,3 +99,26 @@ def test_many_weights_that_are_tiny_beside_one(cuda, dim):
     tol = (half_step(torch.float16) + sums + count / 16 * 2.0 ** -23) * y.abs() + (2.0 ** -11 + 1e-5) * size + count * 2.0 ** -32 * v.abs().amax() + 2.0 ** -25
     assert ((got.cpu().double() - y).abs() <= tol).all(), ((got.cpu().double() - y).abs() / tol).max()
     assert ((lse.cpu().double() - log).abs() <= 2.0 ** -18 * (1 + log) + sums).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scores_past_what_fp32_tells_apart(cuda, dtype, dim, causal):
+    """Scores of 2^20 to 2^140: a row is that of its largest score, or NaN, never one that saw nothing."""
+    n, op = 40, PromptAttention(scale=2.0 ** 10 * 1.1, causal=causal)
+    for power in ((0, 5, 7) if dtype == torch.float16 else range(0, 64, 3)):
+        q, k, v = a_case(n, 2, 1, dim, dtype, seed=power)
+        q, k = q * 2.0 ** power, k * 2.0 ** power
+        got, lse = op(q, k, v, offsets(n), lse=True)
+        bad = torch.isnan(got.float()).any(-1)
+        s = torch.einsum("ihd,jd->ihj", q.cpu().double(), k[:, 0].cpu().double()) * (2.0 ** 10 * 1.1)
+        if causal:
+            s.masked_fill_(torch.arange(n)[None, None] > torch.arange(n)[:, None, None], -INF)
+        top = s.topk(2).values
+        sure = (~bad.cpu()) & (top[..., 0] - top[..., 1] > 2.0 ** -17 * s[torch.isfinite(s)].abs().amax() + 50)  # FP32 sums tell the largest from the next, by far
+        sure[0] = ~bad[0].cpu()
+        want = v[:, 0].cpu().double()[s.argmax(-1)]
+        assert ((got.cpu().double() - want).abs()[sure] <= 2.0 ** -7 * want.abs()[sure]).all(), power
+        assert (torch.isnan(lse) == bad).all() and torch.isfinite(lse[~bad]).all()
+        assert power > 0 or not bad.any()
