@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, worker = static_cast<int>(blockIdx.x) * kWarps + warp;
   GridDependencyWait();
-  GridLaunchDependents();  // the second kernel, which waits for all of this one
+  if (p.parts != nullptr) GridLaunchDependents();  // the second kernel, which waits for all of this one; without it the caller's next one, which has no business here yet
   const Share share = FindShare(p, G::kTile);
   const int units = p.cache.heads * p.row_blocks;
   for (int seq = blockIdx.x; seq < p.seqs; seq += gridDim.x) {
