@@ -168,7 +168,8 @@ class QkNormRope:
         axes = [0] * pairs if axes is None else [int(a) for a in axes]
         if len(inv_freq) != pairs or len(axes) != pairs:
             _refuse(f"QkNormRope: there must be a frequency and an axis for each of {pairs} pairs")
-        self.head_dim, self.rotary_dim, self.axes = head_dim, rotary, max(axes, default=0) + 1
+        self._read = max(axes, default=0) + 1  # rows of positions that any pair goes by are among so many
+        self.head_dim, self.rotary_dim, self.axes = head_dim, rotary, max(self._read, len(sections) if sections is not None else 0)
         check(lib.qfg_qk_norm_rope_create((ctypes.c_double * max(1, pairs))(*inv_freq), (ctypes.c_int32 * max(1, pairs))(*axes), pairs, head_dim, int(bool(interleaved)),
                                           float(rotary_scale), float(eps), float(weight_offset), ctypes.byref(self._h)))
         self._p = self._h.value
@@ -176,6 +177,10 @@ class QkNormRope:
     def __call__(self, q, k, positions=None, q_weight=None, k_weight=None, v=None, cache: KvCache | None = None, slots=None, keys: bool = False):
         """positions [tokens], or [axes, tokens] of as many as `sections` has, int64 or int32; slots [tokens] int64: a token whose slot is negative or lies
         behind the cache is not written; slots must differ."""
+        if self.axes > self._read and self.rotary_dim:  # the last sections have no pairs
+            if not isinstance(positions, torch.Tensor) or positions.dim() != 2 or positions.shape[0] != self.axes:
+                _refuse(f"QkNormRope: positions must be [{self.axes}, tokens]")
+            positions = positions[:self._read]
         r = ops._calls.qk_norm_rope(self._p, q, k, positions, q_weight, k_weight, v, cache._capsule if cache.__class__ is KvCache else cache, slots, keys)
         if r is not None:
             return r if r.__class__ is not int else check(r)
@@ -184,17 +189,17 @@ class QkNormRope:
         of, kv_heads, _, ldk = _heads(op, "k", k, (q.dtype,), dim)
         if of != tokens:
             _refuse(f"{op}: q and k must have as many tokens")
-        where, wide, ldp, axes = None, 8, 0, self.axes
+        where, wide, ldp, axes = None, 8, 0, self._read
         if self.rotary_dim:
             if positions is None:
                 _refuse(f"{op}: no positions")
             p = positions.unsqueeze(0) if isinstance(positions, torch.Tensor) and positions.dim() == 1 else positions
             _whole_numbers(op, "positions", p, tuple(_IDS), 2)
-            if tuple(p.shape) != (self.axes, tokens):
+            if tuple(p.shape) != (axes, tokens):
                 _refuse(f"{op}: positions must be [{tokens}]" if self.axes == 1 else f"{op}: positions must be [{self.axes}, {tokens}]")
-            if self.axes > 1 and tokens > 0 and p.stride(0) < tokens:
+            if axes > 1 and tokens > 0 and p.stride(0) < tokens:
                 _refuse(f"{op}: the axes of positions overlap")
-            where, wide, ldp = p.data_ptr(), _IDS[p.dtype], p.stride(0) if self.axes > 1 else tokens
+            where, wide, ldp = p.data_ptr(), _IDS[p.dtype], p.stride(0) if axes > 1 else tokens
         kind = q.dtype
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
             if w is None:
