@@ -64,6 +64,13 @@ def _table(op: str, table, cache):
     return table.data_ptr(), ld, seqs, most
 
 
+def _workspace_bytes(cache, seqs: int, tokens: int, heads: int, most: int) -> int:
+    """Of a CacheAttention over `most` pages a sequence; what that refuses of its sizes is refused here."""
+    need = ctypes.c_size_t()
+    check(_load().qfg_cache_attention_workspace_bytes(cache._at, seqs, tokens, heads, most, ctypes.byref(need)))
+    return need.value
+
+
 class KvCache:
     """Keys and values of all sequences, cut into pages of `page` tokens (a multiple of 32): torch.uint8, block-16 NVFP4 (9/16 of a byte a value), or
     torch.float8_e4m3fn with a scale for each token and head.
@@ -329,9 +336,8 @@ class CacheAttention:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _given(op, "out", out, q.shape, q.dtype)
         sums = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if lse else None
-        need = ctypes.c_size_t()
-        check(self._lib.qfg_cache_attention_workspace_bytes(at, seqs, tokens, heads, most, ctypes.byref(need)))
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        need = _workspace_bytes(cache, seqs, tokens, heads, most)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         check(self._lib.qfg_cache_attention(_DTYPES[q.dtype], q.data_ptr(), ld_seq, ld_token, seqs, tokens, heads, at, tp, ldt, most, lengths.data_ptr(),
                                             self.scale or 1 / math.sqrt(dim), workspace.data_ptr() if workspace is not None else None, out.data_ptr(),
                                             sums.data_ptr() if lse else None, _stream_ptr()))

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from .attention import CacheAttention, KvCache, PromptAttention, QkNormRope
+from .attention import CacheAttention, KvCache, PromptAttention, QkNormRope, _table, _whole_numbers, _workspace_bytes
 from .ops import QuantGemm, RmsNormQuant, RowQuant
 
 
@@ -21,36 +21,61 @@ class QuantAttention:
     QkNormRope and `cache` a KvCache, which is this layer's own.
 
     x, residual [tokens, hidden] in BF16; positions as the QkNormRope takes them; slots int64 [tokens]: where the tokens go in the cache.
-    A prompt: offsets int32 [sequences + 1], the tokens' sequences, which attend to themselves, with keys and values that no cache has rounded.
-    A step: table and lengths, as CacheAttention takes them; the tokens are the last ones of as many sequences, equally many of each."""
+    A prompt: offsets int32 [sequences + 1], the tokens' sequences, which attend to themselves, with keys and values that no cache has rounded; heads of 64 or 128
+    channels.  A step: table and lengths, as CacheAttention takes them; the tokens are the last ones of as many sequences, equally many of each.  A call that is refused
+    has written nothing into the cache."""
 
     def __init__(self, norm_weight, qkv, qkv_scale, out, out_scale, heads: int, kv_heads: int, rope: QkNormRope, cache: KvCache, q_weight=None, k_weight=None,
                  eps: float = 1e-6, weight_offset: float = 0.0, scale: float | None = None):
         dim = cache.head_dim
         if qkv.dtype != out.dtype or qkv.shape[1] != (heads + 2 * kv_heads) * dim or tuple(out.shape) != (heads * dim, qkv.shape[0]) or cache.kv_heads != kv_heads:
             raise ValueError("QuantAttention: qkv is [hidden, (heads + 2 * kv_heads) * head_dim] and out [heads * head_dim, hidden], of one type, and the cache has kv_heads")
+        if rope.head_dim != dim:
+            raise ValueError(f"QuantAttention: the cache has heads of {dim} channels, the QkNormRope of {rope.head_dim}")
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, dim
         self.norm_weight, self.qkv, self.out, self.q_weight, self.k_weight, self.cache = norm_weight, qkv, out, q_weight, k_weight, cache
-        self._rope = rope
+        self._rope, self._device = rope, cache.k.get_device()
         self._norm = RmsNormQuant(eps=eps, weight_offset=weight_offset, dtype=qkv.dtype)
         self._rows = RowQuant(dtype=qkv.dtype)
         self._qkv, self._out = QuantGemm(w_scale=qkv_scale), QuantGemm(w_scale=out_scale)
         self._prompt, self._step = PromptAttention(scale=scale), CacheAttention(scale=scale)
 
+    def _check_step(self, rows, table, lengths):
+        _, _, seqs, most = _table("QuantAttention", table, self.cache)
+        tokens = rows // max(1, seqs)
+        if _whole_numbers("QuantAttention", "lengths", lengths, (torch.int32,), 1).shape[0] != seqs or tokens * seqs != rows:
+            raise ValueError(f"QuantAttention: there must be a length for each of {seqs} sequences, and equally many tokens")
+        _workspace_bytes(self.cache, seqs, tokens, self.heads, most)
+
     def __call__(self, x, residual, positions, slots, table=None, lengths=None, offsets=None):
-        if (offsets is None) == (table is None):
+        if (offsets is None) == (table is None) or (table is None) != (lengths is None):
             raise ValueError("QuantAttention: a prompt has offsets, a step a table and lengths")
         rows, dim = x.shape[0], self.head_dim
+        # What the operators behind the cache's write would refuse.  Ordinary arguments have passed in a microsecond (the sizes are well within those that a step's counting sets).
+        if offsets is not None:
+            if dim == 256:
+                raise ValueError("QuantAttention: prompts have heads of 64 or 128 channels")
+            plain = offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and offsets.get_device() == self._device
+            if offsets.numel() < 1 or not (plain or _whole_numbers("QuantAttention", "offsets", offsets, (torch.int32,), 1) is offsets):
+                raise ValueError("QuantAttention: there must be one offset more than sequences")
+        else:
+            seqs, tokens = lengths.shape[0] if lengths.dim() == 1 else -1, 0
+            if seqs > 0:
+                tokens = rows // seqs
+            if not (table.dtype == lengths.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == seqs and tokens * seqs == rows and table.is_contiguous() and
+                    lengths.is_contiguous() and table.get_device() == lengths.get_device() == self._device and seqs <= 65536 and tokens <= 1024 and
+                    table.numel() * self.cache.page <= 1 << 22):
+                self._check_step(rows, table, lengths)
         rows8, scale, h = self._norm(x, self.norm_weight, residual)
-        both = self._qkv(rows8, scale, self.qkv).view(rows, -1, dim)
+        both = self._qkv(rows8, scale, self.qkv).view(rows, self.heads + 2 * self.kv_heads, dim)
         q, k, v = both[:, :self.heads], both[:, self.heads:-self.kv_heads], both[:, -self.kv_heads:]
         if offsets is not None:
             q, k = self._rope(q, k, positions, self.q_weight, self.k_weight, v, self.cache, slots, True)
             y = self._prompt(q, k, v, offsets)
         else:
             q = self._rope(q, k, positions, self.q_weight, self.k_weight, v, self.cache, slots)
-            y = self._step(q.view(lengths.shape[0], -1, self.heads, dim), self.cache, table, lengths)
-        rows8, scale = self._rows(y.view(rows, -1))
+            y = self._step(q.view(seqs, tokens, self.heads, dim), self.cache, table, lengths)
+        rows8, scale = self._rows(y.view(rows, self.heads * dim))
         return self._out(rows8, scale, self.out), h
 
 
