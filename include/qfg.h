@@ -389,7 +389,8 @@ typedef struct qfg_kv_cache {
  * Pair i < n_pairs is channels (i, i + n_pairs), interleaved (2 i, 2 i + 1); channels from 2 n_pairs on stay.  n_pairs is a multiple of
  * 16.  `axis` (NULL: all 0) says which of the rows of `positions` a pair goes by: one for text, several for images and video.  Positions
  * are integers of `position_bytes` (4 or 8), rows `ld_positions` apart; angles are exact to 2^-44 of a turn for positions of a million.
- * All in FP32, rounded once to `dtype` (BFLOAT16, FLOAT16, FLOAT) for q_out and k_out, contiguous, and once to the cache's type.
+ * All in FP32, rounded once to `dtype` (BFLOAT16, FLOAT16, FLOAT) for q_out and k_out, contiguous, and once to the cache's type.  A row whose sum of
+ * squares is not a finite FP32 number is NaN; where mean(x^2) + eps lies below 2^-126 it has the bits that a subnormal number has.
  * Without a cache k_out is needed and v is not looked at; with one, k_out may be NULL.  `slots` [tokens]: a token whose slot is negative
  * or lies behind the cache is not written; slots must differ.  q_out and k_out may not overlap the inputs.  tokens == 0 is a no-op.  A node
  * belongs to the device it was made on. */
