@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 from qwen38_flash_ops_b200 import CacheRead, QfgError, attention, ops  # noqa: E402
 
 
-@pytest.mark.parametrize("cache", [5, 4096, 1 << 62, -1, True, 3.0, "cache", None, object()], ids=str)
+@pytest.mark.parametrize("cache", [5, 4096, 1 << 62, -1, True, 3.0, "cache", None, object()], ids=lambda c: "object" if type(c) is object else str(c))
 def test_what_is_no_cache(cache):
     """In a process of its own: an address that is read ends it."""
     table, offsets = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)

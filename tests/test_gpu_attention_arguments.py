@@ -8,7 +8,7 @@ from qwen38_flash_ops_b200 import CacheAttention, CacheRead, CacheWrite, KvCache
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("cache", [0, 5, 4096, 1 << 62, -1, True, 1.5, "cache", object()], ids=str)
+@pytest.mark.parametrize("cache", [0, 5, 4096, 1 << 62, -1, True, 1.5, "cache", object()], ids=lambda c: "object" if type(c) is object else str(c))
 def test_what_is_no_cache(cuda, cache):
     x = torch.zeros(4, 2, 64, device="cuda").bfloat16()
     at, slots, table, n = torch.arange(4).cuda(), torch.arange(4).cuda(), torch.zeros(4, 1, dtype=torch.int32).cuda(), torch.ones(4, dtype=torch.int32).cuda()
