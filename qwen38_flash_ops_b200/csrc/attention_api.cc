@@ -109,6 +109,8 @@ int qfg_qk_norm_rope_create(const double* inv_freq, const int32_t* axis, int n_p
     cudaError_t err = cudaGetDevice(&op->device);
     if (err == cudaSuccess && n_pairs > 0) err = cudaMalloc(reinterpret_cast<void**>(&op->pairs), pairs.size());
     if (err == cudaSuccess && n_pairs > 0) err = cudaMemcpy(op->pairs, pairs.data(), pairs.size(), cudaMemcpyHostToDevice);
+    // a copy from pageable memory may return ahead of its last part, and the node may be used on a stream that does not wait for the default one
+    if (err == cudaSuccess && n_pairs > 0) err = cudaStreamSynchronize(nullptr);
     if (err != cudaSuccess) throw std::runtime_error(cudaGetErrorString(err));
   } catch (const std::invalid_argument& e) {
     delete op;

@@ -45,8 +45,9 @@ int Alignment(const void* base, long long pitch) {
 float* UploadScales(const float* host, size_t n, const char* op) {
   if (host == nullptr || n == 0) return nullptr;
   float* dev = nullptr;
-  if (cudaMalloc(&dev, n * sizeof(float)) != cudaSuccess ||
-      cudaMemcpy(dev, host, n * sizeof(float), cudaMemcpyHostToDevice) != cudaSuccess) {
+  // the wait: a copy from pageable memory may return ahead of its last part, and the node may be used on a stream that does not wait for the default one
+  if (cudaMalloc(&dev, n * sizeof(float)) != cudaSuccess || cudaMemcpy(dev, host, n * sizeof(float), cudaMemcpyHostToDevice) != cudaSuccess ||
+      cudaStreamSynchronize(nullptr) != cudaSuccess) {
     cudaFree(dev);
     cudaGetLastError();
     throw std::runtime_error(std::string(op) + ": failed to upload w_scale");
