@@ -19,7 +19,7 @@
 // are made (from registers, one run ahead, 38.5 us for the 35.4 below, and 286 bytes of them spilt).
 //
 // What bounds them: one read and one write of every head.  4096 tokens of 64 + 8 + 8 heads of 128, BF16, with an E4M3 cache: 35.4 us for 160 MB, 4.5 TB/s; of the issue slots
-// two thirds are taken (the quotients in two parts, the norm's and the rotation's FP32).  Four blocks an SM of 64 registers hide more than five with shorter rings (47 us), and than
+// two thirds are taken (the norm and the rotation in FP32 of 64 + 8 heads, whose weights are read from shared memory for each; without the cache, keys out instead, 31 us).  Four blocks an SM of 64 registers hide more than five with shorter rings (47 us), and than
 // three of 80 did.  Sines and cosines read from shared memory at every row: 46.  Eight tokens: 4.8 us, the launch and one trip to memory: a row for each warp.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

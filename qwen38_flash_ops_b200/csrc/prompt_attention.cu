@@ -14,9 +14,9 @@
 //   ring      128 keys or 128 values a stage, by tensor copies; rows of 128 bytes, swizzled
 //
 // Where there are more blocks than the GPU holds, a block that is done takes on one that has not begun, and never will: the copies go on to its queries and keys while the last
-// ones are worked on, and its first S is made while the rows ahead are written.  Rows are written in runs of 64 bytes: a warp's 16 bytes of 32 rows at a time fill the queue of
-// loads and stores, and waits and the next item's reading stand behind them.  Both together: 8192 tokens of 64 heads 930 -> 829 us, 48 prompts of 256 tokens of 24 heads of 128
-// 102 -> 51.
+// ones are worked on, and its first S is made while the rows ahead are written.  8192 tokens of 64 / 8 heads of 128: 871 us by itself without that, 813 with it; back to back, under
+// the power cap, 890 and 840.  48 prompts of 256 tokens of 24 / 8 heads, back to back: 95 and 50.  Rows are written in runs of 64 bytes: a warp's 16 bytes of 32 rows at a time
+// fill the queue of loads and stores, and waits and the next item's reading stand behind them.
 //
 // One pass: m is taken up only when a score passes it by 8 (in powers of two), and only then are O and the sum scaled again.  In FP16 weights are 2^7 times as large, up to 2^15: its
 // smallest number is 2^-31 of the largest weight then, which keeps those of long sequences that are all small beside one.  S and the sums are FP32; P is rounded to the type of
@@ -24,8 +24,12 @@
 //
 // Products and exponentials take the same time (a tile of 128 x 128 at D = 128: 1024 cycles of the tensor core, 1024 of the unit for exponentials at 16 a cycle), which is
 // what bounds the kernel; a quarter of the exponentials goes to the FMA units for that reason.  No weight is made for tiles that the mask leaves out.  Causal, 8192 tokens of
-// 64 / 8 heads of 128: 802 us by itself, 1.37 PFLOP/s, the tensor pipe busy for 73 % of the cycles; 925 back to back, under the power cap.  Heads of 64: the softmax warps, two a
-// scheduler, 650 instructions a tile each (S apart from P, so that the next is made meanwhile, changed nothing; 8192 tokens of 24 heads 263 us).
+// 64 / 8 heads of 128: 813 to 835 us by itself, 1.32 to 1.35 PFLOP/s, the tensor pipe busy for 72 % of the cycles; 830 to 940 back to back, by the power that the inputs take.
+// Heads of 64: the softmax warps, two a scheduler, 650 instructions a tile each (S apart from P, so that the next is made meanwhile, changed nothing; 8192 tokens of 24 heads
+// 260 us).
+//
+// Two tiles that take turns, a maximum that is seldom taken up, a part of the exponentials by a polynomial and P in the place of S are methods that have been published for
+// attention on GPUs with tensor memory; sums that run along with a maximum are Milakov and Gimelshein's (2018).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -44,8 +48,8 @@ namespace qfg {
 namespace {
 
 constexpr int kTile = 128;
-// Of sixteen pairs of weights those that the FMA units make, so that less waits for the unit for exponentials, which is an eighth as wide.  8192 tokens of 24 heads of 64,
-// us: none 280, two 267, four 263, six 277; of 64 heads of 128 830 to 870 whatever the share.
+// Of sixteen pairs of weights those that the FMA units make, so that less waits for the unit for exponentials, which is an eighth as wide.  8192 tokens, us: of 24 heads of 64 none
+// 280, two 267, four 263, six 277; of 64 heads of 128, by itself, none 848, four 829, and back to back, under the power cap, 863 to 874 and 860 to 870.
 constexpr int kPolyOf16 = 4;
 struct PromptParams {
   CUtensorMap q, k, v;
@@ -291,7 +295,8 @@ __device__ __forceinline__ int UpTo(int v, int lane) {  // the sum of this lane'
   return v;
 }
 // The place of a block of the grid, by its rank among those of its head.  `from` is where the last search of many sequences ended, which is where the next one begins: ranks
-// mostly rise (the last of 32 sequences, and the blocks ahead of them).  512 prompts of up to 300 tokens, 24 / 8 heads of 128: 815 -> 502 us, 2000 of up to 30 3.0 -> 0.73 ms.
+// mostly rise (the last of 32 sequences, and the blocks ahead of them).  512 prompts of up to 300 tokens, 24 / 8 heads of 128: 745 us from the start, 458 so; 2000 of up to 30
+// 4.0 and 1.08 ms.
 struct Cursor {
   int base, before;
 };
