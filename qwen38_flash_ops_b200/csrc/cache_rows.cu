@@ -473,11 +473,11 @@ __global__ void __launch_bounds__(kThreads) CacheReadKernel(const ReadParams p) 
         const int mid = (lo + hi) / 2;
         (p.offsets[mid] <= row ? lo : hi) = mid;
       }
-      const int in = static_cast<int>(row - p.offsets[lo]), page = in / p.cache.page;
+      const long long in = row - p.offsets[lo], room = static_cast<long long>(p.most_pages) * p.cache.page;  // an offset may be as far below 0 as an integer can
       at = -1;
-      if (page < p.most_pages) {
-        const int id = p.table[lo * p.ld_table + page];
-        if (id >= 0 && id < p.cache.pages) at = static_cast<long long>(id) * p.cache.heads * p.cache.page + (in - page * p.cache.page);
+      if (in < room) {  // and so within 32 bits
+        const int page = static_cast<int>(in) / p.cache.page, id = p.table[lo * p.ld_table + page];
+        if (id >= 0 && id < p.cache.pages) at = static_cast<long long>(id) * p.cache.heads * p.cache.page + (static_cast<int>(in) - page * p.cache.page);
       }
     }
     place[threadIdx.x] = at;
