@@ -418,7 +418,8 @@ QFG_API int qfg_cache_read(const qfg_kv_cache* cache, const int32_t* table, int6
  * logarithm of the sum of the exponentials.  Query head h reads key head h / (q_heads / kv_heads).  A row that sees nothing (a length of
  * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it (a table is for 2^34 tokens at most); tokens whose
  * page is none of the cache's are left out.  What lies behind a sequence's length takes no part, whatever it is.  A value within it that is
- * not finite makes all rows of its key head NaN, those of earlier tokens too: their weight for it is 0, and 0 times it is not.  In eight bits
+ * not finite makes all rows of its key head NaN, those of earlier tokens too: their weight for it is 0, and 0 times it is not.  A row of q that
+ * is not finite is NaN, where it sees anything, its lse as well; so is one that sees a key whose scale is NaN.  In eight bits
  * a value's scale may be up to 2^107 (values up to 2^115); rows with larger ones may become NaN.
  * `workspace`: that many bytes (0 where sequences are never cut), on 16 bytes, not looked at before the call and free behind it; calls
  * that run at once need one each. */

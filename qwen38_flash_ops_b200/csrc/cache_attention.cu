@@ -413,7 +413,9 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // 2^(9 - exponent) of the largest and its inverse; the exponent is kept where both are ordinary numbers
         const int e = min(max(static_cast<int>(top >> 23), 20), 254);  // 254: of the largest number there is
-        const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(e - 9) << 23) * p.scale;
+        const float up = __uint_as_float(static_cast<uint32_t>(263 - e) << 23);
+        // of an infinity the scores may all be -infinity, which is not to pass for a row that sees nothing
+        const float down = top >= 0x7F800000u ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(static_cast<uint32_t>(e - 9) << 23) * p.scale;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) q[n][i / 2][i % 2] = Pack16(v[2 * i] * up, v[2 * i + 1] * up);
 #pragma unroll

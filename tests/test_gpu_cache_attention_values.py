@@ -56,3 +56,29 @@ def test_many_weights_that_are_tiny_beside_one(cuda, dim, form):
     tol = (half_step(torch.float16) + sums + count / 16 * 2.0 ** -23) * y.abs() + 2.0 ** -11 * size + tiny + 2.0 ** -25
     assert ((got.cpu().double() - y).abs() <= tol).all(), ((got.cpu().double() - y).abs() / tol).max()
     assert ((lse.cpu().double() - log).abs() <= 2.0 ** -18 * (1 + log) + sums).all()
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_queries_that_are_no_numbers(cuda, form, dim, value):
+    """Infinities as well, whose scores may all be -infinity: rows that see a key are NaN, those that see none 0, and others as they were."""
+    for lengths in ([1, 0], [2, 1], [400, 33]):
+        cache, table, q, n = a_case(form, dim, 1, 3, 2, lengths, torch.bfloat16)
+        for c in (3, 7):  # keys of one sign in channel 3, of the other in channel 7
+            cache.k.view(torch.uint8)[..., c if form == "e4m3" else c // 2] = 0x30 if c == 3 else 0xB0
+        want, log = CacheAttention()(q, cache, table, n, lse=True)
+        for c in (3, 7):
+            bad = q.clone()
+            bad[:, :, 1, c] = value
+            got, lse = CacheAttention()(bad, cache, table, n, lse=True)
+            for i, m in enumerate(lengths):
+                for t in range(2):
+                    sees = m - 1 + t > 0
+                    if sees:
+                        assert torch.isnan(got[i, t, 1].float()).all() and torch.isnan(lse[i, t, 1]), (lengths, c, i, t)
+                    else:
+                        assert (got[i, t] == 0).all() and (lse[i, t] == -math.inf).all()
+            got[:, :, 1], lse[:, :, 1] = want[:, :, 1], log[:, :, 1]
+            assert torch.isfinite(got).all() and ((got.double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs() + 2.0 ** -9).all()
+            assert torch.equal(lse == -math.inf, log == -math.inf) and torch.allclose(lse, log, atol=1e-3)
