@@ -418,9 +418,9 @@ QFG_API int qfg_cache_read(const qfg_kv_cache* cache, const int32_t* table, int6
  * logarithm of the sum of the exponentials.  Query head h reads key head h / (q_heads / kv_heads).  A row that sees nothing (a length of
  * 0, a padded place) is 0, its lse -inf.  Lengths past the table's width are cut to it (a table is for 2^34 tokens at most); tokens whose
  * page is none of the cache's are left out.  What lies behind a sequence's length takes no part, whatever it is.  A value within it that is
- * not finite makes all rows of its key head NaN, those of earlier tokens too: their weight for it is 0, and 0 times it is not.  A row of q that
- * is not finite is NaN, where it sees anything, its lse as well; so is one that sees a key whose scale is NaN.  In eight bits
- * a value's scale may be up to 2^107 (values up to 2^115); rows with larger ones may become NaN.
+ * not finite makes the rows of its key head NaN, those of earlier tokens too (their weight for it is 0, and 0 times it is not), but no row that
+ * sees nothing.  A row of q that is not finite is NaN, where it sees anything, its lse as well; so is one that sees a key whose scale is NaN.
+ * In eight bits a value's scale may be up to 2^107 (values up to 2^115); rows with larger ones may become NaN.
  * `workspace`: that many bytes (0 where sequences are never cut), on 16 bytes, not looked at before the call and free behind it; calls
  * that run at once need one each. */
 QFG_API int qfg_cache_attention_workspace_bytes(const qfg_kv_cache* cache, int64_t seqs, int64_t tokens, int64_t q_heads, int64_t most_pages, size_t* bytes);
@@ -433,10 +433,10 @@ QFG_API int qfg_cache_attention(int dtype, const void* q, int64_t ld_seq, int64_
  * BFLOAT16 and FLOAT16, heads of 64 or 128 channels, bases and tokens on 16 bytes; out [q_rows][q_heads][head_dim] and lse (NULL, or FP32
  * [q_rows][q_heads]) contiguous.  A row that sees nothing is 0, its lse -inf.  Rows ahead of the first and behind the last sequence are left
  * as they were; what lies in keys and values of other sequences takes no part, whatever it is.  Within a sequence a value that is not
- * finite makes rows of the same head that lie up to 128 tokens ahead of it NaN as well: their weight for it is 0, and 0 times it is not;
- * a finite one, however large, takes no part in them.  A row that has a score of NaN or +infinity is NaN, its lse as well; one of -infinity
- * is a weight of 0, and a row of none but those NaN.  Scores (scale q k) have to stay below 2^28: a row whose largest is further from 0 than
- * that may become NaN, and does where FP32 cannot tell what it is. */
+ * finite makes rows of the same head that lie up to 128 tokens ahead of it NaN as well (their weight for it is 0, and 0 times it is not), but
+ * no row that sees nothing; a finite one, however large, takes no part in them.  A row that has a score of NaN or +infinity is NaN, its lse as
+ * well; one of -infinity is a weight of 0, and a row of none but those NaN.  Scores (scale q k) have to stay below 2^28: a row whose largest is
+ * further from 0 than that may become NaN, and does where FP32 cannot tell what it is. */
 QFG_API int qfg_prompt_attention(int dtype, const void* q, int64_t ldq, int64_t q_rows, int64_t q_heads, const void* k, int64_t ldk, const void* v,
                                  int64_t ldv, int64_t k_rows, int64_t kv_heads, int64_t head_dim, const int32_t* q_offsets, const int32_t* k_offsets,
                                  int64_t seqs, int causal, float scale, void* out, float* lse, void* stream);

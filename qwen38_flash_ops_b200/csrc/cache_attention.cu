@@ -671,9 +671,10 @@ __global__ void __launch_bounds__(kThreads, Geometry<D, FP4, NT>::kBlocks) Cache
         if (whole_unit) {
           const long long to = RowOf(p, at.seq, at.unit, row0 + of);
           const float by = total == 0.f ? 0.f : p.cache.v_unit / total;
+          const uint32_t seen = total == 0.f ? 0u : ~0u;  // 0 times what a row does not see may be no number
           uint32_t w[kTilesOfO];
 #pragma unroll
-          for (int t = 0; t < kTilesOfO; ++t) w[t] = Packed(p.bf16, o[n][t][r] * by, o[n][t][2 + r] * by);
+          for (int t = 0; t < kTilesOfO; ++t) w[t] = Packed(p.bf16, o[n][t][r] * by, o[n][t][2 + r] * by) & seen;
           uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D + g * kValueChannels);
 #pragma unroll
           for (int t = 0; t < kTilesOfO / 4; ++t) out[t] = make_uint4(w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]);

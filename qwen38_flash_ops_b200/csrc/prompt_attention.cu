@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(Geometry<D, TILES>::kThreads, Geometry<D, TILE
           LoadColumns(o_at + c, o);
           WaitLoads();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by);
+          for (int i = 0; i < 16; ++i) w[i] = total == 0.f ? 0u : Pack<BF16>(o[2 * i] * by, o[2 * i + 1] * by);  // 0 times what it does not see may be no number
           Exchange(w, lane);
         }
 #pragma unroll

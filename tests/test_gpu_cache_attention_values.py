@@ -82,3 +82,21 @@ def test_queries_that_are_no_numbers(cuda, form, dim, value):
             got[:, :, 1], lse[:, :, 1] = want[:, :, 1], log[:, :, 1]
             assert torch.isfinite(got).all() and ((got.double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs() + 2.0 ** -9).all()
             assert torch.equal(lse == -math.inf, log == -math.inf) and torch.allclose(lse, log, atol=1e-3)
+
+
+@pytest.mark.parametrize("dim,group,tokens", [(64, 4, 3), (128, 8, 3), (256, 2, 3)])
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_that_see_nothing_beside_values_that_are_no_numbers(cuda, form, dim, group, tokens):
+    """A padded place is 0, whatever the tokens hold that only later rows see."""
+    lengths = [1, 2, 0, 3]
+    cache, table, q, n = a_case(form, dim, 2, group, tokens, lengths, torch.bfloat16)
+    want, log = CacheAttention()(q, cache, table, n, lse=True)
+    if form == "e4m3":
+        cache.v_scale.fill_(math.nan)
+    else:
+        cache.v_scale.view(torch.uint8).fill_(0x7F)
+    got, lse = CacheAttention()(q, cache, table, n, lse=True)
+    for i, m in enumerate(lengths):
+        none = max(0, tokens - m)
+        assert (got[i, :none] == 0).all() and (lse[i, :none] == -math.inf).all() and torch.isnan(got[i, none:].float()).all()
+        assert torch.allclose(lse[i, none:], log[i, none:], atol=1e-4)

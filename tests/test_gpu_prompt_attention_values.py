@@ -122,3 +122,18 @@ def test_scores_past_what_fp32_tells_apart(cuda, dtype, dim, causal):
         assert ((got.cpu().double() - want).abs()[sure] <= 2.0 ** -7 * want.abs()[sure]).all(), power
         assert (torch.isnan(lse) == bad).all() and torch.isfinite(lse[~bad]).all()
         assert power > 0 or not bad.any()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_that_see_nothing_beside_values_that_are_no_numbers(cuda, dtype, dim, causal):
+    """More queries than keys: the first ones see none, and are 0 whatever the keys and values are; not causal, only those of a sequence without keys."""
+    for value in (NAN, INF):
+        q, k, v = a_case(90, 2, 1, dim, dtype)
+        k[:], v[:] = value, value
+        at = torch.tensor([0, 10, 90], dtype=torch.int32).cuda()
+        got, lse = PromptAttention(causal=causal)(q, k[:30], v[:30], at, torch.tensor([0, 0, 30], dtype=torch.int32).cuda(), lse=True)
+        none = 60 if causal else 10
+        assert (got[:none] == 0).all() and (lse[:none] == -math.inf).all()
+        assert torch.isnan(got[none:].float()).all() and torch.isnan(lse[none:]).all()
